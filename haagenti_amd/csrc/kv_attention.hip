@@ -1,0 +1,607 @@
+// Attention over the paged 8-bit cache (layout and rules: haagenti_hip.h).
+//
+// With column c = (new row i, head g of the group), i = c / group, both
+// kernels compute, per cache head,
+//   S^T = K Q^T     codes (exact in f16) times f16 queries, f32
+//   z   = S^T (scale of K's block) (softmax scale) log2(e)
+//   m, l, O: running maximum of z, sum of 2^(z - m), and
+//   O^T += V^T P^T  codes times f16 P = 2^(z - m) (scale of V's block) / top,
+//                   top the largest V scale so far (so P <= 1 whatever the
+//                   scales are), O in units of top, f32.
+// Tokens lie on the first product's rows, so its accumulators hold, for one
+// column per lane, just the tokens that the lane supplies to the second
+// product's P^T operand: P never moves between lanes.  Which token a row
+// stands for is free as long as V's operand agrees, and is chosen so that V's
+// operands are contiguous bytes of the cache.  The cache's codes c become the
+// f16 numbers 1024 + c by byte permutation, less 1152 by one packed add.
+//
+// bf16 queries are scaled to a largest magnitude of 1 to 2 per row by a power
+// of two before they become f16 (exact down to 2^-25 of the largest).
+#include "layer_ops.hpp"
+
+namespace hh {
+namespace {
+
+struct AttnArgs {
+    hh_kv_cache cache;
+    hh_kv_attention_args a;
+    uint32_t group;      // q heads per cache head
+    uint32_t splits;     // of a request's tokens, in chunks of:
+    uint32_t chunk;      // a multiple of 256
+    uint32_t tiles;      // column tiles per request (tile kernel)
+    uint32_t small;      // requests with at most this many columns are the step kernel's
+    uint32_t cols;       // most columns of such a request
+    float *part_o;       // [request][head][split][cols][dim]
+    float *part_ml;      // [request][head][split][cols][2]
+};
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// 4 codes as 4 f16 numbers -127..127.
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    const f16x2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - bias);
+    hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - bias);
+}
+__device__ __forceinline__ f16x8 codes8_to_f16(uint32_t a, uint32_t b) {
+    u32x4 v;
+    uint32_t x, y;
+    codes_to_f16(a, x, y);
+    v[0] = x, v[1] = y;
+    codes_to_f16(b, x, y);
+    v[2] = x, v[3] = y;
+    return __builtin_bit_cast(f16x8, v);
+}
+
+// One request's part of the call.
+struct Request {
+    int32_t q0, rows, kv_len, seen;  // seen: tokens within the call's bounds
+};
+__device__ __forceinline__ Request request_of(const AttnArgs &p, uint32_t r) {
+    Request q;
+    q.q0 = p.a.d_start[r];
+    q.rows = p.a.d_start[r + 1] - q.q0;
+    q.kv_len = p.a.d_kv_len[r];
+    const uint64_t room = min((uint64_t)p.a.max_kv, (uint64_t)p.a.table_width * p.cache.block_size);
+    q.seen = (int32_t)min((uint64_t)max(q.kv_len, 0), room);
+    if (q.q0 < 0 || q.rows < 0 || (uint32_t)q.q0 > p.a.tokens || (uint32_t)q.rows > p.a.tokens - (uint32_t)q.q0) q.rows = 0;
+    return q;
+}
+__device__ __forceinline__ uint32_t columns_of(const AttnArgs &p, const Request &q) {
+    return min((uint32_t)q.rows, p.a.max_q) * p.group;
+}
+// Tokens that new row i sees.
+__device__ __forceinline__ int32_t limit_of(const Request &q, int32_t i) {
+    return max(0, min(q.seen, q.kv_len - q.rows + i + 1));
+}
+
+// The cache block of a token below `seen`, or -1.
+__device__ __forceinline__ int32_t block_of(const AttnArgs &p, const int32_t *table, int32_t tok, int32_t end) {
+    if (tok >= end) return -1;
+    const int32_t id = table[(uint32_t)tok / p.cache.block_size];
+    return (uint32_t)id < p.cache.num_blocks ? id : -1;
+}
+
+// N f16 fragments of 8 dimensions of a query row, fragment f at dimension
+// dim(f), as f16 scaled by a power of two of the row; returns what undoes the
+// scaling.  `join` makes a lane's largest magnitude the row's.
+template <int DT, int N, typename Dim, typename Join>
+__device__ __forceinline__ float load_query(const uint16_t *row, bool wide, f16x8 (&q)[N], Dim dim, Join join) {
+    u32x4 raw[N];
+    float top = 0.0f;
+#pragma unroll
+    for (int f = 0; f < N; f++) {
+        raw[f] = u32x4{};
+        if (row) {
+            const uint16_t *at = row + dim(f);
+            if (wide) {
+                raw[f] = *reinterpret_cast<const u32x4 *>(at);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) raw[f][e] = (uint32_t)at[2 * e] | (uint32_t)at[2 * e + 1] << 16;
+            }
+        }
+        if constexpr (DT == HH_F16) q[f] = __builtin_bit_cast(f16x8, raw[f]);
+    }
+    if constexpr (DT == HH_F16) return 1.0f;
+#pragma unroll
+    for (int f = 0; f < N; f++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(half_to_f32<DT>((raw[f][e >> 1] >> (16 * (e & 1))) & 0xffffu)));
+    const uint32_t ex = __float_as_uint(join(top)) >> 23;
+    const bool plain = ex == 0 || ex == 255;  // zeros and subnormals, infinities
+    const float down = plain ? 1.0f : ldexpf(1.0f, 127 - (int)ex), up = plain ? 1.0f : ldexpf(1.0f, (int)ex - 127);
+#pragma unroll
+    for (int f = 0; f < N; f++)
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            q[f][e] = (_Float16)(half_to_f32<DT>((raw[f][e >> 1] >> (16 * (e & 1))) & 0xffffu) * down);
+    return up;
+}
+
+// Rows past the last request's are zeros (one workgroup of the launch).
+__device__ __forceinline__ void zero_tail(const AttnArgs &p, uint32_t dim, uint32_t threads) {
+    const uint32_t total = p.a.tokens, from = (uint32_t)max(0, p.a.d_start[p.a.requests]);
+    uint16_t *out = reinterpret_cast<uint16_t *>(p.a.d_out);
+    for (uint64_t i = (uint64_t)from * p.a.q_heads * dim + threadIdx.x; i < (uint64_t)total * p.a.q_heads * dim;
+         i += threads) {
+        const uint64_t t = i / (p.a.q_heads * dim), e = i % (p.a.q_heads * dim);
+        out[t * p.a.out_token_stride + e / dim * p.a.out_head_stride + e % dim] = 0;
+    }
+}
+
+// 4 consecutive dimensions of an output row.
+template <int DT>
+__device__ __forceinline__ void store4(uint16_t *to, bool wide, const float *v) {
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = f32_to_half<DT>(v[i]);
+    if (wide) {
+        *reinterpret_cast<u32x2 *>(to) = u32x2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) to[i] = (uint16_t)h[i];
+    }
+}
+
+// ---------------------------------------------------------------- few columns
+//
+// A step of a running request: at most 16 columns, one 16 x 16 x 32 tile
+// wide.  Bound by reading the codes once.  A workgroup takes one chunk of a
+// request's tokens for one cache head, its 4 waves every fourth 64 tokens
+// straight from memory to registers; their results are joined in LDS, the
+// chunks' by attn_join_kernel.
+//
+// In a wave's 64 tokens, run u (16 tokens, in one block) supplies rows
+// 4u..4u+3 of each of the 4 row tiles: tile t's row 4u + i is token
+// 16u + 4t + i, so that lane (column, u) ends with tokens 16u..16u+15 of its
+// column, and V's operand is 16 contiguous codes of a dimension.
+
+template <int DT, int D>
+__global__ __launch_bounds__(256) void attn_step_kernel(const AttnArgs p) {
+    constexpr int KS = D / 32, VT = D / 16, KW = D / 16;  // k steps, V tiles, 4-byte words of K per lane and row
+    __shared__ __align__(16) float lds_o[2][16][D + 4];
+    __shared__ float lds_ml[4][16][2];
+    const uint32_t r = blockIdx.x / p.splits, split = blockIdx.x % p.splits, h = blockIdx.y;
+    if (r == p.a.requests - 1 && split == 0 && h == 0) zero_tail(p, D, 256);
+    const Request rq = request_of(p, r);
+    const uint32_t cols = columns_of(p, rq);
+    if (cols == 0 || cols > p.small) return;
+    const int32_t begin = (int32_t)(split * p.chunk), end = min(rq.seen, begin + (int32_t)p.chunk);
+    if (split && begin >= rq.seen) return;
+    const bool whole = rq.seen <= (int32_t)p.chunk;  // no other chunk
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, u = lane >> 4;
+    const int32_t bs = (int32_t)p.cache.block_size;
+    const int32_t *table = p.a.d_table + (uint64_t)r * p.a.table_stride;
+    const bool live = (uint32_t)col < cols;
+    const uint32_t qi = (uint32_t)col / p.group, qh = h * p.group + (uint32_t)col % p.group;
+    const int32_t limit = live ? min(end, limit_of(rq, (int32_t)qi)) : 0;
+
+    f16x8 q[KS];
+    float zs;
+    {
+        const uint16_t *row = live ? reinterpret_cast<const uint16_t *>(p.a.d_q) +
+                                         ((uint64_t)rq.q0 + qi) * p.a.q_token_stride + qh * p.a.q_head_stride
+                                   : nullptr;
+        const bool wide = !((uintptr_t)p.a.d_q & 15u) && !((p.a.q_token_stride | p.a.q_head_stride) & 7u);
+        zs = load_query<DT, KS>(
+            row, wide, q, [&](int f) { return u * (D / 4) + f * 8; },
+            [](float v) { v = fmaxf(v, __shfl_xor(v, 16)); return fmaxf(v, __shfl_xor(v, 32)); });
+        zs *= p.a.scale * kLog2e;
+    }
+
+    f32x4 o[VT];
+#pragma unroll
+    for (int t = 0; t < VT; t++) o[t] = f32x4{0, 0, 0, 0};
+    float m = -__builtin_inff(), l = 0.0f, top = 0.0f;
+
+    for (int32_t base = begin + 64 * wave; base < end; base += 256) {
+        // K rows: this lane's rows are in run col >> 2; V and the scales: run u
+        const int32_t tk = base + 16 * (col >> 2), tv = base + 16 * u;
+        const int32_t bk = block_of(p, table, tk, end), bv = block_of(p, table, tv, end);
+        uint32_t kw[4][KW];
+        u32x4 vw[VT];
+        const uint8_t *kp = p.cache.d_k + (((uint64_t)max(bk, 0) * p.cache.kv_heads + h) * bs + tk % bs + (col & 3)) * D + u * (D / 4);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            if constexpr (KW % 4 == 0) {
+#pragma unroll
+                for (int w = 0; w < KW; w += 4) {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(kp + t * 4 * D + w * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) kw[t][w + e] = x[e];
+                }
+            } else {
+#pragma unroll
+                for (int w = 0; w < KW; w += 2) {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(kp + t * 4 * D + w * 4);
+                    kw[t][w] = x[0], kw[t][w + 1] = x[1];
+                }
+            }
+        }
+        const uint64_t bh = (uint64_t)max(bv, 0) * p.cache.kv_heads + h;
+        const uint8_t *vp = p.cache.d_v + (bh * D + col) * bs + tv % bs;
+#pragma unroll
+        for (int t = 0; t < VT; t++) vw[t] = *reinterpret_cast<const u32x4 *>(vp + (uint64_t)t * 16 * bs);
+        const float ks = p.cache.d_k_scale[bh] * zs, vs = bv >= 0 ? p.cache.d_v_scale[bh] : 0.0f;
+
+        float z[16];
+        const int32_t seen = bv >= 0 ? limit - tv : 0;  // of this lane's 16 tokens
+        float zm = -__builtin_inff();
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+            for (int f = 0; f < KS; f++)
+                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_to_f16(kw[t][2 * f], kw[t][2 * f + 1]), q[f], s, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                z[4 * t + i] = 4 * t + i < seen ? s[i] * ks : -__builtin_inff();
+                zm = fmaxf(zm, z[4 * t + i]);
+            }
+        }
+        zm = fmaxf(zm, __shfl_xor(zm, 16));
+        zm = fmaxf(zm, __shfl_xor(zm, 32));
+        float vt = fmaxf(vs, __shfl_xor(vs, 16));
+        vt = fmaxf(top, fmaxf(vt, __shfl_xor(vt, 32)));
+        const float mn = fmaxf(m, zm), ref = mn == -__builtin_inff() ? 0.0f : mn;
+        const float again = __builtin_amdgcn_exp2f(m - ref);
+        m = mn;
+        const float ov = vt > 0.0f ? top / vt : 1.0f, of = again * ov;
+        top = vt;
+        const float share = vt > 0.0f ? vs / vt : 0.0f;
+        l *= again;
+        f16x8 pv[2];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float e = i < seen ? __builtin_amdgcn_exp2f(z[i] - ref) : 0.0f;
+            l += e;
+            pv[i >> 3][i & 7] = (_Float16)(e * share);
+        }
+        if (__any(of != 1.0f)) {
+#pragma unroll
+            for (int t = 0; t < VT; t++) o[t] *= of;
+        }
+#pragma unroll
+        for (int t = 0; t < VT; t++) {
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_to_f16(vw[t][0], vw[t][1]), pv[0], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_to_f16(vw[t][2], vw[t][3]), pv[1], o[t], 0, 0, 0);
+        }
+    }
+
+    // join the 4 waves: the common maximum, then the sums in a fixed order
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (u == 0) lds_ml[wave][col][0] = m, lds_ml[wave][col][1] = l;
+    __syncthreads();
+    float mm = -__builtin_inff(), ll = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) mm = fmaxf(mm, lds_ml[w][col][0]);
+    const float ref = mm == -__builtin_inff() ? 0.0f : mm;
+#pragma unroll
+    for (int w = 0; w < 4; w++) ll += lds_ml[w][col][1] * __builtin_amdgcn_exp2f(lds_ml[w][col][0] - ref);
+    const float f = __builtin_amdgcn_exp2f(m - ref) * top;
+#pragma unroll
+    for (int t = 0; t < VT; t++) o[t] *= f;
+    if (wave >= 2) {
+#pragma unroll
+        for (int t = 0; t < VT; t++) *reinterpret_cast<f32x4 *>(&lds_o[wave - 2][col][16 * t + 4 * u]) = o[t];
+    }
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+        for (int t = 0; t < VT; t++) o[t] += *reinterpret_cast<const f32x4 *>(&lds_o[wave][col][16 * t + 4 * u]);
+    }
+    __syncthreads();
+    if (wave == 1) {
+#pragma unroll
+        for (int t = 0; t < VT; t++) *reinterpret_cast<f32x4 *>(&lds_o[0][col][16 * t + 4 * u]) = o[t];
+    }
+    __syncthreads();
+    if (wave != 0 || !live) return;
+#pragma unroll
+    for (int t = 0; t < VT; t++) o[t] += *reinterpret_cast<const f32x4 *>(&lds_o[0][col][16 * t + 4 * u]);
+    if (whole) {
+        uint16_t *out = reinterpret_cast<uint16_t *>(p.a.d_out) + ((uint64_t)rq.q0 + qi) * p.a.out_token_stride +
+                        qh * p.a.out_head_stride;
+        const bool wide = !((uintptr_t)p.a.d_out & 7u) && !((p.a.out_token_stride | p.a.out_head_stride) & 3u);
+        const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+#pragma unroll
+        for (int t = 0; t < VT; t++) {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = o[t][i] * inv;
+            store4<DT>(out + 16 * t + 4 * u, wide, v);
+        }
+        return;
+    }
+    const uint64_t at = (((uint64_t)r * p.cache.kv_heads + h) * p.splits + split) * p.cols + col;
+#pragma unroll
+    for (int t = 0; t < VT; t++) *reinterpret_cast<f32x4 *>(p.part_o + at * D + 16 * t + 4 * u) = o[t];
+    if (u == 0) p.part_ml[2 * at] = mm, p.part_ml[2 * at + 1] = ll;
+}
+
+// Joins the chunks of a request's column: one workgroup per request, head and
+// column, its threads over dimensions and every (256 / D)th chunk.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p) {
+    constexpr int W = 256 / D;
+    __shared__ float sum[W][D], lsum[W];
+    const uint32_t r = blockIdx.x, h = blockIdx.y / p.cols, col = blockIdx.y % p.cols;
+    const Request rq = request_of(p, r);
+    const uint32_t cols = columns_of(p, rq);
+    if (col >= cols || cols > p.small || rq.seen <= (int32_t)p.chunk) return;
+    const uint32_t n = ((uint32_t)rq.seen + p.chunk - 1) / p.chunk;
+    const uint64_t at = ((uint64_t)r * p.cache.kv_heads + h) * p.splits * p.cols + col;
+    float m = -__builtin_inff();
+    for (uint32_t s = threadIdx.x & 63u; s < n; s += 64) m = fmaxf(m, p.part_ml[2 * (at + (uint64_t)s * p.cols)]);
+    m = wave_max(m);
+    const float ref = m == -__builtin_inff() ? 0.0f : m;
+    const uint32_t part = threadIdx.x / D, d = threadIdx.x % D;
+    float o = 0.0f, l = 0.0f;
+    if (part < W) {
+#pragma unroll 4
+        for (uint32_t s = part; s < n; s += W) {
+            const uint64_t i = at + (uint64_t)s * p.cols;
+            const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * i] - ref);
+            l += f * p.part_ml[2 * i + 1];
+            o += f * p.part_o[i * D + d];
+        }
+        sum[part][d] = o;
+        if (d == 0) lsum[part] = l;
+    }
+    __syncthreads();
+    if (part != 0) return;
+    l = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; w++) l += lsum[w], o += sum[w][d];
+    uint16_t *out = reinterpret_cast<uint16_t *>(p.a.d_out) + ((uint64_t)rq.q0 + col / p.group) * p.a.out_token_stride +
+                    (h * p.group + col % p.group) * p.a.out_head_stride;
+    out[d] = (uint16_t)f32_to_half<DT>(l != 0.0f ? o / l : 0.0f);
+}
+
+// ---------------------------------------------------------------- many columns
+//
+// Rows of a prompt: NW waves of 32 columns (32 x 32 x 16 tiles) share tiles of
+// 64 tokens, which the workgroup turns into f16 once, in LDS.  Rows of LDS
+// are padded by 16 bytes (an odd number of 16-byte units: rows read together
+// lie in different banks).  A column's accumulators in S^T hold tokens
+// 8 (i / 4) + 4 (lane / 32) + i % 4; V's tokens are stored in the order that
+// makes a lane's 8 of them contiguous (4-7 and 8-11 of 16 change places).
+
+template <int DT, int D, int NW>
+__global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
+    constexpr int KS = D / 16, VT = D / 32, T = 64 * NW;
+    constexpr int KP = D + 8, VP = 64 + 8;  // pitches in f16
+    constexpr int CODES = 64 * D / 16, PER = (CODES + T - 1) / T;  // 16-byte pieces of a tile's codes
+    __shared__ __align__(16) _Float16 lk[64 * KP];
+    __shared__ __align__(16) _Float16 lv[D * VP];
+    __shared__ float lks[4], lvs[4];
+    const uint32_t r = blockIdx.x / p.tiles, tile = p.tiles - 1 - blockIdx.x % p.tiles, h = blockIdx.y;
+    const Request rq = request_of(p, r);
+    const uint32_t cols = columns_of(p, rq);
+    if (cols <= p.small || tile * (32 * NW) >= cols) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hl = lane >> 5;
+    const uint32_t c = tile * (32 * NW) + wave * 32 + (lane & 31);
+    const bool live = c < cols;
+    const uint32_t qi = c / p.group, qh = h * p.group + c % p.group;
+    const int32_t limit = live ? limit_of(rq, (int32_t)qi) : 0;
+    const uint32_t last = min(cols, (tile + 1) * (32 * NW)) - 1;
+    const int32_t end = limit_of(rq, (int32_t)(last / p.group));
+    const int32_t all = limit_of(rq, (int32_t)(tile * (32 * NW) / p.group));  // tokens that every column sees
+    const int32_t bs = (int32_t)p.cache.block_size;
+    const int32_t *table = p.a.d_table + (uint64_t)r * p.a.table_stride;
+
+    f16x8 q[KS];
+    float zs;
+    {
+        const uint16_t *row = live ? reinterpret_cast<const uint16_t *>(p.a.d_q) +
+                                         ((uint64_t)rq.q0 + qi) * p.a.q_token_stride + qh * p.a.q_head_stride
+                                   : nullptr;
+        const bool wide = !((uintptr_t)p.a.d_q & 15u) && !((p.a.q_token_stride | p.a.q_head_stride) & 7u);
+        zs = load_query<DT, KS>(
+            row, wide, q, [&](int f) { return f * 16 + hl * 8; }, [](float v) { return fmaxf(v, __shfl_xor(v, 32)); });
+        zs *= p.a.scale * kLog2e;
+    }
+    f32x16 o[VT];
+#pragma unroll
+    for (int t = 0; t < VT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[t][i] = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f, top = 0.0f;
+
+    // a tile's codes on the way: pieces of 16 dimensions of a token, of 16
+    // tokens of a dimension
+    u32x4 kc[PER], vc[PER];
+    float ksc = 0.0f, vsc = 0.0f;
+    auto fetch = [&](int32_t base) {
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int x = j * T + tid;
+            if (CODES % T && x >= CODES) break;
+            const int kt = x / (D / 16), kd = x % (D / 16), vd = x / 4, vu = x % 4;
+            const int32_t bk = max(block_of(p, table, base + kt, end), 0);
+            kc[j] = *reinterpret_cast<const u32x4 *>(
+                p.cache.d_k + (((uint64_t)bk * p.cache.kv_heads + h) * bs + (base + kt) % bs) * D + kd * 16);
+            const int32_t bv = max(block_of(p, table, base + 16 * vu, end), 0);
+            vc[j] = *reinterpret_cast<const u32x4 *>(
+                p.cache.d_v + (((uint64_t)bv * p.cache.kv_heads + h) * D + vd) * bs + (base + 16 * vu) % bs);
+        }
+        if (tid < 4) {
+            const int32_t b = block_of(p, table, base + 16 * tid, end);
+            const uint64_t bh = (uint64_t)max(b, 0) * p.cache.kv_heads + h;
+            // a run without a block: marked by a negative scale
+            ksc = b >= 0 ? p.cache.d_k_scale[bh] : -1.0f;
+            vsc = b >= 0 ? p.cache.d_v_scale[bh] : 0.0f;
+        }
+    };
+    auto stage = [&]() {
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int x = j * T + tid;
+            if (CODES % T && x >= CODES) break;
+            const int kt = x / (D / 16), kd = x % (D / 16), vd = x / 4, vu = x % 4;
+            *reinterpret_cast<f16x8 *>(&lk[kt * KP + kd * 16]) = codes8_to_f16(kc[j][0], kc[j][1]);
+            *reinterpret_cast<f16x8 *>(&lk[kt * KP + kd * 16 + 8]) = codes8_to_f16(kc[j][2], kc[j][3]);
+            *reinterpret_cast<f16x8 *>(&lv[vd * VP + vu * 16]) = codes8_to_f16(vc[j][0], vc[j][2]);
+            *reinterpret_cast<f16x8 *>(&lv[vd * VP + vu * 16 + 8]) = codes8_to_f16(vc[j][1], vc[j][3]);
+        }
+        if (tid < 4) lks[tid] = ksc, lvs[tid] = vsc;
+    };
+
+    if (end > 0) fetch(0);
+    for (int32_t base = 0; base < end; base += 64) {
+        __syncthreads();
+        stage();
+        __syncthreads();
+        if (base + 64 < end) fetch(base + 64);
+        float ks[4], vs[4], vt = top;
+#pragma unroll
+        for (int i = 0; i < 4; i++) ks[i] = lks[i], vs[i] = lvs[i], vt = fmaxf(vt, vs[i]);
+        const bool masked = base + 64 > all || ks[0] < 0.0f || ks[1] < 0.0f || ks[2] < 0.0f || ks[3] < 0.0f;
+        f32x16 s[2];
+        float zm = -__builtin_inff();
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
+#pragma unroll
+            for (int f = 0; f < KS; f++) {
+                const f16x8 a = *reinterpret_cast<const f16x8 *>(&lk[(t * 32 + (lane & 31)) * KP + f * 16 + hl * 8]);
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[f], s[t], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float z = s[t][i] * (ks[2 * t + (i >> 3)] * zs);
+                if (masked) {
+                    const int32_t tok = base + 32 * t + 8 * (i >> 2) + 4 * hl + (i & 3);
+                    z = tok < limit && ks[2 * t + (i >> 3)] >= 0.0f ? z : -__builtin_inff();
+                }
+                s[t][i] = z;
+                zm = fmaxf(zm, z);
+            }
+        zm = fmaxf(zm, __shfl_xor(zm, 32));
+        const float mn = fmaxf(m, zm), ref = mn == -__builtin_inff() ? 0.0f : mn;
+        const float again = __builtin_amdgcn_exp2f(m - ref), of = again * (vt > 0.0f ? top / vt : 1.0f);
+        m = mn, top = vt;
+        l *= again;
+        if (__any(of != 1.0f)) {
+#pragma unroll
+            for (int t = 0; t < VT; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[t][i] *= of;
+        }
+        f16x8 pv[4];
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float e = __builtin_amdgcn_exp2f(s[t][i] - ref);
+                l += e;
+                pv[2 * t + (i >> 3)][i & 7] = (_Float16)(e * (vt > 0.0f ? vs[2 * t + (i >> 3)] / vt : 0.0f));
+            }
+#pragma unroll
+        for (int t = 0; t < VT; t++)
+#pragma unroll
+            for (int f = 0; f < 4; f++) {
+                const f16x8 a = *reinterpret_cast<const f16x8 *>(&lv[(t * 32 + (lane & 31)) * VP + f * 16 + hl * 8]);
+                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pv[f], o[t], 0, 0, 0);
+            }
+    }
+    l += __shfl_xor(l, 32);
+    if (!live) return;
+    uint16_t *out = reinterpret_cast<uint16_t *>(p.a.d_out) + ((uint64_t)rq.q0 + qi) * p.a.out_token_stride +
+                    qh * p.a.out_head_stride;
+    const bool wide = !((uintptr_t)p.a.d_out & 7u) && !((p.a.out_token_stride | p.a.out_head_stride) & 3u);
+    const float inv = l != 0.0f ? top / l : 0.0f;
+#pragma unroll
+    for (int t = 0; t < VT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = o[t][i + e] * inv;
+            store4<DT>(out + 32 * t + 2 * i + 4 * hl, wide, v);
+        }
+}
+
+constexpr int kTileWaves = 4;
+
+template <int DT, int D>
+hipError_t launch_attention(const AttnArgs &p, hipStream_t s) {
+    hipLaunchKernelGGL((attn_step_kernel<DT, D>), dim3(p.a.requests * p.splits, p.cache.kv_heads), dim3(256), 0, s, p);
+    if (p.splits > 1)
+        hipLaunchKernelGGL((attn_join_kernel<DT, D>), dim3(p.a.requests, p.cache.kv_heads * p.cols), dim3(256), 0, s, p);
+    if (p.tiles)
+        hipLaunchKernelGGL((attn_tile_kernel<DT, D, kTileWaves>), dim3(p.a.requests * p.tiles, p.cache.kv_heads),
+                           dim3(64 * kTileWaves), 0, s, p);
+    return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_dim(const AttnArgs &p, hipStream_t s) {
+    switch (p.cache.head_dim) {
+        case 64: return launch_attention<DT, 64>(p, s);
+        case 96: return launch_attention<DT, 96>(p, s);
+        case 128: return launch_attention<DT, 128>(p, s);
+        case 192: return launch_attention<DT, 192>(p, s);
+        default: return launch_attention<DT, 256>(p, s);
+    }
+}
+
+}  // namespace
+}  // namespace hh
+
+extern "C" int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, const hh_kv_attention_args *a,
+                                   void *stream) {
+    if (!ctx || !a) return HH_ERR_INVALID_ARGUMENT;
+    const int32_t rc = hh::check_kv_cache(cache);
+    if (rc != HH_OK) return rc;
+    if (a->dtype != HH_F16 && a->dtype != HH_BF16) return HH_ERR_UNSUPPORTED;
+    if (a->q_heads == 0 || a->q_heads % cache->kv_heads) return HH_ERR_INVALID_ARGUMENT;
+    if (a->tokens == 0 || a->requests == 0) return HH_OK;
+    if (!a->d_q || !a->d_out || !a->d_start || !a->d_kv_len || (!a->d_table && a->table_width))
+        return HH_ERR_INVALID_ARGUMENT;
+    if ((((uintptr_t)a->d_q | (uintptr_t)a->d_out) & 1u) || a->table_stride < a->table_width) return HH_ERR_INVALID_ARGUMENT;
+    if (a->requests > 65536 || a->tokens >= 1u << 24) return HH_ERR_INVALID_ARGUMENT;
+    const uint32_t group = a->q_heads / cache->kv_heads;
+    const uint64_t most = (uint64_t)(a->max_q < a->tokens ? a->max_q : a->tokens) * group;
+    if (most >= 1ull << 31) return HH_ERR_INVALID_ARGUMENT;
+    hh::DeviceGuard guard(ctx->device);
+    if (guard.status() != hipSuccess) return hh::from_hip(guard.status());
+    hh::AttnArgs p = {};
+    p.cache = *cache;
+    p.a = *a;
+    p.group = group;
+    p.small = 16;
+    p.cols = (uint32_t)(most < 1 ? 1 : most < 16 ? most : 16);
+    const uint64_t room = (uint64_t)a->table_width * cache->block_size;
+    const uint64_t kv = a->max_kv < room ? a->max_kv : room;
+    if (kv > 1ull << 30) return HH_ERR_UNSUPPORTED;  // tokens are counted in 31 bits
+    // chunks: enough workgroups for 4 per CU, none below 256 tokens
+    const uint64_t lanes = (uint64_t)a->requests * cache->kv_heads;
+    const uint64_t want = (4ull * (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256) + lanes - 1) / lanes;
+    uint64_t chunk = (kv + want - 1) / want;
+    chunk = (chunk + 255) / 256 * 256;
+    if (chunk < 256) chunk = 256;
+    p.chunk = (uint32_t)chunk;
+    p.splits = (uint32_t)((kv + chunk - 1) / chunk);
+    if (p.splits < 1) p.splits = 1;
+    p.tiles = most > p.small ? (uint32_t)((most + 32 * hh::kTileWaves - 1) / (32 * hh::kTileWaves)) : 0;
+    if ((uint64_t)a->requests * p.splits >= 1ull << 24 || (uint64_t)a->requests * p.tiles >= 1ull << 24)
+        return HH_ERR_UNSUPPORTED;
+    if (cache->kv_heads * 16ull > 65535) return HH_ERR_UNSUPPORTED;
+    if (p.splits > 1) {
+        const uint64_t n = lanes * p.splits * p.cols;
+        const int32_t e = hh::ensure_scratch(ctx, n * (cache->head_dim + 2) * sizeof(float));
+        if (e != HH_OK) return e;
+        p.part_o = reinterpret_cast<float *>(ctx->d_scratch);
+        p.part_ml = p.part_o + n * cache->head_dim;
+    }
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    return hh::from_hip(a->dtype == HH_BF16 ? hh::launch_dim<HH_BF16>(p, s) : hh::launch_dim<HH_F16>(p, s));
+}

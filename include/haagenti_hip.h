@@ -676,6 +676,139 @@ int32_t hh_spectral_encode_from_dct(const float *coeffs, uint32_t width, uint32_
                                     float retention, float essential_ratio, uint8_t *out, size_t out_cap,
                                     uint64_t *frag_offsets, size_t *written);
 
+/* ---------------------------------------------------------------- decoder layer operators
+ *
+ * What runs on a layer's decoded weights: matrix products with an epilogue
+ * (16-bit weights as the tile decode writes them, or INT4 buffers as they
+ * are), and a paged key / value cache in 8 bits with attention over it.  No
+ * counterpart in the reference, which stops at the decoded tensor.  All are
+ * asynchronous on the stream and read lengths, tables and slots from device
+ * memory, so a step needs no host synchronisation.  Strides are in elements.
+ * The context's scratch grows with the largest call so far; after a first
+ * call of the same sizes a call allocates nothing and may be captured. */
+
+typedef enum hh_activation {
+    HH_ACT_NONE = 0,
+    HH_ACT_RELU = 1,
+    HH_ACT_GELU = 2,      /* 0.5 z (1 + erf(z / sqrt 2)) */
+    HH_ACT_GELU_TANH = 3, /* 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+    HH_ACT_SILU = 4       /* z / (1 + exp(-z)) */
+} hh_activation;
+
+/* w_dtype of a weight in the INT4 layout of hh_quantize_int4 over its n * k
+ * values in row order. */
+#define HH_INT4 16
+
+/* y = act(x W^T + bias) * mul + residual: x is m x k, W n x k (a weight as it
+ * is stored: a row per output), y, mul and residual m x n, bias n values.
+ * bias, mul and residual may be NULL and have x's type; a 16-bit W has it too.
+ * Sums are f32; y is rounded once at the end.  y may be residual or mul
+ * itself (same stride), and overlaps nothing else that is read. */
+typedef struct hh_linear_args {
+    const void *d_x, *d_w, *d_bias, *d_mul, *d_residual;
+    void *d_y;
+    uint64_t x_stride, w_stride, mul_stride, residual_stride, y_stride; /* w_stride: 16-bit W only */
+    uint64_t w_bytes; /* INT4 W: size of its buffer, at least hh_int4_compressed_size(n k) */
+    uint32_t m, n, k;
+    int32_t dtype;    /* HH_F16 or HH_BF16 */
+    int32_t w_dtype;  /* dtype, or HH_INT4 */
+    int32_t y_dtype;  /* dtype, or HH_F32 */
+    int32_t activation;
+} hh_linear_args;
+/* m, n or k of 0 are allowed (k = 0: sums of 0).  Pointers are aligned to
+ * their elements; rows of 16 bytes' alignment (pointers and strides) take the
+ * wide loads.  HH_ERR_UNSUPPORTED for other types, HH_ERR_INVALID_ARGUMENT
+ * for a missing pointer, a stride below the row, a size of 2^31 or more. */
+int32_t hh_linear(hh_context *ctx, const hh_linear_args *args, void *stream);
+
+/* A paged cache: num_blocks blocks of block_size tokens (16, 32, 64 or 128)
+ * for kv_heads heads of head_dim (64, 96, 128, 192 or 256) dimensions.
+ * Byte c stands for (c - 128) * scale, c in 1..255, one f32 scale per block
+ * and head.  Keys lie [block][head][token][dim], values [block][head][dim]
+ * [token] (16 tokens of a dimension are the 16 bytes one lane of the
+ * attention's second product reads).  A slot is block * block_size + token.
+ * num_blocks * block_size is below 2^31; a call takes fewer than 2^24 rows
+ * or blocks. */
+typedef struct hh_kv_cache {
+    uint8_t *d_k, *d_v;           /* 16-byte aligned */
+    float *d_k_scale, *d_v_scale; /* num_blocks x kv_heads */
+    uint32_t num_blocks, block_size, kv_heads, head_dim;
+} hh_kv_cache;
+
+/* One step's plan.  Request r has d_len[r] tokens in the cache, in the blocks
+ * of its row of d_table, and adds d_new[r]; d_new[r] < 0 ends it and frees
+ * its blocks.  d_ring (capacity entries) with d_state = {head, count} is the
+ * queue of free blocks: count ids from entry head on, wrapping around.
+ * Requests are served in order: each takes the blocks that its new length
+ * needs from the head into its row of d_table.  Ended requests' blocks join
+ * the tail, in order, for later steps.
+ * Writes d_start[requests + 1] (first row of each request's new tokens: the
+ * running sum of max(d_new, 0)), d_kv_len (tokens held after the step),
+ * d_slots[tokens] (the slot of each new row, -1 past the last row), d_status
+ * and d_state_out (which is not d_state: give it to the next step).
+ * A request that can't be served takes no block, its slots are -1, its
+ * d_kv_len is 0 and d_status names why: HH_ERR_OUT_OF_MEMORY where the free
+ * blocks are used up (requests after it that need none are served),
+ * HH_ERR_BUFFER_TOO_SMALL where its row of d_table or d_slots is too short,
+ * HH_ERR_INVALID_ARGUMENT for a negative length. */
+typedef struct hh_kv_plan_args {
+    const int32_t *d_len, *d_new;
+    int32_t *d_table;
+    int32_t *d_ring;
+    const int32_t *d_state;
+    int32_t *d_start, *d_kv_len, *d_slots, *d_status, *d_state_out;
+    uint64_t table_stride;
+    uint32_t requests; /* at most 65536 */
+    uint32_t table_width, ring_capacity, block_size, tokens;
+} hh_kv_plan_args;
+int32_t hh_kv_plan(hh_context *ctx, const hh_kv_plan_args *args, void *stream);
+
+/* Rows k and v (tokens x kv_heads x head_dim, f16 or bf16) into the cache at
+ * d_slots; rows whose slot is no slot of the cache are left out.  A block's
+ * new rows are neighbours in the call, at consecutive slots, and the last of
+ * its tokens (as hh_kv_plan gives them; two runs of rows in one block race).
+ * Per block and head: with amax the largest finite magnitude among the new
+ * rows, the scale becomes max(old, amax / 127 rounded up to 8 significant
+ * bits), old being 0 for a block begun at its first token; where it grows,
+ * the tokens before get the code nearest to their value at the new scale.  A
+ * new value gets the code nearest to value / scale (ties to even, infinities
+ * the last code, NaN the code of 0).  With scales of 8 bits no such quotient
+ * lies nearer to a tie than f32 resolves, so codes don't depend on how it is
+ * computed. */
+int32_t hh_kv_append(hh_context *ctx, const hh_kv_cache *cache, const void *d_rows_k, const void *d_rows_v,
+                     int32_t dtype, uint64_t token_stride_k, uint64_t head_stride_k, uint64_t token_stride_v,
+                     uint64_t head_stride_v, const int32_t *d_slots, uint32_t tokens, void *stream);
+
+/* The values of n blocks (d_blocks), as nblocks x block_size x kv_heads x
+ * head_dim of out_dtype: a prefix to keep elsewhere, to check or to use in
+ * another type.  Whole blocks: tokens not yet appended hold what the cache
+ * holds.  A block that the cache doesn't have gives zeros. */
+int32_t hh_kv_read(hh_context *ctx, const hh_kv_cache *cache, const int32_t *d_blocks, uint32_t nblocks,
+                   int32_t out_dtype, void *d_out_k, void *d_out_v, void *stream);
+
+/* o = softmax(scale q K^T) V of each request's new rows over its cached
+ * tokens.  Rows d_start[r] .. d_start[r + 1] of q and out (tokens x q_heads x
+ * head_dim) belong to request r and are its last tokens: row i of c sees the
+ * first d_kv_len[r] - c + 1 + i tokens.  Head h reads head
+ * h / (q_heads / kv_heads) of the cache.  Rows that see no token (a request
+ * that hh_kv_plan left out) and rows past the last request's give zeros;
+ * tokens of a block id that the cache doesn't have are not seen.  max_q and
+ * max_kv bound a request's rows and tokens (what lies beyond is not
+ * computed / not seen): they choose how the work is split, so bounds near
+ * the real sizes are faster.  Sums, maxima and accumulators are f32, codes
+ * are exact, the probabilities times their block's scale are rounded to f16
+ * (11 bits) for the second product, the output once at the end. */
+typedef struct hh_kv_attention_args {
+    const void *d_q;
+    void *d_out;
+    const int32_t *d_table, *d_start, *d_kv_len;
+    uint64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride, table_stride;
+    uint32_t requests, tokens, q_heads, table_width, max_q, max_kv;
+    float scale;
+    int32_t dtype; /* of q and out: HH_F16 or HH_BF16 */
+} hh_kv_attention_args;
+int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, const hh_kv_attention_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
