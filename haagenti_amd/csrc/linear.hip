@@ -122,43 +122,149 @@ __device__ __forceinline__ void finish4(const LinearArgs &p, uint32_t m, uint32_
 
 // ---------------------------------------------------------------- few rows
 //
-// Bound by reading W once.  A workgroup takes 16 rows of W; its 8 waves take
-// every eighth 128 columns of them, straight to registers, and join their
-// sums in LDS.  x (at most 16 MT rows) comes from L1 / L2.
+// Bound by reading W once.  A workgroup takes 16 NT rows of W; its 8 waves
+// take every eighth 128 columns of them, straight to registers (the next 128
+// on their way while these are used), and join their sums in LDS.  x (at most
+// 16 MT rows) comes from L1 / L2; its row is the products' first operand, so
+// a lane's sums belong to one row of W and have one scale.
+//
+// A lane loads 16 bytes of nibbles, one group of its row; four lanes hold the
+// row's 4 groups.  Two swaps between lanes (32 and 16 apart) turn these into
+// a quarter of each group per lane, what the products take.  The nibbles of a
+// word leave it in the order 0 4 1 5 2 6 3 7 (one shift and one and-or per
+// pair); x's values are put in that order too.
 
-template <int DT, int YT, int MT>
+// The 8 nibbles of w as 16 + nibble, in the order 0 4 1 5 2 6 3 7.
+template <int DT>
+__device__ __forceinline__ u32x4 nibbles_0415(uint32_t w) {
+    constexpr uint32_t magic = DT == HH_BF16 ? 0x41804180u : 0x4c004c00u;
+    constexpr int up = DT == HH_BF16 ? 3 : 6;
+    constexpr uint32_t mask = 0x000f000fu << up;
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = ((4 * i > up ? w >> (4 * i - up) : w << (up - 4 * i)) & mask) | magic;
+    return v;
+}
+__device__ __forceinline__ u32x4 order_0415(const u32x4 &x) {
+    return u32x4{__builtin_amdgcn_perm(x[2], x[0], 0x05040100u), __builtin_amdgcn_perm(x[2], x[0], 0x07060302u),
+                 __builtin_amdgcn_perm(x[3], x[1], 0x05040100u), __builtin_amdgcn_perm(x[3], x[1], 0x07060302u)};
+}
+// Lane (r, g) holds words 0..3 of group g; afterwards word g of groups 0..3.
+__device__ __forceinline__ u32x4 groups_across(u32x4 w) {
+    auto s = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+    auto t = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    auto u = __builtin_amdgcn_permlane16_swap(s[0], t[0], false, false);
+    auto v = __builtin_amdgcn_permlane16_swap(s[1], t[1], false, false);
+    return u32x4{u[0], u[1], v[0], v[1]};
+}
+template <int DT>
+__device__ __forceinline__ u32x4 minus24() {
+    constexpr uint32_t v = DT == HH_BF16 ? 0xc1c0c1c0u : 0xce00ce00u;
+    return u32x4{v, v, v, v};
+}
+
+template <int DT, int YT, int MT, int NT, bool INT4>
 __global__ __launch_bounds__(512) void linear_rows_kernel(const LinearArgs p) {
+    constexpr int W = INT4 ? 1 : 4;  // loads of 16 bytes per lane and 128 columns
     __shared__ __align__(16) float part[8][16 * MT][20];
     const hh_linear_args &a = p.a;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = lane & 15u, g = lane >> 4;
-    const uint32_t n0 = blockIdx.x * 16;
-    const uint16_t *w = reinterpret_cast<const uint16_t *>(a.d_w) + (uint64_t)min(n0 + r, a.n - 1) * a.w_stride;
+    const uint32_t n0 = blockIdx.x * (16 * NT);
+    uint64_t row[NT];
+#pragma unroll
+    for (int j = 0; j < NT; j++) row[j] = min(n0 + 16 * j + r, a.n - 1);
     const uint16_t *x[MT];
 #pragma unroll
     for (int t = 0; t < MT; t++)
         x[t] = reinterpret_cast<const uint16_t *>(a.d_x) + (uint64_t)min(16 * t + r, a.m - 1) * a.x_stride;
-    f32x4 acc[MT];
+    f32x4 acc[MT][NT];
 #pragma unroll
-    for (int t = 0; t < MT; t++) acc[t] = f32x4{0, 0, 0, 0};
-    for (uint32_t k = wave * 128 + g * 8; k < (a.k + 127) / 128 * 128; k += 8 * 128) {
-        u32x4 wf[4];
+    for (int t = 0; t < MT; t++)
 #pragma unroll
-        for (uint32_t f = 0; f < 4; f++) wf[f] = row8(w, k + 32 * f, a.k);
+        for (int j = 0; j < NT; j++) acc[t][j] = f32x4{0, 0, 0, 0};
+
+    struct Cols {
+        u32x4 w[NT][W];
+        u32x2 s[NT];
+    };
+    auto fetch = [&](uint32_t k, Cols &c) {
 #pragma unroll
-        for (uint32_t f = 0; f < 4; f++)
+        for (int j = 0; j < NT; j++) {
+            if constexpr (INT4) {
+                const uint64_t at = (row[j] * a.k + k) / 32;  // in groups
+                c.w[j][0] = u32x4{0, 0, 0, 0}, c.s[j] = u32x2{0, 0};
+                if (k + 32 * g < a.k) c.w[j][0] = *reinterpret_cast<const u32x4_any *>(p.nibbles + (at + g) * 16);
+                if (k + 128 <= a.k) {
+                    typedef u32x2 u32x2_any __attribute__((aligned(2)));
+                    c.s[j] = *reinterpret_cast<const u32x2_any *>(p.scales + at);
+                } else {
 #pragma unroll
-            for (int t = 0; t < MT; t++) acc[t] = mma16<DT>(wf[f], row8(x[t], k + 32 * f, a.k), acc[t]);
+                    for (uint32_t e = 0; e < 4; e++)
+                        if (k + 32 * e < a.k) c.s[j][e >> 1] |= (uint32_t)p.scales[at + e] << (16 * (e & 1));
+                }
+            } else {
+                const uint16_t *w = reinterpret_cast<const uint16_t *>(a.d_w) + row[j] * a.w_stride;
+#pragma unroll
+                for (uint32_t f = 0; f < 4; f++) c.w[j][f % W] = row8(w, k + 32 * f + 8 * g, a.k);
+            }
+        }
+    };
+    Cols cur, next;
+    if (wave * 128 < a.k) fetch(wave * 128, cur);
+    for (uint32_t k = wave * 128; k < a.k; k += 1024) {
+        if (k + 1024 < a.k) fetch(k + 1024, next);
+        if constexpr (INT4) {
+#pragma unroll
+            for (int j = 0; j < NT; j++) cur.w[j][0] = groups_across(cur.w[j][0]);
+        }
+#pragma unroll
+        for (uint32_t f = 0; f < 4; f++) {
+            u32x4 xf[MT];
+#pragma unroll
+            for (int t = 0; t < MT; t++) xf[t] = row8(x[t], k + 32 * f + 8 * g, a.k);
+            if constexpr (INT4) {
+                f32x4 corr[MT];
+#pragma unroll
+                for (int t = 0; t < MT; t++) {
+                    xf[t] = order_0415(xf[t]);
+                    corr[t] = mma16<DT>(xf[t], minus24<DT>(), f32x4{0, 0, 0, 0});
+                }
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const u32x4 w = nibbles_0415<DT>(cur.w[j][0][f]);
+                    const float s = half_to_f32<HH_F16>((cur.s[j][f >> 1] >> (16 * (f & 1))) & 0xffffu);
+#pragma unroll
+                    for (int t = 0; t < MT; t++) {
+                        const f32x4 q = mma16<DT>(xf[t], w, corr[t]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[t][j][e] = fmaf(s, q[e], acc[t][j][e]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int t = 0; t < MT; t++) acc[t][j] = mma16<DT>(xf[t], cur.w[j][f % W], acc[t][j]);
+            }
+        }
+        cur = next;
     }
 #pragma unroll
-    for (int t = 0; t < MT; t++) *reinterpret_cast<f32x4 *>(&part[wave][16 * t + r][4 * g]) = acc[t];
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 64 * MT; i += 512) {
-        const uint32_t m = i >> 2, n = (i & 3u) * 4;
-        if (m >= a.m || n0 + n >= a.n) continue;
-        f32x4 s = *reinterpret_cast<const f32x4 *>(&part[0][m][n]);
+    for (int j = 0; j < NT; j++) {
+        if (j) __syncthreads();
 #pragma unroll
-        for (int v = 1; v < 8; v++) s += *reinterpret_cast<const f32x4 *>(&part[v][m][n]);
-        finish4<DT, YT>(p, m, n0 + n, s);
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) part[wave][16 * t + 4 * g + e][r] = acc[t][j][e];
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < 64 * MT; i += 512) {
+            const uint32_t m = i >> 2, n = (i & 3u) * 4, at = n0 + 16 * j + n;
+            if (m >= a.m || at >= a.n) continue;
+            f32x4 s = *reinterpret_cast<const f32x4 *>(&part[0][m][n]);
+#pragma unroll
+            for (int v = 1; v < 8; v++) s += *reinterpret_cast<const f32x4 *>(&part[v][m][n]);
+            finish4<DT, YT>(p, m, at, s);
+        }
     }
 }
 
@@ -302,16 +408,27 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p) {
     }
 }
 
+template <int DT, int YT, int MT, bool INT4>
+hipError_t launch_rows(const LinearArgs &p, hipStream_t s) {
+    const uint32_t tiles = (p.a.n + 15) / 16;
+    if (tiles >= 512)
+        hipLaunchKernelGGL((linear_rows_kernel<DT, YT, MT, 2, INT4>), dim3((tiles + 1) / 2), dim3(512), 0, s, p);
+    else
+        hipLaunchKernelGGL((linear_rows_kernel<DT, YT, MT, 1, INT4>), dim3(tiles), dim3(512), 0, s, p);
+    return hipGetLastError();
+}
+
 template <int DT, int YT>
 hipError_t launch_linear(const LinearArgs &p, hipStream_t s) {
     const hh_linear_args &a = p.a;
-    if (a.w_dtype != HH_INT4 && a.m <= 64) {
-        const dim3 grid((a.n + 15) / 16);
-        auto kernel = a.m <= 16 ? linear_rows_kernel<DT, YT, 1>
-                      : a.m <= 32 ? linear_rows_kernel<DT, YT, 2>
-                                  : linear_rows_kernel<DT, YT, 4>;
-        hipLaunchKernelGGL(kernel, grid, dim3(512), 0, s, p);
-        return hipGetLastError();
+    if (a.m <= 64 && (a.w_dtype != HH_INT4 || a.k % 32 == 0)) {
+        const int rows = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4;
+        return a.w_dtype == HH_INT4 ? (rows == 1   ? launch_rows<DT, YT, 1, true>(p, s)
+                                       : rows == 2 ? launch_rows<DT, YT, 2, true>(p, s)
+                                                   : launch_rows<DT, YT, 4, true>(p, s))
+                                    : (rows == 1   ? launch_rows<DT, YT, 1, false>(p, s)
+                                       : rows == 2 ? launch_rows<DT, YT, 2, false>(p, s)
+                                                   : launch_rows<DT, YT, 4, false>(p, s));
     }
     auto kernel = a.w_dtype != HH_INT4 ? linear_tile_kernel<DT, YT, kHalf>
                   : a.k % 32 == 0      ? linear_tile_kernel<DT, YT, kInt4>
