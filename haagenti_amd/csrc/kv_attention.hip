@@ -6,8 +6,12 @@
 //   z   = S^T (scale of K's block) (softmax scale) log2(e)
 //   m, l, O: running maximum of z, sum of 2^(z - m), and
 //   O^T += V^T P^T  codes times f16 P = 2^(z - m) (scale of V's block) / top,
-//                   top the largest V scale so far (so P <= 1 whatever the
-//                   scales are), O in units of top, f32.
+//                   top the largest V scale so far (so no P is large
+//                   whatever the scales are), O in units of top, f32.
+// The scale's share goes into the exponent; the sum l takes it out again per
+// 16 tokens (a share below 2^-60 counts as 2^-60: such a P is 0 in f16 anyway,
+// and l keeps its tokens).  m follows the maximum only when it is passed by 8,
+// so P < 256 and the accumulators are seldom rescaled.
 // Tokens lie on the first product's rows, so its accumulators hold, for one
 // column per lane, just the tokens that the lane supplies to the second
 // product's P^T operand: P never moves between lanes.  Which token a row
@@ -26,6 +30,8 @@ struct AttnArgs {
     hh_kv_cache cache;
     hh_kv_attention_args a;
     uint32_t group;      // q heads per cache head
+    uint32_t bs_log;     // block_size = 1 << bs_log
+    uint32_t block_step; // bytes of a block: kv_heads * block_size * head_dim
     uint32_t splits;     // of a request's tokens, in chunks of:
     uint32_t chunk;      // a multiple of 256
     uint32_t tiles;      // column tiles per request (tile kernel)
@@ -75,18 +81,25 @@ __device__ __forceinline__ int32_t limit_of(const Request &q, int32_t i) {
     return max(0, min(q.seen, q.kv_len - q.rows + i + 1));
 }
 
-// The cache block of a token below `seen`, or -1.
+// The table's entry for a token, or -1 past the end.
 __device__ __forceinline__ int32_t block_of(const AttnArgs &p, const int32_t *table, int32_t tok, int32_t end) {
     if (tok >= end) return -1;
-    const int32_t id = table[(uint32_t)tok / p.cache.block_size];
-    return (uint32_t)id < p.cache.num_blocks ? id : -1;
+    return table[(uint32_t)tok >> p.bs_log];
 }
+__device__ __forceinline__ bool held(const AttnArgs &p, int32_t id) { return (uint32_t)id < p.cache.num_blocks; }
+// What a V scale's share of the largest does to the exponent.
+__device__ __forceinline__ float share_of(float vs, float log_top) {
+    const float s = __builtin_amdgcn_logf(vs) - log_top;
+    return s > -60.0f ? s : -60.0f;  // also where both are 0
+}
+constexpr float kSlack = 8.0f;
 
 // N f16 fragments of 8 dimensions of a query row, fragment f at dimension
 // dim(f), as f16 scaled by a power of two of the row; returns what undoes the
-// scaling.  `join` makes a lane's largest magnitude the row's.
+// scaling.  `join` makes a lane's largest magnitude the row's; `sign` (of the
+// softmax scale) goes into the row, so that scores are scaled by positives.
 template <int DT, int N, typename Dim, typename Join>
-__device__ __forceinline__ float load_query(const uint16_t *row, bool wide, f16x8 (&q)[N], Dim dim, Join join) {
+__device__ __forceinline__ float load_query(const uint16_t *row, bool wide, float sign, f16x8 (&q)[N], Dim dim, Join join) {
     u32x4 raw[N];
     float top = 0.0f;
 #pragma unroll
@@ -101,7 +114,7 @@ __device__ __forceinline__ float load_query(const uint16_t *row, bool wide, f16x
                 for (int e = 0; e < 4; e++) raw[f][e] = (uint32_t)at[2 * e] | (uint32_t)at[2 * e + 1] << 16;
             }
         }
-        if constexpr (DT == HH_F16) q[f] = __builtin_bit_cast(f16x8, raw[f]);
+        if constexpr (DT == HH_F16) q[f] = __builtin_bit_cast(f16x8, raw[f]) * (_Float16)sign;
     }
     if constexpr (DT == HH_F16) return 1.0f;
 #pragma unroll
@@ -110,7 +123,7 @@ __device__ __forceinline__ float load_query(const uint16_t *row, bool wide, f16x
         for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(half_to_f32<DT>((raw[f][e >> 1] >> (16 * (e & 1))) & 0xffffu)));
     const uint32_t ex = __float_as_uint(join(top)) >> 23;
     const bool plain = ex == 0 || ex == 255;  // zeros and subnormals, infinities
-    const float down = plain ? 1.0f : ldexpf(1.0f, 127 - (int)ex), up = plain ? 1.0f : ldexpf(1.0f, (int)ex - 127);
+    const float down = plain ? sign : ldexpf(sign, 127 - (int)ex), up = plain ? 1.0f : ldexpf(1.0f, (int)ex - 127);
 #pragma unroll
     for (int f = 0; f < N; f++)
 #pragma unroll
@@ -158,7 +171,7 @@ __device__ __forceinline__ void store4(uint16_t *to, bool wide, const float *v) 
 // column, and V's operand is 16 contiguous codes of a dimension.
 
 template <int DT, int D>
-__global__ __launch_bounds__(256) void attn_step_kernel(const AttnArgs p) {
+__global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attn_step_kernel(const AttnArgs p) {
     constexpr int KS = D / 32, VT = D / 16, KW = D / 16;  // k steps, V tiles, 4-byte words of K per lane and row
     __shared__ __align__(16) float lds_o[2][16][D + 4];
     __shared__ float lds_ml[4][16][2];
@@ -176,7 +189,7 @@ __global__ __launch_bounds__(256) void attn_step_kernel(const AttnArgs p) {
     const int32_t *table = p.a.d_table + (uint64_t)r * p.a.table_stride;
     const bool live = (uint32_t)col < cols;
     const uint32_t qi = (uint32_t)col / p.group, qh = h * p.group + (uint32_t)col % p.group;
-    const int32_t limit = live ? min(end, limit_of(rq, (int32_t)qi)) : 0;
+    const int32_t limit = live ? min(end, limit_of(rq, (int32_t)qi)) : end;  // unused columns mask nothing
 
     f16x8 q[KS];
     float zs;
@@ -186,23 +199,27 @@ __global__ __launch_bounds__(256) void attn_step_kernel(const AttnArgs p) {
                                    : nullptr;
         const bool wide = !((uintptr_t)p.a.d_q & 15u) && !((p.a.q_token_stride | p.a.q_head_stride) & 7u);
         zs = load_query<DT, KS>(
-            row, wide, q, [&](int f) { return u * (D / 4) + f * 8; },
+            row, wide, p.a.scale < 0.0f ? -1.0f : 1.0f, q, [&](int f) { return u * (D / 4) + f * 8; },
             [](float v) { v = fmaxf(v, __shfl_xor(v, 16)); return fmaxf(v, __shfl_xor(v, 32)); });
-        zs *= p.a.scale * kLog2e;
+        zs *= fabsf(p.a.scale) * kLog2e;
     }
 
     f32x4 o[VT];
 #pragma unroll
     for (int t = 0; t < VT; t++) o[t] = f32x4{0, 0, 0, 0};
-    float m = -__builtin_inff(), l = 0.0f, top = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f, top = 0.0f, log_top = -__builtin_inff();
 
+    // K rows: this lane's rows are in run col >> 2; V and the scales: run u
+    const int32_t kr = 16 * (col >> 2), vr = 16 * u, mask = bs - 1;
+    const uint8_t *kh = p.cache.d_k + (uint64_t)h * bs * D + (col & 3) * D + u * (D / 4);
+    const uint8_t *vh = p.cache.d_v + (uint64_t)h * bs * D + col * bs;
+    int32_t bk = block_of(p, table, begin + 64 * wave + kr, end), bv = block_of(p, table, begin + 64 * wave + vr, end);
     for (int32_t base = begin + 64 * wave; base < end; base += 256) {
-        // K rows: this lane's rows are in run col >> 2; V and the scales: run u
-        const int32_t tk = base + 16 * (col >> 2), tv = base + 16 * u;
-        const int32_t bk = block_of(p, table, tk, end), bv = block_of(p, table, tv, end);
+        const uint32_t ik = held(p, bk) ? bk : 0, iv = held(p, bv) ? bv : 0;
+        const bool hv = held(p, bv);
         uint32_t kw[4][KW];
         u32x4 vw[VT];
-        const uint8_t *kp = p.cache.d_k + (((uint64_t)max(bk, 0) * p.cache.kv_heads + h) * bs + tk % bs + (col & 3)) * D + u * (D / 4);
+        const uint8_t *kp = kh + (uint64_t)ik * p.block_step + (uint32_t)(((base + kr) & mask) * D);
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             if constexpr (KW % 4 == 0) {
@@ -220,49 +237,53 @@ __global__ __launch_bounds__(256) void attn_step_kernel(const AttnArgs p) {
                 }
             }
         }
-        const uint64_t bh = (uint64_t)max(bv, 0) * p.cache.kv_heads + h;
-        const uint8_t *vp = p.cache.d_v + (bh * D + col) * bs + tv % bs;
+        const uint32_t bh = iv * p.cache.kv_heads + h;
+        const float ks = p.cache.d_k_scale[bh], vs = hv ? p.cache.d_v_scale[bh] : 0.0f;
+        const uint8_t *vp = vh + (uint64_t)iv * p.block_step + (uint32_t)((base + vr) & mask);
 #pragma unroll
-        for (int t = 0; t < VT; t++) vw[t] = *reinterpret_cast<const u32x4 *>(vp + (uint64_t)t * 16 * bs);
-        const float ks = p.cache.d_k_scale[bh] * zs, vs = bv >= 0 ? p.cache.d_v_scale[bh] : 0.0f;
+        for (int t = 0; t < VT; t++) vw[t] = *reinterpret_cast<const u32x4 *>(vp + t * 16 * bs);
+        // the next tokens' blocks, before anything waits for these
+        bk = block_of(p, table, base + 256 + kr, end), bv = block_of(p, table, base + 256 + vr, end);
 
-        float z[16];
-        const int32_t seen = bv >= 0 ? limit - tv : 0;  // of this lane's 16 tokens
-        float zm = -__builtin_inff();
+        f32x4 s[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            f32x4 s = {0, 0, 0, 0};
+            s[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int f = 0; f < KS; f++)
-                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_to_f16(kw[t][2 * f], kw[t][2 * f + 1]), q[f], s, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                z[4 * t + i] = 4 * t + i < seen ? s[i] * ks : -__builtin_inff();
-                zm = fmaxf(zm, z[4 * t + i]);
-            }
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_to_f16(kw[t][2 * f], kw[t][2 * f + 1]), q[f], s[t], 0, 0, 0);
         }
-        zm = fmaxf(zm, __shfl_xor(zm, 16));
-        zm = fmaxf(zm, __shfl_xor(zm, 32));
-        float vt = fmaxf(vs, __shfl_xor(vs, 16));
-        vt = fmaxf(top, fmaxf(vt, __shfl_xor(vt, 32)));
-        const float mn = fmaxf(m, zm), ref = mn == -__builtin_inff() ? 0.0f : mn;
-        const float again = __builtin_amdgcn_exp2f(m - ref);
-        m = mn;
-        const float ov = vt > 0.0f ? top / vt : 1.0f, of = again * ov;
-        top = vt;
-        const float share = vt > 0.0f ? vs / vt : 0.0f;
-        l *= again;
-        f16x8 pv[2];
+        float c = ks * zs;
+        const int32_t seen = hv ? limit - (base + vr) : 0;  // of this lane's 16 tokens
+        if (!__all(seen >= 16)) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float e = i < seen ? __builtin_amdgcn_exp2f(z[i] - ref) : 0.0f;
-            l += e;
-            pv[i >> 3][i & 7] = (_Float16)(e * share);
+            for (int i = 0; i < 16; i++) s[i >> 2][i & 3] = i < seen ? s[i >> 2][i & 3] * c : -__builtin_inff();
+            c = 1.0f;
         }
-        if (__any(of != 1.0f)) {
+        float zm = s[0][0], vt = vs;
+#pragma unroll
+        for (int i = 1; i < 16; i++) zm = fmaxf(zm, s[i >> 2][i & 3]);
+        zm *= c;
+        zm = fmaxf(zm, __shfl_xor(zm, 16)), vt = fmaxf(vt, __shfl_xor(vt, 16));
+        zm = fmaxf(zm, __shfl_xor(zm, 32)), vt = fmaxf(vt, __shfl_xor(vt, 32));
+        if (__any(zm > m + kSlack || vt > top)) {
+            const float mn = zm > m + kSlack ? zm : m, tn = fmaxf(top, vt);
+            const float again = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f, of = again * (tn > top ? top / tn : 1.0f);
+            m = mn, top = tn, log_top = __builtin_amdgcn_logf(tn);
+            l *= again;
 #pragma unroll
             for (int t = 0; t < VT; t++) o[t] *= of;
         }
+        const float share = share_of(vs, log_top), less = share - (m == -__builtin_inff() ? 0.0f : m);
+        f16x8 pv[2];
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], c, less));
+            sum += e;
+            pv[i >> 3][i & 7] = (_Float16)e;
+        }
+        l = fmaf(sum, __builtin_amdgcn_exp2f(-share), l);
 #pragma unroll
         for (int t = 0; t < VT; t++) {
             o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_to_f16(vw[t][0], vw[t][1]), pv[0], o[t], 0, 0, 0);
@@ -323,11 +344,12 @@ __global__ __launch_bounds__(256) void attn_step_kernel(const AttnArgs p) {
 }
 
 // Joins the chunks of a request's column: one workgroup per request, head and
-// column, its threads over dimensions and every (256 / D)th chunk.
+// column, its threads over 4 dimensions and every W-th chunk.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p) {
-    constexpr int W = 256 / D;
-    __shared__ float sum[W][D], lsum[W];
+    constexpr int W = 256 / (D / 4);
+    __shared__ __align__(16) float sum[W][D];
+    __shared__ float lsum[W];
     const uint32_t r = blockIdx.x, h = blockIdx.y / p.cols, col = blockIdx.y % p.cols;
     const Request rq = request_of(p, r);
     const uint32_t cols = columns_of(p, rq);
@@ -338,27 +360,28 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p) {
     for (uint32_t s = threadIdx.x & 63u; s < n; s += 64) m = fmaxf(m, p.part_ml[2 * (at + (uint64_t)s * p.cols)]);
     m = wave_max(m);
     const float ref = m == -__builtin_inff() ? 0.0f : m;
-    const uint32_t part = threadIdx.x / D, d = threadIdx.x % D;
-    float o = 0.0f, l = 0.0f;
+    const uint32_t part = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
     if (part < W) {
-#pragma unroll 4
+        f32x4 o = {0, 0, 0, 0};
+        float l = 0.0f;
+#pragma unroll 8
         for (uint32_t s = part; s < n; s += W) {
             const uint64_t i = at + (uint64_t)s * p.cols;
             const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * i] - ref);
-            l += f * p.part_ml[2 * i + 1];
-            o += f * p.part_o[i * D + d];
+            l = fmaf(f, p.part_ml[2 * i + 1], l);
+            o += f * *reinterpret_cast<const f32x4 *>(p.part_o + i * D + d);
         }
-        sum[part][d] = o;
+        *reinterpret_cast<f32x4 *>(&sum[part][d]) = o;
         if (d == 0) lsum[part] = l;
     }
     __syncthreads();
-    if (part != 0) return;
-    l = 0.0f, o = 0.0f;
+    if (threadIdx.x >= D) return;
+    float l = 0.0f, o = 0.0f;
 #pragma unroll
-    for (int w = 0; w < W; w++) l += lsum[w], o += sum[w][d];
+    for (int w = 0; w < W; w++) l += lsum[w], o += sum[w][threadIdx.x];
     uint16_t *out = reinterpret_cast<uint16_t *>(p.a.d_out) + ((uint64_t)rq.q0 + col / p.group) * p.a.out_token_stride +
                     (h * p.group + col % p.group) * p.a.out_head_stride;
-    out[d] = (uint16_t)f32_to_half<DT>(l != 0.0f ? o / l : 0.0f);
+    out[threadIdx.x] = (uint16_t)f32_to_half<DT>(l != 0.0f ? o / l : 0.0f);
 }
 
 // ---------------------------------------------------------------- many columns
@@ -375,22 +398,22 @@ __global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
     constexpr int KS = D / 16, VT = D / 32, T = 64 * NW;
     constexpr int KP = D + 8, VP = 64 + 8;  // pitches in f16
     constexpr int CODES = 64 * D / 16, PER = (CODES + T - 1) / T;  // 16-byte pieces of a tile's codes
-    __shared__ __align__(16) _Float16 lk[64 * KP];
-    __shared__ __align__(16) _Float16 lv[D * VP];
-    __shared__ float lks[4], lvs[4];
+    __shared__ __align__(16) _Float16 lk[2][64 * KP];
+    __shared__ __align__(16) _Float16 lv[2][D * VP];
+    __shared__ __align__(16) float lks[2][4], lvs[2][4];
     const uint32_t r = blockIdx.x / p.tiles, tile = p.tiles - 1 - blockIdx.x % p.tiles, h = blockIdx.y;
     const Request rq = request_of(p, r);
     const uint32_t cols = columns_of(p, rq);
     if (cols <= p.small || tile * (32 * NW) >= cols) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hl = lane >> 5;
-    const uint32_t c = tile * (32 * NW) + wave * 32 + (lane & 31);
-    const bool live = c < cols;
-    const uint32_t qi = c / p.group, qh = h * p.group + c % p.group;
+    const uint32_t c0 = tile * (32 * NW) + wave * 32 + (lane & 31);
+    const bool live = c0 < cols;
+    const uint32_t qi = c0 / p.group, qh = h * p.group + c0 % p.group;
     const int32_t limit = live ? limit_of(rq, (int32_t)qi) : 0;
     const uint32_t last = min(cols, (tile + 1) * (32 * NW)) - 1;
     const int32_t end = limit_of(rq, (int32_t)(last / p.group));
     const int32_t all = limit_of(rq, (int32_t)(tile * (32 * NW) / p.group));  // tokens that every column sees
-    const int32_t bs = (int32_t)p.cache.block_size;
+    const int32_t bs = (int32_t)p.cache.block_size, mask = bs - 1;
     const int32_t *table = p.a.d_table + (uint64_t)r * p.a.table_stride;
 
     f16x8 q[KS];
@@ -401,114 +424,153 @@ __global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
                                    : nullptr;
         const bool wide = !((uintptr_t)p.a.d_q & 15u) && !((p.a.q_token_stride | p.a.q_head_stride) & 7u);
         zs = load_query<DT, KS>(
-            row, wide, q, [&](int f) { return f * 16 + hl * 8; }, [](float v) { return fmaxf(v, __shfl_xor(v, 32)); });
-        zs *= p.a.scale * kLog2e;
+            row, wide, p.a.scale < 0.0f ? -1.0f : 1.0f, q, [&](int f) { return f * 16 + hl * 8; },
+            [](float v) { return fmaxf(v, __shfl_xor(v, 32)); });
+        zs *= fabsf(p.a.scale) * kLog2e;
     }
     f32x16 o[VT];
 #pragma unroll
     for (int t = 0; t < VT; t++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[t][i] = 0.0f;
-    float m = -__builtin_inff(), l = 0.0f, top = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f, top = 0.0f, log_top = -__builtin_inff();
 
-    // a tile's codes on the way: pieces of 16 dimensions of a token, of 16
-    // tokens of a dimension
+    // A tile's codes on the way: pieces of 16 dimensions of a token, of 16
+    // tokens of a dimension.  The blocks' ids come a tile ahead of the codes,
+    // the codes a tile ahead of their use.
     u32x4 kc[PER], vc[PER];
+    int32_t ik[PER], iv[PER], is = -1;
     float ksc = 0.0f, vsc = 0.0f;
+    const uint8_t *kh = p.cache.d_k + (uint64_t)h * bs * D, *vh = p.cache.d_v + (uint64_t)h * bs * D;
+    auto ids = [&](int32_t base) {
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int x = j * T + tid;
+            ik[j] = block_of(p, table, base + x / (D / 16), end), iv[j] = block_of(p, table, base + 16 * (x % 4), end);
+        }
+        if (tid < 4) is = block_of(p, table, base + 16 * tid, end);
+    };
     auto fetch = [&](int32_t base) {
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int x = j * T + tid;
             if (CODES % T && x >= CODES) break;
             const int kt = x / (D / 16), kd = x % (D / 16), vd = x / 4, vu = x % 4;
-            const int32_t bk = max(block_of(p, table, base + kt, end), 0);
-            kc[j] = *reinterpret_cast<const u32x4 *>(
-                p.cache.d_k + (((uint64_t)bk * p.cache.kv_heads + h) * bs + (base + kt) % bs) * D + kd * 16);
-            const int32_t bv = max(block_of(p, table, base + 16 * vu, end), 0);
-            vc[j] = *reinterpret_cast<const u32x4 *>(
-                p.cache.d_v + (((uint64_t)bv * p.cache.kv_heads + h) * D + vd) * bs + (base + 16 * vu) % bs);
+            kc[j] = *reinterpret_cast<const u32x4 *>(kh + (uint64_t)(held(p, ik[j]) ? ik[j] : 0) * p.block_step +
+                                                     (uint32_t)(((base + kt) & mask) * D + kd * 16));
+            vc[j] = *reinterpret_cast<const u32x4 *>(vh + (uint64_t)(held(p, iv[j]) ? iv[j] : 0) * p.block_step +
+                                                     (uint32_t)(vd * bs + ((base + 16 * vu) & mask)));
         }
         if (tid < 4) {
-            const int32_t b = block_of(p, table, base + 16 * tid, end);
-            const uint64_t bh = (uint64_t)max(b, 0) * p.cache.kv_heads + h;
+            const bool in = held(p, is);
+            const uint32_t bh = (in ? is : 0) * p.cache.kv_heads + h;
             // a run without a block: marked by a negative scale
-            ksc = b >= 0 ? p.cache.d_k_scale[bh] : -1.0f;
-            vsc = b >= 0 ? p.cache.d_v_scale[bh] : 0.0f;
+            ksc = in ? p.cache.d_k_scale[bh] : -1.0f;
+            vsc = in ? p.cache.d_v_scale[bh] : 0.0f;
         }
     };
-    auto stage = [&]() {
+    auto stage = [&](int b) {
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int x = j * T + tid;
             if (CODES % T && x >= CODES) break;
             const int kt = x / (D / 16), kd = x % (D / 16), vd = x / 4, vu = x % 4;
-            *reinterpret_cast<f16x8 *>(&lk[kt * KP + kd * 16]) = codes8_to_f16(kc[j][0], kc[j][1]);
-            *reinterpret_cast<f16x8 *>(&lk[kt * KP + kd * 16 + 8]) = codes8_to_f16(kc[j][2], kc[j][3]);
-            *reinterpret_cast<f16x8 *>(&lv[vd * VP + vu * 16]) = codes8_to_f16(vc[j][0], vc[j][2]);
-            *reinterpret_cast<f16x8 *>(&lv[vd * VP + vu * 16 + 8]) = codes8_to_f16(vc[j][1], vc[j][3]);
+            *reinterpret_cast<f16x8 *>(&lk[b][kt * KP + kd * 16]) = codes8_to_f16(kc[j][0], kc[j][1]);
+            *reinterpret_cast<f16x8 *>(&lk[b][kt * KP + kd * 16 + 8]) = codes8_to_f16(kc[j][2], kc[j][3]);
+            *reinterpret_cast<f16x8 *>(&lv[b][vd * VP + vu * 16]) = codes8_to_f16(vc[j][0], vc[j][2]);
+            *reinterpret_cast<f16x8 *>(&lv[b][vd * VP + vu * 16 + 8]) = codes8_to_f16(vc[j][1], vc[j][3]);
         }
-        if (tid < 4) lks[tid] = ksc, lvs[tid] = vsc;
+        if (tid < 4) lks[b][tid] = ksc, lvs[b][tid] = vsc;
     };
 
-    if (end > 0) fetch(0);
+    if (end > 0) {
+        ids(0);
+        fetch(0);
+        ids(64);
+        stage(0);
+        fetch(64);
+        ids(128);
+    }
     for (int32_t base = 0; base < end; base += 64) {
+        const int b = (base >> 6) & 1;
+        // the one barrier of a tile: its codes are in LDS, and the tile
+        // before, whose buffer the next one takes, is done with
         __syncthreads();
-        stage();
-        __syncthreads();
-        if (base + 64 < end) fetch(base + 64);
-        float ks[4], vs[4], vt = top;
-#pragma unroll
-        for (int i = 0; i < 4; i++) ks[i] = lks[i], vs[i] = lvs[i], vt = fmaxf(vt, vs[i]);
-        const bool masked = base + 64 > all || ks[0] < 0.0f || ks[1] < 0.0f || ks[2] < 0.0f || ks[3] < 0.0f;
         f32x16 s[2];
-        float zm = -__builtin_inff();
 #pragma unroll
         for (int t = 0; t < 2; t++) {
 #pragma unroll
             for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
 #pragma unroll
             for (int f = 0; f < KS; f++) {
-                const f16x8 a = *reinterpret_cast<const f16x8 *>(&lk[(t * 32 + (lane & 31)) * KP + f * 16 + hl * 8]);
+                const f16x8 a = *reinterpret_cast<const f16x8 *>(&lk[b][(t * 32 + (lane & 31)) * KP + f * 16 + hl * 8]);
                 s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[f], s[t], 0, 0, 0);
             }
         }
+        float c[4], vs[4], vt = 0.0f;
+        bool masked = base + 64 > all;
 #pragma unroll
-        for (int t = 0; t < 2; t++)
+        for (int i = 0; i < 4; i++) {
+            const float ks = lks[b][i];
+            vs[i] = lvs[b][i], vt = fmaxf(vt, vs[i]);
+            c[i] = ks * zs;
+            masked = masked || ks < 0.0f;
+        }
+        if (base + 64 < end) {
+            stage(b ^ 1);
+            fetch(base + 128);
+            ids(base + 192);
+        }
+        if (masked) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                float z = s[t][i] * (ks[2 * t + (i >> 3)] * zs);
-                if (masked) {
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int u = 2 * t + (i >> 3);
                     const int32_t tok = base + 32 * t + 8 * (i >> 2) + 4 * hl + (i & 3);
-                    z = tok < limit && ks[2 * t + (i >> 3)] >= 0.0f ? z : -__builtin_inff();
+                    s[t][i] = tok < limit && lks[b][u] >= 0.0f ? s[t][i] * c[u] : -__builtin_inff();
                 }
-                s[t][i] = z;
-                zm = fmaxf(zm, z);
-            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) c[i] = 1.0f;
+        }
+        float zm = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            float um = s[u >> 1][8 * (u & 1)];
+#pragma unroll
+            for (int i = 1; i < 8; i++) um = fmaxf(um, s[u >> 1][8 * (u & 1) + i]);
+            zm = fmaxf(zm, um * c[u]);
+        }
         zm = fmaxf(zm, __shfl_xor(zm, 32));
-        const float mn = fmaxf(m, zm), ref = mn == -__builtin_inff() ? 0.0f : mn;
-        const float again = __builtin_amdgcn_exp2f(m - ref), of = again * (vt > 0.0f ? top / vt : 1.0f);
-        m = mn, top = vt;
-        l *= again;
-        if (__any(of != 1.0f)) {
+        if (__any(zm > m + kSlack || vt > top)) {
+            const float mn = zm > m + kSlack ? zm : m, tn = fmaxf(top, vt);
+            const float again = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f, of = again * (tn > top ? top / tn : 1.0f);
+            m = mn, top = tn, log_top = __builtin_amdgcn_logf(tn);
+            l *= again;
 #pragma unroll
             for (int t = 0; t < VT; t++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[t][i] *= of;
         }
+        const float ref = m == -__builtin_inff() ? 0.0f : m;
         f16x8 pv[4];
 #pragma unroll
-        for (int t = 0; t < 2; t++)
+        for (int u = 0; u < 4; u++) {
+            const float share = share_of(vs[u], log_top), less = share - ref;
+            float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float e = __builtin_amdgcn_exp2f(s[t][i] - ref);
-                l += e;
-                pv[2 * t + (i >> 3)][i & 7] = (_Float16)(e * (vt > 0.0f ? vs[2 * t + (i >> 3)] / vt : 0.0f));
+            for (int i = 0; i < 8; i++) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + i], c[u], less));
+                sum += e;
+                pv[u][i] = (_Float16)e;
             }
+            l = fmaf(sum, __builtin_amdgcn_exp2f(-share), l);
+        }
 #pragma unroll
         for (int t = 0; t < VT; t++)
 #pragma unroll
             for (int f = 0; f < 4; f++) {
-                const f16x8 a = *reinterpret_cast<const f16x8 *>(&lv[(t * 32 + (lane & 31)) * VP + f * 16 + hl * 8]);
+                const f16x8 a = *reinterpret_cast<const f16x8 *>(&lv[b][(t * 32 + (lane & 31)) * VP + f * 16 + hl * 8]);
                 o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pv[f], o[t], 0, 0, 0);
             }
     }
@@ -529,7 +591,10 @@ __global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
         }
 }
 
-constexpr int kTileWaves = 4;
+// 8 waves (two to a SIMD, each tile's codes converted for 256 columns) where
+// their registers fit.
+template <int D>
+constexpr int kTileWaves = D <= 128 ? 8 : 4;
 
 template <int DT, int D>
 hipError_t launch_attention(const AttnArgs &p, hipStream_t s) {
@@ -537,8 +602,8 @@ hipError_t launch_attention(const AttnArgs &p, hipStream_t s) {
     if (p.splits > 1)
         hipLaunchKernelGGL((attn_join_kernel<DT, D>), dim3(p.a.requests, p.cache.kv_heads * p.cols), dim3(256), 0, s, p);
     if (p.tiles)
-        hipLaunchKernelGGL((attn_tile_kernel<DT, D, kTileWaves>), dim3(p.a.requests * p.tiles, p.cache.kv_heads),
-                           dim3(64 * kTileWaves), 0, s, p);
+        hipLaunchKernelGGL((attn_tile_kernel<DT, D, kTileWaves<D>>), dim3(p.a.requests * p.tiles, p.cache.kv_heads),
+                           dim3(64 * kTileWaves<D>), 0, s, p);
     return hipGetLastError();
 }
 
@@ -577,21 +642,24 @@ extern "C" int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, co
     p.cache = *cache;
     p.a = *a;
     p.group = group;
+    p.bs_log = (uint32_t)__builtin_ctz(cache->block_size);
+    p.block_step = cache->kv_heads * cache->block_size * cache->head_dim;
     p.small = 16;
     p.cols = (uint32_t)(most < 1 ? 1 : most < 16 ? most : 16);
     const uint64_t room = (uint64_t)a->table_width * cache->block_size;
     const uint64_t kv = a->max_kv < room ? a->max_kv : room;
     if (kv > 1ull << 30) return HH_ERR_UNSUPPORTED;  // tokens are counted in 31 bits
-    // chunks: enough workgroups for 4 per CU, none below 256 tokens
+    // chunks: enough workgroups for 16 per CU, none below 512 tokens
     const uint64_t lanes = (uint64_t)a->requests * cache->kv_heads;
-    const uint64_t want = (4ull * (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256) + lanes - 1) / lanes;
+    const uint64_t want = (16ull * (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256) + lanes - 1) / lanes;
     uint64_t chunk = (kv + want - 1) / want;
     chunk = (chunk + 255) / 256 * 256;
-    if (chunk < 256) chunk = 256;
+    if (chunk < 512) chunk = 512;
     p.chunk = (uint32_t)chunk;
     p.splits = (uint32_t)((kv + chunk - 1) / chunk);
     if (p.splits < 1) p.splits = 1;
-    p.tiles = most > p.small ? (uint32_t)((most + 32 * hh::kTileWaves - 1) / (32 * hh::kTileWaves)) : 0;
+    const uint32_t tile = 32u * (cache->head_dim <= 128 ? hh::kTileWaves<128> : hh::kTileWaves<256>);
+    p.tiles = most > p.small ? (uint32_t)((most + tile - 1) / tile) : 0;
     if ((uint64_t)a->requests * p.splits >= 1ull << 24 || (uint64_t)a->requests * p.tiles >= 1ull << 24)
         return HH_ERR_UNSUPPORTED;
     if (cache->kv_heads * 16ull > 65535) return HH_ERR_UNSUPPORTED;
