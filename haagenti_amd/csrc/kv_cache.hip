@@ -148,12 +148,13 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(const hh_kv_plan_
 
 // ---------------------------------------------------------------- append
 //
-// One wave per row, head and side (keys, values): the wave of a run's first
-// row (its predecessor's slot is not the one before in the same block) takes
-// the whole run, the others end.  It reads the run twice (largest magnitude,
-// then codes; the second time from cache).  Values are transposed on the way:
-// a lane takes 8 dimensions of 16 tokens and writes each dimension's 16 codes
-// at once.
+// A run is the rows of one block: consecutive slots.  A workgroup takes the
+// runs that begin in its span of rows, for one head and side (keys, values):
+// it holds a run's rows in registers (PER pieces of 8 values per thread),
+// finds their largest magnitude and writes their codes, the keys' at once,
+// the values' through LDS, where they become 16 tokens per dimension.  Bound
+// by reading the rows and, for single rows, by the chain slot, row, maximum,
+// scale, code.
 
 struct AppendArgs {
     uint8_t *k, *v;
@@ -161,7 +162,7 @@ struct AppendArgs {
     const uint16_t *rows_k, *rows_v;
     uint64_t tk, hk, tv, hv;
     const int32_t *slots;
-    uint32_t tokens, heads, dim, bs, slots_end;
+    uint32_t tokens, heads, dim, bs, slots_end, span;
 };
 
 // amax / 127, rounded up to 8 significant bits: a / 127 of an 11-bit a is no
@@ -170,115 +171,198 @@ struct AppendArgs {
 __device__ __forceinline__ float scale_for(float amax) {
     return __uint_as_float((__float_as_uint(amax / 127.0f) + 0xffffu) & 0xffff0000u);
 }
-__device__ __forceinline__ uint32_t code_of(float x, float scale) {
-    const float q = x != x ? 0.0f : fminf(fmaxf(rintf(x / scale), -127.0f), 127.0f);
-    return (uint32_t)(int32_t)q + 128u & 255u;
+// x / scale rounded to a code.  The quotient of an x of at most 16 bits by a
+// scale of 8 is a tie or 2^-18 (relative) away from one; with one correction
+// the product by the reciprocal is within 2^-22 and exact where the quotient
+// is a tie (its correction is the error of the first product, to 2^-23).
+// Scales whose reciprocal leaves f32's normal range are divided by.
+struct Divider {
+    float scale, inverse;
+    __device__ __forceinline__ explicit Divider(float s) : scale(s), inverse(1.0f / s) {}
+    __device__ __forceinline__ float quotient(float x) const {
+        if (scale < 0x1p-120f) return x / scale;
+        const float q = x * inverse;
+        return fmaf(fmaf(-q, scale, x), inverse, q);
+    }
+    // values: infinities give the last codes, NaN that of 0
+    __device__ __forceinline__ uint32_t code(float x) const {
+        const float q = fabsf(x) < __builtin_inff() ? quotient(x) : x;
+        return (uint32_t)(int32_t)(q != q ? 0.0f : fminf(fmaxf(rintf(q), -127.0f), 127.0f)) + 128u;
+    }
+    // The low byte of the result, for a value of at most 127 scales (a whole
+    // run without infinities and NaN) and a scale that is not tiny: the sum
+    // is rounded at its units.
+    __device__ __forceinline__ uint32_t code_in_byte(float x) const {
+        const float q = x * inverse;
+        return __float_as_uint(fmaf(fmaf(-q, scale, x), inverse, q) + 12583040.0f);  // 1.5 * 2^23 + 128
+    }
+};
+// The low bytes of four numbers.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
+}
+// A word of codes at another scale.
+__device__ __forceinline__ uint32_t recode(uint32_t w, float old, const Divider &now) {
+    uint32_t v = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) v |= now.code((float)((int32_t)((w >> (8 * i)) & 255u) - 128) * old) << (8 * i);
+    return v;
 }
 
 // 8 values of a row.  WIDE: 16-byte aligned.
 template <bool WIDE>
 __device__ __forceinline__ u32x4 load8(const uint16_t *p) {
     if constexpr (WIDE) return *reinterpret_cast<const u32x4 *>(p);
-    u32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
-    return v;
+    typedef u32x4 u32x4_any __attribute__((aligned(2)));
+    return *reinterpret_cast<const u32x4_any *>(p);
 }
 template <int DT>
 __device__ __forceinline__ float elem(const u32x4 &v, int i) {
     return half_to_f32<DT>((v[i >> 1] >> (16 * (i & 1))) & 0xffffu);
 }
 
-template <int DT, bool WIDE>
+template <int DT, bool WIDE, int PER>
 __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs p) {
-    const uint32_t lane = threadIdx.x & 63u, task = blockIdx.y * 4 + (threadIdx.x >> 6);
-    const uint32_t h = task >> 1, t = blockIdx.x, bs = p.bs;
-    if (h >= p.heads) return;
-    const int32_t slot = p.slots[t];
-    if (slot < 0 || (uint32_t)slot >= p.slots_end) return;
-    const uint32_t off = (uint32_t)slot % bs;
-    if (off && t && p.slots[t - 1] == slot - 1) return;
-    // the run: consecutive slots of this block (at most 128 rows)
-    uint32_t n = 1;
-    for (uint32_t i = 1; off + i < bs; i += 64) {
-        const uint32_t j = i + lane;
-        const bool in = off + j < bs && (uint64_t)t + j < p.tokens && p.slots[t + j] == slot + (int32_t)j;
-        const uint64_t out = ~__ballot(in);
-        if (out) {
-            n += (uint32_t)__builtin_ctzll(out);
-            break;
+    extern __shared__ __align__(16) uint8_t tile[];
+    __shared__ float tops[4];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, h = blockIdx.y >> 1, bs = p.bs, t0 = blockIdx.x * p.span;
+    const bool values = blockIdx.y & 1u;
+    // 64 slots from the span's first row on: where runs begin, where they go on
+    const int32_t mine = t0 + lane < p.tokens ? p.slots[t0 + lane] : -1;
+    const int32_t ahead = t0 ? p.slots[t0 - 1] : -1;
+    const int32_t below = __shfl_up(mine, 1), prev = lane ? below : ahead;  // every lane takes part in the shuffle
+    const bool sound = mine >= 0 && (uint32_t)mine < p.slots_end, on = sound && (uint32_t)mine % bs && prev == mine - 1;
+    const uint64_t goes_on = __ballot(on);
+    uint64_t first = __ballot(sound && !on && lane < p.span);
+    const uint32_t chunks = p.dim / 8, pitch = bs + 20;
+    // i / chunks of i < 4096: exact, as the error i / 2^16 stays below 1 / chunks
+    const uint32_t inv = 65536u / chunks + (65536u % chunks != 0);
+    for (; first; first &= first - 1) {
+        const uint32_t l0 = (uint32_t)__builtin_ctzll(first), t = t0 + l0;
+        const int32_t slot = __builtin_amdgcn_readlane(mine, (int)l0);
+        const uint32_t off = (uint32_t)slot % bs;
+        const uint64_t rest = ~(goes_on >> l0 >> 1);
+        uint32_t n = 1 + (uint32_t)__builtin_ctzll(rest);  // a bit is set: zeros came in from above
+        if (l0 + n == 64) {
+            // as far as was read: 64 more slots at a time
+            for (uint32_t i = n; off + i < bs; i += 64) {
+                const uint32_t j = i + lane;
+                const bool in = off + j < bs && (uint64_t)t + j < p.tokens && p.slots[t + j] == slot + (int32_t)j;
+                const uint64_t out = ~__ballot(in);
+                n += out ? (uint32_t)__builtin_ctzll(out) : 64u;
+                if (out) break;
+            }
         }
-        n += 64;
-    }
-    const bool values = task & 1u;
-    const uint64_t bh = (uint64_t)((uint32_t)slot / bs) * p.heads + h;
-    const uint64_t ts = values ? p.tv : p.tk;
-    const uint16_t *rows = values ? p.rows_v + t * p.tv + h * p.hv : p.rows_k + t * p.tk + h * p.hk;
-    uint8_t *codes = (values ? p.v : p.k) + bh * bs * p.dim;
-    float *scale = (values ? p.v_scale : p.k_scale) + bh;
-    const float old = off ? *scale : 0.0f;
+        const uint64_t bh = (uint64_t)((uint32_t)slot / bs) * p.heads + h, ts = values ? p.tv : p.tk;
+        const uint16_t *rows = values ? p.rows_v + t * p.tv + h * p.hv : p.rows_k + t * p.tk + h * p.hk;
+        uint8_t *codes = (values ? p.v : p.k) + bh * bs * p.dim;
+        float *scale = (values ? p.v_scale : p.k_scale) + bh;
+        const float old = off ? *scale : 0.0f;
 
-    const uint32_t chunks = p.dim / 8;
-    float amax = 0.0f;
-    for (uint32_t i = lane; i < n * chunks; i += 64) {
-        const u32x4 x = load8<WIDE>(rows + i / chunks * ts + i % chunks * 8);
+        u32x4 x[PER];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float a = fabsf(elem<DT>(x, e));
-            amax = fmaxf(amax, a < __builtin_inff() ? a : 0.0f);
+        for (int j = 0; j < PER; j++) {
+            const uint32_t i = j * 256 + tid;
+            x[j] = i < n * chunks ? load8<WIDE>(rows + (i * inv >> 16) * ts + (i - (i * inv >> 16) * chunks) * 8) : u32x4{0, 0, 0, 0};
         }
-    }
-    amax = wave_max(amax);
-    const float now = fmaxf(old, scale_for(amax)), div = now > 0.0f ? now : 1.0f;
-    if (off && now > old) {
-        // the block's tokens before: off * dim codes, keys in one piece,
-        // values in rows of bs
-        for (uint32_t i = lane; i < off * p.dim; i += 64) {
-            uint8_t *c = codes + (values ? (uint64_t)(i / off) * bs + i % off : i);
-            *c = (uint8_t)code_of((float)((int32_t)*c - 128) * old, div);
+        // magnitudes order as their bits do, infinities and NaN above all
+        u16x2 most = {0, 0};
+#pragma unroll
+        for (int j = 0; j < PER; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[j][e] & 0x7fff7fffu));
+        float amax = half_to_f32<DT>(max(most[0], most[1]));
+        const bool fine = __syncthreads_and(amax < __builtin_inff());
+        if (!fine) {
+            amax = 0.0f;
+#pragma unroll
+            for (int j = 0; j < PER; j++)
+#pragma unroll 1
+                for (int e = 0; e < 8; e++) {
+                    const float v = fabsf(elem<DT>(x[j], e));
+                    amax = fmaxf(amax, v < __builtin_inff() ? v : 0.0f);
+                }
         }
-    }
-    if (lane == 0) *scale = now;
-    if (!values) {
-        for (uint32_t i = lane; i < n * chunks; i += 64) {
-            const uint32_t r = i / chunks, c = i % chunks * 8;
-            const u32x4 x = load8<WIDE>(rows + r * ts + c);
-            u32x2 w = {0u, 0u};
+        amax = wave_max(amax);
+        if (lane == 0) tops[tid >> 6] = amax;
+        __syncthreads();
+        amax = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        const float now = fmaxf(old, scale_for(amax));
+        const Divider div(now > 0.0f ? now : 1.0f);
+        const bool grown = off && now > old, plain = fine && div.scale >= 0x1p-120f;
+        const uint32_t lead = off % 16;  // tile's columns are tokens from the run's first 16 on
+        if (tid == 0) *scale = now;
 #pragma unroll
-            for (int e = 0; e < 8; e++) w[e >> 2] |= code_of(elem<DT>(x, e), div) << (8 * (e & 3));
-            *reinterpret_cast<u32x2 *>(codes + (uint64_t)(off + r) * p.dim + c) = w;
-        }
-        return;
-    }
-    const uint32_t g0 = off / 16, groups = (off + n - 1) / 16 - g0 + 1;
-    for (uint32_t i = lane; i < groups * chunks; i += 64) {
-        const uint32_t g = g0 + i / chunks, c = i % chunks * 8;
-        uint8_t *to = codes + (uint64_t)c * bs + 16 * g;
-        u32x4 w[8] = {};
-        bool whole = true;
+        for (int j = 0; j < PER; j++) {
+            const uint32_t i = j * 256 + tid, r = i * inv >> 16, c = (i - r * chunks) * 8;
+            if (i >= n * chunks) break;
+            u32x2 w;
+            if (plain) {
+                uint32_t b[8];
 #pragma unroll
-        for (uint32_t j = 0; j < 16; j++) {
-            const uint32_t r = 16 * g + j - off;  // wraps below the run
-            if (r < n) {
-                const u32x4 x = load8<WIDE>(rows + r * ts + c);
-#pragma unroll
-                for (int e = 0; e < 8; e++) w[e][j >> 2] |= code_of(elem<DT>(x, e), div) << (8 * (j & 3));
+                for (int e = 0; e < 8; e++) b[e] = div.code_in_byte(elem<DT>(x[j], e));
+                w = u32x2{low_bytes(b[0], b[1], b[2], b[3]), low_bytes(b[4], b[5], b[6], b[7])};
             } else {
-                whole = false;
+                w = u32x2{0u, 0u};
+#pragma unroll
+                for (int e = 0; e < 8; e++) w[e >> 2] |= div.code(elem<DT>(x[j], e)) << (8 * (e & 3));
+            }
+            if (values) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) tile[(c + e) * pitch + lead + r] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+            } else {
+                *reinterpret_cast<u32x2 *>(codes + (uint64_t)(off + r) * p.dim + c) = w;
             }
         }
-        if (whole) {
+        if (values) {
+            // 16 tokens of a dimension at a time, with what is there of
+            // tokens before (at the new scale) and after the run
+            __syncthreads();
+            const uint32_t g0 = grown ? 0 : off / 16, groups = (off + n + 15) / 16 - g0;
+            for (uint32_t i = tid; i < groups * p.dim; i += 256) {
+                const uint32_t d = i / groups, at = (g0 + i % groups) * 16;
+                u32x4 *to = reinterpret_cast<u32x4 *>(codes + (uint64_t)d * bs + at);
+                u32x4 w;
+                if (at >= off && at + 16 <= off + n) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) *reinterpret_cast<u32x4 *>(to + (uint64_t)e * bs) = w[e];
-        } else {
+                    for (int e = 0; e < 4; e++) w[e] = reinterpret_cast<const uint32_t *>(tile + d * pitch + (at - off + lead))[e];
+                } else {
+                    w = *to;
+                    for (uint32_t j = 0; j < 16; j++) {
+                        const uint32_t r = at + j - off;  // wraps below the run
+                        uint32_t c = (w[j >> 2] >> (8 * (j & 3))) & 255u;
+                        if (r < n)
+                            c = tile[d * pitch + lead + r];
+                        else if (grown && at + j < off)
+                            c = div.code((float)((int32_t)c - 128) * old);
+                        w[j >> 2] = (w[j >> 2] & ~(255u << (8 * (j & 3)))) | c << (8 * (j & 3));
+                    }
+                }
+                *to = w;
+            }
+        } else if (grown) {
+            for (uint32_t i = tid; i < off * p.dim / 16; i += 256) {
+                u32x4 *at = reinterpret_cast<u32x4 *>(codes) + i;
+                u32x4 w = *at;
 #pragma unroll
-            for (uint32_t j = 0; j < 16; j++) {
-                if (16 * g + j - off >= n) continue;
-#pragma unroll
-                for (int e = 0; e < 8; e++) to[(uint64_t)e * bs + j] = (uint8_t)(w[e][j >> 2] >> (8 * (j & 3)));
+                for (int e = 0; e < 4; e++) w[e] = recode(w[e], old, div);
+                *at = w;
             }
         }
+        __syncthreads();  // tops and tile are read
     }
+}
+
+template <int DT, bool WIDE>
+void launch_append(const AppendArgs &p, hipStream_t s) {
+    // pieces of 8 values in a full block, over 256 threads
+    const uint32_t per = (p.bs * p.dim / 8 + 255) / 256;
+    auto kernel = per <= 1   ? kv_append_kernel<DT, WIDE, 1>
+                  : per <= 2 ? kv_append_kernel<DT, WIDE, 2>
+                  : per <= 4 ? kv_append_kernel<DT, WIDE, 4>
+                  : per <= 8 ? kv_append_kernel<DT, WIDE, 8>
+                             : kv_append_kernel<DT, WIDE, 16>;
+    hipLaunchKernelGGL(kernel, dim3((p.tokens + p.span - 1) / p.span, 2 * p.heads), dim3(256), p.dim * (p.bs + 20), s, p);
 }
 
 // ---------------------------------------------------------------- read
@@ -304,7 +388,7 @@ __device__ __forceinline__ void store8(void *out, uint64_t at, const float *v) {
 template <int OUT>
 __global__ __launch_bounds__(256) void kv_read_kernel(const hh_kv_cache cache, const int32_t *__restrict__ blocks,
                                                       void *__restrict__ out_k, void *__restrict__ out_v) {
-    extern __shared__ uint32_t tile[];
+    extern __shared__ uint32_t words[];
     const uint32_t bs = cache.block_size, dim = cache.head_dim, heads = cache.kv_heads, h = blockIdx.y;
     const bool values = blockIdx.z, held = (uint32_t)blocks[blockIdx.x] < cache.num_blocks;
     const uint64_t bh = (uint64_t)(held ? blocks[blockIdx.x] : 0) * heads + h;
@@ -318,7 +402,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const hh_kv_cache cache, c
             const uint32_t d = i / (bs / 16), g = i % (bs / 16);
             const u32x4 w = held ? *reinterpret_cast<const u32x4 *>(codes + (uint64_t)i * 16) : u32x4{};
 #pragma unroll
-            for (int j = 0; j < 4; j++) tile[(d * pitch + 16 * g) / 4 + j] = w[j];
+            for (int j = 0; j < 4; j++) words[(d * pitch + 16 * g) / 4 + j] = w[j];
         }
         __syncthreads();
     }
@@ -326,7 +410,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const hh_kv_cache cache, c
         const uint32_t t = i / chunks, c = i % chunks * 8;
         float v[8];
         if (values) {
-            const uint8_t *b = reinterpret_cast<const uint8_t *>(tile);
+            const uint8_t *b = reinterpret_cast<const uint8_t *>(words);
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = (float)((int32_t)b[(c + e) * pitch + t] - 128) * scale;
         } else {
@@ -397,15 +481,19 @@ int32_t hh_kv_append(hh_context *ctx, const hh_kv_cache *cache, const void *d_ro
     if (((uintptr_t)d_rows_k | (uintptr_t)d_rows_v) & 1u) return HH_ERR_INVALID_ARGUMENT;
     hh::DeviceGuard guard(ctx->device);
     if (guard.status() != hipSuccess) return hh::from_hip(guard.status());
+    // Rows in a workgroup's span: one while the grid is small (each row of a
+    // step is a run), up to 16 for prompts, most of whose rows begin none.
+    const uint64_t grid = (uint64_t)tokens * 2 * cache->kv_heads / 2048;
     const hh::AppendArgs p = {cache->d_k, cache->d_v, cache->d_k_scale, cache->d_v_scale,
                               reinterpret_cast<const uint16_t *>(d_rows_k), reinterpret_cast<const uint16_t *>(d_rows_v),
                               tk, hk, tv, hv, d_slots, tokens, cache->kv_heads, cache->head_dim, cache->block_size,
-                              cache->num_blocks * cache->block_size};
+                              cache->num_blocks * cache->block_size, (uint32_t)(grid < 1 ? 1 : grid > 64 ? 64 : grid)};
     const bool wide = !(((uintptr_t)d_rows_k | (uintptr_t)d_rows_v) & 15u) && !((tk | hk | tv | hv) & 7u);
-    auto kernel = dtype == HH_BF16 ? (wide ? hh::kv_append_kernel<HH_BF16, true> : hh::kv_append_kernel<HH_BF16, false>)
-                                   : (wide ? hh::kv_append_kernel<HH_F16, true> : hh::kv_append_kernel<HH_F16, false>);
-    hipLaunchKernelGGL(kernel, dim3(tokens, (2 * cache->kv_heads + 3) / 4), dim3(256), 0,
-                       reinterpret_cast<hipStream_t>(stream), p);
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    if (dtype == HH_BF16)
+        wide ? hh::launch_append<HH_BF16, true>(p, s) : hh::launch_append<HH_BF16, false>(p, s);
+    else
+        wide ? hh::launch_append<HH_F16, true>(p, s) : hh::launch_append<HH_F16, false>(p, s);
     return hh::from_hip(hipGetLastError());
 }
 
