@@ -6,70 +6,45 @@ Tensors are torch tensors on the context's device.  Calls run on torch's
 current stream, where their results are allocated, and don't synchronise.
 What a call can't take raises HaagentiError before anything is launched."""
 import ctypes as C
+import struct
 
 import torch
 
-from . import BF16, F16, F32, INVALID_ARGUMENT, UNSUPPORTED, HaagentiError, _check, _i32, _sig, _sz, _u32, _vp
+from . import BF16, F16, F32, INVALID_ARGUMENT, UNSUPPORTED, HaagentiError, _check, _i32, _sig, _u32, _vp
 
-_u64 = C.c_uint64
 INT4 = 16
 
 ACTIVATIONS = {"none": 0, None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+_HALF = {torch.float16: F16, torch.bfloat16: BF16}
 
+# The argument structures, packed as the header lays them out (natural
+# alignment, no gaps; a step's calls are a few microseconds each, and a packed
+# string costs a quarter of a ctypes structure).
+_LINEAR = struct.Struct("=6Q6Q3I4i4x")      # hh_linear_args
+_CACHE = struct.Struct("=4Q4I")             # hh_kv_cache
+_PLAN = struct.Struct("=10QQ5I4x")          # hh_kv_plan_args
+_ATTENTION = struct.Struct("=5Q5Q6Ifi")     # hh_kv_attention_args
 
-class _LinearArgs(C.Structure):
-    _fields_ = ([(n, _vp) for n in ("d_x", "d_w", "d_bias", "d_mul", "d_residual", "d_y")]
-                + [(n, _u64) for n in ("x_stride", "w_stride", "mul_stride", "residual_stride", "y_stride", "w_bytes")]
-                + [(n, _u32) for n in ("m", "n", "k")]
-                + [(n, _i32) for n in ("dtype", "w_dtype", "y_dtype", "activation")])
+_u64, _bytes = C.c_uint64, C.c_char_p
+_linear = _sig("hh_linear", _i32, [_vp, _bytes, _vp])
+_plan = _sig("hh_kv_plan", _i32, [_vp, _bytes, _vp])
+_append = _sig("hh_kv_append", _i32, [_vp, _bytes, _vp, _vp, _i32, _u64, _u64, _u64, _u64, _vp, _u32, _vp])
+_read = _sig("hh_kv_read", _i32, [_vp, _bytes, _vp, _u32, _i32, _vp, _vp, _vp])
+_attention = _sig("hh_kv_attention", _i32, [_vp, _bytes, _bytes, _vp])
 
-
-class _Cache(C.Structure):
-    _fields_ = ([(n, _vp) for n in ("d_k", "d_v", "d_k_scale", "d_v_scale")]
-                + [(n, _u32) for n in ("num_blocks", "block_size", "kv_heads", "head_dim")])
-
-
-class _PlanArgs(C.Structure):
-    _fields_ = ([(n, _vp) for n in ("d_len", "d_new", "d_table", "d_ring", "d_state", "d_start", "d_kv_len", "d_slots",
-                                    "d_status", "d_state_out")]
-                + [("table_stride", _u64)]
-                + [(n, _u32) for n in ("requests", "table_width", "ring_capacity", "block_size", "tokens")])
-
-
-class _AttentionArgs(C.Structure):
-    _fields_ = ([(n, _vp) for n in ("d_q", "d_out", "d_table", "d_start", "d_kv_len")]
-                + [(n, _u64) for n in ("q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride",
-                                       "table_stride")]
-                + [(n, _u32) for n in ("requests", "tokens", "q_heads", "table_width", "max_q", "max_kv")]
-                + [("scale", C.c_float), ("dtype", _i32)])
-
-
-_linear = _sig("hh_linear", _i32, [_vp, C.POINTER(_LinearArgs), _vp])
-_plan = _sig("hh_kv_plan", _i32, [_vp, C.POINTER(_PlanArgs), _vp])
-_append = _sig("hh_kv_append", _i32, [_vp, C.POINTER(_Cache), _vp, _vp, _i32, _u64, _u64, _u64, _u64, _vp, _u32, _vp])
-_read = _sig("hh_kv_read", _i32, [_vp, C.POINTER(_Cache), _vp, _u32, _i32, _vp, _vp, _vp])
-_attention = _sig("hh_kv_attention", _i32, [_vp, C.POINTER(_Cache), C.POINTER(_AttentionArgs), _vp])
+# torch.cuda.current_stream(device).cuda_stream without the Stream object
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _refuse(code, what):
     raise HaagentiError(code, what)
 
 
-def _on(ctx, what, *tensors):
+def _on(dev, what, *tensors):
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.get_device() != ctx.device):
+        if t is not None and t.get_device() != dev:
             _refuse(INVALID_ARGUMENT, f"{what}: tensors must be on the context's device")
-
-
-def _stream(ctx):
-    return torch.cuda.current_stream(ctx.device).cuda_stream
-
-
-def _half(t, what):
-    if t.dtype not in (torch.float16, torch.bfloat16):
-        _refuse(UNSUPPORTED, f"{what}: {t.dtype} (float16 or bfloat16)")
-    return _CODE[t.dtype]
 
 
 def _ints(what, *tensors):
@@ -89,11 +64,14 @@ class Int4Weight:
         self.data, self.n, self.k = data, int(n), int(k)
 
 
-def _rows(t, m, n, what):
-    """Row stride of an m x n matrix whose rows are contiguous."""
-    if t.dim() != 2 or t.shape[0] != m or t.shape[1] != n or (n > 1 and t.stride(1) != 1):
-        _refuse(INVALID_ARGUMENT, f"{what}: {m} x {n} with contiguous rows, got {tuple(t.shape)}")
-    return t.stride(0) if m > 1 else max(n, 1)
+def _rows(t, m, n, dev, what):
+    """Row stride of an m x n matrix on the device whose rows are contiguous."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != m or shape[1] != n or (n > 1 and stride[1] != 1):
+        _refuse(INVALID_ARGUMENT, f"linear: {what} is {m} x {n} with contiguous rows, got {tuple(shape)}")
+    if t.get_device() != dev:
+        _refuse(INVALID_ARGUMENT, f"linear: {what} must be on the context's device")
+    return stride[0] if m > 1 else n
 
 
 def linear(ctx, x, w, bias=None, act=None, mul=None, residual=None, out=None, out_dtype=None):
@@ -102,45 +80,59 @@ def linear(ctx, x, w, bias=None, act=None, mul=None, residual=None, out=None, ou
     residual m x n, of x's type.  act: a key of ACTIVATIONS.  Rows are
     contiguous, any stride apart.  Returns out (m x n of out_dtype, by default
     x's type; float32 is allowed), which may be residual or mul."""
-    dt = _half(x, "linear")
-    if x.dim() != 2:
+    dtype, dev, shape = x.dtype, ctx.device, x.shape
+    dt = _HALF.get(dtype)
+    if dt is None:
+        _refuse(UNSUPPORTED, f"linear: {dtype} (float16 or bfloat16)")
+    if len(shape) != 2:
         _refuse(INVALID_ARGUMENT, "linear: x is m x k")
-    m, k = x.shape
-    a = _LinearArgs()
+    m, k = shape
     if isinstance(w, Int4Weight):
-        n, wt = w.n, w.data
+        n, w_dtype, w_stride, w_bytes = w.n, INT4, 0, w.data.numel()
         if w.k != k:
             _refuse(INVALID_ARGUMENT, f"linear: x has {k} columns, the weight {w.k}")
-        a.w_dtype, a.w_bytes = INT4, wt.numel()
+        w = w.data
+        _on(dev, "linear", w)
     else:
-        if w.dim() != 2 or w.dtype != x.dtype:
+        if w.dtype != dtype:
             _refuse(INVALID_ARGUMENT, "linear: w is n x k of x's type, or an Int4Weight")
-        n, wt = w.shape[0], w
-        a.w_dtype, a.w_stride = dt, _rows(w, n, k, "linear: w")
-    if act not in ACTIVATIONS:
+        n, w_dtype, w_bytes = w.shape[0], dt, 0
+        w_stride = _rows(w, n, k, dev, "w")
+    code = ACTIVATIONS.get(act)
+    if code is None:
         _refuse(UNSUPPORTED, f"linear: activation {act!r}")
+    x_stride = _rows(x, m, k, dev, "x")
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
-    elif out_dtype is not None and out.dtype != out_dtype:
-        _refuse(INVALID_ARGUMENT, "linear: out has another type than out_dtype")
-    if out.dtype not in (x.dtype, torch.float32):
-        _refuse(UNSUPPORTED, f"linear: output {out.dtype}")
-    _on(ctx, "linear", x, wt, bias, mul, residual, out)
-    a.x_stride, a.y_stride = _rows(x, m, k, "linear: x"), _rows(out, m, n, "linear: out")
-    a.d_x, a.d_w, a.d_y = x.data_ptr(), wt.data_ptr(), out.data_ptr()
+        y_dtype, y_stride = out_dtype or dtype, n
+        if y_dtype is not dtype and y_dtype is not torch.float32:
+            _refuse(UNSUPPORTED, f"linear: output {y_dtype}")
+        out = x.new_empty((m, n), dtype=y_dtype)
+    else:
+        y_dtype = out.dtype
+        if y_dtype is not dtype and y_dtype is not torch.float32:
+            _refuse(UNSUPPORTED, f"linear: output {y_dtype}")
+        if out_dtype is not None and y_dtype is not out_dtype:
+            _refuse(INVALID_ARGUMENT, "linear: out has another type than out_dtype")
+        y_stride = _rows(out, m, n, dev, "out")
+    b = c = d = c_stride = d_stride = 0
     if bias is not None:
-        if bias.dim() != 1 or bias.shape[0] != n or bias.dtype != x.dtype or not bias.is_contiguous():
+        if bias.dim() != 1 or bias.shape[0] != n or bias.dtype is not dtype or not bias.is_contiguous():
             _refuse(INVALID_ARGUMENT, "linear: bias is n contiguous values of x's type")
-        a.d_bias = bias.data_ptr()
+        _on(dev, "linear", bias)
+        b = bias.data_ptr()
     if mul is not None:
-        a.d_mul, a.mul_stride = mul.data_ptr(), _rows(mul, m, n, "linear: mul")
+        c, c_stride = mul.data_ptr(), _rows(mul, m, n, dev, "mul")
+        if mul.dtype is not dtype:
+            _refuse(INVALID_ARGUMENT, "linear: mul has x's type")
     if residual is not None:
-        a.d_residual, a.residual_stride = residual.data_ptr(), _rows(residual, m, n, "linear: residual")
-    for t in (mul, residual):
-        if t is not None and t.dtype != x.dtype:
-            _refuse(INVALID_ARGUMENT, "linear: mul and residual have x's type")
-    a.m, a.n, a.k, a.dtype, a.y_dtype, a.activation = m, n, k, dt, _CODE[out.dtype], ACTIVATIONS[act]
-    _check(_linear(ctx.handle, C.byref(a), _stream(ctx)), "hh_linear")
+        d, d_stride = residual.data_ptr(), _rows(residual, m, n, dev, "residual")
+        if residual.dtype is not dtype:
+            _refuse(INVALID_ARGUMENT, "linear: residual has x's type")
+    rc = _linear(ctx.handle, _LINEAR.pack(x.data_ptr(), w.data_ptr(), b, c, d, out.data_ptr(), x_stride, w_stride, c_stride,
+                                          d_stride, y_stride, w_bytes, m, n, k, dt, w_dtype, _CODE[y_dtype], code),
+                 _stream(dev))
+    if rc:
+        _check(rc, "hh_linear")
     return out
 
 
@@ -164,22 +156,24 @@ def kv_plan(ctx, lens, new, table, ring, state, block_size, tokens):
     lens, new (requests), table (requests x width, updated), ring and state
     (the free queue; ring is updated, the next state returned).  tokens: room
     for the step's new rows."""
-    requests = lens.shape[0]
+    requests, dev, shape = lens.shape[0], ctx.device, table.shape
     _ints("kv_plan", lens, new, ring, state)
-    if (table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1)
-            or table.shape[0] != requests or new.shape != lens.shape or lens.dim() != 1 or state.numel() != 2):
+    if (table.dtype != torch.int32 or len(shape) != 2 or shape[0] != requests or (shape[1] > 1 and table.stride(1) != 1)
+            or new.shape != lens.shape or lens.dim() != 1 or state.numel() != 2):
         _refuse(INVALID_ARGUMENT, "kv_plan: lens and new per request, table requests x width, state of 2")
-    _on(ctx, "kv_plan", lens, new, table, ring, state)
-    tokens = int(tokens)
+    _on(dev, "kv_plan", lens, new, table, ring, state)
+    if tokens < 0:
+        _refuse(INVALID_ARGUMENT, "kv_plan: room for a negative number of rows")
     # one allocation: start, kv_len, status, state, slots
-    buf = torch.empty(3 * requests + 3 + tokens, dtype=torch.int32, device=lens.device)
+    buf = lens.new_empty(3 * requests + 3 + tokens)
     at = buf.data_ptr()
-    a = _PlanArgs(lens.data_ptr(), new.data_ptr(), table.data_ptr(), ring.data_ptr(), state.data_ptr(), at,
-                  at + 4 * (requests + 1), at + 4 * (3 * requests + 3), at + 4 * (2 * requests + 1),
-                  at + 4 * (3 * requests + 1), table.stride(0) if requests > 1 else table.shape[1], requests,
-                  table.shape[1], ring.numel(), int(block_size), tokens)
-    _check(_plan(ctx.handle, C.byref(a), _stream(ctx)), "hh_kv_plan")
-    start, kv_len, status, after, slots = buf.split_with_sizes([requests + 1, requests, requests, 2, tokens])
+    rc = _plan(ctx.handle, _PLAN.pack(lens.data_ptr(), new.data_ptr(), table.data_ptr(), ring.data_ptr(), state.data_ptr(),
+                                      at, at + 4 * requests + 4, at + 12 * requests + 12, at + 8 * requests + 4,
+                                      at + 12 * requests + 4, table.stride(0) if requests > 1 else shape[1], requests,
+                                      shape[1], ring.numel(), block_size, tokens), _stream(dev))
+    if rc:
+        _check(rc, "hh_kv_plan")
+    start, kv_len, status, after, slots = buf.split_with_sizes((requests + 1, requests, requests, 2, tokens))
     return Plan(start, kv_len, slots, status, after)
 
 
@@ -198,12 +192,11 @@ class KvCache:
             _refuse(INVALID_ARGUMENT, "KvCache: shapes of v and the scales must match k's")
         if not all(t.is_contiguous() for t in (k, v, k_scale, v_scale)):
             _refuse(INVALID_ARGUMENT, "KvCache: contiguous tensors")
-        _on(ctx, "KvCache", k, v, k_scale, v_scale)
+        _on(ctx.device, "KvCache", k, v, k_scale, v_scale)
         self.ctx, self.k, self.v, self.k_scale, self.v_scale = ctx, k, v, k_scale, v_scale
         self.num_blocks, self.kv_heads, self.block_size, self.head_dim = blocks, heads, block_size, dim
-        self._c = _Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, block_size, heads,
-                         dim)
-        self._p = C.byref(self._c)
+        self._c = _CACHE.pack(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, block_size,
+                              heads, dim)
 
     @classmethod
     def create(cls, ctx, num_blocks, block_size, kv_heads, head_dim):
@@ -215,35 +208,45 @@ class KvCache:
                    torch.empty(shape, dtype=torch.float32, device=dev),
                    torch.empty(shape, dtype=torch.float32, device=dev))
 
-    def _heads(self, t, heads, what):
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim or t.stride(2) != 1:
-            _refuse(INVALID_ARGUMENT, f"{what}: rows x {heads} x {self.head_dim}, contiguous dimensions")
+    def _heads(self, t, rows, heads, what):
+        """Row and head strides of rows x heads x head_dim on the device."""
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 3 or shape[0] != rows or shape[1] != heads or shape[2] != self.head_dim or stride[2] != 1:
+            _refuse(INVALID_ARGUMENT, f"{what}: {rows} x {heads} x {self.head_dim}, contiguous dimensions")
+        if t.get_device() != self.ctx.device:
+            _refuse(INVALID_ARGUMENT, f"{what} must be on the context's device")
+        return stride[0], stride[1]
 
     def append(self, k, v, slots):
         """Rows k and v (rows x kv_heads x head_dim; any row and head strides)
         at slots (hh_kv_append)."""
-        self._heads(k, self.kv_heads, "append: k")
-        self._heads(v, self.kv_heads, "append: v")
-        dt = _half(k, "append")
-        if v.dtype != k.dtype or v.shape[0] != k.shape[0] or slots.dim() != 1 or slots.shape[0] != k.shape[0]:
+        ctx, rows, dt = self.ctx, k.shape[0], _HALF.get(k.dtype)
+        if dt is None:
+            _refuse(UNSUPPORTED, f"append: {k.dtype} (float16 or bfloat16)")
+        tk, hk = self._heads(k, rows, self.kv_heads, "append: k")
+        tv, hv = self._heads(v, rows, self.kv_heads, "append: v")
+        if v.dtype is not k.dtype or slots.dim() != 1 or slots.shape[0] != rows:
             _refuse(INVALID_ARGUMENT, "append: k, v and slots have the same rows, k and v the same type")
         _ints("append", slots)
-        _on(self.ctx, "append", k, v, slots)
-        _check(_append(self.ctx.handle, self._p, k.data_ptr(), v.data_ptr(), dt, k.stride(0), k.stride(1), v.stride(0),
-                       v.stride(1), slots.data_ptr(), k.shape[0], _stream(self.ctx)), "hh_kv_append")
+        _on(ctx.device, "append", slots)
+        rc = _append(ctx.handle, self._c, k.data_ptr(), v.data_ptr(), dt, tk, hk, tv, hv, slots.data_ptr(), rows,
+                     _stream(ctx.device))
+        if rc:
+            _check(rc, "hh_kv_append")
 
     def read(self, blocks, dtype=torch.float32):
         """The values of whole blocks (int32 ids): k and v as n x block_size x
         kv_heads x head_dim of dtype (hh_kv_read)."""
-        if dtype not in _CODE:
+        ctx, code = self.ctx, _CODE.get(dtype)
+        if code is None:
             _refuse(UNSUPPORTED, f"read: {dtype}")
         _ints("read", blocks)
-        _on(self.ctx, "read", blocks)
+        _on(ctx.device, "read", blocks)
         n = blocks.numel()
-        k, v = torch.empty((2, n, self.block_size, self.kv_heads, self.head_dim), dtype=dtype,
-                           device=self.k.device).unbind(0)
-        _check(_read(self.ctx.handle, self._p, blocks.data_ptr(), n, _CODE[dtype], k.data_ptr(), v.data_ptr(),
-                     _stream(self.ctx)), "hh_kv_read")
+        k, v = self.k_scale.new_empty((2, n, self.block_size, self.kv_heads, self.head_dim), dtype=dtype).unbind(0)
+        rc = _read(ctx.handle, self._c, blocks.data_ptr(), n, code, k.data_ptr(), v.data_ptr(), _stream(ctx.device))
+        if rc:
+            _check(rc, "hh_kv_read")
         return k, v
 
     def attention(self, q, table, start, kv_len, max_q=None, max_kv=None, scale=None, out=None):
@@ -252,29 +255,36 @@ class KvCache:
         width), start and kv_len as kv_plan leaves them.  max_q and max_kv
         bound a request's rows and tokens (default: q's rows, the table's
         width); scale defaults to head_dim ** -0.5."""
-        dt = _half(q, "attention")
-        if q.dim() != 3:
+        ctx, shape, dt = self.ctx, q.shape, _HALF.get(q.dtype)
+        if dt is None:
+            _refuse(UNSUPPORTED, f"attention: {q.dtype} (float16 or bfloat16)")
+        if len(shape) != 3:
             _refuse(INVALID_ARGUMENT, "attention: q is rows x q_heads x head_dim")
-        tokens, heads = q.shape[0], q.shape[1]
-        self._heads(q, heads, "attention: q")
+        tokens, heads = shape[0], shape[1]
+        tq, hq = self._heads(q, tokens, heads, "attention: q")
         if out is None:
-            out = torch.empty((tokens, heads, self.head_dim), dtype=q.dtype, device=q.device)
+            out = q.new_empty((tokens, heads, self.head_dim))
+            to, ho = heads * self.head_dim, self.head_dim
         else:
-            self._heads(out, heads, "attention: out")
-            if out.dtype != q.dtype or out.shape[0] != tokens:
+            to, ho = self._heads(out, tokens, heads, "attention: out")
+            if out.dtype is not q.dtype:
                 _refuse(INVALID_ARGUMENT, "attention: out is like q")
-        requests = kv_len.shape[0]
         _ints("attention", start, kv_len)
-        if (table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != requests
-                or (table.shape[1] > 1 and table.stride(1) != 1) or start.numel() != requests + 1):
+        requests, tshape, tstride = kv_len.shape[0], table.shape, table.stride()
+        if (table.dtype != torch.int32 or len(tshape) != 2 or tshape[0] != requests or (tshape[1] > 1 and tstride[1] != 1)
+                or start.numel() != requests + 1):
             _refuse(INVALID_ARGUMENT, "attention: table requests x width, start requests + 1")
-        _on(self.ctx, "attention", q, table, start, kv_len, out)
-        width = table.shape[1]
-        a = _AttentionArgs(q.data_ptr(), out.data_ptr(), table.data_ptr(), start.data_ptr(), kv_len.data_ptr(),
-                           q.stride(0), q.stride(1), out.stride(0), out.stride(1),
-                           table.stride(0) if requests > 1 else width, requests, tokens, heads, width,
-                           tokens if max_q is None else int(max_q),
-                           width * self.block_size if max_kv is None else int(max_kv),
-                           self.head_dim ** -0.5 if scale is None else float(scale), dt)
-        _check(_attention(self.ctx.handle, self._p, C.byref(a), _stream(self.ctx)), "hh_kv_attention")
+        _on(ctx.device, "attention", table, start, kv_len)
+        width = tshape[1]
+        try:
+            args = _ATTENTION.pack(
+                q.data_ptr(), out.data_ptr(), table.data_ptr(), start.data_ptr(), kv_len.data_ptr(), tq, hq, to, ho,
+                tstride[0] if requests > 1 else width, requests, tokens, heads, width, tokens if max_q is None else max_q,
+                min(width * self.block_size, 1 << 30) if max_kv is None else max_kv,
+                self.head_dim ** -0.5 if scale is None else scale, dt)
+        except struct.error:
+            _refuse(INVALID_ARGUMENT, "attention: max_q, max_kv and scale are numbers in range")
+        rc = _attention(ctx.handle, self._c, args, _stream(ctx.device))
+        if rc:
+            _check(rc, "hh_kv_attention")
         return out
