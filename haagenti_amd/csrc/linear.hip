@@ -44,23 +44,6 @@ __device__ __forceinline__ u32x4 row8(const uint16_t *row, uint32_t at, uint32_t
     return v;
 }
 
-// The 8 nibbles of w as 16 + nibble, in order.
-template <int DT>
-__device__ __forceinline__ u32x4 nibbles_to_half(uint32_t w) {
-    // f16: 16 is 0x4c00 with 6 bits below the units, bf16: 0x4180 with 3
-    constexpr uint32_t magic = DT == HH_BF16 ? 0x41804180u : 0x4c004c00u;
-    constexpr int up = DT == HH_BF16 ? 3 : 6;
-    constexpr uint32_t mask = 0x000f000fu << up;
-    // a value pair 2 i, 2 i + 1 is a byte: spread it to the halves first
-    u32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t b = (w >> (8 * i)) & 255u;
-        v[i] = (((b | b << 12) << up) & mask) | magic;
-    }
-    return v;
-}
-
 __device__ __forceinline__ float act_of(float z, int act) {
     switch (act) {
         case HH_ACT_RELU: return fmaxf(z, 0.0f) + (z != z ? z : 0.0f);
@@ -75,44 +58,57 @@ __device__ __forceinline__ float act_of(float z, int act) {
     }
 }
 
+// What the epilogue of outputs n .. n + 3 of row m reads, where 4 values move
+// at a time.
+struct Side {
+    u32x2 bias, mul, res;
+};
+__device__ __forceinline__ bool whole4(const LinearArgs &p, uint32_t n) { return p.vec && n + 4 <= p.a.n; }
+__device__ __forceinline__ Side load_side(const LinearArgs &p, uint32_t m, uint32_t n) {
+    const hh_linear_args &a = p.a;
+    Side s = {{0, 0}, {0, 0}, {0, 0}};
+    if (a.d_bias) s.bias = *reinterpret_cast<const u32x2 *>(reinterpret_cast<const uint16_t *>(a.d_bias) + n);
+    if (a.d_mul) s.mul = *reinterpret_cast<const u32x2 *>(reinterpret_cast<const uint16_t *>(a.d_mul) + m * a.mul_stride + n);
+    if (a.d_residual)
+        s.res = *reinterpret_cast<const u32x2 *>(reinterpret_cast<const uint16_t *>(a.d_residual) + m * a.residual_stride + n);
+    return s;
+}
+template <int DT, int YT>
+__device__ __forceinline__ void finish_whole4(const LinearArgs &p, uint32_t m, uint32_t n, const f32x4 &sum, const Side &s) {
+    const hh_linear_args &a = p.a;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int sh = 16 * (i & 1);
+        v[i] = sum[i];
+        if (a.d_bias) v[i] += half_to_f32<DT>((s.bias[i >> 1] >> sh) & 0xffffu);
+        v[i] = act_of(v[i], a.activation);
+        if (a.d_mul) v[i] *= half_to_f32<DT>((s.mul[i >> 1] >> sh) & 0xffffu);
+        if (a.d_residual) v[i] += half_to_f32<DT>((s.res[i >> 1] >> sh) & 0xffffu);
+    }
+    if constexpr (YT == HH_F32) {
+        *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.d_y) + m * a.y_stride + n) = f32x4{v[0], v[1], v[2], v[3]};
+    } else {
+        *reinterpret_cast<u32x2 *>(reinterpret_cast<uint16_t *>(a.d_y) + m * a.y_stride + n) =
+            u32x2{f32_to_half<YT>(v[0]) | f32_to_half<YT>(v[1]) << 16, f32_to_half<YT>(v[2]) | f32_to_half<YT>(v[3]) << 16};
+    }
+}
+
 // Writes outputs n .. n + 3 of row m from their sums.
 template <int DT, int YT>
 __device__ __forceinline__ void finish4(const LinearArgs &p, uint32_t m, uint32_t n, const f32x4 &sum) {
     const hh_linear_args &a = p.a;
-    const uint16_t *bias = reinterpret_cast<const uint16_t *>(a.d_bias);
-    const uint16_t *mul = reinterpret_cast<const uint16_t *>(a.d_mul) + m * a.mul_stride + n;
-    const uint16_t *res = reinterpret_cast<const uint16_t *>(a.d_residual) + m * a.residual_stride + n;
-    float v[4];
-    if (p.vec && n + 4 <= a.n) {
-        u32x2 b = {0, 0}, c = {0, 0}, d = {0, 0};
-        if (a.d_bias) b = *reinterpret_cast<const u32x2 *>(bias + n);
-        if (a.d_mul) c = *reinterpret_cast<const u32x2 *>(mul);
-        if (a.d_residual) d = *reinterpret_cast<const u32x2 *>(res);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int sh = 16 * (i & 1);
-            v[i] = sum[i];
-            if (a.d_bias) v[i] += half_to_f32<DT>((b[i >> 1] >> sh) & 0xffffu);
-            v[i] = act_of(v[i], a.activation);
-            if (a.d_mul) v[i] *= half_to_f32<DT>((c[i >> 1] >> sh) & 0xffffu);
-            if (a.d_residual) v[i] += half_to_f32<DT>((d[i >> 1] >> sh) & 0xffffu);
-        }
-        if constexpr (YT == HH_F32) {
-            *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.d_y) + m * a.y_stride + n) = f32x4{v[0], v[1], v[2], v[3]};
-        } else {
-            *reinterpret_cast<u32x2 *>(reinterpret_cast<uint16_t *>(a.d_y) + m * a.y_stride + n) =
-                u32x2{f32_to_half<YT>(v[0]) | f32_to_half<YT>(v[1]) << 16, f32_to_half<YT>(v[2]) | f32_to_half<YT>(v[3]) << 16};
-        }
+    if (whole4(p, n)) {
+        finish_whole4<DT, YT>(p, m, n, sum, load_side(p, m, n));
         return;
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (n + i >= a.n) break;
-        float z = sum[i];
-        if (a.d_bias) z += half_to_f32<DT>(bias[n + i]);
+#pragma unroll 1
+    for (uint32_t i = 0; i < 4 && n + i < a.n; i++) {
+        float z = i == 0 ? sum[0] : i == 1 ? sum[1] : i == 2 ? sum[2] : sum[3];
+        if (a.d_bias) z += half_to_f32<DT>(reinterpret_cast<const uint16_t *>(a.d_bias)[n + i]);
         z = act_of(z, a.activation);
-        if (a.d_mul) z *= half_to_f32<DT>(mul[i]);
-        if (a.d_residual) z += half_to_f32<DT>(res[i]);
+        if (a.d_mul) z *= half_to_f32<DT>(reinterpret_cast<const uint16_t *>(a.d_mul)[m * a.mul_stride + n + i]);
+        if (a.d_residual) z += half_to_f32<DT>(reinterpret_cast<const uint16_t *>(a.d_residual)[m * a.residual_stride + n + i]);
         if constexpr (YT == HH_F32)
             reinterpret_cast<float *>(a.d_y)[m * a.y_stride + n + i] = z;
         else
@@ -268,34 +264,35 @@ __global__ __launch_bounds__(512) void linear_rows_kernel(const LinearArgs p) {
     }
 }
 
-// ---------------------------------------------------------------- many rows
+// ---------------------------------------------------------------- many rows, any layout
 //
-// Tiles of 128 n x 128 m, 32 deep, through LDS; 4 waves of 64 x 64.  INT4
+// Tiles of S n x S m, 32 deep, through registers and LDS; 4 waves.  INT4
 // buffers whose groups cross rows (k not a multiple of 32) give W as the sum
 // of two bf16 numbers (4 + 11 bits of a value fit 8 + 8) and x, if f16, too
 // (11 bits); the products of the parts are exact up to the f32 sums.
 
-template <int DT, int YT, int MODE>
+template <int DT, int YT, int MODE, int S>
 __global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p) {
+    constexpr int H = S / 2, F = H / 16, P = S / 64;  // a wave's side, its tiles, pieces of 8 values per thread
     constexpr int PITCH = 40;  // halves: rows an odd number of 16-byte units apart
     constexpr int WP = MODE == kInt4Any ? 2 : 1, XP = MODE == kInt4Any && DT == HH_F16 ? 2 : 1;
     constexpr int MT = MODE == kInt4Any ? (int)HH_BF16 : DT;
-    __shared__ __align__(16) uint16_t lw[WP][128 * PITCH], lx[XP][128 * PITCH];
-    __shared__ float ls[128];
+    __shared__ __align__(16) uint16_t lw[WP][S * PITCH], lx[XP][S * PITCH];
+    __shared__ __align__(16) float ls[S];
     const hh_linear_args &a = p.a;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r = lane & 15u, g = lane >> 4;
-    const uint32_t n0 = blockIdx.x * 128, m0 = blockIdx.y * 128, wn = (wave & 1u) * 64, wm = (wave >> 1) * 64;
-    f32x4 acc[4][4];
+    const uint32_t n0 = blockIdx.x * S, m0 = blockIdx.y * S, wn = (wave & 1u) * H, wm = (wave >> 1) * H;
+    f32x4 acc[F][F];
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < F; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0, 0, 0, 0};
+        for (int j = 0; j < F; j++) acc[i][j] = f32x4{0, 0, 0, 0};
 
-    u32x4 wv[2][WP], xv[2][XP];
+    u32x4 wv[P][WP], xv[P][XP];
     float sv = 0.0f;
     auto fetch = [&](uint32_t k0) {
 #pragma unroll
-        for (uint32_t j = 0; j < 2; j++) {
+        for (uint32_t j = 0; j < P; j++) {
             const uint32_t row = (j * 256 + tid) >> 2, k = k0 + (tid & 3u) * 8;
             const uint32_t n = n0 + row, m = m0 + row;
 #pragma unroll
@@ -305,7 +302,7 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p) {
             if (m < a.m) {
                 const u32x4 x = row8(reinterpret_cast<const uint16_t *>(a.d_x) + (uint64_t)m * a.x_stride, k, a.k);
                 if constexpr (XP == 1) {
-                    xv[j][0] = x;
+                    xv[j][0] = MODE == kInt4 ? order_0415(x) : x;
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
@@ -324,7 +321,7 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p) {
                 } else if constexpr (MODE == kInt4) {
                     typedef uint32_t u32_any __attribute__((aligned(1)));
                     if (k < a.k)
-                        wv[j][0] = nibbles_to_half<DT>(
+                        wv[j][0] = nibbles_0415<DT>(
                             *reinterpret_cast<const u32_any *>(p.nibbles + ((uint64_t)n * a.k + k) / 2));
                 } else {
 #pragma unroll
@@ -342,7 +339,7 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p) {
             }
         }
         if constexpr (MODE == kInt4) {
-            if (tid < 128)
+            if (tid < S)
                 sv = n0 + tid < a.n && k0 < a.k
                          ? f16_bits_to_f32(p.scales[((uint64_t)(n0 + tid) * a.k + k0) / 32])
                          : 0.0f;
@@ -353,37 +350,36 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p) {
     for (uint32_t k0 = 0; k0 < a.k; k0 += 32) {
         __syncthreads();
 #pragma unroll
-        for (uint32_t j = 0; j < 2; j++) {
+        for (uint32_t j = 0; j < P; j++) {
             const uint32_t at = ((j * 256 + tid) >> 2) * PITCH + (tid & 3u) * 8;
 #pragma unroll
             for (int q = 0; q < WP; q++) *reinterpret_cast<u32x4 *>(&lw[q][at]) = wv[j][q];
 #pragma unroll
             for (int q = 0; q < XP; q++) *reinterpret_cast<u32x4 *>(&lx[q][at]) = xv[j][q];
         }
-        if (MODE == kInt4 && tid < 128) ls[tid] = sv;
+        if (MODE == kInt4 && tid < S) ls[tid] = sv;
         __syncthreads();
         if (k0 + 32 < a.k) fetch(k0 + 32);
 #pragma unroll
         for (int qx = 0; qx < XP; qx++) {
-            u32x4 x[4];
-            f32x4 corr[4];
+            u32x4 x[F];
+            f32x4 corr[F];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
+            for (int j = 0; j < F; j++) {
                 x[j] = *reinterpret_cast<const u32x4 *>(&lx[qx][(wm + 16 * j + r) * PITCH + 8 * g]);
                 if constexpr (MODE == kInt4) {
-                    constexpr uint32_t m24 = DT == HH_BF16 ? 0xc1c0c1c0u : 0xce00ce00u;  // -24
-                    corr[j] = mma16<DT>(u32x4{m24, m24, m24, m24}, x[j], f32x4{0, 0, 0, 0});
+                    corr[j] = mma16<DT>(minus24<DT>(), x[j], f32x4{0, 0, 0, 0});
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < F; i++) {
                 f32x4 s;
                 if constexpr (MODE == kInt4) s = *reinterpret_cast<const f32x4 *>(&ls[wn + 16 * i + 4 * g]);
 #pragma unroll
                 for (int qw = 0; qw < WP; qw++) {
                     const u32x4 w = *reinterpret_cast<const u32x4 *>(&lw[qw][(wn + 16 * i + r) * PITCH + 8 * g]);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
+                    for (int j = 0; j < F; j++) {
                         if constexpr (MODE == kInt4) {
                             const f32x4 part = mma16<DT>(w, x[j], corr[j]);
 #pragma unroll
@@ -397,15 +393,195 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p) {
         }
     }
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < F; j++) {
         const uint32_t m = m0 + wm + 16 * j + r;
         if (m >= a.m) continue;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < F; i++) {
             const uint32_t n = n0 + wn + 16 * i + 4 * g;
             if (n < a.n) finish4<DT, YT>(p, m, n, acc[i][j]);
         }
     }
+}
+
+// ---------------------------------------------------------------- many rows, aligned
+//
+// Tiles of TN n x TM m, 64 deep, copied straight to LDS, two of them in turn:
+// the next tile's copies are under way while this one is multiplied, one
+// barrier per tile.  The buffers are four arrays of their own, so that the
+// compiler sees which of them a copy writes and waits for it at the barrier
+// only.  A row of 64 values is 8 pieces of 16 bytes; row r's piece c lies at
+// place c ^ (r & 7), so that rows read together lie in different banks (the
+// copy's lanes choose their source piece accordingly: LDS is written in lane
+// order).  Rows past the matrices repeat the last one.  Bound by LDS and the
+// matrix pipes alike: at 256 x 256 a tile's reads (192 KiB by 8 waves of
+// 128 x 64) and copies (64 KiB) take as long as its products.
+//
+// Tiles are numbered down the rows of x, and consecutive ones go to one XCD,
+// whose L2 then serves W's panel to all of them.
+
+template <int ROWS, int T>
+__device__ __forceinline__ void tile_offsets(uint32_t stride, uint32_t rows, uint32_t (&off)[ROWS * 8 / T]) {
+#pragma unroll
+    for (int j = 0; j < ROWS * 8 / T; j++) {
+        const uint32_t slot = j * T + threadIdx.x, row = slot >> 3, piece = (slot & 7u) ^ (row & 7u);
+        off[j] = (min(row, rows - 1) * stride + piece * 8) * 2;
+    }
+}
+template <int ROWS, int T, typename Source>
+__device__ __forceinline__ void tile_copy(const Source &from, uint32_t at, const uint32_t (&off)[ROWS * 8 / T], uint16_t *lds,
+                                          uint32_t wave) {
+#if defined(__HIP_DEVICE_COMPILE__)  // 16-byte copies exist in the device's pass only
+#pragma unroll
+    for (int j = 0; j < ROWS * 8 / T; j++)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            from, (__attribute__((address_space(3))) void *)(lds + (j * T + wave * 64) * 8), 16, off[j], at, 0, 0);
+#endif
+}
+
+// Splits of k (blockIdx.y): steps of 64 each takes, sums to `partial`.
+struct Split {
+    uint32_t steps;
+    float *partial;  // [split][m][n], or null: one split, y itself
+};
+
+template <int DT, int YT, int TN, int TM, int WN, int WM>
+__global__ __launch_bounds__(64 * WN * WM) void linear_large_kernel(const LinearArgs p, const Split split) {
+    constexpr int T = 64 * WN * WM, NI = TN / WN / 16, MI = TM / WM / 16;
+    __shared__ __align__(16) uint16_t lw0[TN * 64], lw1[TN * 64], lx0[TM * 64], lx1[TM * 64];
+    const hh_linear_args &a = p.a;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t r = lane & 15u, g = lane >> 4;
+    const uint32_t mt = (a.m + TM - 1) / TM, share = gridDim.x / 8, rest = gridDim.x % 8, xcd = blockIdx.x % 8;
+    const uint32_t id = xcd * share + min(xcd, rest) + blockIdx.x / 8;
+    const uint32_t n0 = id / mt * TN, m0 = id % mt * TM, wn = wave % WN * (TN / WN), wm = wave / WN * (TM / WM);
+    const uint32_t k0 = blockIdx.y * split.steps * 64, k1 = min(a.k, k0 + split.steps * 64);
+    f32x4 acc[NI][MI];
+#pragma unroll
+    for (int i = 0; i < NI; i++)
+#pragma unroll
+        for (int j = 0; j < MI; j++) acc[i][j] = f32x4{0, 0, 0, 0};
+    uint32_t ow[TN * 8 / T], ox[TM * 8 / T];
+    tile_offsets<TN, T>((uint32_t)a.w_stride, a.n - n0, ow);
+    tile_offsets<TM, T>((uint32_t)a.x_stride, a.m - m0, ox);
+    // offsets stay inside the matrices (rows are clamped): no size limit here
+    const auto w = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t *>(reinterpret_cast<const uint16_t *>(a.d_w) + n0 * a.w_stride), 0, 0xffffffffu, 0x00027000);
+    const auto x = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t *>(reinterpret_cast<const uint16_t *>(a.d_x) + m0 * a.x_stride), 0, 0xffffffffu, 0x00027000);
+    auto copy = [&](uint16_t *lw, uint16_t *lx, uint32_t k) {
+        tile_copy<TN, T>(w, 2 * k, ow, lw, wave);
+        tile_copy<TM, T>(x, 2 * k, ox, lx, wave);
+    };
+    auto multiply = [&](const uint16_t *lw, const uint16_t *lx) {
+#pragma unroll
+        for (uint32_t f = 0; f < 2; f++) {
+            const uint32_t piece = ((g + 4 * f) ^ (r & 7u)) * 8;
+            u32x4 wf[NI], xf[MI];
+#pragma unroll
+            for (int j = 0; j < MI; j++) xf[j] = *reinterpret_cast<const u32x4 *>(&lx[(wm + 16 * j + r) * 64 + piece]);
+#pragma unroll
+            for (int i = 0; i < NI; i++) wf[i] = *reinterpret_cast<const u32x4 *>(&lw[(wn + 16 * i + r) * 64 + piece]);
+#pragma unroll
+            for (int i = 0; i < NI; i++)
+#pragma unroll
+                for (int j = 0; j < MI; j++) acc[i][j] = mma16<DT>(wf[i], xf[j], acc[i][j]);
+        }
+        // the first reads, then one between every two products, then the
+        // products that are left
+        constexpr int reads = 2 * (NI + MI), lead = MI + 2;
+        __builtin_amdgcn_sched_group_barrier(0x100, lead, 0);
+#pragma unroll
+        for (int i = 0; i < reads - lead; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 2 * NI * MI - 2 * (reads - lead), 0);
+    };
+    // a barrier waits for the copies into the buffers that are read after it,
+    // and for the reads of the ones that are copied to after it
+    copy(lw0, lx0, k0);
+    for (uint32_t k = k0; k < k1; k += 128) {
+        __syncthreads();
+        if (k + 64 < k1) {
+            copy(lw1, lx1, k + 64);
+        } else {
+            // an odd number of steps ends with one of zeros
+            for (uint32_t i = threadIdx.x; i < TN * 8; i += T) reinterpret_cast<u32x4 *>(lw1)[i] = u32x4{0, 0, 0, 0};
+            for (uint32_t i = threadIdx.x; i < TM * 8; i += T) reinterpret_cast<u32x4 *>(lx1)[i] = u32x4{0, 0, 0, 0};
+        }
+        multiply(lw0, lx0);
+        __syncthreads();
+        if (k + 128 < k1) copy(lw0, lx0, k + 128);
+        multiply(lw1, lx1);
+    }
+    // Sums go out by way of LDS, 16 rows x 64 columns of each wave at a time,
+    // so that a wave writes pieces of rows; a row's groups of 4 lie at q ^ row.
+    constexpr int Q = 16;
+    f32x4 *own = reinterpret_cast<f32x4 *>(TN >= TM ? lw0 : lx0) + wave * 16 * Q;
+    static_assert(WN * WM * 16 * Q * 16 <= (TN >= TM ? TN : TM) * 128, "every wave's piece fits one buffer");
+#pragma unroll
+    for (int j = 0; j < MI; j++)
+#pragma unroll
+        for (int h = 0; h < NI / 4; h++) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; i++) own[r * Q + ((4 * i + g) ^ r)] = acc[4 * h + i][j];
+            __syncthreads();
+            // what the epilogue reads first, all at once
+            Side side[4];
+            uint32_t n = n0 + wn + 64 * h + r * 4, m = m0 + wm + 16 * j + g;
+            asm volatile("" : "+v"(n), "+v"(m));  // no addresses of later pieces in registers meanwhile
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (!split.partial && m + 4 * c < a.m && whole4(p, n)) side[c] = load_side(p, m + 4 * c, n);
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+                const uint32_t row = 4 * c + g, at = m + 4 * c;
+                const f32x4 v = own[row * Q + (r ^ row)];
+                auto pick = [&](u32x2 Side::*f) {
+                    const u32x2 lo = c & 1 ? side[1].*f : side[0].*f, hi = c & 1 ? side[3].*f : side[2].*f;
+                    return c & 2 ? hi : lo;
+                };
+                const Side sd = {pick(&Side::bias), pick(&Side::mul), pick(&Side::res)};
+                if (at >= a.m || n >= a.n) continue;
+                if (split.partial) {
+                    float *to = split.partial + ((uint64_t)blockIdx.y * a.m + at) * a.n + n;
+                    if (n + 4 <= a.n && !(a.n & 3u)) {
+                        *reinterpret_cast<f32x4 *>(to) = v;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (n + e < a.n) to[e] = v[e];
+                    }
+                } else if (whole4(p, n)) {
+                    finish_whole4<DT, YT>(p, at, n, v, sd);
+                } else {
+                    finish4<DT, YT>(p, at, n, v);
+                }
+            }
+        }
+}
+
+// The splits' sums, in order, and the epilogue.
+template <int DT, int YT>
+__global__ __launch_bounds__(256) void linear_join_kernel(const LinearArgs p, const float *partial, uint32_t splits) {
+    const hh_linear_args &a = p.a;
+    const uint32_t quads = (a.n + 3) / 4, i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= quads) return;
+    const uint32_t m = blockIdx.y, n = 4 * i;
+    const float *at = partial + (uint64_t)m * a.n + n;
+    f32x4 s = {0, 0, 0, 0};
+    for (uint32_t j = 0; j < splits; j++, at += (uint64_t)a.m * a.n) {
+        if (!(a.n & 3u)) {
+            s += *reinterpret_cast<const f32x4 *>(at);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (n + e < a.n) s[e] += at[e];
+        }
+    }
+    finish4<DT, YT>(p, m, n, s);
 }
 
 template <int DT, int YT, int MT, bool INT4>
@@ -418,23 +594,90 @@ hipError_t launch_rows(const LinearArgs &p, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <int DT, int YT>
-hipError_t launch_linear(const LinearArgs &p, hipStream_t s) {
-    const hh_linear_args &a = p.a;
-    if (a.m <= 64 && (a.w_dtype != HH_INT4 || a.k % 32 == 0)) {
-        const int rows = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4;
-        return a.w_dtype == HH_INT4 ? (rows == 1   ? launch_rows<DT, YT, 1, true>(p, s)
-                                       : rows == 2 ? launch_rows<DT, YT, 2, true>(p, s)
-                                                   : launch_rows<DT, YT, 4, true>(p, s))
-                                    : (rows == 1   ? launch_rows<DT, YT, 1, false>(p, s)
-                                       : rows == 2 ? launch_rows<DT, YT, 2, false>(p, s)
-                                                   : launch_rows<DT, YT, 4, false>(p, s));
-    }
-    auto kernel = a.w_dtype != HH_INT4 ? linear_tile_kernel<DT, YT, kHalf>
-                  : a.k % 32 == 0      ? linear_tile_kernel<DT, YT, kInt4>
-                                       : linear_tile_kernel<DT, YT, kInt4Any>;
-    hipLaunchKernelGGL(kernel, dim3((a.n + 127) / 128, (a.m + 127) / 128), dim3(256), 0, s, p);
+template <int DT, int YT, int TN, int TM, int WN, int WM>
+void launch_tiles(const LinearArgs &p, const Split &split, uint32_t splits, hipStream_t s) {
+    const uint32_t tiles = ((p.a.n + TN - 1) / TN) * ((p.a.m + TM - 1) / TM);
+    hipLaunchKernelGGL((linear_large_kernel<DT, YT, TN, TM, WN, WM>), dim3(tiles, splits), dim3(64 * WN * WM), 0, s, p, split);
+}
+
+// Tile and splits of k for the aligned kernel: the least of an estimate in
+// microseconds.  Measured per 64 columns of k (all CUs busy): 1.65 for a
+// 256 x 256 tile and 1.0 for 256 x 128 and 128 x 256 (one workgroup to a CU),
+// 1.13 for two of 128 x 128 to a CU and 0.67 for one; 4 for a tile's start
+// and end; the splits' sums are written and read at 4 TB/s and joined by one
+// more launch.
+struct LargePlan {
+    int shape;
+    uint32_t splits, steps;
+};
+inline LargePlan plan_large(const hh_linear_args &a, int cus) {
+    static constexpr struct {
+        uint32_t n, m, per_cu;
+        double us, alone;
+    } shapes[] = {{256, 256, 1, 1.65, 1.65}, {256, 128, 1, 1.0, 1.0}, {128, 256, 1, 1.0, 1.0}, {128, 128, 2, 1.13, 0.67}};
+    LargePlan best = {0, 1, 0};
+    double least = 1e30;
+    const uint32_t steps = a.k / 64;
+    for (int i = 0; i < 4; i++)
+        for (uint32_t want = 1; want <= 16 && want <= steps; want *= 2) {
+            const uint32_t each = (steps + want - 1) / want, splits = (steps + each - 1) / each;
+            const uint64_t tiles = (uint64_t)((a.n + shapes[i].n - 1) / shapes[i].n) * ((a.m + shapes[i].m - 1) / shapes[i].m);
+            const uint64_t slots = (uint64_t)cus * shapes[i].per_cu, work = tiles * splits;
+            const double step = work <= (uint64_t)cus ? shapes[i].alone : shapes[i].us;
+            double us = (double)((work + slots - 1) / slots) * (step * each + 4.0);
+            if (splits > 1) us += 4.0 + (double)a.m * a.n * 8.0 * splits / 4e6;
+            if (us < least) least = us, best = {i, splits, each};
+        }
+    return best;
+}
+
+template <int DT, int YT, int MODE>
+hipError_t launch_any(const LinearArgs &p, int cus, hipStream_t s) {
+    const uint32_t n = p.a.n, m = p.a.m;
+    // tiles of 64 where those of 128 leave CUs without one
+    if ((uint64_t)((n + 127) / 128) * ((m + 127) / 128) >= (uint64_t)cus)
+        hipLaunchKernelGGL((linear_tile_kernel<DT, YT, MODE, 128>), dim3((n + 127) / 128, (m + 127) / 128), dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((linear_tile_kernel<DT, YT, MODE, 64>), dim3((n + 63) / 64, (m + 63) / 64), dim3(256), 0, s, p);
     return hipGetLastError();
+}
+
+template <int DT, int YT>
+int32_t launch_linear(hh_context *ctx, const LinearArgs &p, hipStream_t s) {
+    const hh_linear_args &a = p.a;
+    const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
+    const bool int4 = a.w_dtype == HH_INT4;
+    if (int4 && a.k % 32) return from_hip(launch_any<DT, YT, kInt4Any>(p, cus, s));
+    if (a.m <= 64) {
+        const int rows = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4;
+        return from_hip(int4 ? (rows == 1   ? launch_rows<DT, YT, 1, true>(p, s)
+                                : rows == 2 ? launch_rows<DT, YT, 2, true>(p, s)
+                                            : launch_rows<DT, YT, 4, true>(p, s))
+                             : (rows == 1   ? launch_rows<DT, YT, 1, false>(p, s)
+                                : rows == 2 ? launch_rows<DT, YT, 2, false>(p, s)
+                                            : launch_rows<DT, YT, 4, false>(p, s)));
+    }
+    if (int4) return from_hip(launch_any<DT, YT, kInt4>(p, cus, s));
+    const bool aligned = !(((uintptr_t)a.d_x | (uintptr_t)a.d_w) & 15u) && !((a.x_stride | a.w_stride) & 7u) &&
+                         a.k % 64 == 0 && a.k && a.x_stride < 1u << 22 && a.w_stride < 1u << 22;  // offsets in a tile: 32 bits
+    if (!aligned) return from_hip(launch_any<DT, YT, kHalf>(p, cus, s));
+    const LargePlan plan = plan_large(a, cus);
+    Split split = {plan.steps, nullptr};
+    if (plan.splits > 1) {
+        const int32_t rc = ensure_scratch(ctx, (size_t)plan.splits * a.m * a.n * sizeof(float));
+        if (rc != HH_OK) return rc;
+        split.partial = reinterpret_cast<float *>(ctx->d_scratch);
+    }
+    switch (plan.shape) {
+        case 0: launch_tiles<DT, YT, 256, 256, 2, 4>(p, split, plan.splits, s); break;
+        case 1: launch_tiles<DT, YT, 256, 128, 4, 2>(p, split, plan.splits, s); break;
+        case 2: launch_tiles<DT, YT, 128, 256, 2, 4>(p, split, plan.splits, s); break;
+        default: launch_tiles<DT, YT, 128, 128, 2, 2>(p, split, plan.splits, s); break;
+    }
+    if (split.partial)
+        hipLaunchKernelGGL((linear_join_kernel<DT, YT>), dim3(((a.n + 3) / 4 + 255) / 256, a.m), dim3(256), 0, s, p,
+                           split.partial, plan.splits);
+    return from_hip(hipGetLastError());
 }
 
 }  // namespace
@@ -470,10 +713,8 @@ extern "C" int32_t hh_linear(hh_context *ctx, const hh_linear_args *a, void *str
     hh::DeviceGuard guard(ctx->device);
     if (guard.status() != hipSuccess) return hh::from_hip(guard.status());
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    hipError_t e;
     if (a->dtype == HH_BF16)
-        e = a->y_dtype == HH_F32 ? hh::launch_linear<HH_BF16, HH_F32>(p, s) : hh::launch_linear<HH_BF16, HH_BF16>(p, s);
-    else
-        e = a->y_dtype == HH_F32 ? hh::launch_linear<HH_F16, HH_F32>(p, s) : hh::launch_linear<HH_F16, HH_F16>(p, s);
-    return hh::from_hip(e);
+        return a->y_dtype == HH_F32 ? hh::launch_linear<HH_BF16, HH_F32>(ctx, p, s)
+                                    : hh::launch_linear<HH_BF16, HH_BF16>(ctx, p, s);
+    return a->y_dtype == HH_F32 ? hh::launch_linear<HH_F16, HH_F32>(ctx, p, s) : hh::launch_linear<HH_F16, HH_F16>(ctx, p, s);
 }
