@@ -118,9 +118,9 @@ __device__ __forceinline__ void finish4(const LinearArgs &p, uint32_t m, uint32_
 
 // ---------------------------------------------------------------- few rows
 //
-// Bound by reading W once.  A workgroup takes 16 NT rows of W; its 8 waves
-// take every eighth 128 columns of them, straight to registers (the next 128
-// on their way while these are used), and join their sums in LDS.  x (at most
+// Bound by reading W once.  A workgroup takes 16 NT rows of W; its KW
+// waves take every KW-th 128 columns of them, straight to registers (the next
+// ones on their way while these are used), and join their sums in LDS.  x (at most
 // 16 MT rows) comes from L1 / L2; its row is the products' first operand, so
 // a lane's sums belong to one row of W and have one scale.
 //
@@ -159,16 +159,28 @@ __device__ __forceinline__ u32x4 minus24() {
     return u32x4{v, v, v, v};
 }
 
-template <int DT, int YT, int MT, int NT, bool INT4>
-__global__ __launch_bounds__(512) void linear_rows_kernel(const LinearArgs p) {
-    constexpr int W = INT4 ? 1 : 4;  // loads of 16 bytes per lane and 128 columns
-    __shared__ __align__(16) float part[8][16 * MT][20];
+template <int DT, int YT, int MT, int NT, int KW, bool INT4>
+__global__ __launch_bounds__(64 * KW) void linear_rows_kernel(const LinearArgs p) {
+    constexpr uint32_t STEP = 128 * KW;                       // columns between a wave's 128s
+    constexpr int W = INT4 ? 1 : 4;                           // loads of 16 bytes per lane and 128 columns
+    constexpr int AHEAD = 2;       // 128s of W in registers, one in use
+    constexpr bool XA = MT <= 2;                              // x's values one 128 ahead, where registers allow
+    __shared__ __align__(16) float part[KW][16 * MT][20];
     const hh_linear_args &a = p.a;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = lane & 15u, g = lane >> 4;
-    const uint32_t n0 = blockIdx.x * (16 * NT);
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t r = lane & 15u, g = lane >> 4, n0 = blockIdx.x * (16 * NT);
     uint64_t row[NT];
 #pragma unroll
     for (int j = 0; j < NT; j++) row[j] = min(n0 + 16 * j + r, a.n - 1);
+    // INT4: the lane's group of a row's first four, the row's scales; else
+    // its first 8 columns
+    const uint8_t *nib[NT];
+    const uint16_t *scl[NT], *w[NT];
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+        nib[j] = p.nibbles + row[j] * (a.k / 2) + g * 16, scl[j] = p.scales + row[j] * (a.k / 32);
+        w[j] = reinterpret_cast<const uint16_t *>(a.d_w) + row[j] * a.w_stride + 8 * g;
+    }
     const uint16_t *x[MT];
 #pragma unroll
     for (int t = 0; t < MT; t++)
@@ -179,71 +191,115 @@ __global__ __launch_bounds__(512) void linear_rows_kernel(const LinearArgs p) {
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[t][j] = f32x4{0, 0, 0, 0};
 
+    // W's 128s go around AHEAD sets of registers, x's around two; x's are
+    // loaded first, as loads come back in order.
     struct Cols {
         u32x4 w[NT][W];
         u32x2 s[NT];
     };
     auto fetch = [&](uint32_t k, Cols &c) {
+        typedef u32x2 u32x2_any __attribute__((aligned(2)));
 #pragma unroll
         for (int j = 0; j < NT; j++) {
             if constexpr (INT4) {
-                const uint64_t at = (row[j] * a.k + k) / 32;  // in groups
-                c.w[j][0] = u32x4{0, 0, 0, 0}, c.s[j] = u32x2{0, 0};
-                if (k + 32 * g < a.k) c.w[j][0] = *reinterpret_cast<const u32x4_any *>(p.nibbles + (at + g) * 16);
-                if (k + 128 <= a.k) {
-                    typedef u32x2 u32x2_any __attribute__((aligned(2)));
-                    c.s[j] = *reinterpret_cast<const u32x2_any *>(p.scales + at);
-                } else {
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; e++)
-                        if (k + 32 * e < a.k) c.s[j][e >> 1] |= (uint32_t)p.scales[at + e] << (16 * (e & 1));
-                }
+                c.w[j][0] = *reinterpret_cast<const u32x4_any *>(nib[j] + k / 2);
+                c.s[j] = *reinterpret_cast<const u32x2_any *>(scl[j] + k / 32);
             } else {
-                const uint16_t *w = reinterpret_cast<const uint16_t *>(a.d_w) + row[j] * a.w_stride;
 #pragma unroll
-                for (uint32_t f = 0; f < 4; f++) c.w[j][f % W] = row8(w, k + 32 * f + 8 * g, a.k);
+                for (uint32_t f = 0; f < 4; f++) c.w[j][f % W] = *reinterpret_cast<const u32x4_any *>(w[j] + k + 32 * f);
             }
         }
     };
-    Cols cur, next;
-    if (wave * 128 < a.k) fetch(wave * 128, cur);
-    for (uint32_t k = wave * 128; k < a.k; k += 1024) {
-        if (k + 1024 < a.k) fetch(k + 1024, next);
+    auto fetch_x = [&](uint32_t k, u32x4 (&v)[MT][4]) {
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (uint32_t f = 0; f < 4; f++) v[t][f] = *reinterpret_cast<const u32x4_any *>(x[t] + k + 32 * f + 8 * g);
+    };
+    // one group of 32 columns: word(j) and scale(j) of W's rows in INT4
+    auto group = [&](const u32x4 (&xu)[MT], auto word, auto scale) {
+        u32x4 xf[MT];
+        f32x4 corr[MT];
+#pragma unroll
+        for (int t = 0; t < MT; t++) {
+            xf[t] = order_0415(xu[t]);
+            corr[t] = mma16<DT>(xf[t], minus24<DT>(), f32x4{0, 0, 0, 0});
+        }
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const u32x4 v = nibbles_0415<DT>(word(j));
+            const float s = half_to_f32<HH_F16>(scale(j));
+#pragma unroll
+            for (int t = 0; t < MT; t++) {
+                const f32x4 q = mma16<DT>(xf[t], v, corr[t]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[t][j][e] = fmaf(s, q[e], acc[t][j][e]);
+            }
+        }
+    };
+    auto multiply = [&](Cols &c, const u32x4 (&xu)[MT][4]) {
         if constexpr (INT4) {
 #pragma unroll
-            for (int j = 0; j < NT; j++) cur.w[j][0] = groups_across(cur.w[j][0]);
+            for (int j = 0; j < NT; j++) c.w[j][0] = groups_across(c.w[j][0]);
         }
 #pragma unroll
         for (uint32_t f = 0; f < 4; f++) {
             u32x4 xf[MT];
 #pragma unroll
-            for (int t = 0; t < MT; t++) xf[t] = row8(x[t], k + 32 * f + 8 * g, a.k);
+            for (int t = 0; t < MT; t++) xf[t] = xu[t][f];
             if constexpr (INT4) {
-                f32x4 corr[MT];
-#pragma unroll
-                for (int t = 0; t < MT; t++) {
-                    xf[t] = order_0415(xf[t]);
-                    corr[t] = mma16<DT>(xf[t], minus24<DT>(), f32x4{0, 0, 0, 0});
-                }
-#pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    const u32x4 w = nibbles_0415<DT>(cur.w[j][0][f]);
-                    const float s = half_to_f32<HH_F16>((cur.s[j][f >> 1] >> (16 * (f & 1))) & 0xffffu);
-#pragma unroll
-                    for (int t = 0; t < MT; t++) {
-                        const f32x4 q = mma16<DT>(xf[t], w, corr[t]);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) acc[t][j][e] = fmaf(s, q[e], acc[t][j][e]);
-                    }
-                }
+                group(xf, [&](int j) { return c.w[j][0][f]; },
+                      [&](int j) { return (c.s[j][f >> 1] >> (16 * (f & 1))) & 0xffffu; });
             } else {
 #pragma unroll
                 for (int j = 0; j < NT; j++)
 #pragma unroll
-                    for (int t = 0; t < MT; t++) acc[t][j] = mma16<DT>(xf[t], cur.w[j][f % W], acc[t][j]);
+                    for (int t = 0; t < MT; t++) acc[t][j] = mma16<DT>(xf[t], c.w[j][f % W], acc[t][j]);
             }
         }
-        cur = next;
+    };
+    const uint32_t whole = a.k / 128 * 128;
+    if (wave * 128 < whole) {
+        Cols cols[AHEAD];
+        u32x4 xv[2][MT][4];
+        if (XA) fetch_x(wave * 128, xv[0]);
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) if (wave * 128 + u * STEP < whole) fetch(wave * 128 + u * STEP, cols[u]);
+#pragma unroll 1
+        for (uint32_t k0 = wave * 128; k0 < whole; k0 += AHEAD * STEP) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++) {
+                const uint32_t k = k0 + u * STEP;
+                if (k >= whole) break;
+                if (!XA)
+                    fetch_x(k, xv[0]);
+                else if (k + STEP < whole)
+                    fetch_x(k + STEP, xv[(u + 1) & 1]);
+                multiply(cols[u], xv[XA ? u & 1 : 0]);
+                if (k + AHEAD * STEP < whole) fetch(k + AHEAD * STEP, cols[u]);
+            }
+        }
+    }
+    // what is left of the columns, 32 at a time, the next wave's turn
+    if (whole < a.k && wave == whole / 128 % KW) {
+#pragma unroll 1
+        for (uint32_t k = whole; k < a.k; k += 32) {
+            u32x4 xf[MT];
+#pragma unroll
+            for (int t = 0; t < MT; t++) xf[t] = row8(x[t], k + 8 * g, a.k);
+            if constexpr (INT4) {
+                typedef uint32_t u32_any __attribute__((aligned(2)));
+                group(xf, [&](int j) { return *reinterpret_cast<const u32_any *>(nib[j] + k / 2 + g * 4 - g * 16); },
+                      [&](int j) { return (uint32_t)scl[j][k / 32]; });
+            } else {
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const u32x4 wf = row8(w[j] - 8 * g, k + 8 * g, a.k);
+#pragma unroll
+                    for (int t = 0; t < MT; t++) acc[t][j] = mma16<DT>(xf[t], wf, acc[t][j]);
+                }
+            }
+        }
     }
 #pragma unroll
     for (int j = 0; j < NT; j++) {
@@ -253,12 +309,12 @@ __global__ __launch_bounds__(512) void linear_rows_kernel(const LinearArgs p) {
 #pragma unroll
             for (int e = 0; e < 4; e++) part[wave][16 * t + 4 * g + e][r] = acc[t][j][e];
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < 64 * MT; i += 512) {
+        for (uint32_t i = threadIdx.x; i < 64 * MT; i += 64 * KW) {
             const uint32_t m = i >> 2, n = (i & 3u) * 4, at = n0 + 16 * j + n;
             if (m >= a.m || at >= a.n) continue;
             f32x4 s = *reinterpret_cast<const f32x4 *>(&part[0][m][n]);
 #pragma unroll
-            for (int v = 1; v < 8; v++) s += *reinterpret_cast<const f32x4 *>(&part[v][m][n]);
+            for (int v = 1; v < KW; v++) s += *reinterpret_cast<const f32x4 *>(&part[v][m][n]);
             finish4<DT, YT>(p, m, at, s);
         }
     }
@@ -266,22 +322,52 @@ __global__ __launch_bounds__(512) void linear_rows_kernel(const LinearArgs p) {
 
 // ---------------------------------------------------------------- many rows, any layout
 //
-// Tiles of S n x S m, 32 deep, through registers and LDS; 4 waves.  INT4
-// buffers whose groups cross rows (k not a multiple of 32) give W as the sum
-// of two bf16 numbers (4 + 11 bits of a value fit 8 + 8) and x, if f16, too
-// (11 bits); the products of the parts are exact up to the f32 sums.
+// Tiles of S n x S m, 64 deep, through registers and LDS; 4 waves.  The next
+// 64 columns are loaded while these are multiplied.  INT4 buffers whose groups
+// cross rows (k not a multiple of 32) give W as the sum of two bf16 numbers
+// (4 + 11 bits of a value fit 8 + 8) and x, if f16, too (11 bits); the
+// products of the parts are exact up to the f32 sums.
+
+// Splits of k: steps of 64 each takes, sums to `partial`.
+struct Split {
+    uint32_t steps;
+    float *partial;  // [split][m][n], or null: one split, y itself
+};
+
+// A split's sums of outputs n .. n + 3 of row m.
+__device__ __forceinline__ void store_partial(const LinearArgs &p, const Split &split, uint32_t index, uint32_t m, uint32_t n,
+                                              const f32x4 &v) {
+    float *to = split.partial + ((uint64_t)index * p.a.m + m) * p.a.n + n;
+    if (n + 4 <= p.a.n && !(p.a.n & 3u)) {
+        *reinterpret_cast<f32x4 *>(to) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (n + e < p.a.n) to[e] = v[e];
+    }
+}
+
+// f as the sum of two bf16 numbers, e-th of 8 each; what is not finite is in
+// the first.
+__device__ __forceinline__ void split_bf16(float f, int e, u32x4 &hi, u32x4 &lo) {
+    const uint32_t h = f32_to_half<HH_BF16>(f);
+    const float rest = f - half_to_f32<HH_BF16>(h);
+    hi[e >> 1] |= h << (16 * (e & 1));
+    lo[e >> 1] |= (fabsf(rest) < __builtin_inff() ? f32_to_half<HH_BF16>(rest) : 0u) << (16 * (e & 1));
+}
 
 template <int DT, int YT, int MODE, int S>
-__global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p) {
-    constexpr int H = S / 2, F = H / 16, P = S / 64;  // a wave's side, its tiles, pieces of 8 values per thread
-    constexpr int PITCH = 40;  // halves: rows an odd number of 16-byte units apart
+__global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p, const Split split) {
+    constexpr int H = S / 2, F = H / 16, P = S / 32;  // a wave's side, its tiles, pieces of 8 values per thread
+    constexpr int PITCH = 72;                         // halves: rows an odd number of 16-byte units apart
     constexpr int WP = MODE == kInt4Any ? 2 : 1, XP = MODE == kInt4Any && DT == HH_F16 ? 2 : 1;
     constexpr int MT = MODE == kInt4Any ? (int)HH_BF16 : DT;
     __shared__ __align__(16) uint16_t lw[WP][S * PITCH], lx[XP][S * PITCH];
-    __shared__ __align__(16) float ls[S];
+    __shared__ __align__(16) float ls[2][S];
     const hh_linear_args &a = p.a;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r = lane & 15u, g = lane >> 4;
     const uint32_t n0 = blockIdx.x * S, m0 = blockIdx.y * S, wn = (wave & 1u) * H, wm = (wave >> 1) * H;
+    const uint32_t k1 = (uint32_t)min((uint64_t)a.k, (uint64_t)(blockIdx.z + 1) * split.steps * 64), kb = blockIdx.z * split.steps * 64;
     f32x4 acc[F][F];
 #pragma unroll
     for (int i = 0; i < F; i++)
@@ -289,108 +375,111 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p) {
         for (int j = 0; j < F; j++) acc[i][j] = f32x4{0, 0, 0, 0};
 
     u32x4 wv[P][WP], xv[P][XP];
-    float sv = 0.0f;
+    uint32_t sv = 0;
     auto fetch = [&](uint32_t k0) {
 #pragma unroll
         for (uint32_t j = 0; j < P; j++) {
-            const uint32_t row = (j * 256 + tid) >> 2, k = k0 + (tid & 3u) * 8;
+            const uint32_t row = (j * 256 + tid) >> 3, k = k0 + (tid & 7u) * 8;
             const uint32_t n = n0 + row, m = m0 + row;
 #pragma unroll
             for (int q = 0; q < WP; q++) wv[j][q] = u32x4{0, 0, 0, 0};
 #pragma unroll
             for (int q = 0; q < XP; q++) xv[j][q] = u32x4{0, 0, 0, 0};
-            if (m < a.m) {
-                const u32x4 x = row8(reinterpret_cast<const uint16_t *>(a.d_x) + (uint64_t)m * a.x_stride, k, a.k);
-                if constexpr (XP == 1) {
-                    xv[j][0] = MODE == kInt4 ? order_0415(x) : x;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float f = half_to_f32<DT>((x[e >> 1] >> (16 * (e & 1))) & 0xffffu);
-                        const uint32_t hi = f32_to_half<HH_BF16>(f);
-                        const float rest = f - half_to_f32<HH_BF16>(hi);
-                        xv[j][0][e >> 1] |= hi << (16 * (e & 1));
-                        // infinities and NaN are in the first part
-                        xv[j][1][e >> 1] |= (rest == rest ? f32_to_half<HH_BF16>(rest) : 0u) << (16 * (e & 1));
-                    }
-                }
-            }
+            if (m < a.m) xv[j][0] = row8(reinterpret_cast<const uint16_t *>(a.d_x) + (uint64_t)m * a.x_stride, k, k1);
             if (n < a.n) {
                 if constexpr (MODE == kHalf) {
-                    wv[j][0] = row8(reinterpret_cast<const uint16_t *>(a.d_w) + (uint64_t)n * a.w_stride, k, a.k);
+                    wv[j][0] = row8(reinterpret_cast<const uint16_t *>(a.d_w) + (uint64_t)n * a.w_stride, k, k1);
                 } else if constexpr (MODE == kInt4) {
                     typedef uint32_t u32_any __attribute__((aligned(1)));
-                    if (k < a.k)
-                        wv[j][0] = nibbles_0415<DT>(
-                            *reinterpret_cast<const u32_any *>(p.nibbles + ((uint64_t)n * a.k + k) / 2));
+                    if (k < k1) wv[j][0][0] = *reinterpret_cast<const u32_any *>(p.nibbles + ((uint64_t)n * a.k + k) / 2);
                 } else {
+                    // 8 nibbles: 4 bytes, or 5 from the middle of one; at most two groups
+                    const uint64_t i = (uint64_t)n * a.k + k;
+                    const uint32_t count = k < k1 ? min(k1 - k, 8u) : 0u, odd = (uint32_t)(i & 1);
+                    if (count) {
+                        uint64_t bytes = 0;
 #pragma unroll
-                    for (uint32_t e = 0; e < 8; e++) {
-                        if (k + e >= a.k) break;
-                        const uint64_t i = (uint64_t)n * a.k + k + e;
-                        const int q = (int)((p.nibbles[i / 2] >> (4 * (i & 1))) & 15u) - 8;
-                        const float f = (float)q * f16_bits_to_f32(p.scales[i / 32]);
-                        const uint32_t hi = f32_to_half<HH_BF16>(f);
-                        const float rest = f - half_to_f32<HH_BF16>(hi);
-                        wv[j][0][e >> 1] |= hi << (16 * (e & 1));
-                        wv[j][WP - 1][e >> 1] |= (rest == rest ? f32_to_half<HH_BF16>(rest) : 0u) << (16 * (e & 1));
-                    }
-                }
-            }
-        }
-        if constexpr (MODE == kInt4) {
-            if (tid < S)
-                sv = n0 + tid < a.n && k0 < a.k
-                         ? f16_bits_to_f32(p.scales[((uint64_t)(n0 + tid) * a.k + k0) / 32])
-                         : 0.0f;
-        }
-    };
-
-    if (a.k) fetch(0);
-    for (uint32_t k0 = 0; k0 < a.k; k0 += 32) {
-        __syncthreads();
+                        for (uint32_t e = 0; e < 5; e++)
+                            if (2 * e < count + odd) bytes |= (uint64_t)p.nibbles[i / 2 + e] << (8 * e);
+                        bytes >>= 4 * odd;
+                        const float s0 = f16_bits_to_f32(p.scales[i / 32]), s1 = f16_bits_to_f32(p.scales[(i + count - 1) / 32]);
 #pragma unroll
-        for (uint32_t j = 0; j < P; j++) {
-            const uint32_t at = ((j * 256 + tid) >> 2) * PITCH + (tid & 3u) * 8;
-#pragma unroll
-            for (int q = 0; q < WP; q++) *reinterpret_cast<u32x4 *>(&lw[q][at]) = wv[j][q];
-#pragma unroll
-            for (int q = 0; q < XP; q++) *reinterpret_cast<u32x4 *>(&lx[q][at]) = xv[j][q];
-        }
-        if (MODE == kInt4 && tid < S) ls[tid] = sv;
-        __syncthreads();
-        if (k0 + 32 < a.k) fetch(k0 + 32);
-#pragma unroll
-        for (int qx = 0; qx < XP; qx++) {
-            u32x4 x[F];
-            f32x4 corr[F];
-#pragma unroll
-            for (int j = 0; j < F; j++) {
-                x[j] = *reinterpret_cast<const u32x4 *>(&lx[qx][(wm + 16 * j + r) * PITCH + 8 * g]);
-                if constexpr (MODE == kInt4) {
-                    corr[j] = mma16<DT>(minus24<DT>(), x[j], f32x4{0, 0, 0, 0});
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < F; i++) {
-                f32x4 s;
-                if constexpr (MODE == kInt4) s = *reinterpret_cast<const f32x4 *>(&ls[wn + 16 * i + 4 * g]);
-#pragma unroll
-                for (int qw = 0; qw < WP; qw++) {
-                    const u32x4 w = *reinterpret_cast<const u32x4 *>(&lw[qw][(wn + 16 * i + r) * PITCH + 8 * g]);
-#pragma unroll
-                    for (int j = 0; j < F; j++) {
-                        if constexpr (MODE == kInt4) {
-                            const f32x4 part = mma16<DT>(w, x[j], corr[j]);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(s[e], part[e], acc[i][j][e]);
-                        } else {
-                            acc[i][j] = mma16<MT>(w, x[j], acc[i][j]);
+                        for (uint32_t e = 0; e < 8; e++) {
+                            if (e >= count) break;
+                            const int q = (int)((uint32_t)(bytes >> (4 * e)) & 15u) - 8;
+                            split_bf16((float)q * ((i + e) / 32 == i / 32 ? s0 : s1), e, wv[j][0], wv[j][WP - 1]);
                         }
                     }
                 }
             }
         }
+        if constexpr (MODE == kInt4) {
+            const uint32_t row = tid % S, k = k0 + tid / S * 32;  // 2 S scales
+            if (tid < 2 * S) sv = n0 + row < a.n && k < k1 ? p.scales[((uint64_t)(n0 + row) * a.k + k) / 32] : 0u;
+        }
+    };
+    // what is done to the values on their way to LDS waits until they are here
+    auto stage = [&]() {
+#pragma unroll
+        for (uint32_t j = 0; j < P; j++) {
+            const uint32_t at = ((j * 256 + tid) >> 3) * PITCH + (tid & 7u) * 8;
+            if constexpr (MODE == kInt4) {
+                *reinterpret_cast<u32x4 *>(&lw[0][at]) = nibbles_0415<DT>(wv[j][0][0]);
+                *reinterpret_cast<u32x4 *>(&lx[0][at]) = order_0415(xv[j][0]);
+            } else {
+                if constexpr (XP == 2) {
+                    const u32x4 x = xv[j][0];
+                    xv[j][0] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        split_bf16(half_to_f32<DT>((x[e >> 1] >> (16 * (e & 1))) & 0xffffu), e, xv[j][0], xv[j][XP - 1]);
+                }
+#pragma unroll
+                for (int q = 0; q < WP; q++) *reinterpret_cast<u32x4 *>(&lw[q][at]) = wv[j][q];
+#pragma unroll
+                for (int q = 0; q < XP; q++) *reinterpret_cast<u32x4 *>(&lx[q][at]) = xv[j][q];
+            }
+        }
+        if (MODE == kInt4 && tid < 2 * S) ls[tid / S][tid % S] = f16_bits_to_f32(sv);
+    };
+
+    if (kb < k1) fetch(kb);
+    for (uint32_t k0 = kb; k0 < k1; k0 += 64) {
+        __syncthreads();
+        stage();
+        __syncthreads();
+        if (k0 + 64 < k1) fetch(k0 + 64);
+#pragma unroll
+        for (int f = 0; f < 2; f++)
+#pragma unroll
+            for (int qx = 0; qx < XP; qx++) {
+                u32x4 x[F];
+                f32x4 corr[F];
+#pragma unroll
+                for (int j = 0; j < F; j++) {
+                    x[j] = *reinterpret_cast<const u32x4 *>(&lx[qx][(wm + 16 * j + r) * PITCH + 32 * f + 8 * g]);
+                    if constexpr (MODE == kInt4) corr[j] = mma16<DT>(minus24<DT>(), x[j], f32x4{0, 0, 0, 0});
+                }
+#pragma unroll
+                for (int i = 0; i < F; i++) {
+                    f32x4 s;
+                    if constexpr (MODE == kInt4) s = *reinterpret_cast<const f32x4 *>(&ls[f][wn + 16 * i + 4 * g]);
+#pragma unroll
+                    for (int qw = 0; qw < WP; qw++) {
+                        const u32x4 w = *reinterpret_cast<const u32x4 *>(&lw[qw][(wn + 16 * i + r) * PITCH + 32 * f + 8 * g]);
+#pragma unroll
+                        for (int j = 0; j < F; j++) {
+                            if constexpr (MODE == kInt4) {
+                                const f32x4 part = mma16<DT>(w, x[j], corr[j]);
+#pragma unroll
+                                for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(s[e], part[e], acc[i][j][e]);
+                            } else {
+                                acc[i][j] = mma16<MT>(w, x[j], acc[i][j]);
+                            }
+                        }
+                    }
+                }
+            }
     }
 #pragma unroll
     for (int j = 0; j < F; j++) {
@@ -399,7 +488,11 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p) {
 #pragma unroll
         for (int i = 0; i < F; i++) {
             const uint32_t n = n0 + wn + 16 * i + 4 * g;
-            if (n < a.n) finish4<DT, YT>(p, m, n, acc[i][j]);
+            if (n >= a.n) continue;
+            if (split.partial)
+                store_partial(p, split, blockIdx.z, m, n, acc[i][j]);
+            else
+                finish4<DT, YT>(p, m, n, acc[i][j]);
         }
     }
 }
@@ -438,12 +531,6 @@ __device__ __forceinline__ void tile_copy(const Source &from, uint32_t at, const
             from, (__attribute__((address_space(3))) void *)(lds + (j * T + wave * 64) * 8), 16, off[j], at, 0, 0);
 #endif
 }
-
-// Splits of k (blockIdx.y): steps of 64 each takes, sums to `partial`.
-struct Split {
-    uint32_t steps;
-    float *partial;  // [split][m][n], or null: one split, y itself
-};
 
 template <int DT, int YT, int TN, int TM, int WN, int WM>
 __global__ __launch_bounds__(64 * WN * WM) void linear_large_kernel(const LinearArgs p, const Split split) {
@@ -546,14 +633,7 @@ __global__ __launch_bounds__(64 * WN * WM) void linear_large_kernel(const Linear
                 const Side sd = {pick(&Side::bias), pick(&Side::mul), pick(&Side::res)};
                 if (at >= a.m || n >= a.n) continue;
                 if (split.partial) {
-                    float *to = split.partial + ((uint64_t)blockIdx.y * a.m + at) * a.n + n;
-                    if (n + 4 <= a.n && !(a.n & 3u)) {
-                        *reinterpret_cast<f32x4 *>(to) = v;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (n + e < a.n) to[e] = v[e];
-                    }
+                    store_partial(p, split, blockIdx.y, at, n, v);
                 } else if (whole4(p, n)) {
                     finish_whole4<DT, YT>(p, at, n, v, sd);
                 } else {
@@ -572,6 +652,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const LinearArgs p, co
     const uint32_t m = blockIdx.y, n = 4 * i;
     const float *at = partial + (uint64_t)m * a.n + n;
     f32x4 s = {0, 0, 0, 0};
+#pragma unroll 4
     for (uint32_t j = 0; j < splits; j++, at += (uint64_t)a.m * a.n) {
         if (!(a.n & 3u)) {
             s += *reinterpret_cast<const f32x4 *>(at);
@@ -584,13 +665,19 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const LinearArgs p, co
     finish4<DT, YT>(p, m, n, s);
 }
 
+// 8 waves to a workgroup's rows while there are at most two workgroups to a
+// CU, else 4 (all workgroups resident at once: a row of 8192 x 8192 28 us
+// against 35); two tiles of W's rows where x's values are what a wave loads
+// most.
 template <int DT, int YT, int MT, bool INT4>
-hipError_t launch_rows(const LinearArgs &p, hipStream_t s) {
+hipError_t launch_rows(const LinearArgs &p, int cus, hipStream_t s) {
     const uint32_t tiles = (p.a.n + 15) / 16;
-    if (tiles >= 512)
-        hipLaunchKernelGGL((linear_rows_kernel<DT, YT, MT, 2, INT4>), dim3((tiles + 1) / 2), dim3(512), 0, s, p);
+    if (tiles <= 2 * (uint32_t)cus)
+        hipLaunchKernelGGL((linear_rows_kernel<DT, YT, MT, 1, 8, INT4>), dim3(tiles), dim3(512), 0, s, p);
+    else if (INT4 || MT > 1)
+        hipLaunchKernelGGL((linear_rows_kernel<DT, YT, MT, 2, 4, INT4>), dim3((tiles + 1) / 2), dim3(256), 0, s, p);
     else
-        hipLaunchKernelGGL((linear_rows_kernel<DT, YT, MT, 1, INT4>), dim3(tiles), dim3(512), 0, s, p);
+        hipLaunchKernelGGL((linear_rows_kernel<DT, YT, MT, 1, 4, INT4>), dim3(tiles), dim3(256), 0, s, p);
     return hipGetLastError();
 }
 
@@ -600,27 +687,27 @@ void launch_tiles(const LinearArgs &p, const Split &split, uint32_t splits, hipS
     hipLaunchKernelGGL((linear_large_kernel<DT, YT, TN, TM, WN, WM>), dim3(tiles, splits), dim3(64 * WN * WM), 0, s, p, split);
 }
 
-// Tile and splits of k for the aligned kernel: the least of an estimate in
-// microseconds.  Measured per 64 columns of k (all CUs busy): 1.65 for a
-// 256 x 256 tile and 1.0 for 256 x 128 and 128 x 256 (one workgroup to a CU),
-// 1.13 for two of 128 x 128 to a CU and 0.67 for one; 4 for a tile's start
-// and end; the splits' sums are written and read at 4 TB/s and joined by one
-// more launch.
-struct LargePlan {
+// A tile shape: workgroups to a CU, microseconds per 64 columns of k with all
+// of them and with one alone.
+struct Shape {
+    uint32_t n, m, per_cu;
+    double us, alone;
+};
+struct TilePlan {
     int shape;
     uint32_t splits, steps;
 };
-inline LargePlan plan_large(const hh_linear_args &a, int cus) {
-    static constexpr struct {
-        uint32_t n, m, per_cu;
-        double us, alone;
-    } shapes[] = {{256, 256, 1, 1.65, 1.65}, {256, 128, 1, 1.0, 1.0}, {128, 256, 1, 1.0, 1.0}, {128, 128, 2, 1.13, 0.67}};
-    LargePlan best = {0, 1, 0};
+// Tile and splits of k: the least of an estimate in microseconds.  4 for a
+// tile's start and end; the splits' sums are written and read at 4 TB/s and
+// joined by one more launch.
+template <int N>
+inline TilePlan plan_tiles(const hh_linear_args &a, int cus, const Shape (&shapes)[N]) {
+    TilePlan best = {0, 1, 1};
     double least = 1e30;
-    const uint32_t steps = a.k / 64;
-    for (int i = 0; i < 4; i++)
-        for (uint32_t want = 1; want <= 16 && want <= steps; want *= 2) {
-            const uint32_t each = (steps + want - 1) / want, splits = (steps + each - 1) / each;
+    const uint32_t steps = (a.k + 63) / 64;
+    for (int i = 0; i < N; i++)
+        for (uint32_t want = 1; want <= 16 && (want == 1 || want <= steps); want *= 2) {
+            const uint32_t each = steps ? (steps + want - 1) / want : 1, splits = steps ? (steps + each - 1) / each : 1;
             const uint64_t tiles = (uint64_t)((a.n + shapes[i].n - 1) / shapes[i].n) * ((a.m + shapes[i].m - 1) / shapes[i].m);
             const uint64_t slots = (uint64_t)cus * shapes[i].per_cu, work = tiles * splits;
             const double step = work <= (uint64_t)cus ? shapes[i].alone : shapes[i].us;
@@ -630,16 +717,41 @@ inline LargePlan plan_large(const hh_linear_args &a, int cus) {
         }
     return best;
 }
+// Measured on tiles copied straight to LDS, through registers, and of INT4.
+constexpr Shape kLargeShapes[] = {{256, 256, 1, 1.65, 1.65}, {256, 128, 1, 1.0, 1.0}, {128, 256, 1, 1.0, 1.0},
+                                  {128, 128, 2, 1.13, 0.67}, {128, 64, 3, 1.0, 0.45}};
+constexpr Shape kAnyShapes[] = {{128, 128, 2, 2.0, 1.3}, {64, 64, 4, 1.6, 0.9}};
+
+// Room for the splits' sums in the context's scratch.
+int32_t split_room(hh_context *ctx, const LinearArgs &p, const TilePlan &plan, Split *split) {
+    *split = {plan.steps, nullptr};
+    if (plan.splits == 1) return HH_OK;
+    const int32_t rc = ensure_scratch(ctx, (size_t)plan.splits * p.a.m * p.a.n * sizeof(float));
+    split->partial = reinterpret_cast<float *>(ctx->d_scratch);
+    return rc;
+}
+template <int DT, int YT>
+int32_t join_splits(const LinearArgs &p, const TilePlan &plan, const Split &split, hipStream_t s) {
+    if (split.partial)
+        hipLaunchKernelGGL((linear_join_kernel<DT, YT>), dim3(((p.a.n + 3) / 4 + 255) / 256, p.a.m), dim3(256), 0, s, p,
+                           split.partial, plan.splits);
+    return from_hip(hipGetLastError());
+}
 
 template <int DT, int YT, int MODE>
-hipError_t launch_any(const LinearArgs &p, int cus, hipStream_t s) {
+int32_t launch_any(hh_context *ctx, const LinearArgs &p, int cus, hipStream_t s) {
     const uint32_t n = p.a.n, m = p.a.m;
-    // tiles of 64 where those of 128 leave CUs without one
-    if ((uint64_t)((n + 127) / 128) * ((m + 127) / 128) >= (uint64_t)cus)
-        hipLaunchKernelGGL((linear_tile_kernel<DT, YT, MODE, 128>), dim3((n + 127) / 128, (m + 127) / 128), dim3(256), 0, s, p);
+    const TilePlan plan = plan_tiles(p.a, cus, kAnyShapes);
+    Split split;
+    const int32_t rc = split_room(ctx, p, plan, &split);
+    if (rc != HH_OK) return rc;
+    const uint32_t S = kAnyShapes[plan.shape].n;
+    const dim3 grid((n + S - 1) / S, (m + S - 1) / S, plan.splits);
+    if (S == 128)
+        hipLaunchKernelGGL((linear_tile_kernel<DT, YT, MODE, 128>), grid, dim3(256), 0, s, p, split);
     else
-        hipLaunchKernelGGL((linear_tile_kernel<DT, YT, MODE, 64>), dim3((n + 63) / 64, (m + 63) / 64), dim3(256), 0, s, p);
-    return hipGetLastError();
+        hipLaunchKernelGGL((linear_tile_kernel<DT, YT, MODE, 64>), grid, dim3(256), 0, s, p, split);
+    return join_splits<DT, YT>(p, plan, split, s);
 }
 
 template <int DT, int YT>
@@ -647,37 +759,32 @@ int32_t launch_linear(hh_context *ctx, const LinearArgs &p, hipStream_t s) {
     const hh_linear_args &a = p.a;
     const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
     const bool int4 = a.w_dtype == HH_INT4;
-    if (int4 && a.k % 32) return from_hip(launch_any<DT, YT, kInt4Any>(p, cus, s));
+    if (int4 && a.k % 32) return launch_any<DT, YT, kInt4Any>(ctx, p, cus, s);
     if (a.m <= 64) {
         const int rows = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4;
-        return from_hip(int4 ? (rows == 1   ? launch_rows<DT, YT, 1, true>(p, s)
-                                : rows == 2 ? launch_rows<DT, YT, 2, true>(p, s)
-                                            : launch_rows<DT, YT, 4, true>(p, s))
-                             : (rows == 1   ? launch_rows<DT, YT, 1, false>(p, s)
-                                : rows == 2 ? launch_rows<DT, YT, 2, false>(p, s)
-                                            : launch_rows<DT, YT, 4, false>(p, s)));
+        return from_hip(int4 ? (rows == 1   ? launch_rows<DT, YT, 1, true>(p, cus, s)
+                                : rows == 2 ? launch_rows<DT, YT, 2, true>(p, cus, s)
+                                            : launch_rows<DT, YT, 4, true>(p, cus, s))
+                             : (rows == 1   ? launch_rows<DT, YT, 1, false>(p, cus, s)
+                                : rows == 2 ? launch_rows<DT, YT, 2, false>(p, cus, s)
+                                            : launch_rows<DT, YT, 4, false>(p, cus, s)));
     }
-    if (int4) return from_hip(launch_any<DT, YT, kInt4>(p, cus, s));
+    if (int4) return launch_any<DT, YT, kInt4>(ctx, p, cus, s);
     const bool aligned = !(((uintptr_t)a.d_x | (uintptr_t)a.d_w) & 15u) && !((a.x_stride | a.w_stride) & 7u) &&
                          a.k % 64 == 0 && a.k && a.x_stride < 1u << 22 && a.w_stride < 1u << 22;  // offsets in a tile: 32 bits
-    if (!aligned) return from_hip(launch_any<DT, YT, kHalf>(p, cus, s));
-    const LargePlan plan = plan_large(a, cus);
-    Split split = {plan.steps, nullptr};
-    if (plan.splits > 1) {
-        const int32_t rc = ensure_scratch(ctx, (size_t)plan.splits * a.m * a.n * sizeof(float));
-        if (rc != HH_OK) return rc;
-        split.partial = reinterpret_cast<float *>(ctx->d_scratch);
-    }
+    if (!aligned) return launch_any<DT, YT, kHalf>(ctx, p, cus, s);
+    const TilePlan plan = plan_tiles(a, cus, kLargeShapes);
+    Split split;
+    const int32_t rc = split_room(ctx, p, plan, &split);
+    if (rc != HH_OK) return rc;
     switch (plan.shape) {
         case 0: launch_tiles<DT, YT, 256, 256, 2, 4>(p, split, plan.splits, s); break;
         case 1: launch_tiles<DT, YT, 256, 128, 4, 2>(p, split, plan.splits, s); break;
         case 2: launch_tiles<DT, YT, 128, 256, 2, 4>(p, split, plan.splits, s); break;
-        default: launch_tiles<DT, YT, 128, 128, 2, 2>(p, split, plan.splits, s); break;
+        case 3: launch_tiles<DT, YT, 128, 128, 2, 2>(p, split, plan.splits, s); break;
+        default: launch_tiles<DT, YT, 128, 64, 2, 2>(p, split, plan.splits, s); break;
     }
-    if (split.partial)
-        hipLaunchKernelGGL((linear_join_kernel<DT, YT>), dim3(((a.n + 3) / 4 + 255) / 256, a.m), dim3(256), 0, s, p,
-                           split.partial, plan.splits);
-    return from_hip(hipGetLastError());
+    return join_splits<DT, YT>(p, plan, split, s);
 }
 
 }  // namespace
