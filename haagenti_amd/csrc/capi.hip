@@ -36,6 +36,7 @@ int32_t ensure_scratch(hh_context *ctx, size_t bytes) {
     hipError_t e = hipMalloc(&ctx->d_scratch, sz);
     if (e != hipSuccess) {
         ctx->d_scratch = nullptr;
+        (void)hipGetLastError();  // reported here, not by the next call's launch check
         return from_hip(e);
     }
     ctx->scratch_bytes = sz;

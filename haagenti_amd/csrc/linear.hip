@@ -118,7 +118,11 @@ __device__ __forceinline__ void finish4(const LinearArgs &p, uint32_t m, uint32_
 
 // ---------------------------------------------------------------- few rows
 //
-// Bound by reading W once.  A workgroup takes 16 NT rows of W; its KW
+// Bound by reading W once: a row of 4096 x 4096 in bf16 7.8 us (4.3 TB/s of W,
+// 5.4 at the copy's 6.2), of 14336 x 4096 26 us, of 8192 x 8192 28 us; INT4 of
+// 14336 x 4096 16 us for 1 row, 17.5 for 8 (5.4 at the copy's rate: without
+// the loads of x and of the scales it takes 12, without the products as long
+// as with them).  A workgroup takes 16 NT rows of W; its KW
 // waves take every KW-th 128 columns of them, straight to registers (the next
 // ones on their way while these are used), and join their sums in LDS.  x (at most
 // 16 MT rows) comes from L1 / L2; its row is the products' first operand, so
@@ -508,7 +512,9 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p, co
 // copy's lanes choose their source piece accordingly: LDS is written in lane
 // order).  Rows past the matrices repeat the last one.  Bound by LDS and the
 // matrix pipes alike: at 256 x 256 a tile's reads (192 KiB by 8 waves of
-// 128 x 64) and copies (64 KiB) take as long as its products.
+// 128 x 64) and copies (64 KiB) take as long as its products.  bf16 4096 x
+// 8192 x 8192 takes 440 us (1250 TFLOP/s; 0.85 of the library's product),
+// 2048 x 14336 x 4096 246 (980), 512 x 4096 x 14336 67 (900).
 //
 // Tiles are numbered down the rows of x, and consecutive ones go to one XCD,
 // whose L2 then serves W's panel to all of them.
@@ -647,9 +653,10 @@ __global__ __launch_bounds__(64 * WN * WM) void linear_large_kernel(const Linear
 template <int DT, int YT>
 __global__ __launch_bounds__(256) void linear_join_kernel(const LinearArgs p, const float *partial, uint32_t splits) {
     const hh_linear_args &a = p.a;
-    const uint32_t quads = (a.n + 3) / 4, i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= quads) return;
-    const uint32_t m = blockIdx.y, n = 4 * i;
+    const uint32_t quads = (a.n + 3) / 4;
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (uint64_t)a.m * quads) return;
+    const uint32_t m = (uint32_t)(i / quads), n = (uint32_t)(i % quads) * 4;
     const float *at = partial + (uint64_t)m * a.n + n;
     f32x4 s = {0, 0, 0, 0};
 #pragma unroll 4
@@ -672,12 +679,11 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const LinearArgs p, co
 template <int DT, int YT, int MT, bool INT4>
 hipError_t launch_rows(const LinearArgs &p, int cus, hipStream_t s) {
     const uint32_t tiles = (p.a.n + 15) / 16;
+    constexpr int NT = INT4 || MT > 1 ? 2 : 1;
     if (tiles <= 2 * (uint32_t)cus)
         hipLaunchKernelGGL((linear_rows_kernel<DT, YT, MT, 1, 8, INT4>), dim3(tiles), dim3(512), 0, s, p);
-    else if (INT4 || MT > 1)
-        hipLaunchKernelGGL((linear_rows_kernel<DT, YT, MT, 2, 4, INT4>), dim3((tiles + 1) / 2), dim3(256), 0, s, p);
     else
-        hipLaunchKernelGGL((linear_rows_kernel<DT, YT, MT, 1, 4, INT4>), dim3(tiles), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((linear_rows_kernel<DT, YT, MT, NT, 4, INT4>), dim3((tiles + NT - 1) / NT), dim3(256), 0, s, p);
     return hipGetLastError();
 }
 
@@ -710,6 +716,7 @@ inline TilePlan plan_tiles(const hh_linear_args &a, int cus, const Shape (&shape
             const uint32_t each = steps ? (steps + want - 1) / want : 1, splits = steps ? (steps + each - 1) / each : 1;
             const uint64_t tiles = (uint64_t)((a.n + shapes[i].n - 1) / shapes[i].n) * ((a.m + shapes[i].m - 1) / shapes[i].m);
             const uint64_t slots = (uint64_t)cus * shapes[i].per_cu, work = tiles * splits;
+            if (splits > 1 && (uint64_t)a.m * a.n > 1ull << 30) continue;  // their sums: at most 64 GiB, one launch to join
             const double step = work <= (uint64_t)cus ? shapes[i].alone : shapes[i].us;
             double us = (double)((work + slots - 1) / slots) * (step * each + 4.0);
             if (splits > 1) us += 4.0 + (double)a.m * a.n * 8.0 * splits / 4e6;
@@ -733,7 +740,8 @@ int32_t split_room(hh_context *ctx, const LinearArgs &p, const TilePlan &plan, S
 template <int DT, int YT>
 int32_t join_splits(const LinearArgs &p, const TilePlan &plan, const Split &split, hipStream_t s) {
     if (split.partial)
-        hipLaunchKernelGGL((linear_join_kernel<DT, YT>), dim3(((p.a.n + 3) / 4 + 255) / 256, p.a.m), dim3(256), 0, s, p,
+        hipLaunchKernelGGL((linear_join_kernel<DT, YT>), dim3((uint32_t)(((uint64_t)p.a.m * ((p.a.n + 3) / 4) + 255) / 256)),
+                           dim3(256), 0, s, p,
                            split.partial, plan.splits);
     return from_hip(hipGetLastError());
 }
@@ -798,7 +806,7 @@ extern "C" int32_t hh_linear(hh_context *ctx, const hh_linear_args *a, void *str
     if (a->w_dtype != a->dtype && a->w_dtype != HH_INT4) return HH_ERR_UNSUPPORTED;
     if (a->y_dtype != a->dtype && a->y_dtype != HH_F32) return HH_ERR_UNSUPPORTED;
     if (a->activation < HH_ACT_NONE || a->activation > HH_ACT_SILU) return HH_ERR_UNSUPPORTED;
-    if (a->m >= 1u << 23 || a->n >= 1u << 31 || a->k >= 1u << 31) return HH_ERR_INVALID_ARGUMENT;
+    if (a->m >= 1u << 21 || a->n >= 1u << 26 || a->k >= 1u << 31) return HH_ERR_INVALID_ARGUMENT;
     if (a->m == 0 || a->n == 0) return HH_OK;
     const bool int4 = a->w_dtype == HH_INT4;
     if (!a->d_y || (a->k && (!a->d_x || !a->d_w))) return HH_ERR_INVALID_ARGUMENT;

@@ -684,8 +684,11 @@ int32_t hh_spectral_encode_from_dct(const float *coeffs, uint32_t width, uint32_
  * counterpart in the reference, which stops at the decoded tensor.  All are
  * asynchronous on the stream and read lengths, tables and slots from device
  * memory, so a step needs no host synchronisation.  Strides are in elements.
- * The context's scratch grows with the largest call so far; after a first
- * call of the same sizes a call allocates nothing and may be captured. */
+ * hh_linear and hh_kv_attention may keep partial sums in the context's
+ * scratch, which grows with the largest call so far: after a first call of
+ * the same sizes a call allocates nothing and may be captured.  A later call
+ * that needs more moves the scratch, and what was captured before must be
+ * captured again. */
 
 typedef enum hh_activation {
     HH_ACT_NONE = 0,
@@ -702,7 +705,8 @@ typedef enum hh_activation {
 /* y = act(x W^T + bias) * mul + residual: x is m x k, W n x k (a weight as it
  * is stored: a row per output), y, mul and residual m x n, bias n values.
  * bias, mul and residual may be NULL and have x's type; a 16-bit W has it too.
- * Sums are f32; y is rounded once at the end.  y may be residual or mul
+ * Sums are f32; y is rounded once at the end.  With INT4 weights a row of x
+ * that holds an infinity gives NaN.  y may be residual or mul
  * itself (same stride), and overlaps nothing else that is read. */
 typedef struct hh_linear_args {
     const void *d_x, *d_w, *d_bias, *d_mul, *d_residual;
@@ -718,7 +722,8 @@ typedef struct hh_linear_args {
 /* m, n or k of 0 are allowed (k = 0: sums of 0).  Pointers are aligned to
  * their elements; rows of 16 bytes' alignment (pointers and strides) take the
  * wide loads.  HH_ERR_UNSUPPORTED for other types, HH_ERR_INVALID_ARGUMENT
- * for a missing pointer, a stride below the row, a size of 2^31 or more. */
+ * for a missing pointer, a stride below the row, m of 2^21, n of 2^26 or k of
+ * 2^31 or more, HH_ERR_UNEXPECTED_EOF for an INT4 buffer that is too short. */
 int32_t hh_linear(hh_context *ctx, const hh_linear_args *args, void *stream);
 
 /* A paged cache: num_blocks blocks of block_size tokens (16, 32, 64 or 128)
