@@ -162,7 +162,7 @@ __device__ __forceinline__ void store4(uint16_t *to, bool wide, const float *v) 
 // A step of a running request: at most 16 columns, one 16 x 16 x 32 tile
 // wide.  Bound by reading the codes once: 131,001 tokens of 8 heads of 128
 // dimensions (268 MB) take 43 us (6.2 TB/s) and 7 to join, 48 requests of 100
-// to 8000 tokens (424 MB) 94 and 5 (chunks end unevenly).  A workgroup takes one chunk of a
+// to 8000 tokens (424 MB) 86 and 5 (chunks end unevenly).  A workgroup takes one chunk of a
 // request's tokens for one cache head, its 4 waves every fourth 64 tokens
 // straight from memory to registers; their results are joined in LDS, the
 // chunks' by attn_join_kernel.
@@ -658,15 +658,20 @@ extern "C" int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, co
     const uint64_t room = (uint64_t)a->table_width * cache->block_size;
     const uint64_t kv = a->max_kv < room ? a->max_kv : room;
     if (kv > 1ull << 30) return HH_ERR_UNSUPPORTED;  // tokens are counted in 31 bits
-    // chunks: enough workgroups for 16 per CU, none below 512 tokens
+    // chunks: enough workgroups for 8 per CU (48 requests 86 us; 16 per CU 95,
+    // 24 per CU 87 with twice the chunks to join), none below 512 tokens
     const uint64_t lanes = (uint64_t)a->requests * cache->kv_heads;
-    const uint64_t want = (16ull * (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256) + lanes - 1) / lanes;
+    const uint64_t want = (8ull * (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256) + lanes - 1) / lanes;
     uint64_t chunk = (kv + want - 1) / want;
     chunk = (chunk + 255) / 256 * 256;
     if (chunk < 512) chunk = 512;
     p.chunk = (uint32_t)chunk;
     p.splits = (uint32_t)((kv + chunk - 1) / chunk);
     if (p.splits < 1) p.splits = 1;
+    // Workgroups go around the 8 XCDs: with an odd number of chunks to a
+    // request each XCD gets early and late ones (of ragged requests the late
+    // ones are empty; 48 requests in 16 chunks each 111 us, in 17 87).
+    if (p.splits > 1) p.splits |= 1;
     const uint32_t tile = 32u * (cache->head_dim <= 128 ? hh::kTileWaves<128> : hh::kTileWaves<256>);
     p.tiles = most > p.small ? (uint32_t)((most + tile - 1) / tile) : 0;
     if ((uint64_t)a->requests * p.splits >= 1ull << 24 || (uint64_t)a->requests * p.tiles >= 1ull << 24)

@@ -335,20 +335,15 @@ __global__ __launch_bounds__(64 * KW) void linear_rows_kernel(const LinearArgs p
 // Splits of k: steps of 64 each takes, sums to `partial`.
 struct Split {
     uint32_t steps;
-    float *partial;  // [split][m][n], or null: one split, y itself
+    float *partial;  // [split][m][n rounded up to 4], or null: one split, y itself
 };
 
-// A split's sums of outputs n .. n + 3 of row m.
+// A split's sums of outputs n .. n + 3 of row m.  Rows of the sums are whole
+// groups of 4, so that all are written and read 16 bytes at a time.
+__device__ __forceinline__ uint32_t partial_row(const LinearArgs &p) { return (p.a.n + 3) / 4 * 4; }
 __device__ __forceinline__ void store_partial(const LinearArgs &p, const Split &split, uint32_t index, uint32_t m, uint32_t n,
                                               const f32x4 &v) {
-    float *to = split.partial + ((uint64_t)index * p.a.m + m) * p.a.n + n;
-    if (n + 4 <= p.a.n && !(p.a.n & 3u)) {
-        *reinterpret_cast<f32x4 *>(to) = v;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (n + e < p.a.n) to[e] = v[e];
-    }
+    *reinterpret_cast<f32x4 *>(split.partial + ((uint64_t)index * p.a.m + m) * partial_row(p) + n) = v;
 }
 
 // f as the sum of two bf16 numbers, e-th of 8 each; what is not finite is in
@@ -657,18 +652,11 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const LinearArgs p, co
     const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= (uint64_t)a.m * quads) return;
     const uint32_t m = (uint32_t)(i / quads), n = (uint32_t)(i % quads) * 4;
-    const float *at = partial + (uint64_t)m * a.n + n;
+    const uint64_t step = (uint64_t)a.m * quads * 4;
+    const float *at = partial + (uint64_t)m * quads * 4 + n;
     f32x4 s = {0, 0, 0, 0};
-#pragma unroll 4
-    for (uint32_t j = 0; j < splits; j++, at += (uint64_t)a.m * a.n) {
-        if (!(a.n & 3u)) {
-            s += *reinterpret_cast<const f32x4 *>(at);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (n + e < a.n) s[e] += at[e];
-        }
-    }
+#pragma unroll 8
+    for (uint32_t j = 0; j < splits; j++) s += *reinterpret_cast<const f32x4 *>(at + j * step);
     finish4<DT, YT>(p, m, n, s);
 }
 
@@ -733,7 +721,7 @@ constexpr Shape kAnyShapes[] = {{128, 128, 2, 2.0, 1.3}, {64, 64, 4, 1.6, 0.9}};
 int32_t split_room(hh_context *ctx, const LinearArgs &p, const TilePlan &plan, Split *split) {
     *split = {plan.steps, nullptr};
     if (plan.splits == 1) return HH_OK;
-    const int32_t rc = ensure_scratch(ctx, (size_t)plan.splits * p.a.m * p.a.n * sizeof(float));
+    const int32_t rc = ensure_scratch(ctx, (size_t)plan.splits * p.a.m * ((p.a.n + 3) / 4 * 4) * sizeof(float));
     split->partial = reinterpret_cast<float *>(ctx->d_scratch);
     return rc;
 }
