@@ -1,8 +1,11 @@
 // y = act(x W^T + bias) * mul + residual (hh_linear, include/haagenti_hip.h).
 //
-// Both routes put W's rows on the first operand of the matrix instructions
-// and x's on the second, so a lane ends with 4 consecutive outputs n of one
-// row m: bias, mul, residual and y move 4 values at a time.
+// Three routes: few rows of x (W straight to registers), many rows in tiles
+// copied straight to LDS where the layout is aligned, and tiles through
+// registers for any other layout and for INT4.  The tiles put W's rows on the
+// first operand of the matrix instructions and x's on the second, so a lane
+// ends with 4 consecutive outputs n of one row m; bias, mul, residual and y
+// move 4 values at a time on every route.
 //
 // INT4 weights stay integers: nibbles become the 16-bit numbers 16..31 by
 // shifts and ors (exact in f16 and bf16), and the offset of 24 goes into the
