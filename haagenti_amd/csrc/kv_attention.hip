@@ -4,14 +4,18 @@
 // kernels compute, per cache head,
 //   S^T = K Q^T     codes (exact in f16) times f16 queries, f32
 //   z   = S^T (scale of K's block) (softmax scale) log2(e)
-//   m, l, O: running maximum of z, sum of 2^(z - m), and
-//   O^T += V^T P^T  codes times f16 P = 2^(z - m) (scale of V's block) / top,
-//                   top the largest V scale so far (so no P is large
-//                   whatever the scales are), O in units of top, f32.
-// The scale's share goes into the exponent; the sum l takes it out again per
-// 16 tokens (a share below 2^-60 counts as 2^-60: such a P is 0 in f16 anyway,
-// and l keeps its tokens).  m follows the maximum only when it is passed by 8,
-// so P < 256 and the accumulators are seldom rescaled.
+//   w   = z + log2(scale of V's block)
+//   m, l, M: running maximum of z, sum of 2^(z - m), running maximum of w,
+//   O^T += V^T P^T  codes times f16 P = 2^(w - M), O in units of 2^M, f32,
+// and the output is 2^(M - m) O / l.  Both maxima are the column's own, over
+// tokens that it sees, so whatever the scales are, its largest P is at least 1:
+// a P keeps f16's 11 bits down to 2^-14 and is off by at most 2^-25 below (of
+// terms that small beside the column's largest).
+// P's exponent is z - m + share, share = log2(scale of V's block) - rise, rise
+// standing for M - m; the sum l takes the share out again per 16 tokens (a
+// share below 2^-40 counts as 2^-40: such a P is 0 in f16 anyway, and l keeps
+// its tokens).  m and M follow their maxima only when these pass them by 8, so
+// P < 256 and the accumulators are seldom rescaled.
 // Tokens lie on the first product's rows, so its accumulators hold, for one
 // column per lane, just the tokens that the lane supplies to the second
 // product's P^T operand: P never moves between lanes.  Which token a row
@@ -38,7 +42,7 @@ struct AttnArgs {
     uint32_t small;      // requests with at most this many columns are the step kernel's
     uint32_t cols;       // most columns of such a request
     float *part_o;       // [request][head][split][cols][dim]
-    float *part_ml;      // [request][head][split][cols][2]
+    float *part_ml;      // [request][head][split][cols][m, l, rise]
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -87,12 +91,59 @@ __device__ __forceinline__ int32_t block_of(const AttnArgs &p, const int32_t *ta
     return table[(uint32_t)tok >> p.bs_log];
 }
 __device__ __forceinline__ bool held(const AttnArgs &p, int32_t id) { return (uint32_t)id < p.cache.num_blocks; }
-// What a V scale's share of the largest does to the exponent.
-__device__ __forceinline__ float share_of(float vs, float log_top) {
-    const float s = __builtin_amdgcn_logf(vs) - log_top;
-    return s > -60.0f ? s : -60.0f;  // also where both are 0
+constexpr float kSlack = 8.0f, kNear = 20.0f;
+
+// What a V scale does to the exponent.  Shares of scales that the column
+// doesn't see may be large: of no use, but finite.
+__device__ __forceinline__ float share_of(float log_vs, float rise) {
+    const float s = log_vs - rise;
+    return s > -40.0f ? fminf(s, 300.0f) : -40.0f;
 }
-constexpr float kSlack = 8.0f;
+
+// The larger of lanes 32 (16) apart, by a swap of register halves (rows).
+__device__ __forceinline__ float max_across_32(float v) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float max_across_16(float v) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
+// A maximum to subtract, where there may be none.
+__device__ __forceinline__ float base_of(float top) { return top == -__builtin_inff() ? 0.0f : top; }
+
+// O's unit in units of 2^top, a common m; -inf where there is none.
+__device__ __forceinline__ float unit_of(float m, float rise, float top) {
+    return rise < __builtin_inff() ? m - top + rise : -__builtin_inff();
+}
+
+// A column's running maxima.  rise is infinite while no token seen has a scale
+// above 0; O's unit is 2^(m + rise), and big is that sum for comparing.
+struct Tops {
+    float m = -__builtin_inff(), big = -__builtin_inff(), rise = __builtin_inff();
+    __device__ __forceinline__ bool passed(float zm, float wm) const { return zm > m + kSlack || wm > big + kSlack; }
+    // Takes new maxima where they pass; what that does to l and to O.
+    __device__ __forceinline__ void take(float zm, float wm, float &of_l, float &of_o) {
+        const float mn = zm > m + kSlack ? zm : m, bn = wm > big + kSlack ? wm : big;
+        const float rn = bn > -__builtin_inff() ? bn - mn : __builtin_inff();
+        of_l = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+        of_o = big > -__builtin_inff() ? __builtin_amdgcn_exp2f((m - mn) + (rise - rn)) : 1.0f;
+        m = mn, big = bn, rise = rn;
+    }
+    // Moves both to a new M, as far as that lies above the old.
+    __device__ __forceinline__ float move(float wm) {
+        const float mn = wm > big + kSlack ? m + (wm - big) : m, of = __builtin_amdgcn_exp2f(m - mn);
+        if (wm > big + kSlack) big = wm;
+        m = mn;
+        return of;
+    }
+};
+// The root of 2^rise (the power itself may leave f32's range where the output
+// doesn't); 0 where there is none.
+__device__ __forceinline__ float half_rise(float rise) {
+    return rise < __builtin_inff() ? __builtin_amdgcn_exp2f(0.5f * rise) : 0.0f;
+}
 
 // N f16 fragments of 8 dimensions of a query row, fragment f at dimension
 // dim(f), as f16 scaled by a power of two of the row; returns what undoes the
@@ -176,7 +227,7 @@ template <int DT, int D>
 __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attn_step_kernel(const AttnArgs p) {
     constexpr int KS = D / 32, VT = D / 16, KW = D / 16;  // k steps, V tiles, 4-byte words of K per lane and row
     __shared__ __align__(16) float lds_o[2][16][D + 4];
-    __shared__ float lds_ml[4][16][2];
+    __shared__ float lds_ml[4][16][3];
     const uint32_t r = blockIdx.x / p.splits, split = blockIdx.x % p.splits, h = blockIdx.y;
     if (r == p.a.requests - 1 && split == 0 && h == 0) zero_tail(p, D, 256);
     const Request rq = request_of(p, r);
@@ -209,7 +260,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attn_step_kernel(const 
     f32x4 o[VT];
 #pragma unroll
     for (int t = 0; t < VT; t++) o[t] = f32x4{0, 0, 0, 0};
-    float m = -__builtin_inff(), l = 0.0f, top = 0.0f, log_top = -__builtin_inff();
+    Tops tops;
+    float l = 0.0f;
 
     // K rows: this lane's rows are in run col >> 2; V and the scales: run u
     const int32_t kr = 16 * (col >> 2), vr = 16 * u, mask = bs - 1;
@@ -240,7 +292,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attn_step_kernel(const 
             }
         }
         const uint32_t bh = iv * p.cache.kv_heads + h;
-        const float ks = p.cache.d_k_scale[bh], vs = hv ? p.cache.d_v_scale[bh] : 0.0f;
+        const float ks = p.cache.d_k_scale[bh], log_vs = log2f(hv ? p.cache.d_v_scale[bh] : 0.0f);
         const uint8_t *vp = vh + (uint64_t)iv * p.block_step + (uint32_t)((base + vr) & mask);
 #pragma unroll
         for (int t = 0; t < VT; t++) vw[t] = *reinterpret_cast<const u32x4 *>(vp + t * 16 * bs);
@@ -262,21 +314,20 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attn_step_kernel(const 
             for (int i = 0; i < 16; i++) s[i >> 2][i & 3] = i < seen ? s[i >> 2][i & 3] * c : -__builtin_inff();
             c = 1.0f;
         }
-        float zm = s[0][0], vt = vs;
+        float zm = s[0][0];
 #pragma unroll
         for (int i = 1; i < 16; i++) zm = fmaxf(zm, s[i >> 2][i & 3]);
         zm *= c;
-        zm = fmaxf(zm, __shfl_xor(zm, 16)), vt = fmaxf(vt, __shfl_xor(vt, 16));
-        zm = fmaxf(zm, __shfl_xor(zm, 32)), vt = fmaxf(vt, __shfl_xor(vt, 32));
-        if (__any(zm > m + kSlack || vt > top)) {
-            const float mn = zm > m + kSlack ? zm : m, tn = fmaxf(top, vt);
-            const float again = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f, of = again * (tn > top ? top / tn : 1.0f);
-            m = mn, top = tn, log_top = __builtin_amdgcn_logf(tn);
-            l *= again;
+        float wm = zm + log_vs;  // -inf where nothing is seen
+        zm = max_across_32(max_across_16(zm)), wm = max_across_32(max_across_16(wm));
+        if (__any(tops.passed(zm, wm))) {
+            float of_l, of_o;
+            tops.take(zm, wm, of_l, of_o);
+            l *= of_l;
 #pragma unroll
-            for (int t = 0; t < VT; t++) o[t] *= of;
+            for (int t = 0; t < VT; t++) o[t] *= of_o;
         }
-        const float share = share_of(vs, log_top), less = share - (m == -__builtin_inff() ? 0.0f : m);
+        const float share = share_of(log_vs, tops.rise), less = share - base_of(tops.m);
         f16x8 pv[2];
         float sum = 0.0f;
 #pragma unroll
@@ -293,18 +344,21 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attn_step_kernel(const 
         }
     }
 
-    // join the 4 waves: the common maximum, then the sums in a fixed order
+    // join the 4 waves: the common maxima, then the sums in a fixed order
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (u == 0) lds_ml[wave][col][0] = m, lds_ml[wave][col][1] = l;
+    if (u == 0) lds_ml[wave][col][0] = tops.m, lds_ml[wave][col][1] = l, lds_ml[wave][col][2] = tops.rise;
     __syncthreads();
     float mm = -__builtin_inff(), ll = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; w++) mm = fmaxf(mm, lds_ml[w][col][0]);
-    const float ref = mm == -__builtin_inff() ? 0.0f : mm;
 #pragma unroll
-    for (int w = 0; w < 4; w++) ll += lds_ml[w][col][1] * __builtin_amdgcn_exp2f(lds_ml[w][col][0] - ref);
-    const float f = __builtin_amdgcn_exp2f(m - ref) * top;
+    for (int w = 0; w < 4; w++) ll += lds_ml[w][col][1] * __builtin_amdgcn_exp2f(lds_ml[w][col][0] - base_of(mm));
+    float rise = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < 4; w++) rise = fmaxf(rise, unit_of(lds_ml[w][col][0], lds_ml[w][col][2], mm));
+    const float f = __builtin_amdgcn_exp2f(unit_of(tops.m, tops.rise, mm) - base_of(rise));
+    if (rise == -__builtin_inff()) rise = __builtin_inff();
 #pragma unroll
     for (int t = 0; t < VT; t++) o[t] *= f;
     if (wave >= 2) {
@@ -329,12 +383,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attn_step_kernel(const 
         uint16_t *out = reinterpret_cast<uint16_t *>(p.a.d_out) + ((uint64_t)rq.q0 + qi) * p.a.out_token_stride +
                         qh * p.a.out_head_stride;
         const bool wide = !((uintptr_t)p.a.d_out & 7u) && !((p.a.out_token_stride | p.a.out_head_stride) & 3u);
-        const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+        const float inv = ll != 0.0f ? 1.0f / ll : 0.0f, root = half_rise(rise);
 #pragma unroll
         for (int t = 0; t < VT; t++) {
             float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = o[t][i] * inv;
+            for (int i = 0; i < 4; i++) v[i] = o[t][i] * inv * root * root;
             store4<DT>(out + 16 * t + 4 * u, wide, v);
         }
         return;
@@ -342,7 +396,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attn_step_kernel(const 
     const uint64_t at = (((uint64_t)r * p.cache.kv_heads + h) * p.splits + split) * p.cols + col;
 #pragma unroll
     for (int t = 0; t < VT; t++) *reinterpret_cast<f32x4 *>(p.part_o + at * D + 16 * t + 4 * u) = o[t];
-    if (u == 0) p.part_ml[2 * at] = mm, p.part_ml[2 * at + 1] = ll;
+    if (u == 0) p.part_ml[3 * at] = mm, p.part_ml[3 * at + 1] = ll, p.part_ml[3 * at + 2] = rise;
 }
 
 // Joins the chunks of a request's column: one workgroup per request, head and
@@ -351,39 +405,46 @@ template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p) {
     constexpr int W = 256 / (D / 4);
     __shared__ __align__(16) float sum[W][D];
-    __shared__ float lsum[W];
     const uint32_t r = blockIdx.x, h = blockIdx.y / p.cols, col = blockIdx.y % p.cols;
     const Request rq = request_of(p, r);
     const uint32_t cols = columns_of(p, rq);
     if (col >= cols || cols > p.small || rq.seen <= (int32_t)p.chunk) return;
     const uint32_t n = ((uint32_t)rq.seen + p.chunk - 1) / p.chunk;
     const uint64_t at = ((uint64_t)r * p.cache.kv_heads + h) * p.splits * p.cols + col;
-    float m = -__builtin_inff();
-    for (uint32_t s = threadIdx.x & 63u; s < n; s += 64) m = fmaxf(m, p.part_ml[2 * (at + (uint64_t)s * p.cols)]);
-    m = wave_max(m);
-    const float ref = m == -__builtin_inff() ? 0.0f : m;
+    // l in units of 2^own, the largest of O's units in the same
+    float own = -__builtin_inff(), rise = -__builtin_inff(), l = 0.0f;
+    for (uint32_t s = threadIdx.x & 63u; s < n; s += 64) {
+        const float *ml = p.part_ml + 3 * (at + (uint64_t)s * p.cols);
+        const float now = fmaxf(own, ml[0]), down = own - base_of(now);
+        l = fmaf(ml[1], __builtin_amdgcn_exp2f(ml[0] - base_of(now)), l * __builtin_amdgcn_exp2f(down));
+        rise = fmaxf(rise + down, unit_of(ml[0], ml[2], now));
+        own = now;
+    }
+    const float m = wave_max(own);
+    l *= __builtin_amdgcn_exp2f(own - base_of(m));
+    rise = wave_max(rise + (own - base_of(m)));
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d);
     const uint32_t part = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
     if (part < W) {
         f32x4 o = {0, 0, 0, 0};
-        float l = 0.0f;
 #pragma unroll 8
         for (uint32_t s = part; s < n; s += W) {
             const uint64_t i = at + (uint64_t)s * p.cols;
-            const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * i] - ref);
-            l = fmaf(f, p.part_ml[2 * i + 1], l);
-            o += f * *reinterpret_cast<const f32x4 *>(p.part_o + i * D + d);
+            o += __builtin_amdgcn_exp2f(unit_of(p.part_ml[3 * i], p.part_ml[3 * i + 2], m) - base_of(rise)) *
+                 *reinterpret_cast<const f32x4 *>(p.part_o + i * D + d);
         }
         *reinterpret_cast<f32x4 *>(&sum[part][d]) = o;
-        if (d == 0) lsum[part] = l;
     }
     __syncthreads();
     if (threadIdx.x >= D) return;
-    float l = 0.0f, o = 0.0f;
+    float o = 0.0f;
 #pragma unroll
-    for (int w = 0; w < W; w++) l += lsum[w], o += sum[w][threadIdx.x];
+    for (int w = 0; w < W; w++) o += sum[w][threadIdx.x];
     uint16_t *out = reinterpret_cast<uint16_t *>(p.a.d_out) + ((uint64_t)rq.q0 + col / p.group) * p.a.out_token_stride +
                     (h * p.group + col % p.group) * p.a.out_head_stride;
-    out[threadIdx.x] = (uint16_t)f32_to_half<DT>(l != 0.0f ? o / l : 0.0f);
+    const float root = half_rise(rise > -__builtin_inff() ? rise : __builtin_inff());
+    out[threadIdx.x] = (uint16_t)f32_to_half<DT>(l != 0.0f ? o / l * root * root : 0.0f);
 }
 
 // ---------------------------------------------------------------- many columns
@@ -394,6 +455,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p) {
 // 4100 cached tokens, 32 heads on 8, 434 us (770 TFLOP/s).  4 waves of 32
 // columns instead of 8 take 780 us there (each tile's codes are converted for
 // half the columns).
+//
+// Where all of a tile's V scales lie within 2^20 of the column's rise, m and M
+// move together by w alone: m is then within 28 of the largest z, which costs
+// l nothing.
 //
 // Rows of a prompt: NW waves of 32 columns (32 x 32 x 16 tiles) share tiles of
 // 64 tokens, which the workgroup turns into f16 once, in LDS.  Rows of LDS
@@ -409,7 +474,7 @@ __global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
     constexpr int CODES = 64 * D / 16, PER = (CODES + T - 1) / T;  // 16-byte pieces of a tile's codes
     __shared__ __align__(16) _Float16 lk[2][64 * KP];
     __shared__ __align__(16) _Float16 lv[2][D * VP];
-    __shared__ __align__(16) float lks[2][4], lvs[2][4];
+    __shared__ __align__(16) float lks[2][4], lvs[2][4];  // K's scales, logarithms of V's
     const uint32_t r = blockIdx.x / p.tiles, tile = p.tiles - 1 - blockIdx.x % p.tiles, h = blockIdx.y;
     const Request rq = request_of(p, r);
     const uint32_t cols = columns_of(p, rq);
@@ -442,7 +507,8 @@ __global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
     for (int t = 0; t < VT; t++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[t][i] = 0.0f;
-    float m = -__builtin_inff(), l = 0.0f, top = 0.0f, log_top = -__builtin_inff();
+    Tops tops;
+    float l = 0.0f;
 
     // A tile's codes on the way: pieces of 16 dimensions of a token, of 16
     // tokens of a dimension.  The blocks' ids come a tile ahead of the codes,
@@ -475,7 +541,7 @@ __global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
             const uint32_t bh = (in ? is : 0) * p.cache.kv_heads + h;
             // a run without a block: marked by a negative scale
             ksc = in ? p.cache.d_k_scale[bh] : -1.0f;
-            vsc = in ? p.cache.d_v_scale[bh] : 0.0f;
+            vsc = log2f(in ? p.cache.d_v_scale[bh] : 0.0f);
         }
     };
     auto stage = [&](int b) {
@@ -516,12 +582,12 @@ __global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
                 s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[f], s[t], 0, 0, 0);
             }
         }
-        float c[4], vs[4], vt = 0.0f;
+        float c[4], log_vs[4];
         bool masked = base + 64 > all;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float ks = lks[b][i];
-            vs[i] = lvs[b][i], vt = fmaxf(vt, vs[i]);
+            log_vs[i] = lvs[b][i];
             c[i] = ks * zs;
             masked = masked || ks < 0.0f;
         }
@@ -542,30 +608,44 @@ __global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
 #pragma unroll
             for (int i = 0; i < 4; i++) c[i] = 1.0f;
         }
-        float zm = -__builtin_inff();
+        float um[4], share[4], far = 0.0f, zm = -__builtin_inff(), wm = -__builtin_inff();
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            float um = s[u >> 1][8 * (u & 1)];
+            um[u] = s[u >> 1][8 * (u & 1)];
 #pragma unroll
-            for (int i = 1; i < 8; i++) um = fmaxf(um, s[u >> 1][8 * (u & 1) + i]);
-            zm = fmaxf(zm, um * c[u]);
+            for (int i = 1; i < 8; i++) um[u] = fmaxf(um[u], s[u >> 1][8 * (u & 1) + i]);
+            wm = fmaxf(wm, fmaf(um[u], c[u], log_vs[u]));
+            share[u] = log_vs[u] - tops.rise;
+            far = fmaxf(far, fabsf(share[u]));
         }
-        zm = fmaxf(zm, __shfl_xor(zm, 32));
-        if (__any(zm > m + kSlack || vt > top)) {
-            const float mn = zm > m + kSlack ? zm : m, tn = fmaxf(top, vt);
-            const float again = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f, of = again * (tn > top ? top / tn : 1.0f);
-            m = mn, top = tn, log_top = __builtin_amdgcn_logf(tn);
-            l *= again;
+        wm = max_across_32(wm);
+        const bool near = __all(far <= kNear);
+        if (!near) {
+#pragma unroll
+            for (int u = 0; u < 4; u++) zm = fmaxf(zm, um[u] * c[u]);
+            zm = max_across_32(zm);
+        }
+        if (__any(tops.passed(zm, wm))) {
+            float of_l, of_o;
+            if (near)
+                of_l = of_o = tops.move(wm);
+            else
+                tops.take(zm, wm, of_l, of_o);
+            l *= of_l;
 #pragma unroll
             for (int t = 0; t < VT; t++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[t][i] *= of;
+                for (int i = 0; i < 16; i++) o[t][i] *= of_o;
         }
-        const float ref = m == -__builtin_inff() ? 0.0f : m;
+        if (!near) {
+#pragma unroll
+            for (int u = 0; u < 4; u++) share[u] = share_of(log_vs[u], tops.rise);
+        }
+        const float ref = base_of(tops.m);
         f16x8 pv[4];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const float share = share_of(vs[u], log_top), less = share - ref;
+            const float less = share[u] - ref;
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -573,7 +653,7 @@ __global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
                 sum += e;
                 pv[u][i] = (_Float16)e;
             }
-            l = fmaf(sum, __builtin_amdgcn_exp2f(-share), l);
+            l = fmaf(sum, __builtin_amdgcn_exp2f(-share[u]), l);
         }
 #pragma unroll
         for (int t = 0; t < VT; t++)
@@ -588,14 +668,14 @@ __global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
     uint16_t *out = reinterpret_cast<uint16_t *>(p.a.d_out) + ((uint64_t)rq.q0 + qi) * p.a.out_token_stride +
                     qh * p.a.out_head_stride;
     const bool wide = !((uintptr_t)p.a.d_out & 7u) && !((p.a.out_token_stride | p.a.out_head_stride) & 3u);
-    const float inv = l != 0.0f ? top / l : 0.0f;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f, root = half_rise(tops.rise);
 #pragma unroll
     for (int t = 0; t < VT; t++)
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = o[t][i + e] * inv;
+            for (int e = 0; e < 4; e++) v[e] = o[t][i + e] * inv * root * root;
             store4<DT>(out + 32 * t + 2 * i + 4 * hl, wide, v);
         }
 }
@@ -679,7 +759,7 @@ extern "C" int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, co
     if (cache->kv_heads * 16ull > 65535) return HH_ERR_UNSUPPORTED;
     if (p.splits > 1) {
         const uint64_t n = lanes * p.splits * p.cols;
-        const int32_t e = hh::ensure_scratch(ctx, n * (cache->head_dim + 2) * sizeof(float));
+        const int32_t e = hh::ensure_scratch(ctx, n * (cache->head_dim + 3) * sizeof(float));
         if (e != HH_OK) return e;
         p.part_o = reinterpret_cast<float *>(ctx->d_scratch);
         p.part_ml = p.part_o + n * cache->head_dim;

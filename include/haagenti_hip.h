@@ -801,8 +801,10 @@ int32_t hh_kv_read(hh_context *ctx, const hh_kv_cache *cache, const int32_t *d_b
  * max_kv bound a request's rows and tokens (what lies beyond is not
  * computed / not seen): they choose how the work is split, so bounds near
  * the real sizes are faster.  Sums, maxima and accumulators are f32, codes
- * are exact, the probabilities times their block's scale are rounded to f16
- * (11 bits) for the second product, the output once at the end. */
+ * are exact, the output is rounded once at the end.  A row's probabilities
+ * times their blocks' scales are rounded to f16 for the second product, in
+ * units of the largest of them: 11 bits down to 2^-14 of it, 2^-25 of it
+ * below.  Tokens that a row doesn't see have no part in that. */
 typedef struct hh_kv_attention_args {
     const void *d_q;
     void *d_out;
