@@ -254,7 +254,7 @@ class KvCache:
         (hh_kv_attention): q rows x q_heads x head_dim; table (requests x
         width), start and kv_len as kv_plan leaves them.  max_q and max_kv
         bound a request's rows and tokens (default: q's rows, the table's
-        width); scale defaults to head_dim ** -0.5."""
+        width; rows beyond give zeros, tokens beyond are not seen); scale defaults to head_dim ** -0.5."""
         ctx, shape, dt = self.ctx, q.shape, _HALF.get(q.dtype)
         if dt is None:
             _refuse(UNSUPPORTED, f"attention: {q.dtype} (float16 or bfloat16)")
@@ -271,8 +271,8 @@ class KvCache:
                 _refuse(INVALID_ARGUMENT, "attention: out is like q")
         _ints("attention", start, kv_len)
         requests, tshape, tstride = kv_len.shape[0], table.shape, table.stride()
-        if (table.dtype != torch.int32 or len(tshape) != 2 or tshape[0] != requests or (tshape[1] > 1 and tstride[1] != 1)
-                or start.numel() != requests + 1):
+        if (table.dtype != torch.int32 or len(tshape) != 2 or tshape[0] != requests or start.numel() != requests + 1
+                or (requests and tshape[1] > 1 and tstride[1] != 1)):
             _refuse(INVALID_ARGUMENT, "attention: table requests x width, start requests + 1")
         _on(ctx.device, "attention", table, start, kv_len)
         width = tshape[1]

@@ -183,15 +183,24 @@ __device__ __forceinline__ float load_query(const uint16_t *row, bool wide, floa
     return up;
 }
 
-// Rows past the last request's are zeros (one workgroup of the launch).
-__device__ __forceinline__ void zero_tail(const AttnArgs &p, uint32_t dim, uint32_t threads) {
-    const uint32_t total = p.a.tokens, from = (uint32_t)max(0, p.a.d_start[p.a.requests]);
-    uint16_t *out = reinterpret_cast<uint16_t *>(p.a.d_out);
-    for (uint64_t i = (uint64_t)from * p.a.q_heads * dim + threadIdx.x; i < (uint64_t)total * p.a.q_heads * dim;
-         i += threads) {
-        const uint64_t t = i / (p.a.q_heads * dim), e = i % (p.a.q_heads * dim);
-        out[t * p.a.out_token_stride + e / dim * p.a.out_head_stride + e % dim] = 0;
+// Zeros to rows from .. to - 1 of `heads` heads from h on (a workgroup's work).
+template <int D>
+__device__ __forceinline__ void zero_rows(const AttnArgs &p, uint32_t from, uint32_t to, uint32_t h, uint32_t heads) {
+    for (uint32_t t = from; t < to; t++) {
+        uint16_t *row = reinterpret_cast<uint16_t *>(p.a.d_out) + t * p.a.out_token_stride + h * p.a.out_head_stride;
+        for (uint32_t e = threadIdx.x; e < heads * D; e += blockDim.x) row[e / D * p.a.out_head_stride + e % D] = 0;
     }
+}
+// Rows before the first request's and past the last one's.
+template <int D>
+__device__ __forceinline__ void zero_ends(const AttnArgs &p) {
+    zero_rows<D>(p, 0, (uint32_t)min((int64_t)p.a.tokens, max((int64_t)0, (int64_t)p.a.d_start[0])), 0, p.a.q_heads);
+    zero_rows<D>(p, (uint32_t)max(0, p.a.d_start[p.a.requests]), p.a.tokens, 0, p.a.q_heads);
+}
+// A call without requests.
+template <int D>
+__global__ __launch_bounds__(256) void attn_zero_kernel(const AttnArgs p) {
+    for (uint32_t t = blockIdx.x; t < p.a.tokens; t += gridDim.x) zero_rows<D>(p, t, t + 1, 0, p.a.q_heads);
 }
 
 // 4 consecutive dimensions of an output row.
@@ -229,8 +238,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attn_step_kernel(const 
     __shared__ __align__(16) float lds_o[2][16][D + 4];
     __shared__ float lds_ml[4][16][3];
     const uint32_t r = blockIdx.x / p.splits, split = blockIdx.x % p.splits, h = blockIdx.y;
-    if (r == p.a.requests - 1 && split == 0 && h == 0) zero_tail(p, D, 256);
+    if (r == p.a.requests - 1 && split == 0 && h == 0) zero_ends<D>(p);
     const Request rq = request_of(p, r);
+    if (split == 0 && (uint32_t)rq.rows > p.a.max_q)  // rows beyond the call's bound
+        zero_rows<D>(p, (uint32_t)rq.q0 + p.a.max_q, (uint32_t)(rq.q0 + rq.rows), h * p.group, p.group);
     const uint32_t cols = columns_of(p, rq);
     if (cols == 0 || cols > p.small) return;
     const int32_t begin = (int32_t)(split * p.chunk), end = min(rq.seen, begin + (int32_t)p.chunk);
@@ -687,6 +698,10 @@ constexpr int kTileWaves = D <= 128 ? 8 : 4;
 
 template <int DT, int D>
 hipError_t launch_attention(const AttnArgs &p, hipStream_t s) {
+    if (!p.a.requests) {
+        hipLaunchKernelGGL((attn_zero_kernel<D>), dim3(p.a.tokens < 4096 ? p.a.tokens : 4096), dim3(256), 0, s, p);
+        return hipGetLastError();
+    }
     hipLaunchKernelGGL((attn_step_kernel<DT, D>), dim3(p.a.requests * p.splits, p.cache.kv_heads), dim3(256), 0, s, p);
     if (p.splits > 1)
         hipLaunchKernelGGL((attn_join_kernel<DT, D>), dim3(p.a.requests, p.cache.kv_heads * p.cols), dim3(256), 0, s, p);
@@ -717,8 +732,8 @@ extern "C" int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, co
     if (rc != HH_OK) return rc;
     if (a->dtype != HH_F16 && a->dtype != HH_BF16) return HH_ERR_UNSUPPORTED;
     if (a->q_heads == 0 || a->q_heads % cache->kv_heads) return HH_ERR_INVALID_ARGUMENT;
-    if (a->tokens == 0 || a->requests == 0) return HH_OK;
-    if (!a->d_q || !a->d_out || !a->d_start || !a->d_kv_len || (!a->d_table && a->table_width))
+    if (a->tokens == 0) return HH_OK;
+    if (!a->d_q || !a->d_out || (a->requests && (!a->d_start || !a->d_kv_len || (!a->d_table && a->table_width))))
         return HH_ERR_INVALID_ARGUMENT;
     if ((((uintptr_t)a->d_q | (uintptr_t)a->d_out) & 1u) || a->table_stride < a->table_width) return HH_ERR_INVALID_ARGUMENT;
     if (a->requests > 65536 || a->tokens >= 1u << 24) return HH_ERR_INVALID_ARGUMENT;
@@ -740,7 +755,7 @@ extern "C" int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, co
     if (kv > 1ull << 30) return HH_ERR_UNSUPPORTED;  // tokens are counted in 31 bits
     // chunks: enough workgroups for 8 per CU (48 requests 86 us; 16 per CU 95,
     // 24 per CU 87 with twice the chunks to join), none below 512 tokens
-    const uint64_t lanes = (uint64_t)a->requests * cache->kv_heads;
+    const uint64_t lanes = (uint64_t)(a->requests ? a->requests : 1) * cache->kv_heads;
     const uint64_t want = (8ull * (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256) + lanes - 1) / lanes;
     uint64_t chunk = (kv + want - 1) / want;
     chunk = (chunk + 255) / 256 * 256;
@@ -757,7 +772,7 @@ extern "C" int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, co
     if ((uint64_t)a->requests * p.splits >= 1ull << 24 || (uint64_t)a->requests * p.tiles >= 1ull << 24)
         return HH_ERR_UNSUPPORTED;
     if (cache->kv_heads * 16ull > 65535) return HH_ERR_UNSUPPORTED;
-    if (p.splits > 1) {
+    if (a->requests && p.splits > 1) {
         const uint64_t n = lanes * p.splits * p.cols;
         const int32_t e = hh::ensure_scratch(ctx, n * (cache->head_dim + 3) * sizeof(float));
         if (e != HH_OK) return e;

@@ -796,11 +796,11 @@ int32_t hh_kv_read(hh_context *ctx, const hh_kv_cache *cache, const int32_t *d_b
  * head_dim) belong to request r and are its last tokens: row i of c sees the
  * first d_kv_len[r] - c + 1 + i tokens.  Head h reads head
  * h / (q_heads / kv_heads) of the cache.  Rows that see no token (a request
- * that hh_kv_plan left out) and rows past the last request's give zeros;
- * tokens of a block id that the cache doesn't have are not seen.  max_q and
- * max_kv bound a request's rows and tokens (what lies beyond is not
- * computed / not seen): they choose how the work is split, so bounds near
- * the real sizes are faster.  Sums, maxima and accumulators are f32, codes
+ * that hh_kv_plan left out) and rows before the first request's or past the
+ * last one's give zeros; tokens of a block id that the cache doesn't have are
+ * not seen.  max_q and max_kv bound a request's rows and tokens (rows beyond
+ * give zeros, tokens beyond are not seen): they choose how the work is split,
+ * so bounds near the real sizes are faster.  Sums, maxima and accumulators are f32, codes
  * are exact, the output is rounded once at the end.  A row's probabilities
  * times their blocks' scales are rounded to f16 for the second product, in
  * units of the largest of them: 11 bits down to 2^-14 of it, 2^-25 of it
