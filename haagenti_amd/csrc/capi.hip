@@ -43,6 +43,48 @@ int32_t ensure_scratch(hh_context *ctx, size_t bytes) {
     return HH_OK;
 }
 
+int32_t op_room(hh_context *ctx, hipStream_t stream, size_t bytes, float **out) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream, &status) != hipSuccess) (void)hipGetLastError();
+    const bool captured = status == hipStreamCaptureStatusActive;
+    hh_context::Room *room = nullptr;
+    for (hh_context::Room &r : ctx->rooms)
+        if (r.stream == stream && r.captured == captured) room = &r;
+    if (!room) {
+        ctx->rooms.push_back({stream, captured, nullptr, 0});
+        room = &ctx->rooms.back();
+    }
+    if (room->bytes < bytes) {
+        // what captured calls leave behind stays: at least doubled, all of it
+        // is less than the last
+        size_t size = bytes < (1u << 20) ? (1u << 20) : bytes;
+        if (captured && size < 2 * room->bytes) size = 2 * room->bytes;
+        if (room->at && captured) {
+            ctx->kept_rooms.push_back(room->at);
+        } else if (room->at) {
+            const hipError_t e = hipFree(room->at);  // after the work that uses it
+            if (e != hipSuccess) {
+                (void)hipGetLastError();
+                return from_hip(e);
+            }
+        }
+        room->at = nullptr, room->bytes = 0;
+        // (in the default mode an allocation would end the capture)
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        const bool relaxed = captured && hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+        const hipError_t e = hipMalloc(&room->at, size);
+        if (e != hipSuccess) {
+            room->at = nullptr;
+            (void)hipGetLastError();  // reported here, not by the next call's launch check
+        }
+        if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
+        if (e != hipSuccess) return from_hip(e);
+        room->bytes = size;
+    }
+    *out = reinterpret_cast<float *>(room->at);
+    return HH_OK;
+}
+
 uint8_t *host_stage(hh_context *ctx, size_t bytes, size_t keep) {
     if (bytes <= ctx->stage_bytes) return ctx->h_stage;
     if (bytes > kHostStageMax) return nullptr;
@@ -198,6 +240,9 @@ void hh_context_destroy(hh_context *ctx) {
     if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
     if (ctx->d_basis) (void)hipFree(ctx->d_basis);
     if (ctx->d_scratch) (void)hipFree(ctx->d_scratch);
+    for (const hh_context::Room &r : ctx->rooms)
+        if (r.at) (void)hipFree(r.at);
+    for (void *p : ctx->kept_rooms) (void)hipFree(p);
     if (ctx->h_stage) (void)hipHostFree(ctx->h_stage);
     if (ctx->fork) (void)hipEventDestroy(ctx->fork);
     if (ctx->join) (void)hipEventDestroy(ctx->join);

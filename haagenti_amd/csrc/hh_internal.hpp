@@ -21,6 +21,18 @@ struct hh_context {
     // (grown on demand, kept until the context is destroyed).
     void *d_scratch = nullptr;
     size_t scratch_bytes = 0;
+    // Partial sums of hh_linear and hh_kv_attention: memory per stream, so
+    // that calls on several streams don't share it, and apart for calls that
+    // are captured, whose graphs go on using it; what such calls have grown
+    // out of is kept for their graphs (op_room, capi.hip).
+    struct Room {
+        hipStream_t stream = nullptr;
+        bool captured = false;
+        void *at = nullptr;
+        size_t bytes = 0;
+    };
+    std::vector<Room> rooms;
+    std::vector<void *> kept_rooms;
     // Pinned host memory for what the synchronous entry points upload and
     // fetch: index tables, statuses, a container's bytes.  Grown on demand up
     // to hh::kHostStageMax, kept until the context is destroyed; free
@@ -86,6 +98,10 @@ int32_t check_hctt_tensor(const hh_hctt_tensor &T, size_t *ntiles);
 // (capi.hip).
 int32_t from_hip(hipError_t e);
 int32_t ensure_scratch(hh_context *ctx, size_t bytes);
+// Device memory of at least `bytes` for one call's partial sums on `stream`,
+// valid until the next call of this on the same stream (capi.hip).  The
+// context's device is current.
+int32_t op_room(hh_context *ctx, hipStream_t stream, size_t bytes, float **out);
 // ctx->h_stage grown to at least `bytes` with its first `keep` bytes kept
 // (capi.hip); nullptr above kHostStageMax or when the memory is not to be
 // had, in which case the caller takes ordinary memory.  The context's device

@@ -774,9 +774,9 @@ extern "C" int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, co
     if (cache->kv_heads * 16ull > 65535) return HH_ERR_UNSUPPORTED;
     if (a->requests && p.splits > 1) {
         const uint64_t n = lanes * p.splits * p.cols;
-        const int32_t e = hh::ensure_scratch(ctx, n * (cache->head_dim + 3) * sizeof(float));
+        const int32_t e = hh::op_room(ctx, reinterpret_cast<hipStream_t>(stream), n * (cache->head_dim + 3) * sizeof(float),
+                                      &p.part_o);
         if (e != HH_OK) return e;
-        p.part_o = reinterpret_cast<float *>(ctx->d_scratch);
         p.part_ml = p.part_o + n * cache->head_dim;
     }
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);

@@ -720,13 +720,11 @@ constexpr Shape kLargeShapes[] = {{256, 256, 1, 1.65, 1.65}, {256, 128, 1, 1.0, 
                                   {128, 128, 2, 1.13, 0.67}, {128, 64, 3, 1.0, 0.45}};
 constexpr Shape kAnyShapes[] = {{128, 128, 2, 2.0, 1.3}, {64, 64, 4, 1.6, 0.9}};
 
-// Room for the splits' sums in the context's scratch.
-int32_t split_room(hh_context *ctx, const LinearArgs &p, const TilePlan &plan, Split *split) {
+// Room for the splits' sums.
+int32_t split_room(hh_context *ctx, const LinearArgs &p, const TilePlan &plan, hipStream_t s, Split *split) {
     *split = {plan.steps, nullptr};
     if (plan.splits == 1) return HH_OK;
-    const int32_t rc = ensure_scratch(ctx, (size_t)plan.splits * p.a.m * ((p.a.n + 3) / 4 * 4) * sizeof(float));
-    split->partial = reinterpret_cast<float *>(ctx->d_scratch);
-    return rc;
+    return op_room(ctx, s, (size_t)plan.splits * p.a.m * ((p.a.n + 3) / 4 * 4) * sizeof(float), &split->partial);
 }
 template <int DT, int YT>
 int32_t join_splits(const LinearArgs &p, const TilePlan &plan, const Split &split, hipStream_t s) {
@@ -742,7 +740,7 @@ int32_t launch_any(hh_context *ctx, const LinearArgs &p, int cus, hipStream_t s)
     const uint32_t n = p.a.n, m = p.a.m;
     const TilePlan plan = plan_tiles(p.a, cus, kAnyShapes);
     Split split;
-    const int32_t rc = split_room(ctx, p, plan, &split);
+    const int32_t rc = split_room(ctx, p, plan, s, &split);
     if (rc != HH_OK) return rc;
     const uint32_t S = kAnyShapes[plan.shape].n;
     const dim3 grid((n + S - 1) / S, (m + S - 1) / S, plan.splits);
@@ -776,7 +774,7 @@ int32_t launch_linear(hh_context *ctx, const LinearArgs &p, hipStream_t s) {
     if (!aligned) return launch_any<DT, YT, kHalf>(ctx, p, cus, s);
     const TilePlan plan = plan_tiles(a, cus, kLargeShapes);
     Split split;
-    const int32_t rc = split_room(ctx, p, plan, &split);
+    const int32_t rc = split_room(ctx, p, plan, s, &split);
     if (rc != HH_OK) return rc;
     switch (plan.shape) {
         case 0: launch_tiles<DT, YT, 256, 256, 2, 4>(p, split, plan.splits, s); break;

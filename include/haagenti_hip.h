@@ -18,7 +18,7 @@
  * (LZ4 scratch, whole-matrix transform buffers and tables) is shared by its
  * calls, so the asynchronous calls of one context must be ordered: the
  * same stream, or a synchronisation between calls made on different
- * streams.  Host-pointer entry points are
+ * streams (the decoder layer operators excepted).  Host-pointer entry points are
  * synchronous.  Every entry point makes the context's device current while
  * it runs and restores the calling thread's current device before it
  * returns.
@@ -684,11 +684,13 @@ int32_t hh_spectral_encode_from_dct(const float *coeffs, uint32_t width, uint32_
  * counterpart in the reference, which stops at the decoded tensor.  All are
  * asynchronous on the stream and read lengths, tables and slots from device
  * memory, so a step needs no host synchronisation.  Strides are in elements.
- * hh_linear and hh_kv_attention may keep partial sums in the context's
- * scratch, which grows with the largest call so far: after a first call of
- * the same sizes a call allocates nothing and may be captured.  A later call
- * that needs more moves the scratch, and what was captured before must be
- * captured again. */
+ * hh_linear and hh_kv_attention may keep partial sums in memory that the
+ * context holds for each stream, grown with the largest call there so far, so
+ * their calls on several streams need no order among them.  All may be
+ * captured: captured calls have memory of their own, which stays as it is
+ * until the context is destroyed, whatever is called later (a context outlives
+ * the graphs that were captured with it).  Graphs captured on one stream share
+ * it and so must not run beside each other. */
 
 typedef enum hh_activation {
     HH_ACT_NONE = 0,

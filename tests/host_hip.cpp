@@ -105,6 +105,20 @@ hipError_t hipStreamDestroy(hipStream_t s) {
     std::free(s);
     return hipSuccess;
 }
+// Whether streams are being captured, and the thread's capture mode.
+static bool capturing = false;
+static hipStreamCaptureMode capture_mode = hipStreamCaptureModeGlobal;
+void host_hip_capture(int on) { capturing = on; }
+hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus *s) {
+    *s = capturing ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone;
+    return hipSuccess;
+}
+hipError_t hipThreadExchangeStreamCaptureMode(hipStreamCaptureMode *m) {
+    const hipStreamCaptureMode old = capture_mode;
+    capture_mode = *m;
+    *m = old;
+    return note(capture_mode == hipStreamCaptureModeRelaxed ? "relaxed" : "global", hipErrorInvalidValue);
+}
 hipError_t hipStreamSynchronize(hipStream_t) { return note("synchronize", hipErrorUnknown); }
 
 }  // extern "C"
