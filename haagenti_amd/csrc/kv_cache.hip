@@ -147,6 +147,15 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(const hh_kv_plan_
         p.d_slots[i] = -1;
 }
 
+// The plan's inputs where its results go over them: to[0..1] the state, then
+// the lengths, then the new rows.
+__global__ __launch_bounds__(kPlanThreads) void plan_inputs_kernel(const int32_t *state, const int32_t *len, const int32_t *add,
+                                                                   uint32_t requests, int32_t *to) {
+    const uint32_t i = blockIdx.x * kPlanThreads + threadIdx.x;
+    if (i < 2) to[i] = state[i];
+    if (i < requests) to[2 + i] = len[i], to[2 + requests + i] = add[i];
+}
+
 // ---------------------------------------------------------------- append
 //
 // A run is the rows of one block: consecutive slots.  A workgroup takes the
@@ -460,16 +469,38 @@ int32_t hh_kv_plan(hh_context *ctx, const hh_kv_plan_args *a, void *stream) {
         return HH_ERR_INVALID_ARGUMENT;
     if (a->table_stride < a->table_width || a->tokens >= 1u << 31 || a->ring_capacity >= 1u << 31)
         return HH_ERR_INVALID_ARGUMENT;
-    // a step reads the state in every workgroup and writes the next one
     if (a->d_state < a->d_state_out + 2 && a->d_state_out < a->d_state + 2) return HH_ERR_INVALID_ARGUMENT;
     hh::DeviceGuard guard(ctx->device);
     if (guard.status() != hipSuccess) return hh::from_hip(guard.status());
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    // every workgroup reads the state and all lengths while others write
+    // their results: inputs that these go over are set aside first
+    const uint64_t n = a->requests;
+    const struct {
+        const int32_t *at;
+        uint64_t n;
+    } in[] = {{a->d_len, n}, {a->d_new, n}, {a->d_state, 2}},
+      out[] = {{a->d_start, n + 1}, {a->d_kv_len, n}, {a->d_slots, a->tokens}, {a->d_status, n}, {a->d_state_out, 2}};
+    bool over = false;
+    for (const auto &i : in)
+        for (const auto &o : out) over = over || (i.n && o.n && i.at < o.at + o.n && o.at < i.at + i.n);
+    hh_kv_plan_args p = *a;
+    if (over) {
+        float *room = nullptr;
+        const int32_t rc = hh::op_room(ctx, s, (2 * n + 2) * sizeof(int32_t), &room);
+        if (rc != HH_OK) return rc;
+        int32_t *to = reinterpret_cast<int32_t *>(room);
+        hipLaunchKernelGGL(hh::plan_inputs_kernel, dim3((uint32_t)(n / hh::kPlanThreads) + 1), dim3(hh::kPlanThreads), 0, s,
+                           a->d_state, a->d_len, a->d_new, a->requests, to);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return hh::from_hip(e);
+        p.d_state = to, p.d_len = to + 2, p.d_new = to + 2 + n;
+    }
     const uint32_t columns = a->requests < 1 ? 1 : a->requests < hh::kPlanColumns ? a->requests : hh::kPlanColumns;
     // prompts of thousands of rows: up to 8 workgroups to a request
     const uint32_t per = a->tokens / columns / (4 * hh::kPlanThreads);
     const uint32_t rows = per < 1 ? 1 : per > 8 ? 8 : per;
-    hipLaunchKernelGGL(hh::kv_plan_kernel, dim3(columns, rows), dim3(hh::kPlanThreads), 0,
-                       reinterpret_cast<hipStream_t>(stream), *a);
+    hipLaunchKernelGGL(hh::kv_plan_kernel, dim3(columns, rows), dim3(hh::kPlanThreads), 0, s, p);
     return hh::from_hip(hipGetLastError());
 }
 

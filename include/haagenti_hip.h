@@ -752,9 +752,11 @@ typedef struct hh_kv_cache {
  * Writes d_start[requests + 1] (first row of each request's new tokens: the
  * running sum of max(d_new, 0)), d_kv_len (tokens held after the step),
  * d_slots[tokens] (the slot of each new row, -1 past the last row), d_status
- * and d_state_out (which is not d_state: give it to the next step).
+ * and d_state_out (which is not d_state: give it to the next step).  d_kv_len
+ * may be d_len: an update in place, at the cost of one more launch.
  * A request that can't be served takes no block, its slots are -1, its
- * d_kv_len is 0 and d_status names why: HH_ERR_OUT_OF_MEMORY where the free
+ * d_kv_len is 0 (what it had cached is still there: its length remains the
+ * one that d_len gave) and d_status names why: HH_ERR_OUT_OF_MEMORY where the free
  * blocks are used up (requests after it that need none are served),
  * HH_ERR_BUFFER_TOO_SMALL where its row of d_table or d_slots is too short,
  * HH_ERR_INVALID_ARGUMENT for a negative length. */
