@@ -722,6 +722,22 @@ hipError_t launch_dim(const AttnArgs &p, hipStream_t s) {
     }
 }
 
+// Whether two rows of `dim` elements, `tokens` of them `ts` apart for each of
+// `heads` heads `hs` apart, share an element.
+bool rows_meet(uint64_t tokens, uint64_t heads, uint64_t ts, uint64_t hs, uint64_t dim) {
+    typedef unsigned __int128 u128;
+    if (tokens > 1 && ts < dim) return true;
+    if (heads > 1 && hs < dim) return true;
+    if (tokens == 1 || heads == 1 || ts >= (u128)(heads - 1) * hs + dim || hs >= (u128)(tokens - 1) * ts + dim) return false;
+    // neither stride spans the other: heads j apart against the tokens next to that
+    for (uint64_t j = 1; j < heads; j++) {
+        const u128 d = (u128)j * hs, below = d / ts, rest = d % ts;
+        if (below < tokens && rest < dim) return true;
+        if (below + 1 < tokens && ts - rest < dim) return true;
+    }
+    return false;
+}
+
 }  // namespace
 }  // namespace hh
 
@@ -736,6 +752,8 @@ extern "C" int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, co
     if (!a->d_q || !a->d_out || (a->requests && (!a->d_start || !a->d_kv_len || (!a->d_table && a->table_width))))
         return HH_ERR_INVALID_ARGUMENT;
     if ((((uintptr_t)a->d_q | (uintptr_t)a->d_out) & 1u) || a->table_stride < a->table_width) return HH_ERR_INVALID_ARGUMENT;
+    if (hh::rows_meet(a->tokens, a->q_heads, a->out_token_stride, a->out_head_stride, cache->head_dim))
+        return HH_ERR_INVALID_ARGUMENT;
     if (a->requests > 65536 || a->tokens >= 1u << 24) return HH_ERR_INVALID_ARGUMENT;
     const uint32_t group = a->q_heads / cache->kv_heads;
     const uint64_t most = (uint64_t)(a->max_q < a->tokens ? a->max_q : a->tokens) * group;
