@@ -77,6 +77,26 @@ def _rows(t, m, n, dev, what):
     return stride[0] if m > 1 else n
 
 
+def _apart(a, b):
+    """Whether two matrices with contiguous rows share no memory (columns of
+    one buffer's rows side by side are apart)."""
+    spans = []
+    for t in (a, b):
+        size = t.element_size()
+        rows, width = (t.shape[0], t.shape[1]) if t.dim() == 2 else (1, t.numel())
+        stride = t.stride(0) if rows > 1 else width
+        if not rows or not width:
+            return True
+        spans.append((t.data_ptr(), stride * size, width * size, t.data_ptr() + ((rows - 1) * stride + width) * size))
+    (a0, a_step, a_width, a1), (b0, b_step, b_width, b1) = spans
+    if a1 <= b0 or b1 <= a0:
+        return True
+    if a_step != b_step or not a_step:
+        return False
+    between = (b0 - a0) % a_step
+    return between >= a_width and between + b_width <= a_step
+
+
 def linear(ctx, x, w, bias=None, act=None, mul=None, residual=None, out=None, out_dtype=None):
     """act(x w^T + bias) * mul + residual (hh_linear).  x: m x k, float16 or
     bfloat16; w: n x k of x's type, or an Int4Weight; bias n values, mul and
@@ -117,6 +137,12 @@ def linear(ctx, x, w, bias=None, act=None, mul=None, residual=None, out=None, ou
         if out_dtype is not None and y_dtype is not out_dtype:
             _refuse(INVALID_ARGUMENT, "linear: out has another type than out_dtype")
         y_stride = _rows(out, m, n, dev, "out")
+        for t in (x, w, bias, mul, residual):
+            # (a weight's buffer is compared whole)
+            if t is not None and not _apart(out, t) and not (
+                    (t is mul or t is residual) and t.data_ptr() == out.data_ptr() and t.dtype is y_dtype
+                    and (m == 1 or t.stride(0) == y_stride)):
+                _refuse(INVALID_ARGUMENT, "linear: out lies over what is read (other than mul or residual itself)")
     b = c = d = c_stride = d_stride = 0
     if bias is not None:
         if bias.dim() != 1 or bias.shape[0] != n or bias.dtype is not dtype or not bias.is_contiguous():
