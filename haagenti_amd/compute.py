@@ -7,7 +7,9 @@ current stream, where their results are allocated, and don't synchronise.
 Calls on several streams need no order among them; captured calls keep their
 memory for as long as the context lives, whatever is called later (graphs
 captured on one stream must not run beside each other).
-What a call can't take raises HaagentiError before anything is launched."""
+What a call can't take raises HaagentiError before anything is launched;
+there are no gradients, so tensors that require them are taken under
+torch.no_grad() only."""
 import ctypes as C
 import struct
 
@@ -42,6 +44,12 @@ _stream = torch._C._cuda_getCurrentRawStream
 
 def _refuse(code, what):
     raise HaagentiError(code, what)
+
+
+def _no_grad(what):
+    """For a tensor that requires gradients: refuses it where autograd is asked to follow."""
+    if torch.is_grad_enabled():
+        _refuse(UNSUPPORTED, f"{what}: no gradients (call it under torch.no_grad())")
 
 
 def _on(dev, what, *tensors):
@@ -121,6 +129,8 @@ def linear(ctx, x, w, bias=None, act=None, mul=None, residual=None, out=None, ou
             _refuse(INVALID_ARGUMENT, "linear: w is n x k of x's type, or an Int4Weight")
         n, w_dtype, w_bytes = w.shape[0], dt, 0
         w_stride = _rows(w, n, k, dev, "w")
+    if x.requires_grad or w.requires_grad:
+        _no_grad("linear")
     code = ACTIVATIONS.get(act)
     if code is None:
         _refuse(UNSUPPORTED, f"linear: activation {act!r}")
@@ -143,20 +153,28 @@ def linear(ctx, x, w, bias=None, act=None, mul=None, residual=None, out=None, ou
                     (t is mul or t is residual) and t.data_ptr() == out.data_ptr() and t.dtype is y_dtype
                     and (m == 1 or t.stride(0) == y_stride)):
                 _refuse(INVALID_ARGUMENT, "linear: out lies over what is read (other than mul or residual itself)")
+        if out.requires_grad:
+            _no_grad("linear")
     b = c = d = c_stride = d_stride = 0
     if bias is not None:
         if bias.dim() != 1 or bias.shape[0] != n or bias.dtype is not dtype or not bias.is_contiguous():
             _refuse(INVALID_ARGUMENT, "linear: bias is n contiguous values of x's type")
         _on(dev, "linear", bias)
+        if bias.requires_grad:
+            _no_grad("linear")
         b = bias.data_ptr()
     if mul is not None:
         c, c_stride = mul.data_ptr(), _rows(mul, m, n, dev, "mul")
         if mul.dtype is not dtype:
             _refuse(INVALID_ARGUMENT, "linear: mul has x's type")
+        if mul.requires_grad:
+            _no_grad("linear")
     if residual is not None:
         d, d_stride = residual.data_ptr(), _rows(residual, m, n, dev, "residual")
         if residual.dtype is not dtype:
             _refuse(INVALID_ARGUMENT, "linear: residual has x's type")
+        if residual.requires_grad:
+            _no_grad("linear")
     rc = _linear(ctx.handle, _LINEAR.pack(x.data_ptr(), w.data_ptr(), b, c, d, out.data_ptr(), x_stride, w_stride, c_stride,
                                           d_stride, y_stride, w_bytes, m, n, k, dt, w_dtype, _CODE[y_dtype], code),
                  _stream(dev))
@@ -252,6 +270,8 @@ class KvCache:
         ctx, rows, dt = self.ctx, k.shape[0], _HALF.get(k.dtype)
         if dt is None:
             _refuse(UNSUPPORTED, f"append: {k.dtype} (float16 or bfloat16)")
+        if k.requires_grad or v.requires_grad:
+            _no_grad("append")
         tk, hk = self._heads(k, rows, self.kv_heads, "append: k")
         tv, hv = self._heads(v, rows, self.kv_heads, "append: v")
         if v.dtype is not k.dtype or slots.dim() != 1 or slots.shape[0] != rows:
@@ -289,6 +309,8 @@ class KvCache:
             _refuse(UNSUPPORTED, f"attention: {q.dtype} (float16 or bfloat16)")
         if len(shape) != 3:
             _refuse(INVALID_ARGUMENT, "attention: q is rows x q_heads x head_dim")
+        if q.requires_grad or (out is not None and out.requires_grad):
+            _no_grad("attention")
         tokens, heads = shape[0], shape[1]
         tq, hq = self._heads(q, tokens, heads, "attention: q")
         if out is None:
