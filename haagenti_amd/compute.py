@@ -73,12 +73,14 @@ class Int4Weight:
         if data.dtype != torch.uint8 or not data.is_contiguous():
             _refuse(INVALID_ARGUMENT, "Int4Weight: a contiguous uint8 tensor")
         self.data, self.n, self.k = data, int(n), int(k)
+        if self.n < 0 or self.k < 0:
+            _refuse(INVALID_ARGUMENT, "Int4Weight: a negative size")
 
 
 def _rows(t, m, n, dev, what):
     """Row stride of an m x n matrix on the device whose rows are contiguous."""
     shape, stride = t.shape, t.stride()
-    if len(shape) != 2 or shape[0] != m or shape[1] != n or (n > 1 and stride[1] != 1):
+    if len(shape) != 2 or shape[0] != m or shape[1] != n or (n > 1 and stride[1] != 1 and m):
         _refuse(INVALID_ARGUMENT, f"linear: {what} is {m} x {n} with contiguous rows, got {tuple(shape)}")
     if t.get_device() != dev:
         _refuse(INVALID_ARGUMENT, f"linear: {what} must be on the context's device")
@@ -125,7 +127,7 @@ def linear(ctx, x, w, bias=None, act=None, mul=None, residual=None, out=None, ou
         w = w.data
         _on(dev, "linear", w)
     else:
-        if w.dtype != dtype:
+        if w.dtype != dtype or w.dim() != 2:
             _refuse(INVALID_ARGUMENT, "linear: w is n x k of x's type, or an Int4Weight")
         n, w_dtype, w_bytes = w.shape[0], dt, 0
         w_stride = _rows(w, n, k, dev, "w")
@@ -175,9 +177,12 @@ def linear(ctx, x, w, bias=None, act=None, mul=None, residual=None, out=None, ou
             _refuse(INVALID_ARGUMENT, "linear: residual has x's type")
         if residual.requires_grad:
             _no_grad("linear")
-    rc = _linear(ctx.handle, _LINEAR.pack(x.data_ptr(), w.data_ptr(), b, c, d, out.data_ptr(), x_stride, w_stride, c_stride,
-                                          d_stride, y_stride, w_bytes, m, n, k, dt, w_dtype, _CODE[y_dtype], code),
-                 _stream(dev))
+    try:
+        args = _LINEAR.pack(x.data_ptr(), w.data_ptr(), b, c, d, out.data_ptr(), x_stride, w_stride, c_stride, d_stride,
+                            y_stride, w_bytes, m, n, k, dt, w_dtype, _CODE[y_dtype], code)
+    except struct.error:
+        _refuse(INVALID_ARGUMENT, f"linear: {m} x {n} x {k}")
+    rc = _linear(ctx.handle, args, _stream(dev))
     if rc:
         _check(rc, "hh_linear")
     return out
@@ -203,14 +208,14 @@ def kv_plan(ctx, lens, new, table, ring, state, block_size, tokens):
     lens, new (requests), table (requests x width, updated), ring and state
     (the free queue; ring is updated, the next state returned).  tokens: room
     for the step's new rows."""
-    requests, dev, shape = lens.shape[0], ctx.device, table.shape
+    requests, dev, shape = lens.numel(), ctx.device, table.shape
     _ints("kv_plan", lens, new, ring, state)
-    if (table.dtype != torch.int32 or len(shape) != 2 or shape[0] != requests or (shape[1] > 1 and table.stride(1) != 1)
-            or new.shape != lens.shape or lens.dim() != 1 or state.numel() != 2):
+    if (table.dtype != torch.int32 or len(shape) != 2 or shape[0] != requests or new.shape != lens.shape or lens.dim() != 1
+            or state.numel() != 2 or (requests and shape[1] > 1 and table.stride(1) != 1)):
         _refuse(INVALID_ARGUMENT, "kv_plan: lens and new per request, table requests x width, state of 2")
     _on(dev, "kv_plan", lens, new, table, ring, state)
-    if tokens < 0:
-        _refuse(INVALID_ARGUMENT, "kv_plan: room for a negative number of rows")
+    if not 0 <= tokens < 1 << 31 or not 0 <= block_size < 1 << 31:
+        _refuse(INVALID_ARGUMENT, "kv_plan: sizes below 2^31")
     # one allocation: start, kv_len, status, state, slots
     buf = lens.new_empty(3 * requests + 3 + tokens)
     at = buf.data_ptr()
@@ -230,6 +235,8 @@ class KvCache:
     (blocks, heads); byte c stands for (c - 128) * scale."""
 
     def __init__(self, ctx, k, v, k_scale, v_scale):
+        if k.dim() != 4:
+            _refuse(INVALID_ARGUMENT, "KvCache: k is blocks x heads x block_size x dim")
         blocks, heads, block_size, dim = k.shape
         if k.dtype != torch.uint8 or v.dtype != torch.uint8 or k_scale.dtype != torch.float32 \
                 or v_scale.dtype != torch.float32:
@@ -258,7 +265,7 @@ class KvCache:
     def _heads(self, t, rows, heads, what):
         """Row and head strides of rows x heads x head_dim on the device."""
         shape, stride = t.shape, t.stride()
-        if len(shape) != 3 or shape[0] != rows or shape[1] != heads or shape[2] != self.head_dim or stride[2] != 1:
+        if len(shape) != 3 or shape[0] != rows or shape[1] != heads or shape[2] != self.head_dim or (stride[2] != 1 and rows):
             _refuse(INVALID_ARGUMENT, f"{what}: {rows} x {heads} x {self.head_dim}, contiguous dimensions")
         if t.get_device() != self.ctx.device:
             _refuse(INVALID_ARGUMENT, f"{what} must be on the context's device")
@@ -267,14 +274,14 @@ class KvCache:
     def append(self, k, v, slots):
         """Rows k and v (rows x kv_heads x head_dim; any row and head strides)
         at slots (hh_kv_append)."""
-        ctx, rows, dt = self.ctx, k.shape[0], _HALF.get(k.dtype)
+        ctx, rows, dt = self.ctx, slots.numel(), _HALF.get(k.dtype)
         if dt is None:
             _refuse(UNSUPPORTED, f"append: {k.dtype} (float16 or bfloat16)")
         if k.requires_grad or v.requires_grad:
             _no_grad("append")
         tk, hk = self._heads(k, rows, self.kv_heads, "append: k")
         tv, hv = self._heads(v, rows, self.kv_heads, "append: v")
-        if v.dtype is not k.dtype or slots.dim() != 1 or slots.shape[0] != rows:
+        if v.dtype is not k.dtype or slots.dim() != 1:
             _refuse(INVALID_ARGUMENT, "append: k, v and slots have the same rows, k and v the same type")
         _ints("append", slots)
         _on(ctx.device, "append", slots)
@@ -321,8 +328,8 @@ class KvCache:
             if out.dtype is not q.dtype:
                 _refuse(INVALID_ARGUMENT, "attention: out is like q")
         _ints("attention", start, kv_len)
-        requests, tshape, tstride = kv_len.shape[0], table.shape, table.stride()
-        if (table.dtype != torch.int32 or len(tshape) != 2 or tshape[0] != requests or start.numel() != requests + 1
+        requests, tshape, tstride = kv_len.numel(), table.shape, table.stride()
+        if (kv_len.dim() != 1 or table.dtype != torch.int32 or len(tshape) != 2 or tshape[0] != requests or start.numel() != requests + 1
                 or (requests and tshape[1] > 1 and tstride[1] != 1)):
             _refuse(INVALID_ARGUMENT, "attention: table requests x width, start requests + 1")
         _on(ctx.device, "attention", table, start, kv_len)
