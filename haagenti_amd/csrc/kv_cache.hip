@@ -134,7 +134,11 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(const hh_kv_plan_
         for (uint32_t i = at0; i < w.rows && w.start + i < p.tokens; i += step) {
             const uint32_t pos = w.len + i, b = pos / bs;
             int32_t slot = -1;
-            if (w.served) slot = (int32_t)((uint32_t)(b < w.have ? table[b] : fresh(b - w.have)) * bs + pos % bs);
+            if (w.served) {
+                // an id whose slots pass 31 bits is no block of any cache
+                const uint32_t id = (uint32_t)(b < w.have ? table[b] : fresh(b - w.have));
+                if (id < 0x80000000u / bs) slot = (int32_t)(id * bs + pos % bs);
+            }
             p.d_slots[w.start + i] = slot;
         }
         // entries past the free ones: nobody else reads or writes them

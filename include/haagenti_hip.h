@@ -751,7 +751,8 @@ typedef struct hh_kv_cache {
  * the tail, in order, for later steps.
  * Writes d_start[requests + 1] (first row of each request's new tokens: the
  * running sum of max(d_new, 0)), d_kv_len (tokens held after the step),
- * d_slots[tokens] (the slot of each new row, -1 past the last row), d_status
+ * d_slots[tokens] (the slot of each new row, -1 past the last row and where
+ * the table or the ring holds what can't be a block's id), d_status
  * and d_state_out (which is not d_state: give it to the next step).  d_kv_len
  * may be d_len: an update in place, at the cost of one more launch.
  * A request that can't be served takes no block, its slots are -1, its

@@ -37,3 +37,18 @@ def test_lengths_in_place(n):
                state=out["after"])
     for key, v in got.items():
         assert (v.cpu().numpy() == np.asarray(want[key])).all(), key
+
+
+@pytest.mark.parametrize("bs", [16, 32, 64, 128])
+def test_ids_whose_slots_pass_31_bits(bs):
+    k = G.K()
+    last = (1 << 31) // bs - 1
+    ids = [last, last + 1, (1 << 31) - 1, -1, -(1 << 31), (1 << 32) // bs]
+    want = [last * bs + 3] + [-1] * 5
+    # ids in the table, then from the ring
+    table = np.full((6, 2), 7)
+    table[:, 0] = ids
+    p = k.kv_plan(G.ctx(), G.i32([3] * 6), G.i32([1] * 6), G.i32(table), G.i32([0]), G.i32([0, 0]), bs, 6)
+    assert p.slots.cpu().tolist() == want
+    p = k.kv_plan(G.ctx(), G.i32([bs] * 6), G.i32([1] * 6), G.i32(np.zeros((6, 2))), G.i32(ids), G.i32([0, 6]), bs, 6)
+    assert p.slots.cpu().tolist() == [x - 3 if x >= 0 else x for x in want] and not p.status.any()
