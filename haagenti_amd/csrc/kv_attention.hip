@@ -785,10 +785,11 @@ extern "C" int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, co
     // request each XCD gets early and late ones (of ragged requests the late
     // ones are empty; 48 requests in 16 chunks each 111 us, in 17 87).
     if (p.splits > 1) p.splits |= 1;
-    const uint32_t tile = 32u * (cache->head_dim <= 128 ? hh::kTileWaves<128> : hh::kTileWaves<256>);
+    const uint32_t waves = cache->head_dim <= 128 ? hh::kTileWaves<128> : hh::kTileWaves<256>, tile = 32 * waves;
     p.tiles = most > p.small ? (uint32_t)((most + tile - 1) / tile) : 0;
-    if ((uint64_t)a->requests * p.splits >= 1ull << 24 || (uint64_t)a->requests * p.tiles >= 1ull << 24)
-        return HH_ERR_UNSUPPORTED;
+    // a launch has fewer than 2^32 threads a dimension (chunks are a few
+    // thousand, or a few to a request)
+    if ((uint64_t)a->requests * p.tiles * 64 * waves >= 1ull << 32) return HH_ERR_UNSUPPORTED;
     if (cache->kv_heads * 16ull > 65535) return HH_ERR_UNSUPPORTED;
     if (a->requests && p.splits > 1) {
         const uint64_t n = lanes * p.splits * p.cols;

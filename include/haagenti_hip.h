@@ -805,7 +805,9 @@ int32_t hh_kv_read(hh_context *ctx, const hh_kv_cache *cache, const int32_t *d_b
  * last one's give zeros; tokens of a block id that the cache doesn't have are
  * not seen.  max_q and max_kv bound a request's rows and tokens (rows beyond
  * give zeros, tokens beyond are not seen): they choose how the work is split,
- * so bounds near the real sizes are faster.  Sums, maxima and accumulators are f32, codes
+ * so bounds near the real sizes are faster, and thousands of requests need
+ * them (HH_ERR_UNSUPPORTED where requests times the tiles of max_q rows are
+ * more than one launch holds).  Sums, maxima and accumulators are f32, codes
  * are exact, the output is rounded once at the end.  A row's probabilities
  * times their blocks' scales are rounded to f16 for the second product, in
  * units of the largest of them: 11 bits down to 2^-14 of it, 2^-25 of it
