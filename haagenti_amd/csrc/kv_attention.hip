@@ -23,8 +23,9 @@
 // operands are contiguous bytes of the cache.  The cache's codes c become the
 // f16 numbers 1024 + c by byte permutation, less 1152 by one packed add.
 //
-// bf16 queries are scaled to a largest magnitude of 1 to 2 per row by a power
-// of two before they become f16 (exact down to 2^-25 of the largest).
+// bf16 queries are scaled by a power of two, to a largest magnitude of 2^14 to
+// 2^15 per row, before they become f16: exact down to 2^-31 of the largest, off
+// by at most 2^-39 of it below.
 #include "layer_ops.hpp"
 
 namespace hh {
@@ -172,9 +173,9 @@ __device__ __forceinline__ float load_query(const uint16_t *row, bool wide, floa
     for (int f = 0; f < N; f++)
 #pragma unroll
         for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(half_to_f32<DT>((raw[f][e >> 1] >> (16 * (e & 1))) & 0xffffu)));
-    const uint32_t ex = __float_as_uint(join(top)) >> 23;
-    const bool plain = ex == 0 || ex == 255;  // zeros and subnormals, infinities
-    const float down = plain ? sign : ldexpf(sign, 127 - (int)ex), up = plain ? 1.0f : ldexpf(1.0f, (int)ex - 127);
+    const int ex = (int)(__float_as_uint(join(top)) >> 23);
+    const int by = ex == 255 ? 0 : min(127 + 14 - ex, 127);  // infinities stay; 2^127 is the largest factor
+    const float down = ldexpf(sign, by), up = ldexpf(1.0f, -by);
 #pragma unroll
     for (int f = 0; f < N; f++)
 #pragma unroll

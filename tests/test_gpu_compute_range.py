@@ -10,7 +10,7 @@ import test_gpu_compute as G
 pytestmark = pytest.mark.gpu
 
 
-def attention(q, kq, ks, vq, vs, rows, scale):
+def attention(q, kq, ks, vq, vs, rows, scale, lost=2.0 ** -25):
     """One request, its blocks in order: q (rows, heads, dim), integers of keys and values (blocks, kv heads, tokens,
     dim) with their scales; the output, and what its f16 probabilities and its scores may cost."""
     group = q.shape[1] // kq.shape[1]
@@ -28,12 +28,12 @@ def attention(q, kq, ks, vq, vs, rows, scale):
             p = np.exp(z - z.max())
             p /= p.sum()
             out[i, h] = p @ val[:seen, j]
-            # a score of f32 sums, and of bf16 queries to 2^-25 of the row's largest: its error d changes p and the sum
+            # a score of f32 sums, and of bf16 queries to `lost` of the row's largest: its error d changes p and the sum
             # by d each; p is rounded to 11 bits, or to 2^-25 of the row's largest probability times scale where it is
             # small; exp and the sums to 2^-18
             dim = q.shape[2]
             d = (np.abs(key[:seen, j]) @ np.abs(q[i, h])).max() * scale * (dim + 8) * 2.0 ** -24
-            d += np.abs(key[:seen, j]).sum(1).max() * np.abs(q[i, h]).max() * scale * 2.0 ** -25
+            d += np.abs(key[:seen, j]).sum(1).max() * np.abs(q[i, h]).max() * scale * lost
             d += np.abs(z).max() * 2.0 ** -22
             s = np.repeat(vs[:, j], bs)[:seen]
             err[i, h] = p @ np.abs(val[:seen, j]) * (2 * d + 2.0 ** -11 + 2.0 ** -18) + vi[:seen, j].sum(0) * (p * s).max() * 2.0 ** -25
@@ -127,6 +127,38 @@ def test_all_scales_far_from_one(rows, power):
 def test_scales_of_zero_beside_others(rows):
     check(128, rows, 2, 1, 64, 16, "bf16", lambda rng, n: np.where(np.arange(n) % 3, 0.0, 1.0))
     check(128, rows, 2, 1, 64, 16, "bf16", lambda rng, n: np.where(np.arange(n) < n - 1, 0.0, 2.0 ** 20))
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("power", [-8, -17, -24, -30])
+def test_small_parts_of_queries_beside_a_large_one(rows, power):
+    """A dimension of the query far larger than the others meets keys of 0: the others' scores keep their bits."""
+    t = G.T()
+    c, kq, vq, ks, vs = G.new_cache(6, 16, 2, 64, 5)
+    kq[:, :, :, 7] = 0
+    c.k.copy_(t.from_numpy((kq + 128).astype(np.uint8)))
+    for size in (1.0, 2.0 ** 30, 2.0 ** -60):
+        q = np.random.default_rng(rows).normal(0, 1, (rows, 4, 64))
+        q[:, :, 7] = 2.0 ** -power * np.where(np.arange(rows) % 2, -1.5, 1.0)[:, None]
+        q, qv = G.dev(q * size, "bf16")
+        o = c.attention(q, G.i32(np.arange(6)[None]), G.i32([0, rows]), G.i32([90]), scale=0.125 / size)
+        want, err = attention(qv / size, kq, ks, vq, vs, 90 - rows + 1 + np.arange(rows), 0.125, lost=2.0 ** -39)
+        close(o, want, err, "bf16")
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_queries_of_any_size(rows):
+    t = G.T()
+    c, kq, vq, ks, vs = G.new_cache(6, 16, 2, 64, 5)
+    for power in (-133, -126, -120, -113, -100, 100, 120):
+        q = np.random.default_rng(3).normal(0, 1, (rows, 4, 64)).clip(-3, 3)
+        if power < -120:
+            q = np.rint(q * 8) / 8 if power == -126 else np.rint(q)
+        q, qv = G.dev(q * 2.0 ** power, "bf16")
+        scale = 2.0 ** min(-power, 126) * 0.125
+        o = c.attention(q, G.i32(np.arange(6)[None]), G.i32([0, rows]), G.i32([90]), scale=scale)
+        want, err = attention(qv * scale, kq, ks, vq, vs, 90 - rows + 1 + np.arange(rows), 1.0)
+        close(o, want, err, "bf16")
 
 
 def test_a_request_is_the_same_beside_tokens_that_it_does_not_see():
