@@ -10,6 +10,7 @@
 #include <string>
 
 static std::map<const void *, std::string> names;
+static std::map<std::string, std::pair<dim3, dim3>> shapes;  // of the launches so far
 static std::string calls, fail_name;
 static int fail_in = 0;
 static hipError_t last = hipSuccess;
@@ -27,6 +28,7 @@ const char *host_hip_calls() { return calls.c_str(); }
 // Forgets the calls so far; the n-th call from here whose name holds `name` fails.
 void host_hip_fail(const char *name, int n) {
     calls.clear();
+    shapes.clear();
     fail_name = name;
     fail_in = n;
 }
@@ -41,14 +43,30 @@ void __hipRegisterFunction(void **, const void *host, char *, const char *name, 
     names[host] = name;
 }
 void __hipRegisterVar(void **, void *, char *, char *, int, size_t, int, int) {}
-hipError_t __hipPushCallConfiguration(dim3, dim3, size_t, hipStream_t) { return hipSuccess; }
+static dim3 next_grid(1), next_block(1);
+hipError_t __hipPushCallConfiguration(dim3 grid, dim3 block, size_t, hipStream_t) {
+    next_grid = grid, next_block = block;
+    return hipSuccess;
+}
 hipError_t __hipPopCallConfiguration(dim3 *g, dim3 *b, size_t *m, hipStream_t *s) {
-    *g = *b = dim3(1);
+    *g = next_grid, *b = next_block;
     *m = 0;
     *s = nullptr;
     return hipSuccess;
 }
-hipError_t hipLaunchKernel(const void *f, dim3, dim3, void **, size_t, hipStream_t) {
+// The grid and the workgroup of the latest launch of a kernel whose name holds `name`.
+int host_hip_shape(const char *name, unsigned *out) {
+    for (const auto &s : shapes)
+        if (s.first.find(name) != std::string::npos) {
+            const dim3 g = s.second.first, b = s.second.second;
+            const unsigned v[6] = {g.x, g.y, g.z, b.x, b.y, b.z};
+            std::memcpy(out, v, sizeof(v));
+            return 1;
+        }
+    return 0;
+}
+hipError_t hipLaunchKernel(const void *f, dim3 grid, dim3 block, void **, size_t, hipStream_t) {
+    shapes[names[f]] = {grid, block};
     return note("launch " + names[f], hipErrorLaunchFailure);
 }
 hipError_t hipFuncSetAttribute(const void *, hipFuncAttribute, int) { return hipSuccess; }
