@@ -620,7 +620,8 @@ __global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
 #pragma unroll
             for (int i = 0; i < 4; i++) c[i] = 1.0f;
         }
-        float um[4], share[4], far = 0.0f, zm = -__builtin_inff(), wm = -__builtin_inff();
+        float um[4], share[4], zm = -__builtin_inff(), wm = -__builtin_inff();
+        bool close = true;  // not for NaN
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             um[u] = s[u >> 1][8 * (u & 1)];
@@ -628,10 +629,10 @@ __global__ __launch_bounds__(64 * NW) void attn_tile_kernel(const AttnArgs p) {
             for (int i = 1; i < 8; i++) um[u] = fmaxf(um[u], s[u >> 1][8 * (u & 1) + i]);
             wm = fmaxf(wm, fmaf(um[u], c[u], log_vs[u]));
             share[u] = log_vs[u] - tops.rise;
-            far = fmaxf(far, fabsf(share[u]));
+            close = close && fabsf(share[u]) <= kNear;
         }
         wm = max_across_32(wm);
-        const bool near = __all(far <= kNear);
+        const bool near = __all(close);
         if (!near) {
 #pragma unroll
             for (int u = 0; u < 4; u++) zm = fmaxf(zm, um[u] * c[u]);

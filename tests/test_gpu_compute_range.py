@@ -161,6 +161,22 @@ def test_queries_of_any_size(rows):
         close(o, want, err, "bf16")
 
 
+@pytest.mark.parametrize("rows", [2, 50])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 0.0])
+def test_hidden_blocks_of_any_scale(rows, bad):
+    """Rows don't take part in what later tokens' blocks are scaled by, whatever that is."""
+    t = G.T()
+    outs = []
+    for worst in (0.01, bad):
+        c = G.new_cache(4, 16, 1, 64, 3)[0]
+        c.v_scale[1:], c.k_scale[1:] = worst, worst
+        q = t.randn(rows, 4, 64, generator=t.Generator("cuda").manual_seed(1), device="cuda").bfloat16()
+        outs.append(c.attention(q, G.i32([[0, 1, 2, 3]]), G.i32([0, rows]), G.i32([17 if rows == 2 else 64])))
+    seen = 17 - 1 if rows == 2 else 64 - rows + 1
+    first = 17 - seen if rows == 2 else 16 - seen + 1
+    assert first >= 1 and t.isfinite(outs[1][:first]).all() and t.equal(outs[0][:first], outs[1][:first])
+
+
 def test_a_request_is_the_same_beside_tokens_that_it_does_not_see():
     """A prompt's first rows get bit for bit what they get where the later tokens' values are small."""
     t = G.T()
