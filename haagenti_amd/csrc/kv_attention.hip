@@ -10,7 +10,11 @@
 // and the output is 2^(M - m) O / l.  Both maxima are the column's own, over
 // tokens that it sees, so whatever the scales are, its largest P is at least 1:
 // a P keeps f16's 11 bits down to 2^-14 and is off by at most 2^-25 below (of
-// terms that small beside the column's largest).
+// terms that small beside the column's largest).  The step kernel, which
+// memory bounds, adds the rest of P as a second f16 (22 bits; 48 requests 93.1
+// us, 92.2 without it, 131,001 tokens 52.3 and 51.8); for the tile kernel that
+// is half as much again of the matrix products (two prompts 573 us, 440
+// without) for errors below half a unit of its outputs.
 // P's exponent is z - m + share, share = log2(scale of V's block) - rise, rise
 // standing for M - m; the sum l takes the share out again per 16 tokens (a
 // share below 2^-40 counts as 2^-40: such a P is 0 in f16 anyway, and l keeps
@@ -340,19 +344,23 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attn_step_kernel(const 
             for (int t = 0; t < VT; t++) o[t] *= of_o;
         }
         const float share = share_of(log_vs, tops.rise), less = share - base_of(tops.m);
-        f16x8 pv[2];
+        f16x8 pv[2], rest[2];
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const float e = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], c, less));
             sum += e;
             pv[i >> 3][i & 7] = (_Float16)e;
+            rest[i >> 3][i & 7] = (_Float16)(e - (float)pv[i >> 3][i & 7]);
         }
         l = fmaf(sum, __builtin_amdgcn_exp2f(-share), l);
 #pragma unroll
         for (int t = 0; t < VT; t++) {
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_to_f16(vw[t][0], vw[t][1]), pv[0], o[t], 0, 0, 0);
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_to_f16(vw[t][2], vw[t][3]), pv[1], o[t], 0, 0, 0);
+            const f16x8 a = codes8_to_f16(vw[t][0], vw[t][1]), b = codes8_to_f16(vw[t][2], vw[t][3]);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, rest[0], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, rest[1], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pv[0], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, pv[1], o[t], 0, 0, 0);
         }
     }
 

@@ -811,7 +811,7 @@ int32_t hh_kv_read(hh_context *ctx, const hh_kv_cache *cache, const int32_t *d_b
  * are exact, the output is rounded once at the end.  A row's probabilities
  * times their blocks' scales are rounded to f16 for the second product, in
  * units of the largest of them: 11 bits down to 2^-14 of it, 2^-25 of it
- * below.  Tokens that a row doesn't see have no part in that.  out's rows
+ * below; for requests of at most 16 rows times q_heads / kv_heads 22 bits.  Tokens that a row doesn't see have no part in that.  out's rows
  * share no element (HH_ERR_INVALID_ARGUMENT). */
 typedef struct hh_kv_attention_args {
     const void *d_q;

@@ -10,7 +10,7 @@ import test_gpu_compute as G
 pytestmark = pytest.mark.gpu
 
 
-def attention(q, kq, ks, vq, vs, rows, scale, lost=2.0 ** -25):
+def attention(q, kq, ks, vq, vs, rows, scale, lost=2.0 ** -25, bits=11):
     """One request, its blocks in order: q (rows, heads, dim), integers of keys and values (blocks, kv heads, tokens,
     dim) with their scales; the output, and what its f16 probabilities and its scores may cost."""
     group = q.shape[1] // kq.shape[1]
@@ -29,14 +29,14 @@ def attention(q, kq, ks, vq, vs, rows, scale, lost=2.0 ** -25):
             p /= p.sum()
             out[i, h] = p @ val[:seen, j]
             # a score of f32 sums, and of bf16 queries to `lost` of the row's largest: its error d changes p and the sum
-            # by d each; p is rounded to 11 bits, or to 2^-25 of the row's largest probability times scale where it is
+            # by d each; p is rounded to `bits` bits, or to 2^-25 of the row's largest probability times scale where it is
             # small; exp and the sums to 2^-18
             dim = q.shape[2]
             d = (np.abs(key[:seen, j]) @ np.abs(q[i, h])).max() * scale * (dim + 8) * 2.0 ** -24
             d += np.abs(key[:seen, j]).sum(1).max() * np.abs(q[i, h]).max() * scale * lost
             d += np.abs(z).max() * 2.0 ** -22
             s = np.repeat(vs[:, j], bs)[:seen]
-            err[i, h] = p @ np.abs(val[:seen, j]) * (2 * d + 2.0 ** -11 + 2.0 ** -18) + vi[:seen, j].sum(0) * (p * s).max() * 2.0 ** -25
+            err[i, h] = p @ np.abs(val[:seen, j]) * (2 * d + 2.0 ** -bits + 2.0 ** -18) + vi[:seen, j].sum(0) * (p * s).max() * 2.0 ** -25
     return out, err
 
 
@@ -159,6 +159,20 @@ def test_queries_of_any_size(rows):
         o = c.attention(q, G.i32(np.arange(6)[None]), G.i32([0, rows]), G.i32([90]), scale=scale)
         want, err = attention(qv * scale, kq, ks, vq, vs, 90 - rows + 1 + np.arange(rows), 1.0)
         close(o, want, err, "bf16")
+
+
+@pytest.mark.parametrize("kv_len", [2, 3, 5, 17, 40, 700])
+@pytest.mark.parametrize("q_heads,heads,dim,bs", [(32, 2, 64, 16), (24, 8, 128, 32), (6, 3, 96, 64), (8, 8, 256, 128), (16, 1, 192, 16)])
+def test_few_columns_keep_22_bits(kv_len, q_heads, heads, dim, bs):
+    t = G.T()
+    blocks = (kv_len + bs - 1) // bs
+    c, kq, vq, ks, vs = G.new_cache(blocks, bs, heads, dim, kv_len)
+    vq = np.abs(vq) * np.where(np.arange(bs) % 2, -1, 1)[:, None]  # sums that cancel
+    c.v.copy_(t.from_numpy((np.swapaxes(vq, 2, 3) + 128).astype(np.uint8)))
+    q, qv = G.dev(np.random.default_rng(kv_len).normal(0, 0.3, (1, q_heads, dim)), "f16")
+    o = c.attention(q, G.i32(np.arange(blocks)[None]), G.i32([0, 1]), G.i32([kv_len]), max_q=1, max_kv=kv_len)
+    want, err = attention(qv, kq, ks, vq, vs, [kv_len], dim ** -0.5, lost=0.0, bits=21)
+    close(o, want, err, "f16")
 
 
 @pytest.mark.parametrize("rows", [2, 50])
