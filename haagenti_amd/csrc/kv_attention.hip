@@ -19,7 +19,8 @@
 // standing for M - m; the sum l takes the share out again per 16 tokens (a
 // share below 2^-40 counts as 2^-40: such a P is 0 in f16 anyway, and l keeps
 // its tokens).  m and M follow their maxima only when these pass them by 8, so
-// P < 256 and the accumulators are seldom rescaled.
+// P < 256 and the accumulators are seldom rescaled.  Powers of two are the
+// hardware's, to a unit in the last place.
 // Tokens lie on the first product's rows, so its accumulators hold, for one
 // column per lane, just the tokens that the lane supplies to the second
 // product's P^T operand: P never moves between lanes.  Which token a row
@@ -226,8 +227,8 @@ __device__ __forceinline__ void store4(uint16_t *to, bool wide, const float *v) 
 //
 // A step of a running request: at most 16 columns, one 16 x 16 x 32 tile
 // wide.  Bound by reading the codes once: 131,001 tokens of 8 heads of 128
-// dimensions (268 MB) take 43 us (6.2 TB/s) and 7 to join, 48 requests of 100
-// to 8000 tokens (424 MB) 86 and 5 (chunks end unevenly).  A workgroup takes one chunk of a
+// dimensions (268 MB) take 43 us (6.2 TB/s) and 8 to join, 48 requests of 100
+// to 8000 tokens (424 MB) 87 and 5 (chunks end unevenly).  A workgroup takes one chunk of a
 // request's tokens for one cache head, its 4 waves every fourth 64 tokens
 // straight from memory to registers; their results are joined in LDS, the
 // chunks' by attn_join_kernel.
@@ -472,7 +473,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p) {
 // Bound by the two products' reads of LDS (each wave reads a tile's 32 KiB)
 // and the softmax's vector instructions, about half of the time each beside
 // a third for the matrix pipes: two prompts of 1900 to 2048 rows over 3000 to
-// 4100 cached tokens, 32 heads on 8, 434 us (770 TFLOP/s).  4 waves of 32
+// 4100 cached tokens, 32 heads on 8, 440 to 455 us (740 TFLOP/s).  4 waves of 32
 // columns instead of 8 take 780 us there (each tile's codes are converted for
 // half the columns).
 //
@@ -781,8 +782,9 @@ extern "C" int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, co
     const uint64_t room = (uint64_t)a->table_width * cache->block_size;
     const uint64_t kv = a->max_kv < room ? a->max_kv : room;
     if (kv > 1ull << 30) return HH_ERR_UNSUPPORTED;  // tokens are counted in 31 bits
-    // chunks: enough workgroups for 8 per CU (48 requests 86 us; 16 per CU 95,
-    // 24 per CU 87 with twice the chunks to join), none below 512 tokens
+    // chunks: enough workgroups for 8 per CU, none below 512 tokens (48
+    // requests of up to 8001 tokens, 131,001 tokens of one: 93 and 52 us; 4 per
+    // CU 106 and 50, 16 per CU 100 and 52, 24 per CU 93 and 52)
     const uint64_t lanes = (uint64_t)(a->requests ? a->requests : 1) * cache->kv_heads;
     const uint64_t want = (8ull * (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256) + lanes - 1) / lanes;
     uint64_t chunk = (kv + want - 1) / want;
@@ -793,7 +795,7 @@ extern "C" int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, co
     if (p.splits < 1) p.splits = 1;
     // Workgroups go around the 8 XCDs: with an odd number of chunks to a
     // request each XCD gets early and late ones (of ragged requests the late
-    // ones are empty; 48 requests in 16 chunks each 111 us, in 17 87).
+    // ones are empty; those 48 in 6 chunks each 106 us, in 7 93).
     if (p.splits > 1) p.splits |= 1;
     const uint32_t waves = cache->head_dim <= 128 ? hh::kTileWaves<128> : hh::kTileWaves<256>, tile = 32 * waves;
     p.tiles = most > p.small ? (uint32_t)((most + tile - 1) / tile) : 0;

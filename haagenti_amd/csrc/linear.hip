@@ -12,7 +12,8 @@
 // accumulator's start, -24 sum(x) over the group, from one more product with
 // a constant operand.  A group's 32 values are one product of 32 deep; its
 // sum is multiplied by the group's scale in f32.  So an INT4 weight is exact
-// whatever x's type.
+// whatever x's type; what f32 rounds are sums of up to 31 |x| and 24 |x| where
+// the weight's own integer is at most 8.
 #include "layer_ops.hpp"
 
 namespace hh {
@@ -47,6 +48,8 @@ __device__ __forceinline__ u32x4 row8(const uint16_t *row, uint32_t at, uint32_t
     return v;
 }
 
+// __expf is the hardware's power of two of x log2(e): off by 2^-23 of itself
+// and by 2^-24 |x|, so by less than 2^-20 |z| in what SiLU and GELU make of it.
 __device__ __forceinline__ float act_of(float z, int act) {
     switch (act) {
         case HH_ACT_RELU: return fmaxf(z, 0.0f) + (z != z ? z : 0.0f);
@@ -511,8 +514,9 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(const LinearArgs p, co
 // order).  Rows past the matrices repeat the last one.  Bound by LDS and the
 // matrix pipes alike: at 256 x 256 a tile's reads (192 KiB by 8 waves of
 // 128 x 64) and copies (64 KiB) take as long as its products.  bf16 4096 x
-// 8192 x 8192 takes 440 us (1250 TFLOP/s; 0.85 of the library's product),
-// 2048 x 14336 x 4096 246 (980), 512 x 4096 x 14336 67 (900).
+// 8192 x 8192 takes 413 us (1330 TFLOP/s; 0.82 of the library's product),
+// 2048 x 14336 x 4096 221 (1090; 0.78), with SiLU and a product 239 to 280 by
+// what the caches and clocks hold, 512 x 4096 x 14336 70 (860; the library's 78).
 //
 // Tiles are numbered down the rows of x, and consecutive ones go to one XCD,
 // whose L2 then serves W's panel to all of them.
@@ -715,7 +719,10 @@ inline TilePlan plan_tiles(const hh_linear_args &a, int cus, const Shape (&shape
         }
     return best;
 }
-// Measured on tiles copied straight to LDS, through registers, and of INT4.
+// Of tiles copied straight to LDS, and through registers (16-bit W).  For
+// products of 33 to 4096 rows by 4096 to 14336 columns the estimates are
+// within 30 % of the times, half of them within 10 %; INT4 through registers
+// takes up to 1.2 of them, with groups across rows 2.6 to 4.
 constexpr Shape kLargeShapes[] = {{256, 256, 1, 1.65, 1.65}, {256, 128, 1, 1.0, 1.0}, {128, 256, 1, 1.0, 1.0},
                                   {128, 128, 2, 1.13, 0.67}, {128, 64, 3, 1.0, 0.45}};
 constexpr Shape kAnyShapes[] = {{128, 128, 2, 2.0, 1.3}, {64, 64, 4, 1.6, 0.9}};
@@ -760,7 +767,9 @@ int32_t launch_linear(hh_context *ctx, const LinearArgs &p, hipStream_t s) {
     const bool aligned = !int4 && !(((uintptr_t)a.d_x | (uintptr_t)a.d_w) & 15u) && !((a.x_stride | a.w_stride) & 7u) &&
                          a.k % 64 == 0 && a.k && a.x_stride < 1u << 22 && a.w_stride < 1u << 22;  // offsets in a tile: 32 bits
     // up to 64 rows straight from memory; above 32 aligned tiles are faster
-    // (64 rows of 4096 x 4096 17 us against 22, of 8192 x 8192 39 against 77)
+    // (64 rows of 4096 x 4096 18 us against 22, of 8192 x 8192 43 against 77).
+    // Large products of 33 to 64 rows an odd number of values apart would be
+    // too: 56 and 213 us, in tiles through registers 19 and 47.
     if (a.m <= (aligned ? 32u : 64u)) {
         const int rows = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4;
         return from_hip(int4 ? (rows == 1   ? launch_rows<DT, YT, 1, true>(p, cus, s)
