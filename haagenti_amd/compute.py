@@ -4,8 +4,8 @@ paged 8-bit key / value cache with its plan, append, read and attention.
 
 Tensors are torch tensors on the context's device.  Calls run on torch's
 current stream, where their results are allocated, and don't synchronise.
-Calls on several streams need no order among them; captured calls keep their
-memory for as long as the context lives, whatever is called later (graphs
+Calls on several streams need no order but their tensors' own; captured calls
+keep what they use of the context's memory for as long as the context lives, whatever is called later (graphs
 captured on one stream must not run beside each other).
 What a call can't take raises HaagentiError before anything is launched;
 there are no gradients, so tensors that require them are taken under

@@ -686,7 +686,7 @@ int32_t hh_spectral_encode_from_dct(const float *coeffs, uint32_t width, uint32_
  * memory, so a step needs no host synchronisation.  Strides are in elements.
  * hh_linear and hh_kv_attention may keep partial sums in memory that the
  * context holds for each stream, grown with the largest call there so far, so
- * their calls on several streams need no order among them.  All may be
+ * their calls on several streams need no order but their tensors' own.  All may be
  * captured: captured calls have memory of their own, which stays as it is
  * until the context is destroyed, whatever is called later (a context outlives
  * the graphs that were captured with it).  Graphs captured on one stream share
