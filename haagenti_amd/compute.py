@@ -1,6 +1,8 @@
-"""A decoder layer's operators on decoded weights (hh_linear, hh_kv_*): matrix
-products with their epilogue, over 16-bit weights or INT4 buffers, and a
-paged 8-bit key / value cache with its plan, append, read and attention.
+"""A decoder layer's operators on decoded weights: matrix products with their
+epilogue, over 16-bit weights or INT4 buffers (hh_linear), the norms between
+them and rotary positions with their gradients (hh_norm, hh_rotary), and a
+paged 8-bit key / value cache with its plan, append, read and attention
+(hh_kv_*).
 
 Tensors are torch tensors on the context's device.  Calls run on torch's
 current stream, where their results are allocated, and don't synchronise.
@@ -8,7 +10,8 @@ Calls on several streams need no order but their tensors' own; captured calls
 keep what they use of the context's memory for as long as the context lives, whatever is called later (graphs
 captured on one stream must not run beside each other).
 What a call can't take raises HaagentiError before anything is launched;
-there are no gradients, so tensors that require them are taken under
+gradients are calls of their own (norm_backward, rotary's inverse) that
+autograd doesn't know, so tensors that require them are taken under
 torch.no_grad() only."""
 import ctypes as C
 import struct
@@ -19,6 +22,7 @@ from . import BF16, F16, F32, INVALID_ARGUMENT, UNSUPPORTED, HaagentiError, _che
 
 INT4 = 16
 
+NORMS = {"layer": 0, "rms": 1}
 ACTIVATIONS = {"none": 0, None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _HALF = {torch.float16: F16, torch.bfloat16: BF16}
@@ -27,12 +31,18 @@ _HALF = {torch.float16: F16, torch.bfloat16: BF16}
 # alignment, no gaps; a step's calls are a few microseconds each, and a packed
 # string costs a quarter of a ctypes structure).
 _LINEAR = struct.Struct("=6Q6Q3I4i4x")      # hh_linear_args
+_NORM = struct.Struct("=4Q2Q2If3i")         # hh_norm_args
+_NORM_GRADS = struct.Struct("=6Q")          # hh_norm_grads
+_ROTARY = struct.Struct("=4Q5Q8I3i4x")      # hh_rotary_args
 _CACHE = struct.Struct("=4Q4I")             # hh_kv_cache
 _PLAN = struct.Struct("=10QQ5I4x")          # hh_kv_plan_args
 _ATTENTION = struct.Struct("=5Q5Q6Ifi")     # hh_kv_attention_args
 
 _u64, _bytes = C.c_uint64, C.c_char_p
 _linear = _sig("hh_linear", _i32, [_vp, _bytes, _vp])
+_norm = _sig("hh_norm", _i32, [_vp, _bytes, _vp])
+_norm_backward = _sig("hh_norm_backward", _i32, [_vp, _bytes, _bytes, _vp])
+_rotary = _sig("hh_rotary", _i32, [_vp, _bytes, _vp])
 _plan = _sig("hh_kv_plan", _i32, [_vp, _bytes, _vp])
 _append = _sig("hh_kv_append", _i32, [_vp, _bytes, _vp, _vp, _i32, _u64, _u64, _u64, _u64, _vp, _u32, _vp])
 _read = _sig("hh_kv_read", _i32, [_vp, _bytes, _vp, _u32, _i32, _vp, _vp, _vp])
@@ -77,13 +87,13 @@ class Int4Weight:
             _refuse(INVALID_ARGUMENT, "Int4Weight: a negative size")
 
 
-def _rows(t, m, n, dev, what):
+def _rows(t, m, n, dev, what, of="linear"):
     """Row stride of an m x n matrix on the device whose rows are contiguous."""
     shape, stride = t.shape, t.stride()
     if len(shape) != 2 or shape[0] != m or shape[1] != n or (n > 1 and stride[1] != 1 and m):
-        _refuse(INVALID_ARGUMENT, f"linear: {what} is {m} x {n} with contiguous rows, got {tuple(shape)}")
+        _refuse(INVALID_ARGUMENT, f"{of}: {what} is {m} x {n} with contiguous rows, got {tuple(shape)}")
     if t.get_device() != dev:
-        _refuse(INVALID_ARGUMENT, f"linear: {what} must be on the context's device")
+        _refuse(INVALID_ARGUMENT, f"{of}: {what} must be on the context's device")
     return stride[0] if m > 1 else n
 
 
@@ -186,6 +196,183 @@ def linear(ctx, x, w, bias=None, act=None, mul=None, residual=None, out=None, ou
     if rc:
         _check(rc, "hh_linear")
     return out
+
+
+def _same(a, b, m):
+    """Whether two m x n matrices of one type are the same memory in the same order."""
+    return a.data_ptr() == b.data_ptr() and a.dtype is b.dtype and (m <= 1 or a.stride(0) == b.stride(0))
+
+
+def _out_rows(out, m, n, dtype, dev, of, reads, over=()):
+    """Row stride of a given output: of this type, apart from `reads`, and from `over` unless it is one of these itself."""
+    if out.dtype is not dtype:
+        _refuse(INVALID_ARGUMENT, f"{of}: out is {dtype}")
+    stride = _rows(out, m, n, dev, "out", of)
+    if m > 1 and stride < n:
+        _refuse(INVALID_ARGUMENT, f"{of}: rows of out overlap")
+    if out.requires_grad:
+        _no_grad(of)
+    for t in reads:
+        if t is not None and not _apart(out, t):
+            _refuse(INVALID_ARGUMENT, f"{of}: out lies over what is read")
+    for t in over:
+        if t is not None and not _same(out, t, m) and not _apart(out, t):
+            _refuse(INVALID_ARGUMENT, f"{of}: out lies over part of what is read")
+    return stride
+
+
+def _norm_args(what, ctx, x, weight, bias, kind, eps):
+    """The checks that both passes share: (rows, n, code of x's type, the weights' code, kind)."""
+    dev, dt = ctx.device, _CODE.get(x.dtype)
+    if dt is None:
+        _refuse(UNSUPPORTED, f"{what}: {x.dtype} (float32, float16 or bfloat16)")
+    if kind not in NORMS:
+        _refuse(UNSUPPORTED, f"{what}: kind {kind!r}")
+    if x.dim() != 2:
+        _refuse(INVALID_ARGUMENT, f"{what}: x is rows x n")
+    rows, n = x.shape
+    wt = dt
+    for t in (weight, bias):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or (t.dtype is not x.dtype and t.dtype is not torch.float32):
+            _refuse(INVALID_ARGUMENT, f"{what}: weight and bias are n contiguous values of x's type or float32")
+        _on(dev, what, t)
+        if t.requires_grad:
+            _no_grad(what)
+        wt = _CODE[t.dtype]
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
+        _refuse(INVALID_ARGUMENT, f"{what}: weight and bias have one type")
+    if x.requires_grad:
+        _no_grad(what)
+    return rows, n, dt, wt, NORMS[kind]
+
+
+def norm(ctx, x, weight=None, bias=None, kind="layer", eps=1e-5, out=None):
+    """Layer norm of the rows of x, or with kind "rms" the root mean square
+    norm (hh_norm): (x - mean) / sqrt(variance + eps) * weight + bias.  x:
+    rows x n, float32, float16 or bfloat16, rows contiguous, any stride apart;
+    weight and bias n values of x's type or float32.  Returns out, of x's type,
+    which may be x itself."""
+    rows, n, dt, wt, code = _norm_args("norm", ctx, x, weight, bias, kind, eps)
+    dev = ctx.device
+    x_stride = _rows(x, rows, n, dev, "x", "norm")
+    if out is None:
+        out, y_stride = x.new_empty((rows, n)), n
+    else:
+        y_stride = _out_rows(out, rows, n, x.dtype, dev, "norm", (weight, bias), (x,))
+    try:
+        args = _NORM.pack(x.data_ptr(), 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                          out.data_ptr(), x_stride, y_stride, rows, n, eps, dt, wt, code)
+    except (struct.error, OverflowError):
+        _refuse(INVALID_ARGUMENT, f"norm: {rows} x {n}, eps {eps!r}")
+    rc = _norm(ctx.handle, args, _stream(dev))
+    if rc:
+        _check(rc, "hh_norm")
+    return out
+
+
+def norm_backward(ctx, dy, x, weight=None, bias=False, kind="layer", eps=1e-5, add=None, out=None):
+    """The gradients of norm from dy, that of its output, and its x and weight
+    (hh_norm_backward): (dx, dweight, dbias).  dx is of x's type, `add` (rows x
+    n of that type; what else flows back into x) on top, and may be given as
+    out: dy, x or add itself; dweight (with a weight) and dbias (with bias
+    true) are float32, else None."""
+    rows, n, dt, wt, code = _norm_args("norm_backward", ctx, x, weight, None, kind, eps)
+    dev = ctx.device
+    x_stride = _rows(x, rows, n, dev, "x", "norm_backward")
+    strides = []
+    for t, name in ((dy, "dy"), (add, "add")):
+        if t is None:
+            strides.append(0)
+            continue
+        if t.dtype is not x.dtype:
+            _refuse(INVALID_ARGUMENT, f"norm_backward: {name} has x's type")
+        strides.append(_rows(t, rows, n, dev, name, "norm_backward"))
+        if t.requires_grad:
+            _no_grad("norm_backward")
+    if out is None:
+        out, y_stride = x.new_empty((rows, n)), n
+    else:
+        y_stride = _out_rows(out, rows, n, x.dtype, dev, "norm_backward", (weight,), (x, dy, add))
+    dweight = None if weight is None else x.new_empty(n, dtype=torch.float32)
+    dbias = x.new_empty(n, dtype=torch.float32) if bias else None
+    try:
+        args = _NORM.pack(x.data_ptr(), 0 if weight is None else weight.data_ptr(), 0, out.data_ptr(), x_stride, y_stride, rows,
+                          n, eps, dt, wt, code)
+    except (struct.error, OverflowError):
+        _refuse(INVALID_ARGUMENT, f"norm_backward: {rows} x {n}, eps {eps!r}")
+    grads = _NORM_GRADS.pack(dy.data_ptr(), 0 if add is None else add.data_ptr(), 0 if dweight is None else dweight.data_ptr(),
+                             0 if dbias is None else dbias.data_ptr(), *strides)
+    rc = _norm_backward(ctx.handle, args, grads, _stream(dev))
+    if rc:
+        _check(rc, "hh_norm_backward")
+    return out, dweight, dbias
+
+
+def rotary(ctx, x, positions, inv_freq, sections=None, interleaved=False, inverse=False, out=None):
+    """Rotary positions on x (tokens x heads x dim, float32, float16 or
+    bfloat16; any token and head strides, so the query and key heads of a joint
+    projection are one call) (hh_rotary).  positions: int32, axes x tokens (or
+    tokens, for one axis); inv_freq: float32, one frequency per pair of
+    dimensions; sections: how many of the pairs, in order, each axis turns
+    (default: all the first).  Pair j is dimensions (j, j + pairs), interleaved
+    (2 j, 2 j + 1); dimensions past the pairs are copied.  inverse turns back:
+    the gradient's way.  Returns out, of x's type, which may be x itself."""
+    dev, dt, shape, stride = ctx.device, _CODE.get(x.dtype), x.shape, x.stride()
+    if dt is None:
+        _refuse(UNSUPPORTED, f"rotary: {x.dtype} (float32, float16 or bfloat16)")
+    if len(shape) != 3 or (shape[2] > 1 and stride[2] != 1 and shape[0] and shape[1]):
+        _refuse(INVALID_ARGUMENT, "rotary: x is tokens x heads x dim, contiguous dimensions")
+    tokens, heads, dim = shape
+    if positions.dim() == 1:
+        positions = positions[None]
+    if positions.dtype != torch.int32 or positions.dim() != 2 or positions.shape[1] != tokens \
+            or (tokens > 1 and positions.stride(1) != 1):
+        _refuse(INVALID_ARGUMENT, "rotary: positions are int32, axes x tokens with contiguous rows")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        _refuse(INVALID_ARGUMENT, "rotary: inv_freq is contiguous float32, one per pair")
+    axes = positions.shape[0]
+    sections = [inv_freq.numel()] if sections is None else list(sections)
+    if len(sections) != axes or not 1 <= axes <= 4:
+        _refuse(INVALID_ARGUMENT, "rotary: a section for each of 1 to 4 axes of positions")
+    if any(s < 0 for s in sections) or sum(sections) != inv_freq.numel() or 2 * sum(sections) > dim:
+        _refuse(INVALID_ARGUMENT, "rotary: sections add up to inv_freq's pairs, at most half of dim")
+    _on(dev, "rotary", x, positions, inv_freq)
+    if x.requires_grad or inv_freq.requires_grad:
+        _no_grad("rotary")
+    if out is None:
+        out = x.new_empty((tokens, heads, dim))
+        yt, yh = heads * dim, dim
+    else:
+        if out.dtype is not x.dtype or out.shape != shape or (dim > 1 and out.stride(2) != 1 and tokens and heads):
+            _refuse(INVALID_ARGUMENT, "rotary: out is like x")
+        _on(dev, "rotary", out)
+        if out.requires_grad:
+            _no_grad("rotary")
+        yt, yh = out.stride(0), out.stride(1)
+        same = out.data_ptr() == x.data_ptr() and (tokens <= 1 or yt == stride[0]) and (heads <= 1 or yh == stride[1])
+        if any(not _spans_apart(out, t) for t in ((positions, inv_freq) if same else (positions, inv_freq, x))):
+            _refuse(INVALID_ARGUMENT, "rotary: out is x itself or lies apart from what is read")
+    try:
+        args = _ROTARY.pack(x.data_ptr(), out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), stride[0], stride[1], yt, yh,
+                            positions.stride(0) if axes > 1 else tokens, tokens, heads, dim, axes,
+                            *(sections + [0] * (4 - axes)), bool(interleaved), bool(inverse), dt)
+    except struct.error:
+        _refuse(INVALID_ARGUMENT, f"rotary: {tuple(shape)}")
+    rc = _rotary(ctx.handle, args, _stream(dev))
+    if rc:
+        _check(rc, "hh_rotary")
+    return out
+
+
+def _spans_apart(a, b):
+    """Whether the memory from the first to the last element of two tensors is apart."""
+    if not a.numel() or not b.numel():
+        return True
+    end = [t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size() for t in (a, b)]
+    return end[0] <= b.data_ptr() or end[1] <= a.data_ptr()
+
 
 
 class Plan:

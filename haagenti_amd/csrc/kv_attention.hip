@@ -733,22 +733,6 @@ hipError_t launch_dim(const AttnArgs &p, hipStream_t s) {
     }
 }
 
-// Whether two rows of `dim` elements, `tokens` of them `ts` apart for each of
-// `heads` heads `hs` apart, share an element.
-bool rows_meet(uint64_t tokens, uint64_t heads, uint64_t ts, uint64_t hs, uint64_t dim) {
-    typedef unsigned __int128 u128;
-    if (tokens > 1 && ts < dim) return true;
-    if (heads > 1 && hs < dim) return true;
-    if (tokens == 1 || heads == 1 || ts >= (u128)(heads - 1) * hs + dim || hs >= (u128)(tokens - 1) * ts + dim) return false;
-    // neither stride spans the other: heads j apart against the tokens next to that
-    for (uint64_t j = 1; j < heads; j++) {
-        const u128 d = (u128)j * hs, below = d / ts, rest = d % ts;
-        if (below < tokens && rest < dim) return true;
-        if (below + 1 < tokens && ts - rest < dim) return true;
-    }
-    return false;
-}
-
 }  // namespace
 }  // namespace hh
 

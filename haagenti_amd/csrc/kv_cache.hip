@@ -445,6 +445,20 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const hh_kv_cache cache, c
 
 }  // namespace
 
+bool rows_meet(uint64_t tokens, uint64_t heads, uint64_t ts, uint64_t hs, uint64_t dim) {
+    typedef unsigned __int128 u128;
+    if (tokens > 1 && ts < dim) return true;
+    if (heads > 1 && hs < dim) return true;
+    if (tokens == 1 || heads == 1 || ts >= (u128)(heads - 1) * hs + dim || hs >= (u128)(tokens - 1) * ts + dim) return false;
+    // neither stride spans the other: heads j apart against the tokens next to that
+    for (uint64_t j = 1; j < heads; j++) {
+        const u128 d = (u128)j * hs, below = d / ts, rest = d % ts;
+        if (below < tokens && rest < dim) return true;
+        if (below + 1 < tokens && ts - rest < dim) return true;
+    }
+    return false;
+}
+
 int32_t check_kv_cache(const hh_kv_cache *c) {
     if (!c || !c->d_k || !c->d_v || !c->d_k_scale || !c->d_v_scale) return HH_ERR_INVALID_ARGUMENT;
     if (((uintptr_t)c->d_k | (uintptr_t)c->d_v) & 15u) return HH_ERR_INVALID_ARGUMENT;

@@ -1,5 +1,5 @@
-// What the decoder-layer operators (linear.hip, kv_cache.hip,
-// kv_attention.hip) share on the device.
+// What the decoder-layer operators (linear.hip, gated.hip, norm.hip,
+// rotary.hip, kv_cache.hip, kv_attention.hip) share.
 #pragma once
 
 #include "hh_internal.hpp"
@@ -33,6 +33,9 @@ __device__ __forceinline__ uint32_t f32_to_half(float f) {
 
 // The checks of a cache that its entry points share (kv_cache.hip).
 int32_t check_kv_cache(const hh_kv_cache *c);
+// Whether two rows of `dim` elements, `tokens` of them `ts` apart for each of
+// `heads` heads `hs` apart, share an element (kv_cache.hip).
+bool rows_meet(uint64_t tokens, uint64_t heads, uint64_t ts, uint64_t hs, uint64_t dim);
 
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll

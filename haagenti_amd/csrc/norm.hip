@@ -1,0 +1,457 @@
+// Layer norm and root mean square norm with their gradients (hh_norm,
+// hh_norm_backward; rules: haagenti_hip.h).
+//
+// With g = dy w, h = (x - mean) rstd (mean 0 in the rms form):
+//   y  = h w + b
+//   dx = rstd (g - mean(g) - h mean(g h)) + add   (no mean(g) in the rms form)
+//   dw = sum over rows of dy h,  db = sum over rows of dy
+//
+// Bound by memory: x in and y out; dy, x (and add) in and dx out.  A row lies
+// in the registers of W waves, C pieces of 16 bytes a lane, so it is read once
+// and its variance is summed about its mean, in f32.  The backward pass
+// recomputes both from x, which it reads anyway: two sums over registers cost
+// less than statistics kept, passed and checked.  W = 1 needs no LDS and no
+// barrier; more waves take rows too long for one wave, and few rows.
+#include "layer_ops.hpp"
+
+namespace hh {
+namespace {
+
+struct NormArgs {
+    hh_norm_args a;
+    const void *dy, *add;
+    uint64_t dy_stride, add_stride;
+    float *dw, *db;       // the sums' outputs, or null
+    float *part;          // [workgroup][2][n]: dw's and db's sums, where rows are many
+    int w32;              // weight and bias are f32
+};
+
+template <int XT>
+struct Elem {
+    static constexpr int V = XT == HH_F32 ? 4 : 8;      // values to 16 bytes
+    static constexpr int S = XT == HH_F32 ? 4 : 2;
+};
+typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
+typedef u32x2 u32x2_at2 __attribute__((aligned(2)));
+
+// Value e of 16 bytes.
+template <int XT>
+__device__ __forceinline__ float value(const u32x4 &r, int e) {
+    if constexpr (XT == HH_F32)
+        return __uint_as_float(r[e]);
+    else
+        return half_to_f32<XT>((r[e >> 1] >> (16 * (e & 1))) & 0xffffu);
+}
+template <int XT>
+__device__ __forceinline__ u32x4 packed(const float (&v)[Elem<XT>::V]) {
+    u32x4 r;
+    if constexpr (XT == HH_F32) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) r[e] = __float_as_uint(v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) r[e] = f32_to_half<XT>(v[2 * e]) | f32_to_half<XT>(v[2 * e + 1]) << 16;
+    }
+    return r;
+}
+// 16 bytes of a row at value `at`, of which `left` are the row's (zeros past them).
+template <int XT>
+__device__ __forceinline__ u32x4 load16(const void *row, uint32_t at, int32_t left) {
+    const uint8_t *p = reinterpret_cast<const uint8_t *>(row) + (uint64_t)at * Elem<XT>::S;
+    if (left >= Elem<XT>::V) return *reinterpret_cast<const u32x4_at2 *>(p);
+    u32x4 r = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < Elem<XT>::V; e++)
+        if (e < left) {
+            if constexpr (XT == HH_F32)
+                r[e] = reinterpret_cast<const uint32_t *>(p)[e];
+            else
+                r[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[e] << (16 * (e & 1));
+        }
+    return r;
+}
+template <int XT>
+__device__ __forceinline__ void store16(void *row, uint32_t at, int32_t left, const u32x4 &r) {
+    uint8_t *p = reinterpret_cast<uint8_t *>(row) + (uint64_t)at * Elem<XT>::S;
+    if (left >= Elem<XT>::V) {
+        *reinterpret_cast<u32x4_at2 *>(p) = r;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < Elem<XT>::V; e++)
+        if (e < left) {
+            if constexpr (XT == HH_F32)
+                reinterpret_cast<uint32_t *>(p)[e] = r[e];
+            else
+                reinterpret_cast<uint16_t *>(p)[e] = (uint16_t)(r[e >> 1] >> (16 * (e & 1)));
+        }
+}
+// V parameters (weight or bias) from column `at` on, `none` where there are
+// none and past the row.
+template <int XT>
+__device__ __forceinline__ void params(const void *p, int w32, uint32_t at, int32_t left, float none, float (&v)[Elem<XT>::V]) {
+    constexpr int V = Elem<XT>::V;
+#pragma unroll
+    for (int e = 0; e < V; e++) v[e] = none;
+    if (!p) return;
+    if (XT != HH_F32 && !w32) {
+        const u32x4 r = load16<XT>(p, at, left);
+#pragma unroll
+        for (int e = 0; e < V; e++) v[e] = e < left ? value<XT>(r, e) : none;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 4; i++) {
+            const u32x4 r = load16<HH_F32>(p, at + 4 * i, left - 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[4 * i + e] = 4 * i + e < left ? __uint_as_float(r[e]) : none;
+        }
+    }
+}
+
+// Sums over a wave, and over the W waves of a row (by way of `lds`, which
+// takes turns: one barrier a sum).
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    return v;
+}
+template <int W, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float (*lds)[W][2], int &turn) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = wave_sum(v[i]);
+    if constexpr (W > 1) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63u) == 0)
+#pragma unroll
+            for (int i = 0; i < N; i++) lds[turn][wave][i] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            v[i] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; w++) v[i] += lds[turn][w][i];
+        }
+        turn ^= 1;
+    }
+}
+
+// A row's mean (0 in the rms form) and 1 / sqrt(variance + eps) from its
+// pieces; left[c] values of piece c are the row's.
+template <int XT, int W, int C>
+__device__ __forceinline__ void statistics(const NormArgs &p, const u32x4 (&x)[C], const int32_t (&left)[C],
+                                           float (*lds)[W][2], int &turn, float &mean, float &rstd) {
+    constexpr int V = Elem<XT>::V;
+    const float inv = 1.0f / (float)p.a.n;
+    float s[1] = {0.0f};
+    mean = 0.0f;
+    if (p.a.kind == HH_NORM_LAYER) {
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int e = 0; e < V; e++) s[0] += value<XT>(x[c], e);
+        row_sum<W>(s, lds, turn);
+        mean = s[0] * inv;
+    }
+    s[0] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        if (left[c] >= V) {
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float d = value<XT>(x[c], e) - mean;
+                s[0] = fmaf(d, d, s[0]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float d = e < left[c] ? value<XT>(x[c], e) - mean : 0.0f;
+                s[0] = fmaf(d, d, s[0]);
+            }
+        }
+    }
+    row_sum<W>(s, lds, turn);
+    rstd = 1.0f / sqrtf(s[0] * inv + p.a.eps);
+}
+
+// W waves to a row, G rows to a workgroup at a time.
+template <int XT, int W, int G, int C>
+__global__ __launch_bounds__(64 * W * G) void norm_kernel(const NormArgs p) {
+    constexpr int V = Elem<XT>::V, T = 64 * W;
+    __shared__ float lds[2][W][2];
+    const uint32_t t = threadIdx.x % T, first = blockIdx.x * G + threadIdx.x / T, step = gridDim.x * G;
+    const hh_norm_args &a = p.a;
+    int32_t left[C];
+    float w[C][V], b[C][V];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        left[c] = (int32_t)a.n - (int32_t)((c * T + t) * V);
+        params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], 1.0f, w[c]);
+        params<XT>(a.d_bias, p.w32, (c * T + t) * V, left[c], 0.0f, b[c]);
+    }
+    auto fetch = [&](uint32_t row, u32x4 (&x)[C]) {
+        const uint8_t *at = reinterpret_cast<const uint8_t *>(a.d_x) + (uint64_t)row * a.x_stride * Elem<XT>::S;
+#pragma unroll
+        for (int c = 0; c < C; c++) x[c] = load16<XT>(at, (c * T + t) * V, left[c]);
+    };
+    u32x4 x[C], next[C];
+    int turn = 0;
+    if (first < a.rows) fetch(first, x);
+    // (W > 1: the row is the workgroup's, so all its waves go around together)
+    for (uint32_t row = first; row < a.rows; row += step) {
+        if (row + step < a.rows) fetch(row + step, next);
+        float mean, rstd;
+        statistics<XT, W, C>(p, x, left, lds, turn, mean, rstd);
+        uint8_t *to = reinterpret_cast<uint8_t *>(a.d_y) + (uint64_t)row * a.y_stride * Elem<XT>::S;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            float y[V];
+#pragma unroll
+            for (int e = 0; e < V; e++) y[e] = fmaf((value<XT>(x[c], e) - mean) * rstd, w[c][e], b[c][e]);
+            store16<XT>(to, (c * T + t) * V, left[c], packed<XT>(y));
+        }
+#pragma unroll
+        for (int c = 0; c < C; c++) x[c] = next[c];
+    }
+}
+
+// The gradients; dw's and db's sums over the workgroup's rows stay in
+// registers, are joined over its G rows in LDS and written to `part`.
+template <int XT, int W, int G, int C>
+__global__ __launch_bounds__(64 * W * G) void norm_backward_kernel(const NormArgs p) {
+    constexpr int V = Elem<XT>::V, T = 64 * W;
+    __shared__ float lds[2][W][2];
+    __shared__ __align__(16) float join[G > 1 ? G : 1][G > 1 ? T * 4 : 4];
+    const uint32_t t = threadIdx.x % T, group = threadIdx.x / T, first = blockIdx.x * G + group, step = gridDim.x * G;
+    const hh_norm_args &a = p.a;
+    const float inv = 1.0f / (float)a.n;
+    int32_t left[C];
+    float sw[C][V], sb[C][V];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        left[c] = (int32_t)a.n - (int32_t)((c * T + t) * V);
+#pragma unroll
+        for (int e = 0; e < V; e++) sw[c][e] = 0.0f, sb[c][e] = 0.0f;
+    }
+    int turn = 0;
+    for (uint32_t row = first; row < a.rows; row += step) {
+        u32x4 x[C], dy[C], add[C];
+        const uint8_t *xr = reinterpret_cast<const uint8_t *>(a.d_x) + (uint64_t)row * a.x_stride * Elem<XT>::S;
+        const uint8_t *dr = reinterpret_cast<const uint8_t *>(p.dy) + (uint64_t)row * p.dy_stride * Elem<XT>::S;
+        const uint8_t *ar = reinterpret_cast<const uint8_t *>(p.add) + (uint64_t)row * p.add_stride * Elem<XT>::S;
+#pragma unroll
+        for (int c = 0; c < C; c++) x[c] = load16<XT>(xr, (c * T + t) * V, left[c]);
+#pragma unroll
+        for (int c = 0; c < C; c++) dy[c] = load16<XT>(dr, (c * T + t) * V, left[c]);
+        if (p.add)
+#pragma unroll
+            for (int c = 0; c < C; c++) add[c] = load16<XT>(ar, (c * T + t) * V, left[c]);
+        float mean, rstd;
+        statistics<XT, W, C>(p, x, left, lds, turn, mean, rstd);
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            float w[V];
+            params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], 1.0f, w);
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float d = value<XT>(dy[c], e), h = (value<XT>(x[c], e) - mean) * rstd, g = d * w[e];  // d: 0 past the row
+                s[0] += g;
+                s[1] = fmaf(g, h, s[1]);
+                sw[c][e] = fmaf(d, h, sw[c][e]);
+                sb[c][e] += d;
+            }
+        }
+        row_sum<W>(s, lds, turn);
+        const float mg = a.kind == HH_NORM_LAYER ? s[0] * inv : 0.0f, mgh = s[1] * inv;
+        uint8_t *to = reinterpret_cast<uint8_t *>(a.d_y) + (uint64_t)row * a.y_stride * Elem<XT>::S;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            float w[V], v[V];
+            params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], 1.0f, w);
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float h = (value<XT>(x[c], e) - mean) * rstd, g = value<XT>(dy[c], e) * w[e];
+                v[e] = (g - mg - h * mgh) * rstd;
+                if (p.add) v[e] += value<XT>(add[c], e);
+            }
+            store16<XT>(to, (c * T + t) * V, left[c], packed<XT>(v));
+        }
+    }
+    if (!p.part) return;
+    // sums of dw, then of db: joined over the groups in a fixed order
+    float *out = p.part + (uint64_t)blockIdx.x * 2 * a.n;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        if (!(k ? p.db : p.dw)) continue;
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int q = 0; q < V / 4; q++) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = k ? sb[c][4 * q + e] : sw[c][4 * q + e];
+                if constexpr (G > 1) {
+                    __syncthreads();
+                    *reinterpret_cast<f32x4 *>(&join[group][t * 4]) = v;
+                    __syncthreads();
+                    if (group) continue;
+#pragma unroll
+                    for (int i = 1; i < G; i++) v += *reinterpret_cast<const f32x4 *>(&join[i][t * 4]);
+                }
+                const uint32_t at = (c * T + t) * V + 4 * q;
+                float *o = out + (uint64_t)k * a.n + at;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (at + e < a.n) o[e] = v[e];
+            }
+    }
+}
+
+// The workgroups' sums, in order: 32 columns to a workgroup, its 32 rows of
+// threads over every 32nd of them.
+__global__ __launch_bounds__(1024) void norm_join_kernel(const NormArgs p, uint32_t parts) {
+    __shared__ float sum[32][33];
+    const uint32_t col = blockIdx.x * 32 + (threadIdx.x & 31u), q = threadIdx.x >> 5, k = blockIdx.y;
+    float *out = k ? p.db : p.dw;
+    if (!out) return;
+    float s = 0.0f;
+    if (col < p.a.n)
+        for (uint32_t i = q; i < parts; i += 32) s += p.part[((uint64_t)i * 2 + k) * p.a.n + col];
+    sum[q][threadIdx.x & 31u] = s;
+    __syncthreads();
+    if (q || col >= p.a.n) return;
+    for (int i = 1; i < 32; i++) s += sum[i][threadIdx.x & 31u];
+    out[col] = s;
+}
+// No rows: sums of nothing.
+__global__ __launch_bounds__(256) void norm_zero_kernel(const NormArgs p) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= p.a.n) return;
+    if (p.dw) p.dw[i] = 0.0f;
+    if (p.db) p.db[i] = 0.0f;
+}
+
+// Waves to a row and pieces to a lane: one wave for rows that fit 8 pieces a
+// lane, where there are enough of them for two waves to a SIMD; else 4 waves,
+// or 16.
+struct NormPlan {
+    int w, c;
+    uint32_t groups, grid;
+};
+NormPlan plan_norm(const hh_norm_args &a, int cus, bool back) {
+    const uint32_t v = a.dtype == HH_F32 ? 4 : 8, pieces = (a.n + v - 1) / v;
+    NormPlan pl;
+    if (pieces <= 64 * 8 && a.rows > 4u * cus)
+        pl.w = 1;
+    else
+        pl.w = pieces <= 256 * 8 ? 4 : 16;
+    const uint32_t each = (pieces + 64 * pl.w - 1) / (64 * pl.w);
+    pl.c = pl.w == 16 ? 4 : each <= 1 ? 1 : each <= 2 ? 2 : each <= 4 ? 4 : 8;
+    pl.groups = pl.w == 1 ? 8 : 1;
+    const uint32_t most = (uint32_t)cus * (pl.w == 4 ? 2 : 1) * (back ? 1 : pl.w == 16 ? 1 : 2);
+    const uint32_t need = (a.rows + pl.groups - 1) / pl.groups;
+    pl.grid = need < most ? need : most;
+    return pl;
+}
+template <int XT, int W, int G, int C>
+void launch_one(const NormArgs &p, const NormPlan &pl, bool back, hipStream_t s) {
+    if (back)
+        hipLaunchKernelGGL((norm_backward_kernel<XT, W, G, C>), dim3(pl.grid), dim3(64 * W * G), 0, s, p);
+    else
+        hipLaunchKernelGGL((norm_kernel<XT, W, G, C>), dim3(pl.grid), dim3(64 * W * G), 0, s, p);
+}
+template <int XT, int W, int G>
+void launch_c(const NormArgs &p, const NormPlan &pl, bool back, hipStream_t s) {
+    switch (pl.c) {
+        case 1: launch_one<XT, W, G, 1>(p, pl, back, s); break;
+        case 2: launch_one<XT, W, G, 2>(p, pl, back, s); break;
+        case 4: launch_one<XT, W, G, 4>(p, pl, back, s); break;
+        default: launch_one<XT, W, G, 8>(p, pl, back, s); break;
+    }
+}
+template <int XT>
+int32_t launch_norm(const NormArgs &p, const NormPlan &pl, bool back, hipStream_t s) {
+    if (pl.w == 1)
+        launch_c<XT, 1, 8>(p, pl, back, s);
+    else if (pl.w == 4)
+        launch_c<XT, 4, 1>(p, pl, back, s);
+    else
+        launch_one<XT, 16, 1, 4>(p, pl, back, s);
+    return from_hip(hipGetLastError());
+}
+
+int32_t check_norm(const hh_norm_args *a, uint32_t *size) {
+    if (a->dtype != HH_F32 && a->dtype != HH_F16 && a->dtype != HH_BF16) return HH_ERR_UNSUPPORTED;
+    if (a->kind != HH_NORM_LAYER && a->kind != HH_NORM_RMS) return HH_ERR_UNSUPPORTED;
+    if (a->weight_dtype != a->dtype && a->weight_dtype != HH_F32) return HH_ERR_UNSUPPORTED;
+    if (a->rows >= 1u << 31) return HH_ERR_INVALID_ARGUMENT;
+    if (a->n > (a->dtype == HH_F32 ? 16384u : 32768u)) return HH_ERR_UNSUPPORTED;
+    if (!(a->eps >= 0.0f)) return HH_ERR_INVALID_ARGUMENT;
+    *size = a->dtype == HH_F32 ? 4 : 2;
+    const uint32_t ws = a->weight_dtype == HH_F32 ? 4 : 2;
+    if (a->rows && a->n && (!a->d_x || !a->d_y)) return HH_ERR_INVALID_ARGUMENT;
+    if ((((uintptr_t)a->d_x | (uintptr_t)a->d_y) & (*size - 1)) || (((uintptr_t)a->d_weight | (uintptr_t)a->d_bias) & (ws - 1)))
+        return HH_ERR_INVALID_ARGUMENT;
+    if (a->x_stride < a->n || a->y_stride < a->n) return HH_ERR_INVALID_ARGUMENT;
+    return HH_OK;
+}
+
+int32_t launch_type(const NormArgs &p, const NormPlan &pl, bool back, hipStream_t s) {
+    switch (p.a.dtype) {
+        case HH_F32: return launch_norm<HH_F32>(p, pl, back, s);
+        case HH_F16: return launch_norm<HH_F16>(p, pl, back, s);
+        default: return launch_norm<HH_BF16>(p, pl, back, s);
+    }
+}
+
+}  // namespace
+}  // namespace hh
+
+extern "C" int32_t hh_norm(hh_context *ctx, const hh_norm_args *a, void *stream) {
+    if (!ctx || !a) return HH_ERR_INVALID_ARGUMENT;
+    uint32_t size;
+    const int32_t rc = hh::check_norm(a, &size);
+    if (rc != HH_OK) return rc;
+    if (!a->rows || !a->n) return HH_OK;
+    hh::DeviceGuard guard(ctx->device);
+    if (guard.status() != hipSuccess) return hh::from_hip(guard.status());
+    hh::NormArgs p = {};
+    p.a = *a;
+    p.w32 = a->weight_dtype == HH_F32;
+    return hh::launch_type(p, hh::plan_norm(*a, ctx->num_cus > 0 ? ctx->num_cus : 256, false), false,
+                           reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" int32_t hh_norm_backward(hh_context *ctx, const hh_norm_args *a, const hh_norm_grads *d, void *stream) {
+    if (!ctx || !a || !d) return HH_ERR_INVALID_ARGUMENT;
+    uint32_t size;
+    const int32_t rc = hh::check_norm(a, &size);
+    if (rc != HH_OK) return rc;
+    if (!a->n) return HH_OK;
+    if (a->rows && !d->d_dy) return HH_ERR_INVALID_ARGUMENT;
+    if ((((uintptr_t)d->d_dy | (uintptr_t)d->d_add) & (size - 1)) || (((uintptr_t)d->d_dweight | (uintptr_t)d->d_dbias) & 3u))
+        return HH_ERR_INVALID_ARGUMENT;
+    if (d->dy_stride < a->n || (d->d_add && d->add_stride < a->n)) return HH_ERR_INVALID_ARGUMENT;
+    hh::DeviceGuard guard(ctx->device);
+    if (guard.status() != hipSuccess) return hh::from_hip(guard.status());
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    hh::NormArgs p = {};
+    p.a = *a;
+    p.w32 = a->weight_dtype == HH_F32;
+    p.dy = d->d_dy, p.add = d->d_add, p.dy_stride = d->dy_stride, p.add_stride = d->add_stride;
+    p.dw = reinterpret_cast<float *>(d->d_dweight), p.db = reinterpret_cast<float *>(d->d_dbias);
+    const bool sums = p.dw || p.db;
+    if (!a->rows) {
+        if (sums) hipLaunchKernelGGL(hh::norm_zero_kernel, dim3((a->n + 255) / 256), dim3(256), 0, s, p);
+        return hh::from_hip(hipGetLastError());
+    }
+    const hh::NormPlan pl = hh::plan_norm(*a, ctx->num_cus > 0 ? ctx->num_cus : 256, true);
+    if (sums) {
+        const int32_t e = hh::op_room(ctx, s, (size_t)pl.grid * 2 * a->n * sizeof(float), &p.part);
+        if (e != HH_OK) return e;
+    }
+    const int32_t e = hh::launch_type(p, pl, true, s);
+    if (e != HH_OK || !sums) return e;
+    hipLaunchKernelGGL(hh::norm_join_kernel, dim3((a->n + 31) / 32, 2), dim3(1024), 0, s, p, pl.grid);
+    return hh::from_hip(hipGetLastError());
+}

@@ -684,7 +684,7 @@ int32_t hh_spectral_encode_from_dct(const float *coeffs, uint32_t width, uint32_
  * counterpart in the reference, which stops at the decoded tensor.  All are
  * asynchronous on the stream and read lengths, tables and slots from device
  * memory, so a step needs no host synchronisation.  Strides are in elements.
- * hh_linear and hh_kv_attention may keep partial sums in memory that the
+ * hh_linear, hh_kv_attention and their like may keep partial sums in memory that the
  * context holds for each stream, grown with the largest call there so far, so
  * their calls on several streams need no order but their tensors' own.  All may be
  * captured: captured calls have memory of their own, which stays as it is
@@ -727,6 +727,59 @@ typedef struct hh_linear_args {
  * for a missing pointer, a stride below the row, m of 2^21, n of 2^26 or k of
  * 2^31 or more, HH_ERR_UNEXPECTED_EOF for an INT4 buffer that is too short. */
 int32_t hh_linear(hh_context *ctx, const hh_linear_args *args, void *stream);
+
+/* Norms of rows: y = (x - mean) / sqrt(variance + eps) * weight + bias, mean
+ * and variance (about the mean, over n) of the row; HH_NORM_RMS: without the
+ * mean, the mean square in the variance's place.  weight and bias (n values
+ * each) may be NULL.  Everything between x and y is f32. */
+typedef enum hh_norm_kind { HH_NORM_LAYER = 0, HH_NORM_RMS = 1 } hh_norm_kind;
+typedef struct hh_norm_args {
+    const void *d_x, *d_weight, *d_bias;
+    void *d_y; /* may be d_x (same stride); overlaps nothing else */
+    uint64_t x_stride, y_stride;
+    uint32_t rows, n;
+    float eps;            /* 0 or more */
+    int32_t dtype;        /* of x and y: HH_F32, HH_F16 or HH_BF16 */
+    int32_t weight_dtype; /* of weight and bias: dtype or HH_F32 */
+    int32_t kind;
+} hh_norm_args;
+/* Rows of at most 32768 values (f32: 16384), else HH_ERR_UNSUPPORTED. */
+int32_t hh_norm(hh_context *ctx, const hh_norm_args *args, void *stream);
+
+/* Its gradients: from dy (that of y) and x to dx = d_y of args, with `add`
+ * (what else flows back into x: a residual path's gradient; may be NULL) on
+ * top, and the f32 sums over the rows for weight and bias (either may be
+ * NULL).  args as for the forward pass; its d_bias is not read.  The row's
+ * statistics are computed again from x.  dx may be dy, x or add itself (same
+ * stride).  Sums are taken in a fixed order: the same call gives the same bits. */
+typedef struct hh_norm_grads {
+    const void *d_dy, *d_add; /* x's type */
+    float *d_dweight, *d_dbias;
+    uint64_t dy_stride, add_stride;
+} hh_norm_grads;
+int32_t hh_norm_backward(hh_context *ctx, const hh_norm_args *args, const hh_norm_grads *grads, void *stream);
+
+/* Rotary positions over heads of x (tokens x heads x dim): pair j of a head
+ * turns by d_positions[axis of j][token] * d_freq[j] radians,
+ * (a, b) -> (a cos - b sin, b cos + a sin); `inverse` turns back, which is
+ * also the gradient (dx from dy).  The first sections[0] pairs belong to axis
+ * 0, the next sections[1] to axis 1, and so on; their sum is the number of
+ * pairs P, at most 512.  Pair j is dimensions (j, j + P), interleaved (2 j,
+ * 2 j + 1); dimensions from 2 P on are copied.  Angles are reduced in 64 bits,
+ * so far positions lose nothing. */
+typedef struct hh_rotary_args {
+    const void *d_x;
+    void *d_y;                  /* may be d_x (same strides); rows share no element */
+    const int32_t *d_positions; /* axes rows of `tokens`, position_stride (0: one row for all) apart */
+    const float *d_freq;        /* P */
+    uint64_t x_token_stride, x_head_stride, y_token_stride, y_head_stride, position_stride;
+    uint32_t tokens, heads, dim;
+    uint32_t axes; /* 1 to 4 */
+    uint32_t sections[4];
+    int32_t interleaved, inverse;
+    int32_t dtype; /* HH_F32, HH_F16 or HH_BF16 */
+} hh_rotary_args;
+int32_t hh_rotary(hh_context *ctx, const hh_rotary_args *args, void *stream);
 
 /* A paged cache: num_blocks blocks of block_size tokens (16, 32, 64 or 128)
  * for kv_heads heads of head_dim (64, 96, 128, 192 or 256) dimensions.
