@@ -37,6 +37,23 @@ int32_t check_kv_cache(const hh_kv_cache *c);
 // `heads` heads `hs` apart, share an element (kv_cache.hip).
 bool rows_meet(uint64_t tokens, uint64_t heads, uint64_t ts, uint64_t hs, uint64_t dim);
 
+// A wave's sum, in every lane and the same in all of them: neighbours, pairs
+// and halves of a row of 16 lanes by DPP, rows by swaps (no LDS).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v += dpp<0xb1>(v);   // lane ^ 1
+    v += dpp<0x4e>(v);   // lane ^ 2
+    v += dpp<0x141>(v);  // 7 - lane of 8
+    v += dpp<0x140>(v);  // 15 - lane of 16
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+}
+
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) v = fmaxf(v, __shfl_xor(v, d));

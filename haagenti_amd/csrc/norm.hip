@@ -108,15 +108,10 @@ __device__ __forceinline__ void params(const void *p, int w32, uint32_t at, int3
     }
 }
 
-// Sums over a wave, and over the W waves of a row (by way of `lds`, which
-// takes turns: one barrier a sum).
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-    return v;
-}
-template <int W, int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float (*lds)[W][2], int &turn) {
+// Sums over the W waves of a row (by way of `lds`, which takes turns: one
+// barrier a sum).
+template <int W, int G, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float (*lds)[W * G][3], int &turn) {
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = wave_sum(v[i]);
     if constexpr (W > 1) {
@@ -129,57 +124,51 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*lds)[W][2], int &
         for (int i = 0; i < N; i++) {
             v[i] = 0.0f;
 #pragma unroll
-            for (int w = 0; w < W; w++) v[i] += lds[turn][w][i];
+            for (int w = 0; w < W; w++) v[i] += lds[turn][wave / W * W + w][i];
         }
         turn ^= 1;
     }
 }
 
-// A row's mean (0 in the rms form) and 1 / sqrt(variance + eps) from its
-// pieces; left[c] values of piece c are the row's.
-template <int XT, int W, int C>
-__device__ __forceinline__ void statistics(const NormArgs &p, const u32x4 (&x)[C], const int32_t (&left)[C],
-                                           float (*lds)[W][2], int &turn, float &mean, float &rstd) {
+// A row's values less its mean (0 in the rms form), zeros past the row.
+template <int XT, int W, int G, int C>
+__device__ __forceinline__ void off_mean(const NormArgs &p, const u32x4 (&x)[C], const int32_t (&left)[C], float inv,
+                                         float (*lds)[W * G][3], int &turn, float (&d)[C][Elem<XT>::V]) {
     constexpr int V = Elem<XT>::V;
-    const float inv = 1.0f / (float)p.a.n;
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int e = 0; e < V; e++) d[c][e] = value<XT>(x[c], e);
+    if (p.a.kind != HH_NORM_LAYER) return;
     float s[1] = {0.0f};
-    mean = 0.0f;
-    if (p.a.kind == HH_NORM_LAYER) {
 #pragma unroll
-        for (int c = 0; c < C; c++)
+    for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int e = 0; e < V; e++) s[0] += value<XT>(x[c], e);
-        row_sum<W>(s, lds, turn);
-        mean = s[0] * inv;
-    }
-    s[0] = 0.0f;
+        for (int e = 0; e < V; e++) s[0] += d[c][e];
+    row_sum<W, G>(s, lds, turn);
+    const float mean = s[0] * inv;
 #pragma unroll
-    for (int c = 0; c < C; c++) {
-        if (left[c] >= V) {
+    for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float d = value<XT>(x[c], e) - mean;
-                s[0] = fmaf(d, d, s[0]);
-            }
-        } else {
+        for (int e = 0; e < V; e++) d[c][e] -= mean;
+    if (p.a.n == C * 64 * W * V) return;
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float d = e < left[c] ? value<XT>(x[c], e) - mean : 0.0f;
-                s[0] = fmaf(d, d, s[0]);
-            }
-        }
-    }
-    row_sum<W>(s, lds, turn);
-    rstd = 1.0f / sqrtf(s[0] * inv + p.a.eps);
+    for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int e = 0; e < V; e++)
+            if (e >= left[c]) d[c][e] = 0.0f;
 }
 
-// W waves to a row, G rows to a workgroup at a time.
+// W waves to a row, G rows to a workgroup at a time.  All of a workgroup's
+// waves go around together (they meet at barriers where W > 1); past the last
+// row they read that row again and keep nothing of it.
 template <int XT, int W, int G, int C>
 __global__ __launch_bounds__(64 * W * G) void norm_kernel(const NormArgs p) {
     constexpr int V = Elem<XT>::V, T = 64 * W;
-    __shared__ float lds[2][W][2];
-    const uint32_t t = threadIdx.x % T, first = blockIdx.x * G + threadIdx.x / T, step = gridDim.x * G;
+    __shared__ float lds[2][W * G][3];
+    const uint32_t t = threadIdx.x % T, group = threadIdx.x / T, step = gridDim.x * G;
     const hh_norm_args &a = p.a;
+    const float inv = 1.0f / (float)a.n;
     int32_t left[C];
     float w[C][V], b[C][V];
 #pragma unroll
@@ -189,26 +178,33 @@ __global__ __launch_bounds__(64 * W * G) void norm_kernel(const NormArgs p) {
         params<XT>(a.d_bias, p.w32, (c * T + t) * V, left[c], 0.0f, b[c]);
     }
     auto fetch = [&](uint32_t row, u32x4 (&x)[C]) {
-        const uint8_t *at = reinterpret_cast<const uint8_t *>(a.d_x) + (uint64_t)row * a.x_stride * Elem<XT>::S;
+        const uint8_t *at = reinterpret_cast<const uint8_t *>(a.d_x) + (uint64_t)min(row, a.rows - 1) * a.x_stride * Elem<XT>::S;
 #pragma unroll
         for (int c = 0; c < C; c++) x[c] = load16<XT>(at, (c * T + t) * V, left[c]);
     };
     u32x4 x[C], next[C];
     int turn = 0;
-    if (first < a.rows) fetch(first, x);
-    // (W > 1: the row is the workgroup's, so all its waves go around together)
-    for (uint32_t row = first; row < a.rows; row += step) {
-        if (row + step < a.rows) fetch(row + step, next);
-        float mean, rstd;
-        statistics<XT, W, C>(p, x, left, lds, turn, mean, rstd);
+    fetch(blockIdx.x * G + group, x);
+    for (uint32_t base = blockIdx.x * G; base < a.rows; base += step) {
+        const uint32_t row = base + group;
+        if (base + step < a.rows) fetch(row + step, next);
+        float d[C][V], s[1] = {0.0f};
+        off_mean<XT, W, G, C>(p, x, left, inv, lds, turn, d);
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int e = 0; e < V; e++) s[0] = fmaf(d[c][e], d[c][e], s[0]);
+        row_sum<W, G>(s, lds, turn);
+        const float rstd = 1.0f / sqrtf(s[0] * inv + a.eps);
         uint8_t *to = reinterpret_cast<uint8_t *>(a.d_y) + (uint64_t)row * a.y_stride * Elem<XT>::S;
+        if (row < a.rows)
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            float y[V];
+            for (int c = 0; c < C; c++) {
+                float y[V];
 #pragma unroll
-            for (int e = 0; e < V; e++) y[e] = fmaf((value<XT>(x[c], e) - mean) * rstd, w[c][e], b[c][e]);
-            store16<XT>(to, (c * T + t) * V, left[c], packed<XT>(y));
-        }
+                for (int e = 0; e < V; e++) y[e] = fmaf(d[c][e] * rstd, w[c][e], b[c][e]);
+                store16<XT>(to, (c * T + t) * V, left[c], packed<XT>(y));
+            }
 #pragma unroll
         for (int c = 0; c < C; c++) x[c] = next[c];
     }
@@ -219,63 +215,90 @@ __global__ __launch_bounds__(64 * W * G) void norm_kernel(const NormArgs p) {
 template <int XT, int W, int G, int C>
 __global__ __launch_bounds__(64 * W * G) void norm_backward_kernel(const NormArgs p) {
     constexpr int V = Elem<XT>::V, T = 64 * W;
-    __shared__ float lds[2][W][2];
+    constexpr bool AHEAD = C * V <= 16;   // the next row on its way and the weights in registers, where these allow
+    __shared__ float lds[2][W * G][3];
     __shared__ __align__(16) float join[G > 1 ? G : 1][G > 1 ? T * 4 : 4];
-    const uint32_t t = threadIdx.x % T, group = threadIdx.x / T, first = blockIdx.x * G + group, step = gridDim.x * G;
+    const uint32_t t = threadIdx.x % T, group = threadIdx.x / T, step = gridDim.x * G;
     const hh_norm_args &a = p.a;
     const float inv = 1.0f / (float)a.n;
     int32_t left[C];
-    float sw[C][V], sb[C][V];
+    float sw[C][V], sb[C][V], held[AHEAD ? C : 1][V];
 #pragma unroll
     for (int c = 0; c < C; c++) {
         left[c] = (int32_t)a.n - (int32_t)((c * T + t) * V);
+        if (AHEAD) params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], 1.0f, held[AHEAD ? c : 0]);
 #pragma unroll
         for (int e = 0; e < V; e++) sw[c][e] = 0.0f, sb[c][e] = 0.0f;
     }
-    int turn = 0;
-    for (uint32_t row = first; row < a.rows; row += step) {
+    struct Row {
         u32x4 x[C], dy[C], add[C];
-        const uint8_t *xr = reinterpret_cast<const uint8_t *>(a.d_x) + (uint64_t)row * a.x_stride * Elem<XT>::S;
-        const uint8_t *dr = reinterpret_cast<const uint8_t *>(p.dy) + (uint64_t)row * p.dy_stride * Elem<XT>::S;
-        const uint8_t *ar = reinterpret_cast<const uint8_t *>(p.add) + (uint64_t)row * p.add_stride * Elem<XT>::S;
+    };
+    auto fetch = [&](uint32_t row, Row &r) {
+        const uint64_t i = min(row, a.rows - 1);
+        const uint8_t *xr = reinterpret_cast<const uint8_t *>(a.d_x) + i * a.x_stride * Elem<XT>::S;
+        const uint8_t *dr = reinterpret_cast<const uint8_t *>(p.dy) + i * p.dy_stride * Elem<XT>::S;
+        const uint8_t *ar = reinterpret_cast<const uint8_t *>(p.add) + i * p.add_stride * Elem<XT>::S;
 #pragma unroll
-        for (int c = 0; c < C; c++) x[c] = load16<XT>(xr, (c * T + t) * V, left[c]);
+        for (int c = 0; c < C; c++) r.x[c] = load16<XT>(xr, (c * T + t) * V, left[c]);
 #pragma unroll
-        for (int c = 0; c < C; c++) dy[c] = load16<XT>(dr, (c * T + t) * V, left[c]);
+        for (int c = 0; c < C; c++) r.dy[c] = load16<XT>(dr, (c * T + t) * V, left[c]);
         if (p.add)
 #pragma unroll
-            for (int c = 0; c < C; c++) add[c] = load16<XT>(ar, (c * T + t) * V, left[c]);
-        float mean, rstd;
-        statistics<XT, W, C>(p, x, left, lds, turn, mean, rstd);
-        float s[2] = {0.0f, 0.0f};
+            for (int c = 0; c < C; c++) r.add[c] = load16<XT>(ar, (c * T + t) * V, left[c]);
+    };
+    auto weights = [&](int c, float (&w)[V]) {
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int e = 0; e < V; e++) w[e] = held[c][e];
+        } else {
+            params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], 1.0f, w);
+        }
+    };
+    int turn = 0;
+    Row now, next;
+    if (AHEAD) fetch(blockIdx.x * G + group, now);
+    for (uint32_t base = blockIdx.x * G; base < a.rows; base += step) {
+        const uint32_t row = base + group;
+        if (!AHEAD)
+            fetch(row, now);
+        else if (base + step < a.rows)
+            fetch(row + step, next);
+        float d[C][V], dy[C][V];
+        off_mean<XT, W, G, C>(p, now.x, left, inv, lds, turn, d);
+        float s[3] = {0.0f, 0.0f, 0.0f};  // of (x - mean)^2, g, g (x - mean)
 #pragma unroll
         for (int c = 0; c < C; c++) {
             float w[V];
-            params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], 1.0f, w);
+            weights(c, w);
 #pragma unroll
             for (int e = 0; e < V; e++) {
-                const float d = value<XT>(dy[c], e), h = (value<XT>(x[c], e) - mean) * rstd, g = d * w[e];  // d: 0 past the row
-                s[0] += g;
-                s[1] = fmaf(g, h, s[1]);
-                sw[c][e] = fmaf(d, h, sw[c][e]);
-                sb[c][e] += d;
+                dy[c][e] = value<XT>(now.dy[c], e);
+                const float g = dy[c][e] * w[e];
+                s[0] = fmaf(d[c][e], d[c][e], s[0]);
+                s[1] += g;
+                s[2] = fmaf(g, d[c][e], s[2]);
             }
         }
-        row_sum<W>(s, lds, turn);
-        const float mg = a.kind == HH_NORM_LAYER ? s[0] * inv : 0.0f, mgh = s[1] * inv;
+        row_sum<W, G>(s, lds, turn);
+        // dx = g rstd - mean(g) rstd - (x - mean) rstd^3 mean(g (x - mean))
+        const float rstd = 1.0f / sqrtf(s[0] * inv + a.eps);
+        const float mg = a.kind == HH_NORM_LAYER ? s[1] * inv * rstd : 0.0f, mgd = s[2] * inv * rstd * rstd * rstd;
         uint8_t *to = reinterpret_cast<uint8_t *>(a.d_y) + (uint64_t)row * a.y_stride * Elem<XT>::S;
+        if (row < a.rows)
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            float w[V], v[V];
-            params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], 1.0f, w);
+            for (int c = 0; c < C; c++) {
+                float w[V], v[V];
+                weights(c, w);
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float h = (value<XT>(x[c], e) - mean) * rstd, g = value<XT>(dy[c], e) * w[e];
-                v[e] = (g - mg - h * mgh) * rstd;
-                if (p.add) v[e] += value<XT>(add[c], e);
+                for (int e = 0; e < V; e++) {
+                    sw[c][e] = fmaf(dy[c][e] * rstd, d[c][e], sw[c][e]);
+                    sb[c][e] += dy[c][e];
+                    v[e] = fmaf(dy[c][e] * w[e], rstd, fmaf(-d[c][e], mgd, -mg));
+                    if (p.add) v[e] += value<XT>(now.add[c], e);
+                }
+                store16<XT>(to, (c * T + t) * V, left[c], packed<XT>(v));
             }
-            store16<XT>(to, (c * T + t) * V, left[c], packed<XT>(v));
-        }
+        if (AHEAD) now = next;
     }
     if (!p.part) return;
     // sums of dw, then of db: joined over the groups in a fixed order
@@ -331,25 +354,27 @@ __global__ __launch_bounds__(256) void norm_zero_kernel(const NormArgs p) {
     if (p.db) p.db[i] = 0.0f;
 }
 
-// Waves to a row and pieces to a lane: one wave for rows that fit 8 pieces a
-// lane, where there are enough of them for two waves to a SIMD; else 4 waves,
-// or 16.
+// Waves to a row, rows to a workgroup at a time, pieces to a lane, workgroups
+// to a CU.  Few pieces to a lane, so that the next row is on its way while one
+// is worked on: layer norm of 8192 x 4096 bf16 takes 25 us with 4 waves of 2
+// pieces (30 with 2 of 4, 38 with one of 8), its gradients 70 (96, 127).
 struct NormPlan {
-    int w, c;
-    uint32_t groups, grid;
+    int w, g, c;
+    uint32_t grid;
 };
 NormPlan plan_norm(const hh_norm_args &a, int cus, bool back) {
     const uint32_t v = a.dtype == HH_F32 ? 4 : 8, pieces = (a.n + v - 1) / v;
     NormPlan pl;
-    if (pieces <= 64 * 8 && a.rows > 4u * cus)
-        pl.w = 1;
+    uint32_t per_cu;
+    if (pieces <= 128)
+        pl.w = 1, pl.g = 4, pl.c = pieces <= 64 ? 1 : 2, per_cu = back ? 2 : 4;
+    else if (pieces <= 512)
+        pl.w = 4, pl.g = 1, pl.c = pieces <= 256 ? 1 : 2, per_cu = back ? 2 : 4;
+    else if (pieces <= 1024)
+        pl.w = 8, pl.g = 1, pl.c = 2, per_cu = back ? 1 : 2;
     else
-        pl.w = pieces <= 256 * 8 ? 4 : 16;
-    const uint32_t each = (pieces + 64 * pl.w - 1) / (64 * pl.w);
-    pl.c = pl.w == 16 ? 4 : each <= 1 ? 1 : each <= 2 ? 2 : each <= 4 ? 4 : 8;
-    pl.groups = pl.w == 1 ? 8 : 1;
-    const uint32_t most = (uint32_t)cus * (pl.w == 4 ? 2 : 1) * (back ? 1 : pl.w == 16 ? 1 : 2);
-    const uint32_t need = (a.rows + pl.groups - 1) / pl.groups;
+        pl.w = 16, pl.g = 1, pl.c = pieces <= 2048 ? 2 : 4, per_cu = 1;
+    const uint32_t need = (a.rows + pl.g - 1) / pl.g, most = (uint32_t)cus * per_cu;
     pl.grid = need < most ? need : most;
     return pl;
 }
@@ -360,23 +385,17 @@ void launch_one(const NormArgs &p, const NormPlan &pl, bool back, hipStream_t s)
     else
         hipLaunchKernelGGL((norm_kernel<XT, W, G, C>), dim3(pl.grid), dim3(64 * W * G), 0, s, p);
 }
-template <int XT, int W, int G>
-void launch_c(const NormArgs &p, const NormPlan &pl, bool back, hipStream_t s) {
-    switch (pl.c) {
-        case 1: launch_one<XT, W, G, 1>(p, pl, back, s); break;
-        case 2: launch_one<XT, W, G, 2>(p, pl, back, s); break;
-        case 4: launch_one<XT, W, G, 4>(p, pl, back, s); break;
-        default: launch_one<XT, W, G, 8>(p, pl, back, s); break;
-    }
-}
 template <int XT>
 int32_t launch_norm(const NormArgs &p, const NormPlan &pl, bool back, hipStream_t s) {
-    if (pl.w == 1)
-        launch_c<XT, 1, 8>(p, pl, back, s);
-    else if (pl.w == 4)
-        launch_c<XT, 4, 1>(p, pl, back, s);
-    else
-        launch_one<XT, 16, 1, 4>(p, pl, back, s);
+    switch (pl.w * 10 + pl.c) {
+        case 11: launch_one<XT, 1, 4, 1>(p, pl, back, s); break;
+        case 12: launch_one<XT, 1, 4, 2>(p, pl, back, s); break;
+        case 41: launch_one<XT, 4, 1, 1>(p, pl, back, s); break;
+        case 42: launch_one<XT, 4, 1, 2>(p, pl, back, s); break;
+        case 82: launch_one<XT, 8, 1, 2>(p, pl, back, s); break;
+        case 162: launch_one<XT, 16, 1, 2>(p, pl, back, s); break;
+        default: launch_one<XT, 16, 1, 4>(p, pl, back, s); break;
+    }
     return from_hip(hipGetLastError());
 }
 
