@@ -238,7 +238,7 @@ EXPORTS = [
     "hh_pipeline_wait", "hh_pipeline_stream_wait", "hh_pipeline_get_times", "hh_pipeline_finish",
     "hh_pipeline_get_stats", "hh_pipeline_reset_stats", "hh_hbm_copy",
     "hh_linear", "hh_kv_plan", "hh_kv_append", "hh_kv_read", "hh_kv_attention",
-    "hh_norm", "hh_norm_backward", "hh_rotary",
+    "hh_norm", "hh_norm_backward", "hh_rotary", "hh_gated_linear",
 ]
 
 CORRUPT_HEADER_CHECKSUM, CORRUPT_BLOCK_CHECKSUM, CORRUPT_QUANT_SCHEME = 6, 7, 8

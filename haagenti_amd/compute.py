@@ -34,6 +34,7 @@ _LINEAR = struct.Struct("=6Q6Q3I4i4x")      # hh_linear_args
 _NORM = struct.Struct("=4Q2Q2If3i")         # hh_norm_args
 _NORM_GRADS = struct.Struct("=6Q")          # hh_norm_grads
 _ROTARY = struct.Struct("=4Q5Q8I3i4x")      # hh_rotary_args
+_GATED = struct.Struct("=7Q6Q3I4i4x")       # hh_gated_args
 _CACHE = struct.Struct("=4Q4I")             # hh_kv_cache
 _PLAN = struct.Struct("=10QQ5I4x")          # hh_kv_plan_args
 _ATTENTION = struct.Struct("=5Q5Q6Ifi")     # hh_kv_attention_args
@@ -43,6 +44,7 @@ _linear = _sig("hh_linear", _i32, [_vp, _bytes, _vp])
 _norm = _sig("hh_norm", _i32, [_vp, _bytes, _vp])
 _norm_backward = _sig("hh_norm_backward", _i32, [_vp, _bytes, _bytes, _vp])
 _rotary = _sig("hh_rotary", _i32, [_vp, _bytes, _vp])
+_gated = _sig("hh_gated_linear", _i32, [_vp, _bytes, _vp])
 _plan = _sig("hh_kv_plan", _i32, [_vp, _bytes, _vp])
 _append = _sig("hh_kv_append", _i32, [_vp, _bytes, _vp, _vp, _i32, _u64, _u64, _u64, _u64, _vp, _u32, _vp])
 _read = _sig("hh_kv_read", _i32, [_vp, _bytes, _vp, _u32, _i32, _vp, _vp, _vp])
@@ -372,6 +374,77 @@ def _spans_apart(a, b):
         return True
     end = [t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size() for t in (a, b)]
     return end[0] <= b.data_ptr() or end[1] <= a.data_ptr()
+
+
+
+def _gated_args(what, ctx, x, gate, up, act):
+    """The checks that both passes share: (m, n, k, x's code, the weights' code, the pointers, strides and buffer sizes)."""
+    dev, dt = ctx.device, _HALF.get(x.dtype)
+    if dt is None:
+        _refuse(UNSUPPORTED, f"{what}: {x.dtype} (float16 or bfloat16)")
+    if x.dim() != 2:
+        _refuse(INVALID_ARGUMENT, f"{what}: x is m x k")
+    m, k = x.shape
+    if isinstance(gate, Int4Weight) != isinstance(up, Int4Weight):
+        _refuse(INVALID_ARGUMENT, f"{what}: gate and up are both tensors or both Int4Weights")
+    if isinstance(gate, Int4Weight):
+        if (gate.n, gate.k) != (up.n, up.k) or gate.k != k:
+            _refuse(INVALID_ARGUMENT, f"{what}: x has {k} columns, the weights {gate.k} and {up.k}, of {gate.n} and {up.n} rows")
+        n, wt, strides, sizes, held = gate.n, INT4, (0, 0), (gate.data.numel(), up.data.numel()), (gate.data, up.data)
+        _on(dev, what, *held)
+    else:
+        if gate.dtype is not x.dtype or up.dtype is not x.dtype or gate.dim() != 2:
+            _refuse(INVALID_ARGUMENT, f"{what}: gate and up are n x k of x's type, or Int4Weights")
+        n, wt, sizes, held = gate.shape[0], dt, (0, 0), (gate, up)
+        strides = _rows(gate, n, k, dev, "gate", what), _rows(up, n, k, dev, "up", what)
+    code = ACTIVATIONS.get(act)
+    if code is None:
+        _refuse(UNSUPPORTED, f"{what}: activation {act!r}")
+    if x.requires_grad or held[0].requires_grad or held[1].requires_grad:
+        _no_grad(what)
+    return m, n, k, dt, wt, code, held, (_rows(x, m, k, dev, "x", what), *strides), sizes
+
+
+def gated_linear(ctx, x, gate, up, gate_bias=None, up_bias=None, act="silu", save=False, out=None, out_dtype=None):
+    """act(x gate^T + gate_bias) * (x up^T + up_bias) in one launch
+    (hh_gated_linear).  x: m x k, float16 or bfloat16; gate and up: n x k of
+    x's type, or two Int4Weights; biases n values of x's type.  act: a key of
+    ACTIVATIONS.  Returns out (m x n of out_dtype, by default x's type; float32
+    is allowed), with save (out, saved): saved is what
+    gated_linear_backward takes, m x 2 n float32."""
+    m, n, k, dt, wt, code, held, strides, sizes = _gated_args("gated_linear", ctx, x, gate, up, act)
+    dev, dtype = ctx.device, x.dtype
+    biases = []
+    for b in (gate_bias, up_bias):
+        if b is None:
+            biases.append(0)
+            continue
+        if b.dim() != 1 or b.shape[0] != n or b.dtype is not dtype or not b.is_contiguous():
+            _refuse(INVALID_ARGUMENT, "gated_linear: biases are n contiguous values of x's type")
+        _on(dev, "gated_linear", b)
+        if b.requires_grad:
+            _no_grad("gated_linear")
+        biases.append(b.data_ptr())
+    if out is None:
+        y_dtype, y_stride = out_dtype or dtype, n
+        if y_dtype is not dtype and y_dtype is not torch.float32:
+            _refuse(UNSUPPORTED, f"gated_linear: output {y_dtype}")
+        out = x.new_empty((m, n), dtype=y_dtype)
+    else:
+        y_dtype = out.dtype
+        if y_dtype is not dtype and y_dtype is not torch.float32:
+            _refuse(UNSUPPORTED, f"gated_linear: output {y_dtype}")
+        y_stride = _out_rows(out, m, n, out_dtype or y_dtype, dev, "gated_linear", (x, *held, gate_bias, up_bias))
+    saved = x.new_empty((m, 2 * n), dtype=torch.float32) if save else None
+    try:
+        args = _GATED.pack(x.data_ptr(), held[0].data_ptr(), held[1].data_ptr(), *biases, out.data_ptr(),
+                           saved.data_ptr() if save else 0, *strides, y_stride, *sizes, m, n, k, dt, wt, _CODE[y_dtype], code)
+    except struct.error:
+        _refuse(INVALID_ARGUMENT, f"gated_linear: {m} x {n} x {k}")
+    rc = _gated(ctx.handle, args, _stream(dev))
+    if rc:
+        _check(rc, "hh_gated_linear")
+    return (out, saved) if save else out
 
 
 

@@ -33,6 +33,8 @@ __device__ __forceinline__ uint32_t f32_to_half(float f) {
 
 // The checks of a cache that its entry points share (kv_cache.hip).
 int32_t check_kv_cache(const hh_kv_cache *c);
+// The checks that the gated products' two passes share (gated.hip).
+int32_t check_gated(const hh_gated_args *a);
 // Whether two rows of `dim` elements, `tokens` of them `ts` apart for each of
 // `heads` heads `hs` apart, share an element (kv_cache.hip).
 bool rows_meet(uint64_t tokens, uint64_t heads, uint64_t ts, uint64_t hs, uint64_t dim);

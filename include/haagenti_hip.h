@@ -781,6 +781,43 @@ typedef struct hh_rotary_args {
 } hh_rotary_args;
 int32_t hh_rotary(hh_context *ctx, const hh_rotary_args *args, void *stream);
 
+/* A gated feed-forward's first half in one launch: y = act(x G^T + gate_bias)
+ * * (x U^T + up_bias), G and U n x k as for hh_linear (both 16-bit of x's
+ * type, or both INT4 buffers).  With d_saved (m x 2 n f32, a row's n gate
+ * sums and then its n up sums, biases included) what the backward pass needs
+ * is kept.  y and d_saved overlap nothing that is read.  Limits and errors as
+ * hh_linear's, n below 2^25. */
+typedef struct hh_gated_args {
+    const void *d_x, *d_gate, *d_up, *d_gate_bias, *d_up_bias;
+    void *d_y;
+    float *d_saved; /* 16-byte aligned, or NULL */
+    uint64_t x_stride, gate_stride, up_stride, y_stride; /* gate_stride, up_stride: 16-bit weights only */
+    uint64_t gate_bytes, up_bytes;                       /* INT4 buffers' sizes */
+    uint32_t m, n, k;
+    int32_t dtype;   /* HH_F16 or HH_BF16 */
+    int32_t w_dtype; /* dtype, or HH_INT4 */
+    int32_t y_dtype; /* dtype, or HH_F32 */
+    int32_t activation;
+} hh_gated_args;
+int32_t hh_gated_linear(hh_context *ctx, const hh_gated_args *args, void *stream);
+
+/* Its gradients from dy (m x n, x's type) and d_saved of the forward call:
+ * with dg = dy up act'(gate) and du = dy act(gate),
+ *   dx = dg G + du U,  dG = dg^T x,  dU = du^T x,  sums of dg and du over the
+ * rows for the biases (f32).  Any of the outputs may be NULL, dG and dU both
+ * or neither.  dg and du are computed in f32 and rounded to x's type for the
+ * products (the biases' sums are not), whose sums are f32; outputs are
+ * rounded once, to x's type.  16-bit weights only (HH_ERR_UNSUPPORTED for
+ * INT4 buffers).  d_y and the biases of args are not read.  relu's slope at 0
+ * is 0. */
+typedef struct hh_gated_grads {
+    const void *d_dy;
+    void *d_dx, *d_dgate, *d_dup;
+    float *d_dgate_bias, *d_dup_bias;
+    uint64_t dy_stride, dx_stride, dgate_stride, dup_stride;
+} hh_gated_grads;
+int32_t hh_gated_linear_backward(hh_context *ctx, const hh_gated_args *args, const hh_gated_grads *grads, void *stream);
+
 /* A paged cache: num_blocks blocks of block_size tokens (16, 32, 64 or 128)
  * for kv_heads heads of head_dim (64, 96, 128, 192 or 256) dimensions.
  * Byte c stands for (c - 128) * scale, c in 1..255, one f32 scale per block
