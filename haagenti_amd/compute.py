@@ -35,6 +35,7 @@ _NORM = struct.Struct("=4Q2Q2If3i")         # hh_norm_args
 _NORM_GRADS = struct.Struct("=6Q")          # hh_norm_grads
 _ROTARY = struct.Struct("=4Q5Q8I3i4x")      # hh_rotary_args
 _GATED = struct.Struct("=7Q6Q3I4i4x")       # hh_gated_args
+_GATED_GRADS = struct.Struct("=6Q4Q")       # hh_gated_grads
 _CACHE = struct.Struct("=4Q4I")             # hh_kv_cache
 _PLAN = struct.Struct("=10QQ5I4x")          # hh_kv_plan_args
 _ATTENTION = struct.Struct("=5Q5Q6Ifi")     # hh_kv_attention_args
@@ -45,6 +46,7 @@ _norm = _sig("hh_norm", _i32, [_vp, _bytes, _vp])
 _norm_backward = _sig("hh_norm_backward", _i32, [_vp, _bytes, _bytes, _vp])
 _rotary = _sig("hh_rotary", _i32, [_vp, _bytes, _vp])
 _gated = _sig("hh_gated_linear", _i32, [_vp, _bytes, _vp])
+_gated_backward = _sig("hh_gated_linear_backward", _i32, [_vp, _bytes, _bytes, _vp])
 _plan = _sig("hh_kv_plan", _i32, [_vp, _bytes, _vp])
 _append = _sig("hh_kv_append", _i32, [_vp, _bytes, _vp, _vp, _i32, _u64, _u64, _u64, _u64, _vp, _u32, _vp])
 _read = _sig("hh_kv_read", _i32, [_vp, _bytes, _vp, _u32, _i32, _vp, _vp, _vp])
@@ -445,6 +447,50 @@ def gated_linear(ctx, x, gate, up, gate_bias=None, up_bias=None, act="silu", sav
     if rc:
         _check(rc, "hh_gated_linear")
     return (out, saved) if save else out
+
+
+
+class GatedGrads:
+    """What gated_linear_backward gives: dx, dgate, dup (of x's type) and the biases' dgate_bias, dup_bias (float32); None for
+    what was not asked for."""
+    __slots__ = ("dx", "dgate", "dup", "dgate_bias", "dup_bias")
+
+    def __init__(self, dx, dgate, dup, dgate_bias, dup_bias):
+        self.dx, self.dgate, self.dup, self.dgate_bias, self.dup_bias = dx, dgate, dup, dgate_bias, dup_bias
+
+
+def gated_linear_backward(ctx, dy, x, gate, up, saved, act="silu", dx=True, dw=True, bias=False):
+    """The gradients of gated_linear from dy, that of its output (m x n of x's
+    type), its x, gate and up (16-bit tensors), act, and what it saved
+    (hh_gated_linear_backward).  dx, dw (both weights'), bias (both): which are
+    computed.  Returns GatedGrads."""
+    what = "gated_linear_backward"
+    if isinstance(gate, Int4Weight) or isinstance(up, Int4Weight):
+        _refuse(UNSUPPORTED, f"{what}: 16-bit weights")
+    m, n, k, dt, wt, code, held, strides, sizes = _gated_args(what, ctx, x, gate, up, act)
+    dev = ctx.device
+    if dy.dtype is not x.dtype:
+        _refuse(INVALID_ARGUMENT, f"{what}: dy has x's type")
+    dy_stride = _rows(dy, m, n, dev, "dy", what)
+    if saved.dtype != torch.float32 or tuple(saved.shape) != (m, 2 * n) or not saved.is_contiguous():
+        _refuse(INVALID_ARGUMENT, f"{what}: saved is what gated_linear gave, {m} x {2 * n}")
+    _on(dev, what, saved)
+    if dy.requires_grad or saved.requires_grad:
+        _no_grad(what)
+    gx = x.new_empty((m, k)) if dx else None
+    gw = x.new_empty((2, n, k)).unbind(0) if dw else (None, None)
+    gb = saved.new_empty((2, n)).unbind(0) if bias else (None, None)
+    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    try:
+        args = _GATED.pack(x.data_ptr(), held[0].data_ptr(), held[1].data_ptr(), 0, 0, 0, saved.data_ptr(), *strides, n, *sizes,
+                           m, n, k, dt, wt, dt, code)
+    except struct.error:
+        _refuse(INVALID_ARGUMENT, f"{what}: {m} x {n} x {k}")
+    rc = _gated_backward(ctx.handle, args, _GATED_GRADS.pack(dy.data_ptr(), at(gx), at(gw[0]), at(gw[1]), at(gb[0]), at(gb[1]),
+                                                             dy_stride, k, k, k), _stream(dev))
+    if rc:
+        _check(rc, "hh_gated_linear_backward")
+    return GatedGrads(gx, *gw, *gb)
 
 
 

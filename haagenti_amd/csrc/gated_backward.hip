@@ -1,0 +1,641 @@
+// The gradients of y = act(x G^T + gate bias) * (x U^T + up bias)
+// (hh_gated_linear_backward, include/haagenti_hip.h).
+//
+// 1. slope: dg = dy up act'(gate), du = dy act(gate), in f32 from the sums
+//    that the forward pass kept, rounded to x's type (half a step, what the
+//    matrix instructions take) into D = [dg | du]: m rows of 2 N columns, N =
+//    n rounded up to 64, zeros past both.  The biases' sums are taken here,
+//    before the rounding.  Bound by memory (14 bytes an element).
+// 2. dx = D [G; U]: a product over D's columns, the weights' rows.
+// 3. [dG; dU] = D^T x: a product over the rows of both.
+//
+// The products' sums run over the slow index of their operands (both in 3).
+// Tiles come to LDS as they lie in memory, 64 of that index deep, and are
+// transposed on their way to registers: ds_read_b64_tr_b16 gives lane i of 16
+// column i of 4 rows that the 16 lanes read.  Nothing is transposed through
+// memory (the weights alone would cost 85 us at 2 x 14336 x 4096).
+#include "layer_ops.hpp"
+
+namespace hh {
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+template <int DT>
+__device__ __forceinline__ f32x4 mma16(const u32x4 &a, const u32x4 &b, const f32x4 &c) {
+    if constexpr (DT == HH_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------- slope
+
+struct SlopeArgs {
+    const uint16_t *dy;
+    const float *saved;   // [m][gate's n, up's n]
+    uint16_t *d;          // [rows][2 N]
+    float *part;          // [row block][2 n]: the biases' sums, or null
+    float *gate_bias, *up_bias;
+    uint64_t dy_stride;
+    uint32_t m, n, wide;  // wide: N
+    uint32_t rows;        // m, or m rounded up to 64 where the rows past it are read
+    int act;
+};
+constexpr uint32_t kSlopeRows = 32;  // of a workgroup
+
+// act(z) and act'(z).
+__device__ __forceinline__ void act_and_slope(float z, int act, float &a, float &s) {
+    switch (act) {
+        case HH_ACT_RELU: a = fmaxf(z, 0.0f) + (z != z ? z : 0.0f), s = z > 0.0f ? 1.0f : z != z ? z : 0.0f; break;
+        case HH_ACT_GELU: {
+            const float p = 0.5f * (1.0f + erff(z * 0.70710678118654752440f));
+            a = z * p, s = fmaf(z * 0.39894228040143267794f, __expf(-0.5f * z * z), p);
+            break;
+        }
+        case HH_ACT_GELU_TANH: {
+            // 0.5 (1 + tanh u) = p = 1 / (1 + exp(-2 u)); its slope 2 p (1 - p) u'
+            const float u = 0.79788456080286535588f * (z + 0.044715f * z * z * z);
+            const float p = 1.0f / (1.0f + __expf(-2.0f * u));
+            a = z * p;
+            const float du = 0.79788456080286535588f * (1.0f + 0.134145f * z * z);
+            const float q = p * (1.0f - p);
+            s = q == 0.0f ? p : fmaf(2.0f * z * q, du, p);  // far out du may be infinite
+            break;
+        }
+        case HH_ACT_SILU: {
+            const float p = 1.0f / (1.0f + __expf(-z));
+            a = z * p;
+            const float q = p * (1.0f - p);
+            s = q == 0.0f ? p : fmaf(z, q, p);
+            break;
+        }
+        default: a = z, s = 1.0f;
+    }
+}
+
+// 4 columns a lane, 256 a wave, every 4th row of the block a wave.
+template <int DT>
+__global__ __launch_bounds__(256) void gated_slope_kernel(const SlopeArgs p) {
+    __shared__ __align__(16) float sums[2][4][256];
+    const uint32_t across = (p.wide + 255) / 256, block = blockIdx.x / across, c0 = blockIdx.x % across * 256;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = c0 + lane * 4, r0 = block * kSlopeRows;
+    f32x4 sg = {0, 0, 0, 0}, su = {0, 0, 0, 0};
+    if (c < p.wide) {
+#pragma unroll 2
+        for (uint32_t r = r0 + wave; r < min(r0 + kSlopeRows, p.rows); r += 4) {
+            f32x4 dg = {0, 0, 0, 0}, du = {0, 0, 0, 0};
+            if (r < p.m && c < p.n) {
+                const uint16_t *dy = p.dy + r * p.dy_stride + c;
+                const float *s = p.saved + (uint64_t)r * 2 * p.n + c;
+                float d[4] = {0, 0, 0, 0}, g[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
+                if (c + 4 <= p.n) {
+                    const u32x2 v = *reinterpret_cast<const u32x2_any *>(dy);
+                    const f32x4 a = *reinterpret_cast<const f32x4_any *>(s), b = *reinterpret_cast<const f32x4_any *>(s + p.n);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        d[e] = half_to_f32<DT>((v[e >> 1] >> (16 * (e & 1))) & 0xffffu);
+                        g[e] = a[e], u[e] = b[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (c + e < p.n) d[e] = half_to_f32<DT>(dy[e]), g[e] = s[e], u[e] = s[p.n + e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float a, slope;
+                    act_and_slope(g[e], p.act, a, slope);
+                    dg[e] = d[e] * u[e] * slope, du[e] = d[e] * a;
+                }
+                sg += dg, su += du;
+            }
+            uint16_t *to = p.d + (uint64_t)r * 2 * p.wide + c;
+            *reinterpret_cast<u32x2 *>(to) = u32x2{f32_to_half<DT>(dg[0]) | f32_to_half<DT>(dg[1]) << 16,
+                                                   f32_to_half<DT>(dg[2]) | f32_to_half<DT>(dg[3]) << 16};
+            *reinterpret_cast<u32x2 *>(to + p.wide) = u32x2{f32_to_half<DT>(du[0]) | f32_to_half<DT>(du[1]) << 16,
+                                                            f32_to_half<DT>(du[2]) | f32_to_half<DT>(du[3]) << 16};
+        }
+    }
+    if (!p.part) return;
+    *reinterpret_cast<f32x4 *>(&sums[0][wave][lane * 4]) = sg;
+    *reinterpret_cast<f32x4 *>(&sums[1][wave][lane * 4]) = su;
+    __syncthreads();
+    const uint32_t col = c0 + threadIdx.x;
+    if (col >= p.n) return;
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+        p.part[((uint64_t)block * 2 + k) * p.n + col] = (sums[k][0][threadIdx.x] + sums[k][1][threadIdx.x]) +
+                                                             (sums[k][2][threadIdx.x] + sums[k][3][threadIdx.x]);
+}
+// The row blocks' sums, in order: 32 columns to a workgroup, its 32 rows of
+// threads over every 32nd block.
+__global__ __launch_bounds__(1024) void gated_bias_kernel(const SlopeArgs p, uint32_t blocks) {
+    __shared__ float sum[32][33];
+    const uint32_t col = blockIdx.x * 32 + (threadIdx.x & 31u), q = threadIdx.x >> 5, k = blockIdx.y;
+    float *out = k ? p.up_bias : p.gate_bias;
+    if (!out) return;
+    float s = 0.0f;
+    if (col < p.n)
+        for (uint32_t i = q; i < blocks; i += 32) s += p.part[((uint64_t)i * 2 + k) * p.n + col];
+    sum[q][threadIdx.x & 31u] = s;
+    __syncthreads();
+    if (q || col >= p.n) return;
+    for (int i = 1; i < 32; i++) s += sum[i][threadIdx.x & 31u];
+    out[col] = s;
+}
+
+// ---------------------------------------------------------------- products
+//
+// C[r][c] = sum over t of R[r][t] L[t][c].  For dx: r the rows of x, c its
+// columns, t the weights' rows (G's, zeros up to N, U's), R = D.  For the
+// weights (TURN: both operands are transposed): r D's columns, c x's columns,
+// t the rows, R[r][t] = D[t][r].
+
+struct BackArgs {
+    const uint16_t *l[2];    // the left matrix's parts: G and U, or x
+    uint64_t l_stride[2];
+    const uint16_t *d;
+    uint16_t *out[2];        // dx, or dG and dU
+    uint64_t out_stride[2];
+    float *partial;          // [split][rows][cols rounded up to 4], or null
+    uint32_t rows, cols;     // of C; TURN: rows counts 2 N
+    uint32_t depth;          // t of one part
+    uint32_t n, wide;
+    uint32_t steps;          // of 64 t to a split
+};
+
+// Where 16 columns' unit of 32 bytes of row t of a transposed tile lies: rows
+// that are read together (t = 8 g + 0..3) in different banks.
+__device__ __forceinline__ uint32_t twist(uint32_t t, uint32_t units) { return ((t & 3u) | (t >> 1 & 4u)) & (units - 1); }
+
+// The next 64 t of a split: the part, its first t.
+__device__ __forceinline__ uint32_t steps_of(uint32_t depth) { return (depth + 63) / 64; }
+
+template <int W>
+struct Turned {
+    // LDS offsets (elements) of this lane's reads: fragment i's rows t = 8 g + (lane / 4 % 4)
+    template <int N>
+    static __device__ __forceinline__ void places(uint32_t lane, uint32_t first, uint32_t (&at)[N]) {
+        const uint32_t t = (lane >> 4) * 8 + (lane >> 2 & 3u);
+#pragma unroll
+        for (int i = 0; i < N; i++) at[i] = t * W + ((first / 16 + i) ^ twist(t, W / 16)) * 16 + (lane & 3u) * 4;
+    }
+    // 8 t of a column: t = 32 f + 8 g + 0..7
+    static __device__ __forceinline__ u32x4 read(const uint16_t *lds, uint32_t at, uint32_t f) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(lds + at + f * 32 * W));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(lds + at + f * 32 * W + 4 * W));
+        const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+        return u32x4{a[0], a[1], b[0], b[1]};
+#else
+        return u32x4{};
+#endif
+    }
+};
+
+// The tile of a workgroup: bands of 8 tiles of r, in them down the band and
+// then along c, consecutive ones on one XCD (32 of them at a time read 8 + 4
+// tiles' operands).
+struct Place {
+    uint32_t r, c;
+};
+__device__ __forceinline__ Place place_of(uint32_t rt, uint32_t ct) {
+    const uint32_t share = gridDim.x / 8, rest = gridDim.x % 8, xcd = blockIdx.x % 8;
+    const uint32_t id = xcd * share + min(xcd, rest) + blockIdx.x / 8;
+    const uint32_t band = id / (8 * ct), in = id % (8 * ct), high = min(8u, rt - 8 * band);
+    return {8 * band + in % high, in / high};
+}
+
+// Outputs c .. c + 3 of row r.
+template <int DT, bool TURN>
+__device__ __forceinline__ void store_back(const BackArgs &p, uint32_t split, uint32_t r, uint32_t c, const f32x4 &v, bool wide) {
+    if (p.partial) {
+        *reinterpret_cast<f32x4 *>(p.partial + ((uint64_t)split * p.rows + r) * ((p.cols + 3) / 4 * 4) + c) = v;
+        return;
+    }
+    const uint32_t side = TURN && r >= p.wide, row = TURN && side ? r - p.wide : r;
+    if (TURN && row >= p.n) return;
+    uint16_t *to = p.out[side] + row * p.out_stride[side] + c;
+    if (wide && c + 4 <= p.cols) {
+        *reinterpret_cast<u32x2_any *>(to) =
+            u32x2{f32_to_half<DT>(v[0]) | f32_to_half<DT>(v[1]) << 16, f32_to_half<DT>(v[2]) | f32_to_half<DT>(v[3]) << 16};
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (c + i < p.cols) to[i] = (uint16_t)f32_to_half<DT>(v[i]);
+}
+
+// Aligned operands, copied straight to LDS, two tiles in turn (as the forward
+// products' large tiles): 16-byte pieces at places that depend on their row.
+template <int ROWS, int T>
+__device__ __forceinline__ void plain_offsets(uint32_t stride, uint32_t rows, uint32_t (&off)[ROWS * 8 / T]) {
+#pragma unroll
+    for (int j = 0; j < ROWS * 8 / T; j++) {
+        const uint32_t slot = j * T + threadIdx.x, row = slot >> 3, piece = (slot & 7u) ^ (row & 7u);
+        off[j] = (min(row, rows - 1) * stride + piece * 8) * 2;
+    }
+}
+template <int W, int T>
+__device__ __forceinline__ void turned_offsets(uint32_t cols, uint32_t (&t)[W * 8 / T], uint32_t (&off)[W * 8 / T]) {
+#pragma unroll
+    for (int j = 0; j < W * 8 / T; j++) {
+        const uint32_t slot = j * T + threadIdx.x, piece = (slot % (W / 8)) ^ (2 * twist(slot / (W / 8), W / 16));
+        t[j] = slot / (W / 8);
+        off[j] = min(piece * 8, cols - 8) * 2;  // cols: a multiple of 8, at least 8
+    }
+}
+template <int N, int T, typename Source>
+__device__ __forceinline__ void copy_pieces(const Source &from, uint32_t at, const uint32_t (&off)[N], uint16_t *lds, uint32_t wave) {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+    for (int j = 0; j < N; j++)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            from, (__attribute__((address_space(3))) void *)(lds + (j * T + wave * 64) * 8), 16, off[j], at, 0, 0);
+#endif
+}
+__device__ __forceinline__ auto source(const uint16_t *p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0, 0xffffffffu, 0x00027000);
+}
+
+template <int DT, bool TURN, int TC, int TR, int WC, int WR>
+__global__ __launch_bounds__(64 * WC * WR) void gated_back_kernel(const BackArgs p) {
+    constexpr int T = 64 * WC * WR, NI = TC / WC / 16, MI = TR / WR / 16, LP = TC * 8 / T, RP = TR * 8 / T;
+    __shared__ __align__(16) uint16_t ll0[TC * 64], ll1[TC * 64], lr0[TR * 64], lr1[TR * 64];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t r = lane & 15u, g = lane >> 4;
+    const Place at = place_of((p.rows + TR - 1) / TR, (p.cols + TC - 1) / TC);
+    const uint32_t c0 = at.c * TC, r0 = at.r * TR, wc = wave % WC * (TC / WC), wr = wave / WC * (TR / WR);
+    const uint32_t each = steps_of(p.depth), all = TURN ? each : 2 * each;
+    const uint32_t s0 = blockIdx.y * p.steps, s1 = min(all, s0 + p.steps);
+    f32x4 acc[NI][MI];
+#pragma unroll
+    for (int i = 0; i < NI; i++)
+#pragma unroll
+        for (int j = 0; j < MI; j++) acc[i][j] = f32x4{0, 0, 0, 0};
+    uint32_t lt[LP], lo[LP], rt[RP], ro[RP], la[NI], ra[MI];
+    turned_offsets<TC, T>(p.cols - c0, lt, lo);
+    if constexpr (TURN)
+        turned_offsets<TR, T>(p.rows - r0, rt, ro);
+    else
+        plain_offsets<TR, T>(2 * p.wide, p.rows - r0, ro);
+    Turned<TC>::places(lane, wc, la);
+    if constexpr (TURN) Turned<TR>::places(lane, wr, ra);
+    // Step s: rows of a part from t on; those past the part repeat its last
+    // one and are cleared where they have come (D's are zeros).
+    auto copy = [&](uint16_t *ll, uint16_t *lr, uint32_t s) {
+        const uint32_t part = !TURN && s >= each, t = (s - (part ? each : 0)) * 64, left = p.depth - t;
+        uint32_t off[LP];
+#pragma unroll
+        for (int j = 0; j < LP; j++) off[j] = min(lt[j], left - 1) * (uint32_t)p.l_stride[part] * 2 + lo[j];
+        copy_pieces<LP, T>(source(p.l[part] + (uint64_t)t * p.l_stride[part] + c0), 0, off, ll, wave);
+        if constexpr (TURN) {
+            uint32_t of[RP];
+#pragma unroll
+            for (int j = 0; j < RP; j++) of[j] = rt[j] * (4 * p.wide) + ro[j];
+            copy_pieces<RP, T>(source(p.d + (uint64_t)t * 2 * p.wide + r0), 0, of, lr, wave);
+        } else {
+            copy_pieces<RP, T>(source(p.d + (uint64_t)r0 * 2 * p.wide), 2 * (t + (part ? p.wide : 0)), ro, lr, wave);
+        }
+    };
+    auto clear = [&](uint16_t *ll, uint32_t s) {
+        const uint32_t t = (s >= each ? s - each : s) * 64, left = p.depth - t;
+        if (left >= 64) return;
+        for (uint32_t i = left * (TC / 8) + threadIdx.x; i < 64 * (TC / 8); i += T) reinterpret_cast<u32x4 *>(ll)[i] = u32x4{0, 0, 0, 0};
+        __syncthreads();
+    };
+    auto multiply = [&](const uint16_t *ll, const uint16_t *lr) {
+#pragma unroll
+        for (uint32_t f = 0; f < 2; f++) {
+            u32x4 lf[NI], rf[MI];
+#pragma unroll
+            for (int j = 0; j < MI; j++) {
+                if constexpr (TURN)
+                    rf[j] = Turned<TR>::read(lr, ra[j], f);
+                else
+                    rf[j] = *reinterpret_cast<const u32x4 *>(&lr[(wr + 16 * j + r) * 64 + ((g + 4 * f) ^ (r & 7u)) * 8]);
+            }
+#pragma unroll
+            for (int i = 0; i < NI; i++) lf[i] = Turned<TC>::read(ll, la[i], f);
+#pragma unroll
+            for (int i = 0; i < NI; i++)
+#pragma unroll
+                for (int j = 0; j < MI; j++) acc[i][j] = mma16<DT>(lf[i], rf[j], acc[i][j]);
+        }
+    };
+    if (s0 < s1) copy(ll0, lr0, s0);
+    for (uint32_t s = s0; s < s1; s += 2) {
+        __syncthreads();
+        clear(ll0, s);
+        if (s + 1 < s1) {
+            copy(ll1, lr1, s + 1);
+        } else {
+            // an odd number of steps ends with one of zeros
+            for (uint32_t i = threadIdx.x; i < TC * 8; i += T) reinterpret_cast<u32x4 *>(ll1)[i] = u32x4{0, 0, 0, 0};
+            for (uint32_t i = threadIdx.x; i < TR * 8; i += T) reinterpret_cast<u32x4 *>(lr1)[i] = u32x4{0, 0, 0, 0};
+        }
+        multiply(ll0, lr0);
+        __syncthreads();
+        if (s + 1 < s1) clear(ll1, s + 1);
+        if (s + 2 < s1) copy(ll0, lr0, s + 2);
+        multiply(ll1, lr1);
+    }
+    // Sums go out by way of LDS, 16 rows x 64 columns of each wave at a time
+    constexpr int Q = 16;
+    f32x4 *own = reinterpret_cast<f32x4 *>(TC >= TR ? ll0 : lr0) + wave * 16 * Q;
+    static_assert(WC * WR * 16 * Q * 16 <= (TC >= TR ? TC : TR) * 128, "every wave's piece fits one buffer");
+#pragma unroll
+    for (int j = 0; j < MI; j++)
+#pragma unroll
+        for (int h = 0; h < NI / 4; h++) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; i++) own[r * Q + ((4 * i + g) ^ r)] = acc[4 * h + i][j];
+            __syncthreads();
+            uint32_t c = c0 + wc + 64 * h + r * 4, row = r0 + wr + 16 * j + g;
+            asm volatile("" : "+v"(c), "+v"(row));  // no addresses of later pieces in registers meanwhile
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const f32x4 v = own[(4 * q + g) * Q + (r ^ (4 * q + g))];
+                if (row + 4 * q < p.rows && c < p.cols) store_back<DT, TURN>(p, blockIdx.y, row + 4 * q, c, v, true);
+            }
+        }
+}
+
+// Any layout: tiles of S x S through registers, the next ones on their way
+// while these are multiplied; 4 waves.
+template <int DT, bool TURN, int S>
+__global__ __launch_bounds__(256) void gated_back_any_kernel(const BackArgs p) {
+    constexpr int F = S / 32, P = S / 32;  // fragments of a wave's side, pieces of 16 bytes a thread
+    __shared__ __align__(16) uint16_t ll[S * 64], lr[S * 64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = lane & 15u, g = lane >> 4;
+    const Place at = place_of((p.rows + S - 1) / S, (p.cols + S - 1) / S);
+    const uint32_t c0 = at.c * S, r0 = at.r * S, wc = (wave & 1u) * (S / 2), wr = (wave >> 1) * (S / 2);
+    const uint32_t each = steps_of(p.depth), all = TURN ? each : 2 * each;
+    const uint32_t s0 = blockIdx.y * p.steps, s1 = min(all, s0 + p.steps);
+    f32x4 acc[F][F];
+#pragma unroll
+    for (int i = 0; i < F; i++)
+#pragma unroll
+        for (int j = 0; j < F; j++) acc[i][j] = f32x4{0, 0, 0, 0};
+    uint32_t la[F], ra[F];
+    Turned<S>::places(lane, wc, la);
+    if constexpr (TURN) Turned<S>::places(lane, wr, ra);
+    u32x4 lv[P], rv[P];
+    auto fetch = [&](uint32_t s) {
+        const uint32_t part = !TURN && s >= each, t0 = (s - (part ? each : 0)) * 64;
+#pragma unroll
+        for (int j = 0; j < P; j++) {
+            const uint32_t slot = j * 256 + threadIdx.x, t = t0 + slot / (S / 8), c = c0 + slot % (S / 8) * 8;
+            lv[j] = u32x4{0, 0, 0, 0};
+            if (t < p.depth && c < p.cols) {
+                const uint16_t *from = p.l[part] + (uint64_t)t * p.l_stride[part] + c;
+                if (c + 8 <= p.cols) {
+                    lv[j] = *reinterpret_cast<const u32x4_any *>(from);
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; e++)
+                        if (c + e < p.cols) lv[j][e >> 1] |= (uint32_t)from[e] << (16 * (e & 1));
+                }
+            }
+            rv[j] = u32x4{0, 0, 0, 0};
+            if constexpr (TURN) {  // (D has whole steps of rows, and N whole pieces of 64 columns)
+                const uint32_t d = r0 + slot % (S / 8) * 8;
+                if (d < p.rows) rv[j] = *reinterpret_cast<const u32x4 *>(p.d + (uint64_t)t * 2 * p.wide + d);
+            } else {
+                const uint32_t row = r0 + (slot >> 3);
+                if (row < p.rows)
+                    rv[j] = *reinterpret_cast<const u32x4 *>(p.d + (uint64_t)row * 2 * p.wide + (part ? p.wide : 0) + t0 + (slot & 7u) * 8);
+            }
+        }
+    };
+    auto stage = [&]() {
+#pragma unroll
+        for (int j = 0; j < P; j++) {
+            const uint32_t slot = j * 256 + threadIdx.x, t = slot / (S / 8), piece = slot % (S / 8), row = slot >> 3;
+            const uint32_t turned = t * S + (piece ^ (2 * twist(t, S / 16))) * 8;
+            *reinterpret_cast<u32x4 *>(&ll[turned]) = lv[j];
+            *reinterpret_cast<u32x4 *>(&lr[TURN ? turned : row * 64 + ((slot & 7u) ^ (row & 7u)) * 8]) = rv[j];
+        }
+    };
+    if (s0 < s1) fetch(s0);
+    for (uint32_t s = s0; s < s1; s++) {
+        __syncthreads();
+        stage();
+        __syncthreads();
+        if (s + 1 < s1) fetch(s + 1);
+#pragma unroll
+        for (uint32_t f = 0; f < 2; f++) {
+            u32x4 rf[F];
+#pragma unroll
+            for (int j = 0; j < F; j++) {
+                if constexpr (TURN)
+                    rf[j] = Turned<S>::read(lr, ra[j], f);
+                else
+                    rf[j] = *reinterpret_cast<const u32x4 *>(&lr[(wr + 16 * j + r) * 64 + ((g + 4 * f) ^ (r & 7u)) * 8]);
+            }
+#pragma unroll
+            for (int i = 0; i < F; i++) {
+                const u32x4 lf = Turned<S>::read(ll, la[i], f);
+#pragma unroll
+                for (int j = 0; j < F; j++) acc[i][j] = mma16<DT>(lf, rf[j], acc[i][j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < F; j++)
+#pragma unroll
+        for (int i = 0; i < F; i++) {
+            const uint32_t row = r0 + wr + 16 * j + r, c = c0 + wc + 16 * i + 4 * g;
+            if (row < p.rows && c < p.cols) store_back<DT, TURN>(p, blockIdx.y, row, c, acc[i][j], true);
+        }
+}
+
+// The splits' sums, in order.
+template <int DT, bool TURN>
+__global__ __launch_bounds__(256) void gated_back_join_kernel(const BackArgs p, uint32_t splits) {
+    const uint32_t quads = (p.cols + 3) / 4;
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (uint64_t)p.rows * quads) return;
+    const uint32_t r = (uint32_t)(i / quads), c = (uint32_t)(i % quads) * 4;
+    const uint64_t step = (uint64_t)p.rows * quads * 4;
+    f32x4 s = {0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t j = 0; j < splits; j++) s += *reinterpret_cast<const f32x4 *>(p.partial + j * step + (uint64_t)r * quads * 4 + c);
+    BackArgs q = p;
+    q.partial = nullptr;
+    store_back<DT, TURN>(q, 0, r, c, s, true);
+}
+
+// ---------------------------------------------------------------- host
+
+// A tile shape (columns, rows), workgroups to a CU, microseconds per 64 t with
+// all of them and with one alone.
+struct Shape {
+    uint32_t c, r, per_cu;
+    double us, alone;
+};
+constexpr Shape kBackShapes[] = {{256, 256, 1, 1.65, 1.65}, {256, 128, 1, 1.0, 1.0}, {128, 256, 1, 1.0, 1.0},
+                                 {128, 128, 2, 1.13, 0.67}, {128, 64, 3, 1.0, 0.45}};
+constexpr Shape kBackAnyShapes[] = {{128, 128, 2, 2.0, 1.3}, {64, 64, 4, 1.6, 0.9}};
+struct BackPlan {
+    int shape;
+    uint32_t splits, steps;
+    uint64_t tiles;
+    size_t room;  // bytes of the splits' sums
+};
+// The least of an estimate in microseconds: 4 for a tile's start and end; the
+// splits' sums are written and read at 4 TB/s and joined by one more launch.
+template <int N>
+BackPlan plan_back(uint32_t rows, uint32_t cols, uint32_t steps, int cus, const Shape (&shapes)[N]) {
+    BackPlan best = {0, 1, steps, 0, 0};
+    double least = 1e30;
+    const uint64_t sums = (uint64_t)rows * ((cols + 3) / 4 * 4);
+    for (int i = 0; i < N; i++)
+        for (uint32_t want = 1; want <= 16 && want <= steps; want *= 2) {
+            const uint32_t each = (steps + want - 1) / want, splits = (steps + each - 1) / each;
+            const uint64_t tiles = (uint64_t)((cols + shapes[i].c - 1) / shapes[i].c) * ((rows + shapes[i].r - 1) / shapes[i].r);
+            const uint64_t slots = (uint64_t)cus * shapes[i].per_cu, work = tiles * splits;
+            if (splits > 1 && sums > 1ull << 30) continue;  // 64 GiB at most, and one launch to join
+            const double step = work <= (uint64_t)cus ? shapes[i].alone : shapes[i].us;
+            double us = (double)((work + slots - 1) / slots) * (step * each + 4.0);
+            if (splits > 1) us += 4.0 + (double)sums * 8.0 * splits / 4e6;
+            if (us < least) least = us, best = {i, splits, each, tiles, splits > 1 ? splits * sums * sizeof(float) : 0};
+        }
+    return best;
+}
+
+template <int DT, bool TURN>
+int32_t launch_back(BackArgs p, const BackPlan &plan, bool aligned, float *room, hipStream_t s) {
+    p.steps = plan.steps;
+    p.partial = plan.splits > 1 ? room : nullptr;
+    const dim3 grid((uint32_t)plan.tiles, plan.splits);
+#define HH_BACK(TC, TR, WC, WR) hipLaunchKernelGGL((gated_back_kernel<DT, TURN, TC, TR, WC, WR>), grid, dim3(64 * WC * WR), 0, s, p)
+    if (aligned) {
+        switch (plan.shape) {
+            case 0: HH_BACK(256, 256, 2, 4); break;
+            case 1: HH_BACK(256, 128, 4, 2); break;
+            case 2: HH_BACK(128, 256, 2, 4); break;
+            case 3: HH_BACK(128, 128, 2, 2); break;
+            default: HH_BACK(128, 64, 2, 2); break;
+        }
+    } else if (plan.shape == 0) {
+        hipLaunchKernelGGL((gated_back_any_kernel<DT, TURN, 128>), grid, dim3(256), 0, s, p);
+    } else {
+        hipLaunchKernelGGL((gated_back_any_kernel<DT, TURN, 64>), grid, dim3(256), 0, s, p);
+    }
+#undef HH_BACK
+    const int32_t rc = from_hip(hipGetLastError());
+    if (rc != HH_OK || plan.splits == 1) return rc;
+    hipLaunchKernelGGL((gated_back_join_kernel<DT, TURN>),
+                       dim3((uint32_t)(((uint64_t)p.rows * ((p.cols + 3) / 4) + 255) / 256)), dim3(256), 0, s, p, plan.splits);
+    return from_hip(hipGetLastError());
+}
+
+template <int DT>
+int32_t gated_backward(hh_context *ctx, const hh_gated_args &a, const hh_gated_grads &d, hipStream_t s) {
+    const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
+    const uint32_t wide = (a.n + 63) / 64 * 64, rows = (a.m + 63) / 64 * 64;
+    const bool dx = d.d_dx && a.k, dw = d.d_dgate && a.k, bias = d.d_dgate_bias || d.d_dup_bias;
+    // offsets in a tile: 32 bits
+    auto fits = [](const void *p, uint64_t stride) { return !((uintptr_t)p & 15u) && !(stride & 7u) && stride < 1u << 22; };
+    const bool narrow = a.k % 8 == 0 && wide < 1u << 21;
+    const bool x_aligned = narrow && fits(a.d_gate, a.gate_stride) && fits(a.d_up, a.up_stride);
+    const bool w_aligned = narrow && fits(a.d_x, a.x_stride);
+    BackPlan px = {}, pw = {};
+    if (dx) px = x_aligned ? plan_back(a.m, a.k, 2 * (wide / 64), cus, kBackShapes) : plan_back(a.m, a.k, 2 * (wide / 64), cus, kBackAnyShapes);
+    if (dw) pw = w_aligned ? plan_back(2 * wide, a.k, rows / 64, cus, kBackShapes) : plan_back(2 * wide, a.k, rows / 64, cus, kBackAnyShapes);
+    // a launch has fewer than 2^32 threads
+    const uint32_t blocks = (rows + kSlopeRows - 1) / kSlopeRows;
+    if ((uint64_t)blocks * ((wide + 255) / 256) >= 1u << 24 || px.tiles >= 1u << 23 || pw.tiles >= 1u << 23) return HH_ERR_UNSUPPORTED;
+    // D, the biases' sums of row blocks, the larger of the products' sums
+    const size_t d_bytes = (size_t)rows * 2 * wide * sizeof(uint16_t);
+    const size_t b_bytes = bias ? ((size_t)blocks * 2 * a.n * sizeof(float) + 255) / 256 * 256 : 0;
+    float *room = nullptr;
+    const int32_t rc = op_room(ctx, s, d_bytes + b_bytes + (px.room > pw.room ? px.room : pw.room), &room);
+    if (rc != HH_OK) return rc;
+    uint8_t *at = reinterpret_cast<uint8_t *>(room);
+    SlopeArgs sl = {};
+    sl.dy = reinterpret_cast<const uint16_t *>(d.d_dy), sl.dy_stride = d.dy_stride;
+    sl.saved = a.d_saved, sl.d = reinterpret_cast<uint16_t *>(at);
+    sl.part = bias ? reinterpret_cast<float *>(at + d_bytes) : nullptr;
+    sl.gate_bias = d.d_dgate_bias, sl.up_bias = d.d_dup_bias;
+    sl.m = a.m, sl.n = a.n, sl.wide = wide, sl.rows = dw ? rows : a.m, sl.act = a.activation;
+    hipLaunchKernelGGL((gated_slope_kernel<DT>), dim3((wide + 255) / 256 * blocks), dim3(256), 0, s, sl);
+    int32_t e = from_hip(hipGetLastError());
+    if (e == HH_OK && bias) {
+        hipLaunchKernelGGL(gated_bias_kernel, dim3((a.n + 31) / 32, 2), dim3(1024), 0, s, sl, blocks);
+        e = from_hip(hipGetLastError());
+    }
+    float *sums = reinterpret_cast<float *>(at + d_bytes + b_bytes);
+    BackArgs p = {};
+    p.d = sl.d, p.cols = a.k, p.n = a.n, p.wide = wide;
+    if (e == HH_OK && dx) {
+        p.l[0] = reinterpret_cast<const uint16_t *>(a.d_gate), p.l[1] = reinterpret_cast<const uint16_t *>(a.d_up);
+        p.l_stride[0] = a.gate_stride, p.l_stride[1] = a.up_stride;
+        p.out[0] = reinterpret_cast<uint16_t *>(d.d_dx), p.out_stride[0] = d.dx_stride;
+        p.rows = a.m, p.depth = a.n;
+        e = launch_back<DT, false>(p, px, x_aligned, sums, s);
+    }
+    if (e == HH_OK && dw) {
+        p.l[0] = reinterpret_cast<const uint16_t *>(a.d_x), p.l_stride[0] = a.x_stride;
+        p.out[0] = reinterpret_cast<uint16_t *>(d.d_dgate), p.out[1] = reinterpret_cast<uint16_t *>(d.d_dup);
+        p.out_stride[0] = d.dgate_stride, p.out_stride[1] = d.dup_stride;
+        p.rows = 2 * wide, p.depth = a.m;
+        e = launch_back<DT, true>(p, pw, w_aligned, sums, s);
+    }
+    return e;
+}
+
+// Gradients of nothing: dx without weights' rows, the weights' without rows.
+__global__ __launch_bounds__(256) void gated_zero_kernel(uint16_t *out, uint64_t stride, uint32_t rows, uint32_t cols) {
+    for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y)
+        for (uint32_t c = blockIdx.x * 256 + threadIdx.x; c < cols; c += gridDim.x * 256) out[r * stride + c] = 0;
+}
+__global__ __launch_bounds__(256) void gated_zero_bias_kernel(float *out, uint32_t n) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) out[i] = 0.0f;
+}
+int32_t gated_zero(void *out, uint64_t stride, uint32_t rows, uint32_t cols, hipStream_t s) {
+    if (!out || !rows || !cols) return HH_OK;
+    hipLaunchKernelGGL(gated_zero_kernel, dim3(cols < 4096 ? (cols + 255) / 256 : 16, rows < 4096 ? rows : 4096), dim3(256), 0, s,
+                       reinterpret_cast<uint16_t *>(out), stride, rows, cols);
+    return from_hip(hipGetLastError());
+}
+
+}  // namespace
+}  // namespace hh
+
+extern "C" int32_t hh_gated_linear_backward(hh_context *ctx, const hh_gated_args *a, const hh_gated_grads *d, void *stream) {
+    if (!ctx || !a || !d) return HH_ERR_INVALID_ARGUMENT;
+    int32_t rc = hh::check_gated(a);
+    if (rc != HH_OK) return rc;
+    if (a->w_dtype == HH_INT4) return HH_ERR_UNSUPPORTED;
+    if (!d->d_dgate != !d->d_dup) return HH_ERR_INVALID_ARGUMENT;
+    if (((uintptr_t)d->d_dy | (uintptr_t)d->d_dx | (uintptr_t)d->d_dgate | (uintptr_t)d->d_dup) & 1u) return HH_ERR_INVALID_ARGUMENT;
+    if (((uintptr_t)d->d_dgate_bias | (uintptr_t)d->d_dup_bias) & 3u) return HH_ERR_INVALID_ARGUMENT;
+    if (a->m && a->n && (!d->d_dy || !a->d_saved || d->dy_stride < a->n)) return HH_ERR_INVALID_ARGUMENT;
+    if ((d->d_dx && d->dx_stride < a->k) || (d->d_dgate && (d->dgate_stride < a->k || d->dup_stride < a->k)))
+        return HH_ERR_INVALID_ARGUMENT;
+    hh::DeviceGuard guard(ctx->device);
+    if (guard.status() != hipSuccess) return hh::from_hip(guard.status());
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    if (!a->m || !a->n) {
+        rc = hh::gated_zero(d->d_dx, d->dx_stride, a->m, a->k, s);
+        if (rc == HH_OK) rc = hh::gated_zero(d->d_dgate, d->dgate_stride, a->n, a->k, s);
+        if (rc == HH_OK) rc = hh::gated_zero(d->d_dup, d->dup_stride, a->n, a->k, s);
+        for (float *b : {d->d_dgate_bias, d->d_dup_bias})
+            if (rc == HH_OK && b && a->n) {
+                hipLaunchKernelGGL(hh::gated_zero_bias_kernel, dim3((a->n + 255) / 256), dim3(256), 0, s, b, a->n);
+                rc = hh::from_hip(hipGetLastError());
+            }
+        return rc;
+    }
+    if ((!d->d_dx || !a->k) && (!d->d_dgate || !a->k) && !d->d_dgate_bias && !d->d_dup_bias) return HH_OK;
+    return a->dtype == HH_BF16 ? hh::gated_backward<HH_BF16>(ctx, *a, *d, s) : hh::gated_backward<HH_F16>(ctx, *a, *d, s);
+}
