@@ -241,13 +241,14 @@ __device__ __forceinline__ void plain_offsets(uint32_t stride, uint32_t rows, ui
         off[j] = (min(row, rows - 1) * stride + piece * 8) * 2;
     }
 }
+// Rows of a transposed tile: `rows` of them are there, others repeat the last;
+// columns past the matrix (`cols` of it, a multiple of 8) its last piece.
 template <int W, int T>
-__device__ __forceinline__ void turned_offsets(uint32_t cols, uint32_t (&t)[W * 8 / T], uint32_t (&off)[W * 8 / T]) {
+__device__ __forceinline__ void turned_offsets(uint32_t stride, uint32_t rows, uint32_t cols, uint32_t (&off)[W * 8 / T]) {
 #pragma unroll
     for (int j = 0; j < W * 8 / T; j++) {
-        const uint32_t slot = j * T + threadIdx.x, piece = (slot % (W / 8)) ^ (2 * twist(slot / (W / 8), W / 16));
-        t[j] = slot / (W / 8);
-        off[j] = min(piece * 8, cols - 8) * 2;  // cols: a multiple of 8, at least 8
+        const uint32_t slot = j * T + threadIdx.x, t = slot / (W / 8), piece = (slot % (W / 8)) ^ (2 * twist(t, W / 16));
+        off[j] = (min(t, rows - 1) * stride + min(piece * 8, cols - 8)) * 2;
     }
 }
 template <int N, int T, typename Source>
@@ -278,10 +279,9 @@ __global__ __launch_bounds__(64 * WC * WR) void gated_back_kernel(const BackArgs
     for (int i = 0; i < NI; i++)
 #pragma unroll
         for (int j = 0; j < MI; j++) acc[i][j] = f32x4{0, 0, 0, 0};
-    uint32_t lt[LP], lo[LP], rt[RP], ro[RP], la[NI], ra[MI];
-    turned_offsets<TC, T>(p.cols - c0, lt, lo);
+    uint32_t lo[LP], ro[RP], la[NI], ra[MI];
     if constexpr (TURN)
-        turned_offsets<TR, T>(p.rows - r0, rt, ro);
+        turned_offsets<TR, T>(2 * p.wide, 64, p.rows - r0, ro);
     else
         plain_offsets<TR, T>(2 * p.wide, p.rows - r0, ro);
     Turned<TC>::places(lane, wc, la);
@@ -290,15 +290,11 @@ __global__ __launch_bounds__(64 * WC * WR) void gated_back_kernel(const BackArgs
     // one and are cleared where they have come (D's are zeros).
     auto copy = [&](uint16_t *ll, uint16_t *lr, uint32_t s) {
         const uint32_t part = !TURN && s >= each, t = (s - (part ? each : 0)) * 64, left = p.depth - t;
-        uint32_t off[LP];
-#pragma unroll
-        for (int j = 0; j < LP; j++) off[j] = min(lt[j], left - 1) * (uint32_t)p.l_stride[part] * 2 + lo[j];
-        copy_pieces<LP, T>(source(p.l[part] + (uint64_t)t * p.l_stride[part] + c0), 0, off, ll, wave);
+        if (s == s0 || (!TURN && s == each) || left < 64)
+            turned_offsets<TC, T>((uint32_t)p.l_stride[part], min(left, 64u), p.cols - c0, lo);
+        copy_pieces<LP, T>(source(p.l[part] + (uint64_t)t * p.l_stride[part] + c0), 0, lo, ll, wave);
         if constexpr (TURN) {
-            uint32_t of[RP];
-#pragma unroll
-            for (int j = 0; j < RP; j++) of[j] = rt[j] * (4 * p.wide) + ro[j];
-            copy_pieces<RP, T>(source(p.d + (uint64_t)t * 2 * p.wide + r0), 0, of, lr, wave);
+            copy_pieces<RP, T>(source(p.d + (uint64_t)t * 2 * p.wide + r0), 0, ro, lr, wave);
         } else {
             copy_pieces<RP, T>(source(p.d + (uint64_t)r0 * 2 * p.wide), 2 * (t + (part ? p.wide : 0)), ro, lr, wave);
         }
@@ -326,6 +322,19 @@ __global__ __launch_bounds__(64 * WC * WR) void gated_back_kernel(const BackArgs
             for (int i = 0; i < NI; i++)
 #pragma unroll
                 for (int j = 0; j < MI; j++) acc[i][j] = mma16<DT>(lf[i], rf[j], acc[i][j]);
+        }
+        // the first reads, then one after every one or two products
+        constexpr int right = TURN ? 2 * MI : MI, reads = 2 * (2 * NI + right), lead = right + 4, rest = reads - lead;
+        constexpr int products = 2 * NI * MI, pairs = products - rest;
+        static_assert(pairs >= 0 && pairs <= rest, "one or two products to a read");
+        __builtin_amdgcn_sched_group_barrier(0x100, lead, 0);
+#pragma unroll
+        for (int i = 0; i < rest; i++) {
+            if (i < pairs)
+                __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+            else
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
     };
     if (s0 < s1) copy(ll0, lr0, s0);
