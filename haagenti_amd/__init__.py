@@ -239,7 +239,7 @@ EXPORTS = [
     "hh_pipeline_get_stats", "hh_pipeline_reset_stats", "hh_hbm_copy",
     "hh_linear", "hh_kv_plan", "hh_kv_append", "hh_kv_read", "hh_kv_attention",
     "hh_norm", "hh_norm_backward", "hh_rotary", "hh_gated_linear",
-    "hh_gated_linear_backward",
+    "hh_gated_linear_backward", "hh_kv_diff_attention",
 ]
 
 CORRUPT_HEADER_CHECKSUM, CORRUPT_BLOCK_CHECKSUM, CORRUPT_QUANT_SCHEME = 6, 7, 8

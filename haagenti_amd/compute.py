@@ -39,6 +39,7 @@ _GATED_GRADS = struct.Struct("=6Q4Q")       # hh_gated_grads
 _CACHE = struct.Struct("=4Q4I")             # hh_kv_cache
 _PLAN = struct.Struct("=10QQ5I4x")          # hh_kv_plan_args
 _ATTENTION = struct.Struct("=5Q5Q6Ifi")     # hh_kv_attention_args
+_DIFF = struct.Struct("=2Q2f")              # hh_kv_diff_args
 
 _u64, _bytes = C.c_uint64, C.c_char_p
 _linear = _sig("hh_linear", _i32, [_vp, _bytes, _vp])
@@ -50,6 +51,7 @@ _gated_backward = _sig("hh_gated_linear_backward", _i32, [_vp, _bytes, _bytes, _
 _plan = _sig("hh_kv_plan", _i32, [_vp, _bytes, _vp])
 _append = _sig("hh_kv_append", _i32, [_vp, _bytes, _vp, _vp, _i32, _u64, _u64, _u64, _u64, _vp, _u32, _vp])
 _read = _sig("hh_kv_read", _i32, [_vp, _bytes, _vp, _u32, _i32, _vp, _vp, _vp])
+_diff_attention = _sig("hh_kv_diff_attention", _i32, [_vp, _bytes, _bytes, _bytes, _vp])
 _attention = _sig("hh_kv_attention", _i32, [_vp, _bytes, _bytes, _vp])
 
 # torch.cuda.current_stream(device).cuda_stream without the Stream object
@@ -611,44 +613,84 @@ class KvCache:
             _check(rc, "hh_kv_read")
         return k, v
 
-    def attention(self, q, table, start, kv_len, max_q=None, max_kv=None, scale=None, out=None):
-        """softmax(scale q K^T) V of each request's new rows over its tokens
-        (hh_kv_attention): q rows x q_heads x head_dim; table (requests x
-        width), start and kv_len as kv_plan leaves them.  max_q and max_kv
-        bound a request's rows and tokens (default: q's rows, the table's
-        width; rows beyond give zeros, tokens beyond are not seen); scale defaults to head_dim ** -0.5."""
+    def _attention_args(self, what, q, table, start, kv_len, max_q, max_kv, scale, out):
+        """The checks and arguments of an attention call: (out, packed)."""
         ctx, shape, dt = self.ctx, q.shape, _HALF.get(q.dtype)
         if dt is None:
-            _refuse(UNSUPPORTED, f"attention: {q.dtype} (float16 or bfloat16)")
+            _refuse(UNSUPPORTED, f"{what}: {q.dtype} (float16 or bfloat16)")
         if len(shape) != 3:
-            _refuse(INVALID_ARGUMENT, "attention: q is rows x q_heads x head_dim")
+            _refuse(INVALID_ARGUMENT, f"{what}: q is rows x q_heads x head_dim")
         if q.requires_grad or (out is not None and out.requires_grad):
-            _no_grad("attention")
+            _no_grad(what)
         tokens, heads = shape[0], shape[1]
-        tq, hq = self._heads(q, tokens, heads, "attention: q")
+        tq, hq = self._heads(q, tokens, heads, f"{what}: q")
         if out is None:
             out = q.new_empty((tokens, heads, self.head_dim))
             to, ho = heads * self.head_dim, self.head_dim
         else:
-            to, ho = self._heads(out, tokens, heads, "attention: out")
+            to, ho = self._heads(out, tokens, heads, f"{what}: out")
             if out.dtype is not q.dtype:
-                _refuse(INVALID_ARGUMENT, "attention: out is like q")
-        _ints("attention", start, kv_len)
+                _refuse(INVALID_ARGUMENT, f"{what}: out is like q")
+        _ints(what, start, kv_len)
         requests, tshape, tstride = kv_len.numel(), table.shape, table.stride()
         if (kv_len.dim() != 1 or table.dtype != torch.int32 or len(tshape) != 2 or tshape[0] != requests or start.numel() != requests + 1
                 or (requests and tshape[1] > 1 and tstride[1] != 1)):
-            _refuse(INVALID_ARGUMENT, "attention: table requests x width, start requests + 1")
-        _on(ctx.device, "attention", table, start, kv_len)
+            _refuse(INVALID_ARGUMENT, f"{what}: table requests x width, start requests + 1")
+        _on(ctx.device, what, table, start, kv_len)
         width = tshape[1]
         try:
             args = _ATTENTION.pack(
                 q.data_ptr(), out.data_ptr(), table.data_ptr(), start.data_ptr(), kv_len.data_ptr(), tq, hq, to, ho,
                 tstride[0] if requests > 1 else width, requests, tokens, heads, width, tokens if max_q is None else max_q,
                 min(width * self.block_size, 1 << 30) if max_kv is None else max_kv,
-                self.head_dim ** -0.5 if scale is None else scale, dt)
+                scale, dt)
         except struct.error:
-            _refuse(INVALID_ARGUMENT, "attention: max_q, max_kv and scale are numbers in range")
-        rc = _attention(ctx.handle, self._c, args, _stream(ctx.device))
+            _refuse(INVALID_ARGUMENT, f"{what}: max_q, max_kv and scale are numbers in range")
+        return out, args
+
+    def attention(self, q, table, start, kv_len, max_q=None, max_kv=None, scale=None, out=None):
+        """softmax(scale q K^T) V of each request's new rows over its tokens
+        (hh_kv_attention): q rows x q_heads x head_dim; table (requests x
+        width), start and kv_len as kv_plan leaves them.  max_q and max_kv
+        bound a request's rows and tokens (default: q's rows, the table's
+        width; rows beyond give zeros, tokens beyond are not seen); scale defaults to head_dim ** -0.5."""
+        out, args = self._attention_args("attention", q, table, start, kv_len, max_q, max_kv,
+                                         self.head_dim ** -0.5 if scale is None else scale, out)
+        rc = _attention(self.ctx.handle, self._c, args, _stream(self.ctx.device))
         if rc:
             _check(rc, "hh_kv_attention")
+        return out
+
+    def diff_attention(self, q, lam, table, start, kv_len, max_q=None, max_kv=None, scale=None, norm_weight=None, eps=1e-5,
+                       gain=1.0, out=None):
+        """Differential attention (hh_kv_diff_attention): a head's dimensions
+        are two halves with a softmax map each,
+        softmax(scale q1 K1^T) V - lam softmax(scale q2 K2^T) V over all of V's
+        dimensions; with norm_weight (head_dim float32 values) the root mean
+        square norm of each head's outputs times norm_weight, then times gain.
+        lam: q_heads float32 values; scale defaults to (head_dim / 2) ** -0.5;
+        the rest as for attention."""
+        what, ctx = "diff_attention", self.ctx
+        if q.dim() != 3:
+            _refuse(INVALID_ARGUMENT, f"{what}: q is rows x q_heads x head_dim")
+        for t, n, name in ((lam, q.shape[1], "lam"), (norm_weight, self.head_dim, "norm_weight")):
+            if t is None and name == "norm_weight":
+                continue
+            if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+                _refuse(INVALID_ARGUMENT, f"{what}: {name} is {n} contiguous float32 values")
+            _on(ctx.device, what, t)
+            if t.requires_grad:
+                _no_grad(what)
+        if out is not None and any(t is not None and not _spans_apart(out, t) for t in (q, lam, norm_weight, table, start, kv_len,
+                                                                                       self.k, self.v, self.k_scale, self.v_scale)):
+            _refuse(INVALID_ARGUMENT, f"{what}: out lies over what is read")
+        out, args = self._attention_args(what, q, table, start, kv_len, max_q, max_kv,
+                                         (self.head_dim / 2) ** -0.5 if scale is None else scale, out)
+        try:
+            diff = _DIFF.pack(lam.data_ptr(), 0 if norm_weight is None else norm_weight.data_ptr(), eps, gain)
+        except (struct.error, OverflowError):
+            _refuse(INVALID_ARGUMENT, f"{what}: eps and gain are numbers in range")
+        rc = _diff_attention(ctx.handle, self._c, args, diff, _stream(ctx.device))
+        if rc:
+            _check(rc, "hh_kv_diff_attention")
         return out

@@ -914,6 +914,24 @@ typedef struct hh_kv_attention_args {
 } hh_kv_attention_args;
 int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, const hh_kv_attention_args *args, void *stream);
 
+/* Differential attention over the cache: a head's dimensions are two halves,
+ * each with a softmax map of its own over the same values,
+ *   o = softmax(scale q1 K1^T) V - lambda[head] softmax(scale q2 K2^T) V,
+ * q1, K1 the first half of the dimensions of q and of the cached keys, q2, K2
+ * the second, V all of head_dim; then, with d_norm_weight (head_dim values),
+ * o / sqrt(mean(o^2) + eps) * norm_weight * gain over each head's dimensions,
+ * else o * gain.  Arguments, limits and what rows see are hh_kv_attention's
+ * (args); rows that see no token give zeros.  A row's probabilities are
+ * rounded as there, each map's in units of its own largest: 22 bits for
+ * requests of at most 8 rows times q_heads / kv_heads, else 11. */
+typedef struct hh_kv_diff_args {
+    const float *d_lambda;      /* q_heads */
+    const float *d_norm_weight; /* head_dim, or NULL */
+    float eps, gain;            /* eps 0 or more */
+} hh_kv_diff_args;
+int32_t hh_kv_diff_attention(hh_context *ctx, const hh_kv_cache *cache, const hh_kv_attention_args *args,
+                             const hh_kv_diff_args *diff, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
