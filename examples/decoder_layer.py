@@ -3,10 +3,10 @@ LZ4 blocks of HCT-T tiles are decoded on the GPU in one launch, and requests
 of several lengths run through it with the operators of haagenti_amd.compute
 -- a prompt first, then one token at a time -- over a paged 8-bit cache.
 
-    python examples/decoder_layer.py [--hidden 4096 --heads 32 --kv-heads 8 --ffn 14336]
+    python examples/decoder_layer.py [--hidden 4096 --heads 32 --kv-heads 8 --ffn 14336 --theta 500000]
 
-Weights are random (there is no checkpoint to load); normalisation is plain
-torch, positions are left out."""
+Weights are random (there is no checkpoint to load); norms have no weight, and
+positions are left out without --theta."""
 import argparse
 import os
 import sys
@@ -55,36 +55,35 @@ def decode(ctx, names, blob, lens, tensors):
     return outs
 
 
-def norm(x):
-    """Root mean square norm, in f32."""
-    f = x.float()
-    return (f * torch.rsqrt(f.square().mean(-1, keepdim=True) + 1e-5)).to(x.dtype)
-
-
 class Layer:
-    def __init__(self, ctx, weights, heads, kv_heads, blocks, block_size=64, requests=4, width=64):
+    def __init__(self, ctx, weights, heads, kv_heads, blocks, block_size=64, requests=4, width=64, theta=None):
         self.ctx, self.w, self.heads, self.kv_heads = ctx, weights, heads, kv_heads
         self.dim = weights["o"].shape[0] // heads
         self.cache = K.KvCache.create(ctx, blocks, block_size, kv_heads, self.dim)
         self.ring, self.state = K.free_ring(blocks)
         self.table = torch.full((requests, width), -1, dtype=torch.int32, device="cuda")
         self.lens = torch.zeros(requests, dtype=torch.int32, device="cuda")
+        pairs = self.dim // 2
+        self.inv_freq = None if theta is None else float(theta) ** (-torch.arange(pairs, device="cuda") / pairs)
 
     def step(self, x, new, max_q, max_kv):
         """Hidden states x of the requests' new tokens (new per request) through the layer."""
         ctx, w, h, kv, d = self.ctx, self.w, self.heads, self.kv_heads, self.dim
         plan = K.kv_plan(ctx, self.lens, new, self.table, self.ring, self.state, self.cache.block_size, x.shape[0])
-        qkv = K.linear(ctx, norm(x), w["qkv"]).view(-1, h + 2 * kv, d)
+        qkv = K.linear(ctx, K.norm(ctx, x, kind="rms"), w["qkv"]).view(-1, h + 2 * kv, d)
+        if self.inv_freq is not None:       # queries and keys turn by their place in their request
+            first = torch.repeat_interleave(self.lens - plan.start[:-1], new, output_size=x.shape[0])
+            at = first + torch.arange(x.shape[0], dtype=torch.int32, device="cuda")
+            K.rotary(ctx, qkv[:, :h + kv], at, self.inv_freq, out=qkv[:, :h + kv])
         self.cache.append(qkv[:, h:h + kv], qkv[:, h + kv:], plan.slots)
         o = self.cache.attention(qkv[:, :h], self.table, plan.start, plan.kv_len, max_q=max_q, max_kv=max_kv)
         x = K.linear(ctx, o.view(-1, h * d), w["o"], residual=x)
-        y = norm(x)
-        y = K.linear(ctx, y, w["gate"], act="silu", mul=K.linear(ctx, y, w["up"]))
+        y = K.gated_linear(ctx, K.norm(ctx, x, kind="rms"), w["gate"], w["up"], act="silu")
         self.lens, self.state = plan.kv_len, plan.state
         return K.linear(ctx, y, w["down"], residual=x)
 
 
-def run(hidden, heads, kv_heads, ffn, prompts, steps, retention=0.3, seed=0):
+def run(hidden, heads, kv_heads, ffn, prompts, steps, retention=0.3, seed=0, theta=None):
     """Prompts of these lengths, then `steps` tokens each; returns (the weights decoded, the inputs of every step, the
     outputs of every step, milliseconds per single-token step)."""
     rng = np.random.default_rng(seed)
@@ -94,7 +93,7 @@ def run(hidden, heads, kv_heads, ffn, prompts, steps, retention=0.3, seed=0):
     weights = decode(ctx, list(sh), *encode(host, retention))
     longest = max(prompts) + steps
     blocks = sum((p + steps + 63) // 64 for p in prompts)
-    layer = Layer(ctx, weights, heads, kv_heads, blocks, 64, len(prompts), (longest + 63) // 64)
+    layer = Layer(ctx, weights, heads, kv_heads, blocks, 64, len(prompts), (longest + 63) // 64, theta)
     ins, outs, t0 = [], [], 0.0
     gen = torch.Generator(device="cuda").manual_seed(seed)
     for i in range(steps + 1):
@@ -116,8 +115,9 @@ def main():
     for name, value in (("hidden", 1024), ("heads", 8), ("kv-heads", 2), ("ffn", 3584), ("steps", 32)):
         p.add_argument("--" + name, type=int, default=value)
     p.add_argument("--prompts", type=int, nargs="+", default=[200, 31, 1, 500])
+    p.add_argument("--theta", type=float, default=None)
     a = p.parse_args()
-    _, _, outs, ms = run(a.hidden, a.heads, a.kv_heads, a.ffn, a.prompts, a.steps)
+    _, _, outs, ms = run(a.hidden, a.heads, a.kv_heads, a.ffn, a.prompts, a.steps, theta=a.theta)
     print(f"{len(a.prompts)} prompts of {a.prompts} tokens and {a.steps} steps: {ms:.3f} ms a step, "
           f"hidden states of rms {float(outs[-1].float().square().mean().sqrt()):.3f}")
 

@@ -70,10 +70,11 @@ assert back(dw=0, db=0) == 0 and len(launches("launch")) == 1, calls()
 
 # XT, W, G, C of the kernel's template: waves to a row, rows to a workgroup, pieces to a lane
 KERNELS = [
-    ("rows=8, n=4096", "norm_kernelILi2ELi4ELi1ELi2E"), ("rows=2000, n=4096", "norm_kernelILi2ELi1ELi8ELi8E"),
-    ("rows=2000, n=4097", "norm_kernelILi2ELi4ELi1ELi4E"), ("rows=1, n=1", "norm_kernelILi2ELi4ELi1ELi1E"),
-    ("rows=1, n=16384", "norm_kernelILi2ELi4ELi1ELi8E"), ("rows=1, n=16385", "norm_kernelILi2ELi16ELi1ELi4E"),
-    ("rows=2000, n=512, dtype=0", "norm_kernelILi0ELi1ELi8ELi2E"),
+    ("n=1", "norm_kernelILi2ELi1ELi4ELi1E"), ("n=512", "norm_kernelILi2ELi1ELi4ELi1E"), ("n=513", "norm_kernelILi2ELi1ELi4ELi2E"),
+    ("n=1024", "norm_kernelILi2ELi1ELi4ELi2E"), ("n=1025", "norm_kernelILi2ELi4ELi1ELi1E"),
+    ("n=2049", "norm_kernelILi2ELi4ELi1ELi2E"), ("n=4096", "norm_kernelILi2ELi4ELi1ELi2E"),
+    ("n=4097", "norm_kernelILi2ELi8ELi1ELi2E"), ("n=8193", "norm_kernelILi2ELi16ELi1ELi2E"),
+    ("n=16385", "norm_kernelILi2ELi16ELi1ELi4E"), ("n=512, dtype=0", "norm_kernelILi0ELi1ELi4ELi2E"),
 ]
 
 
