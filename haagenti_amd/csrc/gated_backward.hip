@@ -14,6 +14,8 @@
 // transposed on their way to registers: ds_read_b64_tr_b16 gives lane i of 16
 // column i of 4 rows that the 16 lanes read.  Nothing is transposed through
 // memory (the weights alone would cost 85 us at 2 x 14336 x 4096).
+#include <type_traits>
+
 #include "layer_ops.hpp"
 
 namespace hh {
@@ -165,15 +167,15 @@ struct BackArgs {
     uint32_t rows, cols;     // of C; TURN: rows counts 2 N
     uint32_t depth;          // t of one part
     uint32_t n, wide;
-    uint32_t steps;          // of 64 t to a split
+    uint32_t steps;          // of a split: of 32 t, through registers of 64
 };
 
 // Where 16 columns' unit of 32 bytes of row t of a transposed tile lies: rows
 // that are read together (t = 8 g + 0..3) in different banks.
 __device__ __forceinline__ uint32_t twist(uint32_t t, uint32_t units) { return ((t & 3u) | (t >> 1 & 4u)) & (units - 1); }
 
-// The next 64 t of a split: the part, its first t.
-__device__ __forceinline__ uint32_t steps_of(uint32_t depth) { return (depth + 63) / 64; }
+// Steps of 32 t of a part (D has zeros where its last one ends later).
+__device__ __forceinline__ uint32_t steps_of(uint32_t depth) { return (depth + 31) / 32; }
 
 template <int W>
 struct Turned {
@@ -231,43 +233,120 @@ __device__ __forceinline__ void store_back(const BackArgs &p, uint32_t split, ui
         if (c + i < p.cols) to[i] = (uint16_t)f32_to_half<DT>(v[i]);
 }
 
-// Aligned operands, copied straight to LDS, two tiles in turn (as the forward
-// products' large tiles): 16-byte pieces at places that depend on their row.
+// Aligned operands, copied straight to LDS in tiles 32 deep, four of them in
+// turn: three are on their way while one is multiplied (64 deep and two in
+// turn, a copy has one tile's products to arrive in: 483 and 479 us where
+// these take XXX), 16-byte pieces at places that depend on their row.  One
+// barrier a tile: before it a wave waits for its own part of the next tile's
+// copies, the oldest under way, and for its reads of the last one.
 template <int ROWS, int T>
-__device__ __forceinline__ void plain_offsets(uint32_t stride, uint32_t rows, uint32_t (&off)[ROWS * 8 / T]) {
+__device__ __forceinline__ void plain_offsets(uint32_t stride, uint32_t rows, uint32_t (&off)[ROWS * 4 / T]) {
 #pragma unroll
-    for (int j = 0; j < ROWS * 8 / T; j++) {
-        const uint32_t slot = j * T + threadIdx.x, row = slot >> 3, piece = (slot & 7u) ^ (row & 7u);
+    for (int j = 0; j < ROWS * 4 / T; j++) {
+        const uint32_t slot = j * T + threadIdx.x, row = slot >> 2, piece = (slot & 3u) ^ (row >> 2 & 3u);
         off[j] = (min(row, rows - 1) * stride + piece * 8) * 2;
     }
 }
-// Rows of a transposed tile: `rows` of them are there, others repeat the last;
-// columns past the matrix (`cols` of it, a multiple of 8) its last piece.
-template <int W, int T>
-__device__ __forceinline__ void turned_offsets(uint32_t stride, uint32_t rows, uint32_t cols, uint32_t (&off)[W * 8 / T]) {
-#pragma unroll
-    for (int j = 0; j < W * 8 / T; j++) {
-        const uint32_t slot = j * T + threadIdx.x, t = slot / (W / 8), piece = (slot % (W / 8)) ^ (2 * twist(t, W / 16));
-        off[j] = (min(t, rows - 1) * stride + min(piece * 8, cols - 8)) * 2;
+// A transposed tile of 32 rows t by W columns: chunks of 1 KiB, what a wave
+// copies at once, hold 512 / W rows; which ones, the unit of 16 columns that a
+// row's own is swapped with and the gap after a chunk are chosen so that the 8
+// rows of 32 bytes that half a wave reads together lie in different banks, and
+// so that few registers hold a lane's places: fragment i's is the (i mod 512 /
+// W)-th and a constant.
+template <int W>
+struct Chunks {
+    static constexpr int ROWS = 512 / W, GAP = W == 64 ? 0 : 16 * ROWS, SIZE = 512 + GAP, ALL = 32 / ROWS * SIZE;  // elements
+    static constexpr int NEXT = W == 256 ? 4 * SIZE : W == 128 ? 2 * SIZE : SIZE;  // from t to t + 4
+    static constexpr int PLACES = W == 64 ? 4 : ROWS;
+    static __device__ __forceinline__ uint32_t sub(uint32_t t) {
+        return W == 256 ? t >> 3 & 1u : W == 128 ? (t >> 2 & 2u) | (t & 1u) : (t >> 1 & 4u) | (t & 3u);
     }
-}
-template <int N, int T, typename Source>
+    static __device__ __forceinline__ uint32_t chunk(uint32_t t) {
+        return W == 256 ? (t & 7u) | (t >> 1 & 8u) : W == 128 ? (t >> 1 & 3u) | (t >> 2 & 4u) : (t >> 2 & 1u) | (t >> 3 & 2u);
+    }
+    static __device__ __forceinline__ uint32_t row(uint32_t chunk, uint32_t sub) {
+        return W == 256   ? (chunk & 7u) | sub << 3 | (chunk & 8u) << 1
+               : W == 128 ? (sub & 1u) | (chunk & 3u) << 1 | (sub & 2u) << 2 | (chunk & 4u) << 2
+                          : (sub & 3u) | (chunk & 1u) << 2 | (sub & 4u) << 1 | (chunk & 2u) << 3;
+    }
+    // the row and the column of what piece `place` of a chunk holds
+    static __device__ __forceinline__ void held(uint32_t chunk, uint32_t place, uint32_t &t, uint32_t &c) {
+        const uint32_t s = place / (64 / ROWS), piece = place % (64 / ROWS);
+        t = row(chunk, s), c = ((piece >> 1 ^ (s & (PLACES - 1))) * 2 + (piece & 1u)) * 8;
+    }
+    // this lane's reads: rows t = 8 g + (lane / 4 % 4), columns from `first` on
+    static __device__ __forceinline__ void places(uint32_t lane, uint32_t first, uint32_t (&at)[PLACES]) {
+        const uint32_t t = (lane >> 4) * 8 + (lane >> 2 & 3u), s = sub(t);
+#pragma unroll
+        for (int i = 0; i < PLACES; i++)
+            at[i] = chunk(t) * SIZE + s * W + ((first / 16 + i) ^ (s & (PLACES - 1))) * 16 + (lane & 3u) * 4;
+    }
+    // 8 t of fragment i's column
+    static __device__ __forceinline__ u32x4 read(const uint16_t *lds, const uint32_t (&at)[PLACES], int i) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
+        const uint16_t *from = lds + at[i % PLACES] + i / PLACES * PLACES * 16;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)from);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(from + NEXT));
+        const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+        return u32x4{a[0], a[1], b[0], b[1]};
+#else
+        return u32x4{};
+#endif
+    }
+    // Offsets of a lane's pieces in the matrix (bytes): `rows` rows of it are
+    // there, others repeat the last; columns past it (`cols` of it, a multiple
+    // of 8) its last piece.
+    template <int T>
+    static __device__ __forceinline__ void offsets(uint32_t thread, uint32_t stride, uint32_t rows, uint32_t cols,
+                                                   uint32_t (&off)[W * 4 / T]) {
+#pragma unroll
+        for (int j = 0; j < W * 4 / T; j++) {
+            uint32_t t, c;
+            held(j * (T / 64) + thread / 64, thread & 63u, t, c);
+            off[j] = (min(t, rows - 1) * stride + min(c, cols - 8)) * 2;
+        }
+    }
+    // Zeros to rows from `rows` on.
+    template <int T>
+    static __device__ __forceinline__ void clear(uint32_t thread, uint16_t *lds, uint32_t rows) {
+#pragma unroll
+        for (int j = 0; j < W * 4 / T; j++) {
+            uint32_t t, c;
+            const uint32_t chunk = j * (T / 64) + thread / 64;
+            held(chunk, thread & 63u, t, c);
+            if (t >= rows) *reinterpret_cast<u32x4 *>(lds + chunk * SIZE + (thread & 63u) * 8) = u32x4{0, 0, 0, 0};
+        }
+    }
+};
+template <int N, int T, int SIZE, typename Source>
 __device__ __forceinline__ void copy_pieces(const Source &from, uint32_t at, const uint32_t (&off)[N], uint16_t *lds, uint32_t wave) {
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
     for (int j = 0; j < N; j++)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            from, (__attribute__((address_space(3))) void *)(lds + (j * T + wave * 64) * 8), 16, off[j], at, 0, 0);
+            from, (__attribute__((address_space(3))) void *)(lds + (j * (T / 64) + wave) * SIZE), 16, off[j], at, 0, 0);
 #endif
 }
 __device__ __forceinline__ auto source(const uint16_t *p) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0, 0xffffffffu, 0x00027000);
 }
+// Waits until at most N of the wave's loads are under way and all its LDS
+// reads are done.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (N >> 4) << 14);
+}
 
 template <int DT, bool TURN, int TC, int TR, int WC, int WR>
 __global__ __launch_bounds__(64 * WC * WR) void gated_back_kernel(const BackArgs p) {
-    constexpr int T = 64 * WC * WR, NI = TC / WC / 16, MI = TR / WR / 16, LP = TC * 8 / T, RP = TR * 8 / T;
-    __shared__ __align__(16) uint16_t ll0[TC * 64], ll1[TC * 64], lr0[TR * 64], lr1[TR * 64];
+    constexpr int T = 64 * WC * WR, NI = TC / WC / 16, MI = TR / WR / 16, LP = TC * 4 / T, RP = TR * 4 / T;
+    // a tile of the left matrix, then one of the right; arrays of their own, so
+    // that the compiler sees which of them a copy writes
+    typedef Chunks<TC> Left;
+    typedef Chunks<TR> Right;
+    constexpr int L = Left::ALL, ALL = L + (TURN ? Right::ALL : TR * 32);
+    __shared__ __align__(16) uint16_t t0[ALL], t1[ALL], t2[ALL], t3[ALL];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t r = lane & 15u, g = lane >> 4;
     const Place at = place_of((p.rows + TR - 1) / TR, (p.cols + TC - 1) / TC);
@@ -279,85 +358,116 @@ __global__ __launch_bounds__(64 * WC * WR) void gated_back_kernel(const BackArgs
     for (int i = 0; i < NI; i++)
 #pragma unroll
         for (int j = 0; j < MI; j++) acc[i][j] = f32x4{0, 0, 0, 0};
-    uint32_t lo[LP], ro[RP], la[NI], ra[MI];
+    uint32_t lo[LP], ro[RP], la[Left::PLACES], ra[Right::PLACES];
     if constexpr (TURN)
-        turned_offsets<TR, T>(2 * p.wide, 64, p.rows - r0, ro);
+        Right::template offsets<T>(threadIdx.x, 2 * p.wide, 32, p.rows - r0, ro);
     else
         plain_offsets<TR, T>(2 * p.wide, p.rows - r0, ro);
-    Turned<TC>::places(lane, wc, la);
-    if constexpr (TURN) Turned<TR>::places(lane, wr, ra);
+    Left::places(lane, wc, la);
+    if constexpr (TURN)
+        Right::places(lane, wr, ra);
+    else
+        ra[0] = (wr + r) * 32 + (g ^ (r >> 2 & 3u)) * 8;
+    // (what is computed from this is computed where it is needed, and not kept
+    // in registers through all steps)
+    auto thread = []() {
+        uint32_t t = threadIdx.x;
+        asm volatile("" : "+v"(t));
+        return t;
+    };
     // Step s: rows of a part from t on; those past the part repeat its last
     // one and are cleared where they have come (D's are zeros).
-    auto copy = [&](uint16_t *ll, uint16_t *lr, uint32_t s) {
-        const uint32_t part = !TURN && s >= each, t = (s - (part ? each : 0)) * 64, left = p.depth - t;
-        if (s == s0 || (!TURN && s == each) || left < 64)
-            turned_offsets<TC, T>((uint32_t)p.l_stride[part], min(left, 64u), p.cols - c0, lo);
-        copy_pieces<LP, T>(source(p.l[part] + (uint64_t)t * p.l_stride[part] + c0), 0, lo, ll, wave);
+    auto copy = [&](uint16_t *to, uint32_t s) {
+        const uint32_t part = !TURN && s >= each, t = (s - (part ? each : 0)) * 32, left = p.depth - t;
+        if (s == s0 || (!TURN && s == each) || left < 32)
+            Left::template offsets<T>(thread(), (uint32_t)p.l_stride[part], min(left, 32u), p.cols - c0, lo);
+        copy_pieces<LP, T, Left::SIZE>(source(p.l[part] + (uint64_t)t * p.l_stride[part] + c0), 0, lo, to, wave);
         if constexpr (TURN) {
-            copy_pieces<RP, T>(source(p.d + (uint64_t)t * 2 * p.wide + r0), 0, ro, lr, wave);
+            copy_pieces<RP, T, Right::SIZE>(source(p.d + (uint64_t)t * 2 * p.wide + r0), 0, ro, to + L, wave);
         } else {
-            copy_pieces<RP, T>(source(p.d + (uint64_t)r0 * 2 * p.wide), 2 * (t + (part ? p.wide : 0)), ro, lr, wave);
+            copy_pieces<RP, T, 512>(source(p.d + (uint64_t)r0 * 2 * p.wide), 2 * (t + (part ? p.wide : 0)), ro, to + L, wave);
         }
     };
-    auto clear = [&](uint16_t *ll, uint32_t s) {
-        const uint32_t t = (s >= each ? s - each : s) * 64, left = p.depth - t;
-        if (left >= 64) return;
-        for (uint32_t i = left * (TC / 8) + threadIdx.x; i < 64 * (TC / 8); i += T) reinterpret_cast<u32x4 *>(ll)[i] = u32x4{0, 0, 0, 0};
+    // Zeros in the tile of step s: rows past the part's end, all of a step past
+    // the last (the steps go around in fours).
+    auto clear = [&](uint16_t *at, uint32_t s) {
+        const uint32_t t = (s >= each ? s - each : s) * 32, left = p.depth - t;
+        if (s >= s1) {
+            for (uint32_t i = thread(); i < ALL / 8; i += T) reinterpret_cast<u32x4 *>(at)[i] = u32x4{0, 0, 0, 0};
+        } else {
+            if (left >= 32) return;
+            Left::template clear<T>(thread(), at, left);
+        }
         __syncthreads();
     };
-    auto multiply = [&](const uint16_t *ll, const uint16_t *lr) {
+    // Until at most AHEAD tiles are under way, and all waves are here.
+    auto meet = [](auto ahead) {
+        wait_loads<decltype(ahead)::value * (LP + RP)>();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    struct Fragments {
+        u32x4 l[NI], r[MI];
+    };
+    auto read = [&](const uint16_t *ll, Fragments &f) {
+        const uint16_t *lr = ll + L;
 #pragma unroll
-        for (uint32_t f = 0; f < 2; f++) {
-            u32x4 lf[NI], rf[MI];
-#pragma unroll
-            for (int j = 0; j < MI; j++) {
-                if constexpr (TURN)
-                    rf[j] = Turned<TR>::read(lr, ra[j], f);
-                else
-                    rf[j] = *reinterpret_cast<const u32x4 *>(&lr[(wr + 16 * j + r) * 64 + ((g + 4 * f) ^ (r & 7u)) * 8]);
-            }
-#pragma unroll
-            for (int i = 0; i < NI; i++) lf[i] = Turned<TC>::read(ll, la[i], f);
-#pragma unroll
-            for (int i = 0; i < NI; i++)
-#pragma unroll
-                for (int j = 0; j < MI; j++) acc[i][j] = mma16<DT>(lf[i], rf[j], acc[i][j]);
-        }
-        // the first reads, then one after every one or two products
-        constexpr int right = TURN ? 2 * MI : MI, reads = 2 * (2 * NI + right), lead = right + 4, rest = reads - lead;
-        constexpr int products = 2 * NI * MI, pairs = products - rest;
-        static_assert(pairs >= 0 && pairs <= rest, "one or two products to a read");
-        __builtin_amdgcn_sched_group_barrier(0x100, lead, 0);
-#pragma unroll
-        for (int i = 0; i < rest; i++) {
-            if (i < pairs)
-                __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+        for (int j = 0; j < MI; j++) {
+            if constexpr (TURN)
+                f.r[j] = Right::read(lr, ra, j);
             else
-                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                f.r[j] = *reinterpret_cast<const u32x4 *>(&lr[ra[0] + 16 * j * 32]);
+        }
+#pragma unroll
+        for (int i = 0; i < NI; i++) f.l[i] = Left::read(ll, la, i);
+    };
+    // Step s: its products, from the registers `now`; the next step's tile,
+    // which is here once all waves are, goes to `after` meanwhile; the buffer
+    // of this step's, which all waves have read, takes the tile 4 steps on.
+    // (Tiles past the last are that one again, until they are cleared: so as
+    // many copies are under way at every step, and the compiler, which counts
+    // them too, adds no waits of its own.)
+    auto step = [&](uint32_t s, uint16_t *own, const uint16_t *next, Fragments &now, Fragments &after) {
+        meet(std::integral_constant<int, 2>());
+        clear(const_cast<uint16_t *>(next), s + 1);
+        copy(own, min(s + 4, s1 - 1));
+        read(next, after);
+#pragma unroll
+        for (int i = 0; i < NI; i++)
+#pragma unroll
+            for (int j = 0; j < MI; j++) acc[i][j] = mma16<DT>(now.l[i], now.r[j], acc[i][j]);
+        // a read after every one or two products
+        constexpr int reads = 2 * NI + (TURN ? 2 * MI : MI), products = NI * MI, few = products / reads, more = products % reads;
+#pragma unroll
+        for (int i = 0; i < reads; i++) {
+            if (i < more)
+                __builtin_amdgcn_sched_group_barrier(0x8, few + 1, 0);
+            else
+                __builtin_amdgcn_sched_group_barrier(0x8, few, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
     };
-    if (s0 < s1) copy(ll0, lr0, s0);
-    for (uint32_t s = s0; s < s1; s += 2) {
-        __syncthreads();
-        clear(ll0, s);
-        if (s + 1 < s1) {
-            copy(ll1, lr1, s + 1);
-        } else {
-            // an odd number of steps ends with one of zeros
-            for (uint32_t i = threadIdx.x; i < TC * 8; i += T) reinterpret_cast<u32x4 *>(ll1)[i] = u32x4{0, 0, 0, 0};
-            for (uint32_t i = threadIdx.x; i < TR * 8; i += T) reinterpret_cast<u32x4 *>(lr1)[i] = u32x4{0, 0, 0, 0};
+    if (s0 < s1) {
+        Fragments a, b;
+        copy(t0, s0);
+        copy(t1, min(s0 + 1, s1 - 1));
+        copy(t2, min(s0 + 2, s1 - 1));
+        copy(t3, min(s0 + 3, s1 - 1));
+        meet(std::integral_constant<int, 3>());
+        clear(t0, s0);
+        read(t0, a);
+        for (uint32_t s = s0; s < s1; s += 4) {
+            step(s, t0, t1, a, b);
+            step(s + 1, t1, t2, b, a);
+            step(s + 2, t2, t3, a, b);
+            step(s + 3, t3, t0, b, a);
         }
-        multiply(ll0, lr0);
-        __syncthreads();
-        if (s + 1 < s1) clear(ll1, s + 1);
-        if (s + 2 < s1) copy(ll0, lr0, s + 2);
-        multiply(ll1, lr1);
     }
     // Sums go out by way of LDS, 16 rows x 64 columns of each wave at a time
-    constexpr int Q = 16;
-    f32x4 *own = reinterpret_cast<f32x4 *>(TC >= TR ? ll0 : lr0) + wave * 16 * Q;
-    static_assert(WC * WR * 16 * Q * 16 <= (TC >= TR ? TC : TR) * 128, "every wave's piece fits one buffer");
+    constexpr int Q = 16, PER = (TC + TR) * 64 / (16 * Q * 16);  // waves' pieces to a buffer
+    static_assert(2 * PER >= WC * WR, "every wave's piece fits two buffers");
+    f32x4 *own = reinterpret_cast<f32x4 *>(wave < PER ? t0 : t1) + wave % PER * 16 * Q;
 #pragma unroll
     for (int j = 0; j < MI; j++)
 #pragma unroll
@@ -385,7 +495,7 @@ __global__ __launch_bounds__(256) void gated_back_any_kernel(const BackArgs p) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = lane & 15u, g = lane >> 4;
     const Place at = place_of((p.rows + S - 1) / S, (p.cols + S - 1) / S);
     const uint32_t c0 = at.c * S, r0 = at.r * S, wc = (wave & 1u) * (S / 2), wr = (wave >> 1) * (S / 2);
-    const uint32_t each = steps_of(p.depth), all = TURN ? each : 2 * each;
+    const uint32_t each = (p.depth + 63) / 64, all = TURN ? each : 2 * each;
     const uint32_t s0 = blockIdx.y * p.steps, s1 = min(all, s0 + p.steps);
     f32x4 acc[F][F];
 #pragma unroll
@@ -521,7 +631,7 @@ BackPlan plan_back(uint32_t rows, uint32_t cols, uint32_t steps, int cus, const 
 
 template <int DT, bool TURN>
 int32_t launch_back(BackArgs p, const BackPlan &plan, bool aligned, float *room, hipStream_t s) {
-    p.steps = plan.steps;
+    p.steps = aligned ? 2 * plan.steps : plan.steps;
     p.partial = plan.splits > 1 ? room : nullptr;
     const dim3 grid((uint32_t)plan.tiles, plan.splits);
 #define HH_BACK(TC, TR, WC, WR) hipLaunchKernelGGL((gated_back_kernel<DT, TURN, TC, TR, WC, WR>), grid, dim3(64 * WC * WR), 0, s, p)
