@@ -239,11 +239,12 @@ __device__ __forceinline__ void store_back(const BackArgs &p, uint32_t split, ui
 // these take XXX), 16-byte pieces at places that depend on their row.  One
 // barrier a tile: before it a wave waits for its own part of the next tile's
 // copies, the oldest under way, and for its reads of the last one.
+__device__ __forceinline__ uint32_t shift_of(uint32_t row) { return (0u - (row >> 2)) & 3u; }
 template <int ROWS, int T>
 __device__ __forceinline__ void plain_offsets(uint32_t stride, uint32_t rows, uint32_t (&off)[ROWS * 4 / T]) {
 #pragma unroll
     for (int j = 0; j < ROWS * 4 / T; j++) {
-        const uint32_t slot = j * T + threadIdx.x, row = slot >> 2, piece = (slot & 3u) ^ (row >> 2 & 3u);
+        const uint32_t slot = j * T + threadIdx.x, row = slot >> 2, piece = (slot & 3u) ^ shift_of(row);
         off[j] = (min(row, rows - 1) * stride + piece * 8) * 2;
     }
 }
@@ -367,7 +368,7 @@ __global__ __launch_bounds__(64 * WC * WR) void gated_back_kernel(const BackArgs
     if constexpr (TURN)
         Right::places(lane, wr, ra);
     else
-        ra[0] = (wr + r) * 32 + (g ^ (r >> 2 & 3u)) * 8;
+        ra[0] = (wr + r) * 32 + (g ^ shift_of(r)) * 8;
     // (what is computed from this is computed where it is needed, and not kept
     // in registers through all steps)
     auto thread = []() {
