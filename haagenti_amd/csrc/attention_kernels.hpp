@@ -629,7 +629,13 @@ __global__ __launch_bounds__(64 * NW) void ATTENTION(tile_kernel)(const AttnArgs
     __shared__ __align__(16) _Float16 lk[2][64 * KP];
     __shared__ __align__(16) _Float16 lv[2][D * VP];
     __shared__ __align__(16) float lks[2][4], lvs[2][4];  // K's scales, logarithms of V's
-    const uint32_t r = blockIdx.x / p.tiles, tile = p.tiles - 1 - blockIdx.x % p.tiles, h = blockIdx.y;
+    // the last tiles of all requests and heads, which see most, first (by head
+    // and request first: two prompts' 496 workgroups 520 us, so 486; two
+    // maps' 384 266 us, so 236)
+    const uint32_t lanes = p.a.requests * p.cache.kv_heads;
+    const uint64_t id = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    const uint32_t lane_of = (uint32_t)(id % lanes), r = lane_of / p.cache.kv_heads, h = lane_of % p.cache.kv_heads;
+    const uint32_t tile = p.tiles - 1 - (uint32_t)(id / lanes);
     const Request rq = request_of(p, r);
     const uint32_t cols = columns_of(p, rq);
     if (cols <= p.small || tile * TILE >= cols) return;
