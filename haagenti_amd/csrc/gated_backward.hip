@@ -45,9 +45,9 @@ struct SlopeArgs {
     uint64_t dy_stride;
     uint32_t m, n, wide;  // wide: N
     uint32_t rows;        // m, or m rounded up to 64 where the rows past it are read
+    uint32_t block_rows;  // of a workgroup
     int act;
 };
-constexpr uint32_t kSlopeRows = 32;  // of a workgroup
 
 // act(z) and act'(z).
 __device__ __forceinline__ void act_and_slope(float z, int act, float &a, float &s) {
@@ -79,47 +79,60 @@ __device__ __forceinline__ void act_and_slope(float z, int act, float &a, float 
     }
 }
 
-// 4 columns a lane, 256 a wave, every 4th row of the block a wave.
-template <int DT>
+// 4 columns a lane, 256 a wave, every 4th row of the block a wave, R of them at
+// a time: all their loads are done, at places that are there (behind
+// conditions they wait for one another: 77 x 1003 14 us, so 4).  2048 x 14336:
+// 84 us, 411 MB at 4.9 TB/s.
+template <int DT, int R>
 __global__ __launch_bounds__(256) void gated_slope_kernel(const SlopeArgs p) {
     __shared__ __align__(16) float sums[2][4][256];
     const uint32_t across = (p.wide + 255) / 256, block = blockIdx.x / across, c0 = blockIdx.x % across * 256;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = c0 + lane * 4, r0 = block * kSlopeRows;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = c0 + lane * 4, r0 = block * p.block_rows;
+    const uint32_t end = min(r0 + p.block_rows, p.rows);
     f32x4 sg = {0, 0, 0, 0}, su = {0, 0, 0, 0};
     if (c < p.wide) {
-#pragma unroll 2
-        for (uint32_t r = r0 + wave; r < min(r0 + kSlopeRows, p.rows); r += 4) {
-            f32x4 dg = {0, 0, 0, 0}, du = {0, 0, 0, 0};
-            if (r < p.m && c < p.n) {
-                const uint16_t *dy = p.dy + r * p.dy_stride + c;
-                const float *s = p.saved + (uint64_t)r * 2 * p.n + c;
-                float d[4] = {0, 0, 0, 0}, g[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
-                if (c + 4 <= p.n) {
-                    const u32x2 v = *reinterpret_cast<const u32x2_any *>(dy);
-                    const f32x4 a = *reinterpret_cast<const f32x4_any *>(s), b = *reinterpret_cast<const f32x4_any *>(s + p.n);
+        for (uint32_t first = r0 + wave; first < end; first += 4 * R) {
+            f32x4 d[R], g[R], u[R];
+            if (c0 + 256 <= p.n) {
+#pragma unroll
+                for (int k = 0; k < R; k++) {
+                    const uint32_t r = min(first + 4 * k, p.m - 1);
+                    const float *s = p.saved + (uint64_t)r * 2 * p.n + c;
+                    const u32x2 v = *reinterpret_cast<const u32x2_any *>(p.dy + r * p.dy_stride + c);
+                    g[k] = *reinterpret_cast<const f32x4_any *>(s), u[k] = *reinterpret_cast<const f32x4_any *>(s + p.n);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) d[k][e] = half_to_f32<DT>((v[e >> 1] >> (16 * (e & 1))) & 0xffffu);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < R; k++) {
+                    const uint32_t r = min(first + 4 * k, p.m - 1);
+                    const float *s = p.saved + (uint64_t)r * 2 * p.n;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        d[e] = half_to_f32<DT>((v[e >> 1] >> (16 * (e & 1))) & 0xffffu);
-                        g[e] = a[e], u[e] = b[e];
+                        const uint32_t col = min(c + e, p.n - 1);
+                        d[k][e] = half_to_f32<DT>(p.dy[r * p.dy_stride + col]), g[k][e] = s[col], u[k][e] = s[p.n + col];
                     }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (c + e < p.n) d[e] = half_to_f32<DT>(dy[e]), g[e] = s[e], u[e] = s[p.n + e];
                 }
+            }
+#pragma unroll
+            for (int k = 0; k < R; k++) {
+                const uint32_t r = first + 4 * k;
+                if (r >= end) break;
+                f32x4 dg = {0, 0, 0, 0}, du = {0, 0, 0, 0};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     float a, slope;
-                    act_and_slope(g[e], p.act, a, slope);
-                    dg[e] = d[e] * u[e] * slope, du[e] = d[e] * a;
+                    act_and_slope(g[k][e], p.act, a, slope);
+                    if (r < p.m && c + e < p.n) dg[e] = d[k][e] * u[k][e] * slope, du[e] = d[k][e] * a;
                 }
                 sg += dg, su += du;
+                uint16_t *to = p.d + (uint64_t)r * 2 * p.wide + c;
+                *reinterpret_cast<u32x2 *>(to) = u32x2{f32_to_half<DT>(dg[0]) | f32_to_half<DT>(dg[1]) << 16,
+                                                       f32_to_half<DT>(dg[2]) | f32_to_half<DT>(dg[3]) << 16};
+                *reinterpret_cast<u32x2 *>(to + p.wide) = u32x2{f32_to_half<DT>(du[0]) | f32_to_half<DT>(du[1]) << 16,
+                                                                f32_to_half<DT>(du[2]) | f32_to_half<DT>(du[3]) << 16};
             }
-            uint16_t *to = p.d + (uint64_t)r * 2 * p.wide + c;
-            *reinterpret_cast<u32x2 *>(to) = u32x2{f32_to_half<DT>(dg[0]) | f32_to_half<DT>(dg[1]) << 16,
-                                                   f32_to_half<DT>(dg[2]) | f32_to_half<DT>(dg[3]) << 16};
-            *reinterpret_cast<u32x2 *>(to + p.wide) = u32x2{f32_to_half<DT>(du[0]) | f32_to_half<DT>(du[1]) << 16,
-                                                            f32_to_half<DT>(du[2]) | f32_to_half<DT>(du[3]) << 16};
         }
     }
     if (!p.part) return;
@@ -236,7 +249,7 @@ __device__ __forceinline__ void store_back(const BackArgs &p, uint32_t split, ui
 // Aligned operands, copied straight to LDS in tiles 32 deep, four of them in
 // turn: three are on their way while one is multiplied (64 deep and two in
 // turn, a copy has one tile's products to arrive in: 483 and 479 us where
-// these take XXX), 16-byte pieces at places that depend on their row.  One
+// these take 440 and 457), 16-byte pieces at places that depend on their row.  One
 // barrier a tile: before it a wave waits for its own part of the next tile's
 // copies, the oldest under way, and for its reads of the last one.
 __device__ __forceinline__ uint32_t shift_of(uint32_t row) { return (0u - (row >> 2)) & 3u; }
@@ -507,46 +520,62 @@ __global__ __launch_bounds__(256) void gated_back_any_kernel(const BackArgs p) {
     Turned<S>::places(lane, wc, la);
     if constexpr (TURN) Turned<S>::places(lane, wr, ra);
     u32x4 lv[P], rv[P];
-    auto fetch = [&](uint32_t s) {
+    // Every load is done, at a place that is there, so that all of a step's are
+    // under way at once; what is not this step's is put right on its way to LDS.
+    // (Loads behind conditions wait for one another: 2048 x 14331 x 4093 2240
+    // and 950 us with the slope, so 745 and 775.)  Columns and rows past C's hold
+    // anything: only sums that are not stored take from them.
+    auto fetch_all = [&](uint32_t s, auto less) __attribute__((always_inline)) {
+        constexpr bool few = decltype(less)::value;  // rows of less than 8 values
         const uint32_t part = !TURN && s >= each, t0 = (s - (part ? each : 0)) * 64;
 #pragma unroll
         for (int j = 0; j < P; j++) {
             const uint32_t slot = j * 256 + threadIdx.x, t = t0 + slot / (S / 8), c = c0 + slot % (S / 8) * 8;
-            lv[j] = u32x4{0, 0, 0, 0};
-            if (t < p.depth && c < p.cols) {
-                const uint16_t *from = p.l[part] + (uint64_t)t * p.l_stride[part] + c;
-                if (c + 8 <= p.cols) {
-                    lv[j] = *reinterpret_cast<const u32x4_any *>(from);
-                } else {
-#pragma unroll
-                    for (uint32_t e = 0; e < 8; e++)
-                        if (c + e < p.cols) lv[j][e >> 1] |= (uint32_t)from[e] << (16 * (e & 1));
-                }
-            }
-            rv[j] = u32x4{0, 0, 0, 0};
-            if constexpr (TURN) {  // (D has whole steps of rows, and N whole pieces of 64 columns)
-                const uint32_t d = r0 + slot % (S / 8) * 8;
-                if (d < p.rows) rv[j] = *reinterpret_cast<const u32x4 *>(p.d + (uint64_t)t * 2 * p.wide + d);
+            const uint16_t *from = p.l[part] + (uint64_t)min(t, p.depth - 1) * p.l_stride[part];
+            if constexpr (!few) {
+                lv[j] = *reinterpret_cast<const u32x4_any *>(from + min(c, p.cols - 8));
             } else {
-                const uint32_t row = r0 + (slot >> 3);
-                if (row < p.rows)
-                    rv[j] = *reinterpret_cast<const u32x4 *>(p.d + (uint64_t)row * 2 * p.wide + (part ? p.wide : 0) + t0 + (slot & 7u) * 8);
+                lv[j] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++)
+                    if (c + e < p.cols) lv[j][e >> 1] |= (uint32_t)from[e] << (16 * (e & 1));
+            }
+            if constexpr (TURN) {  // (D has whole steps of rows, and N whole pieces of 64 columns)
+                rv[j] = *reinterpret_cast<const u32x4 *>(p.d + (uint64_t)t * 2 * p.wide + r0 + slot % (S / 8) * 8);
+            } else {
+                const uint32_t row = min(r0 + (slot >> 3), p.rows - 1);
+                rv[j] = *reinterpret_cast<const u32x4 *>(p.d + (uint64_t)row * 2 * p.wide + (part ? p.wide : 0) + t0 + (slot & 7u) * 8);
             }
         }
     };
-    auto stage = [&]() {
+    auto fetch = [&](uint32_t s) __attribute__((always_inline)) {
+        if (p.cols < 8)
+            fetch_all(s, std::true_type());
+        else
+            fetch_all(s, std::false_type());
+    };
+    auto stage = [&](uint32_t s) {
+        const uint32_t t0 = (!TURN && s >= each ? s - each : s) * 64;
 #pragma unroll
         for (int j = 0; j < P; j++) {
             const uint32_t slot = j * 256 + threadIdx.x, t = slot / (S / 8), piece = slot % (S / 8), row = slot >> 3;
             const uint32_t turned = t * S + (piece ^ (2 * twist(t, S / 16))) * 8;
-            *reinterpret_cast<u32x4 *>(&ll[turned]) = lv[j];
+            u32x4 v = lv[j];
+            if (p.cols >= 8 && c0 + S > p.cols) {  // a row's last piece: read that much further left
+                const uint32_t c = c0 + piece * 8, over = c + 8 > p.cols ? c + 8 - p.cols : 0;
+                if (over & 4u) v = u32x4{v[2], v[3], 0, 0};
+                if (over & 2u) v = u32x4{v[1], v[2], v[3], 0};
+                if (over & 1u) v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+            }
+            if (t0 + t >= p.depth) v = u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4 *>(&ll[turned]) = v;
             *reinterpret_cast<u32x4 *>(&lr[TURN ? turned : row * 64 + ((slot & 7u) ^ (row & 7u)) * 8]) = rv[j];
         }
     };
     if (s0 < s1) fetch(s0);
     for (uint32_t s = s0; s < s1; s++) {
         __syncthreads();
-        stage();
+        stage(s);
         __syncthreads();
         if (s + 1 < s1) fetch(s + 1);
 #pragma unroll
@@ -671,8 +700,10 @@ int32_t gated_backward(hh_context *ctx, const hh_gated_args &a, const hh_gated_g
     if (dx) px = x_aligned ? plan_back(a.m, a.k, 2 * (wide / 64), cus, kBackShapes) : plan_back(a.m, a.k, 2 * (wide / 64), cus, kBackAnyShapes);
     if (dw) pw = w_aligned ? plan_back(2 * wide, a.k, rows / 64, cus, kBackShapes) : plan_back(2 * wide, a.k, rows / 64, cus, kBackAnyShapes);
     // a launch has fewer than 2^32 threads
-    const uint32_t blocks = (rows + kSlopeRows - 1) / kSlopeRows;
-    if ((uint64_t)blocks * ((wide + 255) / 256) >= 1u << 24 || px.tiles >= 1u << 23 || pw.tiles >= 1u << 23) return HH_ERR_UNSUPPORTED;
+    // 32 rows to a workgroup, or 4 where that leaves CUs idle
+    const uint32_t across = (wide + 255) / 256, block_rows = (uint64_t)(rows / 32) * across < 4 * (uint32_t)cus ? 4 : 32;
+    const uint32_t blocks = rows / block_rows;
+    if ((uint64_t)blocks * across >= 1u << 24 || px.tiles >= 1u << 23 || pw.tiles >= 1u << 23) return HH_ERR_UNSUPPORTED;
     // D, the biases' sums of row blocks, the larger of the products' sums
     const size_t d_bytes = (size_t)rows * 2 * wide * sizeof(uint16_t);
     const size_t b_bytes = bias ? ((size_t)blocks * 2 * a.n * sizeof(float) + 255) / 256 * 256 : 0;
@@ -686,7 +717,11 @@ int32_t gated_backward(hh_context *ctx, const hh_gated_args &a, const hh_gated_g
     sl.part = bias ? reinterpret_cast<float *>(at + d_bytes) : nullptr;
     sl.gate_bias = d.d_dgate_bias, sl.up_bias = d.d_dup_bias;
     sl.m = a.m, sl.n = a.n, sl.wide = wide, sl.rows = dw ? rows : a.m, sl.act = a.activation;
-    hipLaunchKernelGGL((gated_slope_kernel<DT>), dim3((wide + 255) / 256 * blocks), dim3(256), 0, s, sl);
+    sl.block_rows = block_rows;
+    if (block_rows == 4)
+        hipLaunchKernelGGL((gated_slope_kernel<DT, 1>), dim3(across * blocks), dim3(256), 0, s, sl);
+    else
+        hipLaunchKernelGGL((gated_slope_kernel<DT, 4>), dim3(across * blocks), dim3(256), 0, s, sl);
     int32_t e = from_hip(hipGetLastError());
     if (e == HH_OK && bias) {
         hipLaunchKernelGGL(gated_bias_kernel, dim3((a.n + 31) / 32, 2), dim3(1024), 0, s, sl, blocks);

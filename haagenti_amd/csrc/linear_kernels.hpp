@@ -24,6 +24,8 @@
 // A file that includes this says which it makes: HH_GATED 0 or 1.
 #pragma once
 
+#include <type_traits>
+
 #include "layer_ops.hpp"
 
 #if HH_GATED
@@ -97,6 +99,19 @@ __device__ __forceinline__ u32x4 row8(const uint16_t *row, uint32_t at, uint32_t
     for (uint32_t e = 0; e < 8; e++)
         if (at + e < k) v[e >> 1] |= (uint32_t)row[at + e] << (16 * (e & 1));
     return v;
+}
+
+// The same in two parts, for a row of 8 values or more: a load without a
+// condition (of the row's last 8 past their start), and what puts it right.
+__device__ __forceinline__ u32x4 load8(const uint16_t *row, uint32_t at, uint32_t k) {
+    return *reinterpret_cast<const u32x4_any *>(row + min(at, k - 8));
+}
+__device__ __forceinline__ u32x4 last8(u32x4 v, uint32_t at, uint32_t k) {
+    const uint32_t over = at + 8 > k ? at + 8 - k : 0;
+    if (over & 4u) v = u32x4{v[2], v[3], 0, 0};
+    if (over & 2u) v = u32x4{v[1], v[2], v[3], 0};
+    if (over & 1u) v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+    return over < 8 ? v : u32x4{0, 0, 0, 0};
 }
 
 // __expf is the hardware's power of two of x log2(e): off by 2^-23 of itself
@@ -500,24 +515,37 @@ __global__ __launch_bounds__(256) void PRODUCT(tile_kernel)(const Args p, const 
 
     u32x4 wv[P][WP], xv[P][XP];
     uint32_t sv = 0;
-    auto fetch = [&](uint32_t k0) {
+    auto fetch_all = [&](uint32_t k0, auto less) __attribute__((always_inline)) {
+        constexpr bool few = decltype(less)::value;  // rows of less than 8 values
 #pragma unroll
         for (uint32_t j = 0; j < P; j++) {
             const uint32_t row = (j * 256 + tid) >> 3, k = k0 + (tid & 7u) * 8;
             const uint32_t n = n0 + row_of(row), m = m0 + row, side = side_of(row);
-#pragma unroll
-            for (int q = 0; q < WP; q++) wv[j][q] = u32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int q = 0; q < XP; q++) xv[j][q] = u32x4{0, 0, 0, 0};
-            if (m < a.m) xv[j][0] = row8(reinterpret_cast<const uint16_t *>(a.d_x) + (uint64_t)m * a.x_stride, k, k1);
-            if (n < a.n) {
-                if constexpr (MODE == kHalf) {
-                    wv[j][0] = row8(weight_of(p, side) + (uint64_t)n * stride_of(p, side), k, k1);
-                } else if constexpr (MODE == kInt4) {
+            if constexpr (MODE != kInt4Any) {
+                // every load is done, at a place that is there: behind conditions
+                // they would wait for one another.  Rows past the ends hold
+                // anything (their sums are not stored), columns are put right below.
+                const uint16_t *from = reinterpret_cast<const uint16_t *>(a.d_x) + (uint64_t)min(m, a.m - 1) * a.x_stride;
+                const uint64_t wr = min(n, a.n - 1);
+                if constexpr (MODE == kInt4) {
                     typedef uint32_t u32_any __attribute__((aligned(1)));
-                    if (k < k1)
-                        wv[j][0][0] = *reinterpret_cast<const u32_any *>(nibbles_of(p, side) + ((uint64_t)n * a.k + k) / 2);
+                    xv[j][0] = load8(from, k, a.k);
+                    wv[j][0][0] = *reinterpret_cast<const u32_any *>(nibbles_of(p, side) + (wr * a.k + min(k, a.k - 8)) / 2);
                 } else {
+                    const uint16_t *wf = weight_of(p, side) + wr * stride_of(p, side);
+                    if (few) {
+                        xv[j][0] = row8(from, k, a.k), wv[j][0] = row8(wf, k, a.k);
+                    } else {
+                        xv[j][0] = load8(from, k, a.k), wv[j][0] = load8(wf, k, a.k);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < WP; q++) wv[j][q] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int q = 0; q < XP; q++) xv[j][q] = u32x4{0, 0, 0, 0};
+                if (m < a.m) xv[j][0] = row8(reinterpret_cast<const uint16_t *>(a.d_x) + (uint64_t)m * a.x_stride, k, k1);
+                if (n < a.n) {
                     // 8 nibbles: 4 bytes, or 5 from the middle of one; at most two groups
                     const uint8_t *nibbles = nibbles_of(p, side);
                     const uint16_t *scales = scales_of(p, side);
@@ -543,14 +571,24 @@ __global__ __launch_bounds__(256) void PRODUCT(tile_kernel)(const Args p, const 
         if constexpr (MODE == kInt4) {
             const uint32_t row = tid % S, k = k0 + tid / S * 32;  // 2 S scales
             const uint32_t n = n0 + row_of(row);
-            if (tid < 2 * S) sv = n < a.n && k < k1 ? scales_of(p, side_of(row))[((uint64_t)n * a.k + k) / 32] : 0u;
+            if (tid < 2 * S) sv = scales_of(p, side_of(row))[((uint64_t)min(n, a.n - 1) * a.k + min(k, a.k - 32)) / 32];
         }
     };
+    auto fetch = [&](uint32_t k0) __attribute__((always_inline)) {
+        if (MODE == kHalf && a.k < 8)
+            fetch_all(k0, std::true_type());
+        else
+            fetch_all(k0, std::false_type());
+    };
     // what is done to the values on their way to LDS waits until they are here
-    auto stage = [&]() {
+    auto stage = [&](uint32_t k0) {
 #pragma unroll
         for (uint32_t j = 0; j < P; j++) {
-            const uint32_t at = ((j * 256 + tid) >> 3) * PITCH + (tid & 7u) * 8;
+            const uint32_t at = ((j * 256 + tid) >> 3) * PITCH + (tid & 7u) * 8, k = k0 + (tid & 7u) * 8;
+            if (MODE != kInt4Any && k0 + 64 > a.k && a.k >= 8) {
+                xv[j][0] = last8(xv[j][0], k, a.k);
+                if (MODE == kHalf) wv[j][0] = last8(wv[j][0], k, a.k);
+            }
             if constexpr (MODE == kInt4) {
                 *reinterpret_cast<u32x4 *>(&lw[0][at]) = nibbles_0415<DT>(wv[j][0][0]);
                 *reinterpret_cast<u32x4 *>(&lx[0][at]) = order_0415(xv[j][0]);
@@ -568,13 +606,13 @@ __global__ __launch_bounds__(256) void PRODUCT(tile_kernel)(const Args p, const 
                 for (int q = 0; q < XP; q++) *reinterpret_cast<u32x4 *>(&lx[q][at]) = xv[j][q];
             }
         }
-        if (MODE == kInt4 && tid < 2 * S) ls[tid / S][tid % S] = f16_bits_to_f32(sv);
+        if (MODE == kInt4 && tid < 2 * S) ls[tid / S][tid % S] = k0 + tid / S * 32 < a.k ? f16_bits_to_f32(sv) : 0.0f;
     };
 
     if (kb < k1) fetch(kb);
     for (uint32_t k0 = kb; k0 < k1; k0 += 64) {
         __syncthreads();
-        stage();
+        stage(k0);
         __syncthreads();
         if (k0 + 64 < k1) fetch(k0 + 64);
 #pragma unroll
