@@ -54,11 +54,31 @@ __device__ __forceinline__ u32x4 packed(const float (&v)[Elem<XT>::V]) {
     }
     return r;
 }
-// 16 bytes of a row at value `at`, of which `left` are the row's (zeros past them).
+// 16 bytes of a row of n at value `at`, of which `left` are the row's.  In two
+// parts: a load without a condition, of the row's last 16 bytes past their
+// start, so that many are under way at once (with the ends loaded a value at a
+// time 8192 rows of 4093 bfloat16 took 39 us and their gradients 87, so 32 and
+// 65); and, once it is here, its values moved to their places, zeros past them.
 template <int XT>
-__device__ __forceinline__ u32x4 load16(const void *row, uint32_t at, int32_t left) {
+__device__ __forceinline__ u32x4 load16(const void *row, uint32_t at, uint32_t n) {
+    const uint8_t *p = reinterpret_cast<const uint8_t *>(row) + (uint64_t)min(at, n - Elem<XT>::V) * Elem<XT>::S;
+    return *reinterpret_cast<const u32x4_at2 *>(p);
+}
+template <int XT>
+__device__ __forceinline__ u32x4 ended(u32x4 r, int32_t left) {
+    constexpr int V = Elem<XT>::V;
+    if (left >= V) return r;
+    if (left <= 0) return u32x4{0, 0, 0, 0};
+    const uint32_t halves = (V - left) * (8 / V);
+    if (halves & 4u) r = u32x4{r[2], r[3], 0, 0};
+    if (halves & 2u) r = u32x4{r[1], r[2], r[3], 0};
+    if (halves & 1u) r = u32x4{r[0] >> 16 | r[1] << 16, r[1] >> 16 | r[2] << 16, r[2] >> 16 | r[3] << 16, r[3] >> 16};
+    return r;
+}
+// A row of less than 16 bytes.
+template <int XT>
+__device__ __forceinline__ u32x4 load_few(const void *row, uint32_t at, int32_t left) {
     const uint8_t *p = reinterpret_cast<const uint8_t *>(row) + (uint64_t)at * Elem<XT>::S;
-    if (left >= Elem<XT>::V) return *reinterpret_cast<const u32x4_at2 *>(p);
     u32x4 r = {0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < Elem<XT>::V; e++)
@@ -69,6 +89,10 @@ __device__ __forceinline__ u32x4 load16(const void *row, uint32_t at, int32_t le
                 r[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[e] << (16 * (e & 1));
         }
     return r;
+}
+template <int XT>
+__device__ __forceinline__ u32x4 row16(const void *row, uint32_t at, int32_t left, uint32_t n) {
+    return n < Elem<XT>::V ? load_few<XT>(row, at, left) : ended<XT>(load16<XT>(row, at, n), left);
 }
 template <int XT>
 __device__ __forceinline__ void store16(void *row, uint32_t at, int32_t left, const u32x4 &r) {
@@ -89,19 +113,20 @@ __device__ __forceinline__ void store16(void *row, uint32_t at, int32_t left, co
 // V parameters (weight or bias) from column `at` on, `none` where there are
 // none and past the row.
 template <int XT>
-__device__ __forceinline__ void params(const void *p, int w32, uint32_t at, int32_t left, float none, float (&v)[Elem<XT>::V]) {
+__device__ __forceinline__ void params(const void *p, int w32, uint32_t at, int32_t left, uint32_t n, float none,
+                                       float (&v)[Elem<XT>::V]) {
     constexpr int V = Elem<XT>::V;
 #pragma unroll
     for (int e = 0; e < V; e++) v[e] = none;
     if (!p) return;
     if (XT != HH_F32 && !w32) {
-        const u32x4 r = load16<XT>(p, at, left);
+        const u32x4 r = row16<XT>(p, at, left, n);
 #pragma unroll
         for (int e = 0; e < V; e++) v[e] = e < left ? value<XT>(r, e) : none;
     } else {
 #pragma unroll
         for (int i = 0; i < V / 4; i++) {
-            const u32x4 r = load16<HH_F32>(p, at + 4 * i, left - 4 * i);
+            const u32x4 r = row16<HH_F32>(p, at + 4 * i, left - 4 * i, n);
 #pragma unroll
             for (int e = 0; e < 4; e++) v[4 * i + e] = 4 * i + e < left ? __uint_as_float(r[e]) : none;
         }
@@ -169,18 +194,23 @@ __global__ __launch_bounds__(64 * W * G) void norm_kernel(const NormArgs p) {
     const uint32_t t = threadIdx.x % T, group = threadIdx.x / T, step = gridDim.x * G;
     const hh_norm_args &a = p.a;
     const float inv = 1.0f / (float)a.n;
+    const bool few = C == 1 && W == 1 && a.n < V;
     int32_t left[C];
     float w[C][V], b[C][V];
 #pragma unroll
     for (int c = 0; c < C; c++) {
         left[c] = (int32_t)a.n - (int32_t)((c * T + t) * V);
-        params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], 1.0f, w[c]);
-        params<XT>(a.d_bias, p.w32, (c * T + t) * V, left[c], 0.0f, b[c]);
+        params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], a.n, 1.0f, w[c]);
+        params<XT>(a.d_bias, p.w32, (c * T + t) * V, left[c], a.n, 0.0f, b[c]);
     }
     auto fetch = [&](uint32_t row, u32x4 (&x)[C]) {
         const uint8_t *at = reinterpret_cast<const uint8_t *>(a.d_x) + (uint64_t)min(row, a.rows - 1) * a.x_stride * Elem<XT>::S;
+        if (few) {
+            x[0] = load_few<XT>(at, t * V, left[0]);
+            return;
+        }
 #pragma unroll
-        for (int c = 0; c < C; c++) x[c] = load16<XT>(at, (c * T + t) * V, left[c]);
+        for (int c = 0; c < C; c++) x[c] = load16<XT>(at, (c * T + t) * V, a.n);
     };
     u32x4 x[C], next[C];
     int turn = 0;
@@ -188,6 +218,9 @@ __global__ __launch_bounds__(64 * W * G) void norm_kernel(const NormArgs p) {
     for (uint32_t base = blockIdx.x * G; base < a.rows; base += step) {
         const uint32_t row = base + group;
         if (base + step < a.rows) fetch(row + step, next);
+        if (!few)
+#pragma unroll
+            for (int c = 0; c < C; c++) x[c] = ended<XT>(x[c], left[c]);
         float d[C][V], s[1] = {0.0f};
         off_mean<XT, W, G, C>(p, x, left, inv, lds, turn, d);
 #pragma unroll
@@ -221,12 +254,13 @@ __global__ __launch_bounds__(64 * W * G) void norm_backward_kernel(const NormArg
     const uint32_t t = threadIdx.x % T, group = threadIdx.x / T, step = gridDim.x * G;
     const hh_norm_args &a = p.a;
     const float inv = 1.0f / (float)a.n;
+    const bool few = C == 1 && W == 1 && a.n < V;
     int32_t left[C];
     float sw[C][V], sb[C][V], held[AHEAD ? C : 1][V];
 #pragma unroll
     for (int c = 0; c < C; c++) {
         left[c] = (int32_t)a.n - (int32_t)((c * T + t) * V);
-        if (AHEAD) params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], 1.0f, held[AHEAD ? c : 0]);
+        if (AHEAD) params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], a.n, 1.0f, held[AHEAD ? c : 0]);
 #pragma unroll
         for (int e = 0; e < V; e++) sw[c][e] = 0.0f, sb[c][e] = 0.0f;
     }
@@ -238,20 +272,25 @@ __global__ __launch_bounds__(64 * W * G) void norm_backward_kernel(const NormArg
         const uint8_t *xr = reinterpret_cast<const uint8_t *>(a.d_x) + i * a.x_stride * Elem<XT>::S;
         const uint8_t *dr = reinterpret_cast<const uint8_t *>(p.dy) + i * p.dy_stride * Elem<XT>::S;
         const uint8_t *ar = reinterpret_cast<const uint8_t *>(p.add) + i * p.add_stride * Elem<XT>::S;
+        if (few) {
+            r.x[0] = load_few<XT>(xr, t * V, left[0]), r.dy[0] = load_few<XT>(dr, t * V, left[0]);
+            if (p.add) r.add[0] = load_few<XT>(ar, t * V, left[0]);
+            return;
+        }
 #pragma unroll
-        for (int c = 0; c < C; c++) r.x[c] = load16<XT>(xr, (c * T + t) * V, left[c]);
+        for (int c = 0; c < C; c++) r.x[c] = load16<XT>(xr, (c * T + t) * V, a.n);
 #pragma unroll
-        for (int c = 0; c < C; c++) r.dy[c] = load16<XT>(dr, (c * T + t) * V, left[c]);
+        for (int c = 0; c < C; c++) r.dy[c] = load16<XT>(dr, (c * T + t) * V, a.n);
         if (p.add)
 #pragma unroll
-            for (int c = 0; c < C; c++) r.add[c] = load16<XT>(ar, (c * T + t) * V, left[c]);
+            for (int c = 0; c < C; c++) r.add[c] = load16<XT>(ar, (c * T + t) * V, a.n);
     };
     auto weights = [&](int c, float (&w)[V]) {
         if constexpr (AHEAD) {
 #pragma unroll
             for (int e = 0; e < V; e++) w[e] = held[c][e];
         } else {
-            params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], 1.0f, w);
+            params<XT>(a.d_weight, p.w32, (c * T + t) * V, left[c], a.n, 1.0f, w);
         }
     };
     int turn = 0;
@@ -263,6 +302,12 @@ __global__ __launch_bounds__(64 * W * G) void norm_backward_kernel(const NormArg
             fetch(row, now);
         else if (base + step < a.rows)
             fetch(row + step, next);
+        if (!few)
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                now.x[c] = ended<XT>(now.x[c], left[c]), now.dy[c] = ended<XT>(now.dy[c], left[c]);
+                if (p.add) now.add[c] = ended<XT>(now.add[c], left[c]);
+            }
         float d[C][V], dy[C][V];
         off_mean<XT, W, G, C>(p, now.x, left, inv, lds, turn, d);
         float s[3] = {0.0f, 0.0f, 0.0f};  // of (x - mean)^2, g, g (x - mean)
@@ -357,7 +402,8 @@ __global__ __launch_bounds__(256) void norm_zero_kernel(const NormArgs p) {
 // Waves to a row, rows to a workgroup at a time, pieces to a lane, workgroups
 // to a CU.  Few pieces to a lane, so that the next row is on its way while one
 // is worked on: layer norm of 8192 x 4096 bf16 takes 25 us with 4 waves of 2
-// pieces (30 with 2 of 4, 38 with one of 8), its gradients 70 (96, 127).
+// pieces (30 with 2 of 4, 38 with one of 8), its gradients 70 (96,
+// 127; 64 since).
 struct NormPlan {
     int w, g, c;
     uint32_t grid;
