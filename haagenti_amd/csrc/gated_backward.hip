@@ -525,14 +525,13 @@ __global__ __launch_bounds__(256) void gated_back_any_kernel(const BackArgs p) {
     // (Loads behind conditions wait for one another: 2048 x 14331 x 4093 2240
     // and 950 us with the slope, so 745 and 775.)  Columns and rows past C's hold
     // anything: only sums that are not stored take from them.
-    auto fetch_all = [&](uint32_t s, auto less) __attribute__((always_inline)) {
-        constexpr bool few = decltype(less)::value;  // rows of less than 8 values
+    auto fetch = [&](uint32_t s) {
         const uint32_t part = !TURN && s >= each, t0 = (s - (part ? each : 0)) * 64;
 #pragma unroll
         for (int j = 0; j < P; j++) {
             const uint32_t slot = j * 256 + threadIdx.x, t = t0 + slot / (S / 8), c = c0 + slot % (S / 8) * 8;
             const uint16_t *from = p.l[part] + (uint64_t)min(t, p.depth - 1) * p.l_stride[part];
-            if constexpr (!few) {
+            if (p.cols >= 8) {
                 lv[j] = *reinterpret_cast<const u32x4_any *>(from + min(c, p.cols - 8));
             } else {
                 lv[j] = u32x4{0, 0, 0, 0};
@@ -547,12 +546,6 @@ __global__ __launch_bounds__(256) void gated_back_any_kernel(const BackArgs p) {
                 rv[j] = *reinterpret_cast<const u32x4 *>(p.d + (uint64_t)row * 2 * p.wide + (part ? p.wide : 0) + t0 + (slot & 7u) * 8);
             }
         }
-    };
-    auto fetch = [&](uint32_t s) __attribute__((always_inline)) {
-        if (p.cols < 8)
-            fetch_all(s, std::true_type());
-        else
-            fetch_all(s, std::false_type());
     };
     auto stage = [&](uint32_t s) {
         const uint32_t t0 = (!TURN && s >= each ? s - each : s) * 64;

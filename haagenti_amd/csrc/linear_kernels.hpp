@@ -220,12 +220,17 @@ __device__ __forceinline__ void finish_gated(const GatedArgs &p, uint32_t m, uin
                 u32x2{f32_to_half<YT>(v[0]) | f32_to_half<YT>(v[1]) << 16, f32_to_half<YT>(v[2]) | f32_to_half<YT>(v[3]) << 16};
         return;
     }
+    // the biases all at once (those past the row's end are not used)
+    if (bg)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) gate[i] += half_to_f32<DT>(bg[min(n + i, a.n - 1)]);
+    if (bu)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) up[i] += half_to_f32<DT>(bu[min(n + i, a.n - 1)]);
 #pragma unroll 1
     for (uint32_t i = 0; i < 4 && n + i < a.n; i++) {
         float z = i == 0 ? gate[0] : i == 1 ? gate[1] : i == 2 ? gate[2] : gate[3];
-        float u = i == 0 ? up[0] : i == 1 ? up[1] : i == 2 ? up[2] : up[3];
-        if (bg) z += half_to_f32<DT>(bg[n + i]);
-        if (bu) u += half_to_f32<DT>(bu[n + i]);
+        const float u = i == 0 ? up[0] : i == 1 ? up[1] : i == 2 ? up[2] : up[3];
         if (p.saved) {
             float *s = p.saved + (uint64_t)m * 2 * a.n + n + i;
             s[0] = z, s[a.n] = u;
