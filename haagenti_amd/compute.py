@@ -1,8 +1,9 @@
 """A decoder layer's operators on decoded weights: matrix products with their
-epilogue, over 16-bit weights or INT4 buffers (hh_linear), the norms between
-them and rotary positions with their gradients (hh_norm, hh_rotary), and a
-paged 8-bit key / value cache with its plan, append, read and attention
-(hh_kv_*).
+epilogue, over 16-bit weights or INT4 buffers (hh_linear), the gated
+feed-forward's two in one launch (hh_gated_linear), the norms between them and
+rotary positions (hh_norm, hh_rotary), all three with their gradients, and a
+paged 8-bit key / value cache with its plan, append, read, attention and
+differential attention (hh_kv_*).
 
 Tensors are torch tensors on the context's device.  Calls run on torch's
 current stream, where their results are allocated, and don't synchronise.
@@ -10,8 +11,8 @@ Calls on several streams need no order but their tensors' own; captured calls
 keep what they use of the context's memory for as long as the context lives, whatever is called later (graphs
 captured on one stream must not run beside each other).
 What a call can't take raises HaagentiError before anything is launched;
-gradients are calls of their own (norm_backward, rotary's inverse) that
-autograd doesn't know, so tensors that require them are taken under
+gradients are calls of their own (norm_backward, gated_linear_backward,
+rotary's inverse) that autograd doesn't know, so tensors that require them are taken under
 torch.no_grad() only."""
 import ctypes as C
 import struct

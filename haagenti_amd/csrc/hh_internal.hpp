@@ -21,10 +21,11 @@ struct hh_context {
     // (grown on demand, kept until the context is destroyed).
     void *d_scratch = nullptr;
     size_t scratch_bytes = 0;
-    // Partial sums of hh_linear and hh_kv_attention: memory per stream, so
-    // that calls on several streams don't share it, and apart for calls that
-    // are captured, whose graphs go on using it; what such calls have grown
-    // out of is kept for their graphs (op_room, capi.hip).
+    // What the decoder-layer operators keep between a call's launches (partial
+    // sums, the gated gradients' slopes): memory per stream, so that calls on
+    // several streams don't share it, and apart for calls that are captured,
+    // whose graphs go on using it; what such calls have grown out of is kept
+    // for their graphs (op_room, capi.hip).
     struct Room {
         hipStream_t stream = nullptr;
         bool captured = false;

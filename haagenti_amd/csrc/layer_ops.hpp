@@ -1,5 +1,6 @@
-// What the decoder-layer operators (linear.hip, gated.hip, norm.hip,
-// rotary.hip, kv_cache.hip, kv_attention.hip) share.
+// What the decoder-layer operators (linear.hip, gated.hip, gated_backward.hip,
+// norm.hip, rotary.hip, kv_cache.hip, kv_attention.hip, diff_attention.hip)
+// share.
 #pragma once
 
 #include "hh_internal.hpp"

@@ -11,7 +11,9 @@
 // and its variance is summed about its mean, in f32.  The backward pass
 // recomputes both from x, which it reads anyway: two sums over registers cost
 // less than statistics kept, passed and checked.  W = 1 needs no LDS and no
-// barrier; more waves take rows too long for one wave, and few rows.
+// barrier; more waves take rows too long for one wave, and few rows.  8192 rows
+// of 4096 bf16: 24 us, 134 MB at 5.6 TB/s; gradients with add 58 us, 268 MB at
+// 4.7 TB/s, and 6 us to join the workgroups' sums; 8 rows 3.9 us.
 #include "layer_ops.hpp"
 
 namespace hh {
@@ -402,8 +404,8 @@ __global__ __launch_bounds__(256) void norm_zero_kernel(const NormArgs p) {
 // Waves to a row, rows to a workgroup at a time, pieces to a lane, workgroups
 // to a CU.  Few pieces to a lane, so that the next row is on its way while one
 // is worked on: layer norm of 8192 x 4096 bf16 takes 25 us with 4 waves of 2
-// pieces (30 with 2 of 4, 38 with one of 8), its gradients 70 (96,
-// 127; 64 since).
+// pieces (30 with 2 of 4, 38 with one of 8), its gradients 70 (96, 127; 64
+// since).
 struct NormPlan {
     int w, g, c;
     uint32_t grid;
