@@ -7,8 +7,8 @@
 // once, up's output not written and read between, and one launch less.  bf16,
 // 14336 x 4096: a token 41 us (235 MB of weights at 5.7 TB/s); 16 tokens of
 // INT4 33 us (66 MB at 2 TB/s: loads of 64 bytes a row, and their scales); 2048
-// tokens with what is kept 490 to 510 us (960 TFLOP/s; the library's bare
-// product 415), bound by LDS beside the matrix pipes.
+// tokens with what is kept 405 and 99 us in two launches (950 TFLOP/s; the
+// library's bare product 415), bound by LDS beside the matrix pipes.
 #define HH_GATED 1
 #include "linear_kernels.hpp"
 
@@ -35,8 +35,32 @@ TilePlan plan_gated(const hh_linear_args &a, int cus, const Shape (&shapes)[N]) 
     both.n = (a.n + 15) / 16 * 32;
     return plan_tiles(both, cus, shapes);
 }
+// Where a last round of tiles leaves CUs idle, whole rounds and then a launch
+// of smaller tiles for the other columns, if that is expected to be faster: the
+// first launch's columns (all of them: n) and the second's shape.  2048 x 14336
+// x 4096: 896 tiles of 256 x 256 on 256 CUs 561 us, 768 and 256 of 256 x 128
+// 542; 3000 x 5504 x 2048 174, so 148.
+uint32_t whole_rounds(const hh_linear_args &a, int cus, const TilePlan &plan, int *rest_shape) {
+    if (plan.splits > 1) return a.n;
+    const Shape &s = kLargeShapes[plan.shape];
+    const uint64_t mt = (a.m + s.m - 1) / s.m, slots = (uint64_t)cus * s.per_cu;
+    const uint64_t nt = ((uint64_t)a.n * 2 + s.n - 1) / s.n, first = nt * mt / slots * slots / mt;  // tiles of columns
+    if (!first || first >= nt) return a.n;
+    auto time = [&](const Shape &t, uint64_t cols) {
+        const uint64_t tiles = (2 * cols + t.n - 1) / t.n * ((a.m + t.m - 1) / t.m), all = (uint64_t)cus * t.per_cu;
+        return (double)((tiles + all - 1) / all) * ((tiles <= (uint64_t)cus ? t.alone : t.us) * plan.steps + 4.0);
+    };
+    const uint32_t cols = (uint32_t)(first * s.n / 2);
+    double least = time(s, a.n) - time(s, cols) - 4.0;  // (a launch)
+    uint32_t whole = a.n;
+    for (int i = 0; i < (int)(sizeof(kLargeShapes) / sizeof(Shape)); i++) {
+        const double rest = time(kLargeShapes[i], a.n - cols);
+        if (rest < least) least = rest, whole = cols, *rest_shape = i;
+    }
+    return whole;
+}
 int32_t gated_room(hh_context *ctx, const GatedArgs &p, const TilePlan &plan, hipStream_t s, Split *split) {
-    *split = {plan.steps, nullptr};
+    *split = {plan.steps, nullptr, 0};
     if (plan.splits == 1) return HH_OK;
     return op_room(ctx, s, (size_t)plan.splits * p.a.m * partial_row(p.a.n) * sizeof(float), &split->partial);
 }
@@ -64,8 +88,8 @@ int32_t launch_gated_any(hh_context *ctx, const GatedArgs &p, int cus, hipStream
     return join_gated<DT, YT>(p, plan, split, s);
 }
 template <int DT, int YT, int TN, int TM, int WN, int WM>
-void launch_gated_tiles(const GatedArgs &p, const Split &split, uint32_t splits, hipStream_t s) {
-    const uint32_t tiles = ((p.a.n + TN / 2 - 1) / (TN / 2)) * ((p.a.m + TM - 1) / TM);
+void launch_gated_tiles(const GatedArgs &p, const Split &split, uint32_t cols, uint32_t splits, hipStream_t s) {
+    const uint32_t tiles = ((cols + TN / 2 - 1) / (TN / 2)) * ((p.a.m + TM - 1) / TM);
     hipLaunchKernelGGL((gated_large_kernel<DT, YT, TN, TM, WN, WM>), dim3(tiles, splits), dim3(64 * WN * WM), 0, s, p,
                        split);
 }
@@ -94,12 +118,23 @@ int32_t launch_gated(hh_context *ctx, const GatedArgs &p, hipStream_t s) {
     Split split;
     const int32_t rc = gated_room(ctx, p, plan, s, &split);
     if (rc != HH_OK) return rc;
-    switch (plan.shape) {
-        case 0: launch_gated_tiles<DT, YT, 256, 256, 2, 4>(p, split, plan.splits, s); break;
-        case 1: launch_gated_tiles<DT, YT, 256, 128, 4, 2>(p, split, plan.splits, s); break;
-        case 2: launch_gated_tiles<DT, YT, 128, 256, 2, 4>(p, split, plan.splits, s); break;
-        case 3: launch_gated_tiles<DT, YT, 128, 128, 2, 2>(p, split, plan.splits, s); break;
-        default: launch_gated_tiles<DT, YT, 128, 64, 2, 2>(p, split, plan.splits, s); break;
+    int rest_shape = 0;
+    const uint32_t whole = whole_rounds(a, cus, plan, &rest_shape);
+    auto launch = [&](int shape, uint32_t cols) {
+        switch (shape) {
+            case 0: launch_gated_tiles<DT, YT, 256, 256, 2, 4>(p, split, cols, plan.splits, s); break;
+            case 1: launch_gated_tiles<DT, YT, 256, 128, 4, 2>(p, split, cols, plan.splits, s); break;
+            case 2: launch_gated_tiles<DT, YT, 128, 256, 2, 4>(p, split, cols, plan.splits, s); break;
+            case 3: launch_gated_tiles<DT, YT, 128, 128, 2, 2>(p, split, cols, plan.splits, s); break;
+            default: launch_gated_tiles<DT, YT, 128, 64, 2, 2>(p, split, cols, plan.splits, s); break;
+        }
+    };
+    launch(plan.shape, whole);
+    if (whole < a.n) {
+        const int32_t e = from_hip(hipGetLastError());
+        if (e != HH_OK) return e;
+        split.first = whole;
+        launch(rest_shape, a.n - whole);
     }
     return join_gated<DT, YT>(p, plan, split, s);
 }

@@ -30,7 +30,7 @@ void launch_tiles(const LinearArgs &p, const Split &split, uint32_t splits, hipS
 
 // Room for the splits' sums.
 int32_t split_room(hh_context *ctx, const LinearArgs &p, const TilePlan &plan, hipStream_t s, Split *split) {
-    *split = {plan.steps, nullptr};
+    *split = {plan.steps, nullptr, 0};
     if (plan.splits == 1) return HH_OK;
     return op_room(ctx, s, (size_t)plan.splits * p.a.m * ((p.a.n + 3) / 4 * 4) * sizeof(float), &split->partial);
 }

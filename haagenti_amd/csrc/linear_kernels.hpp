@@ -475,6 +475,7 @@ __global__ __launch_bounds__(64 * KW) void PRODUCT(rows_kernel)(const Args p) {
 struct Split {
     uint32_t steps;
     float *partial;  // [split][m][n rounded up to 4 (gated: twice that)], or null: one split, y itself
+    uint32_t first;  // gated, aligned tiles: the first output column of the launch
 };
 
 // A split's sums of outputs n .. n + 3 of row m.  Rows of the sums are whole
@@ -722,7 +723,7 @@ __global__ __launch_bounds__(64 * WN * WM) void PRODUCT(large_kernel)(const Args
     const uint32_t r = lane & 15u, g = lane >> 4;
     const uint32_t mt = (a.m + TM - 1) / TM, share = gridDim.x / 8, rest = gridDim.x % 8, xcd = blockIdx.x % 8;
     const uint32_t id = xcd * share + min(xcd, rest) + blockIdx.x / 8;
-    const uint32_t n0 = id / mt * (kGated ? TN / 2 : TN), m0 = id % mt * TM, wn = wave % WN * (TN / WN), wm = wave / WN * (TM / WM);
+    const uint32_t n0 = id / mt * (kGated ? TN / 2 : TN) + (kGated ? split.first : 0), m0 = id % mt * TM, wn = wave % WN * (TN / WN), wm = wave / WN * (TM / WM);
     const uint32_t k0 = blockIdx.y * split.steps * 64, k1 = min(a.k, k0 + split.steps * 64);
     f32x4 acc[NI][MI];
 #pragma unroll

@@ -28,6 +28,10 @@ ROWS = [
     (16, 819, 1184, "int4", 1, 8), (19, 100, 2080, "int4", 2, 8), (64, 812, 416, "int4", 4, 8),
 ]
 
+# whole rounds of one shape, then the other columns in another: m, n, k, the first launch's shape and columns, the second's shape
+TWO = [(1544, 5875, 448, (256, 256), 4608, (256, 128)), (1562, 5278, 320, (256, 256), 4608, (128, 128)),
+       (1429, 5496, 256, (256, 256), 5376, (128, 64)), (1538, 4997, 896, (256, 128), 4992, (128, 64))]
+
 
 def cases():
     """(m, n, k, weight, the kernel's mangled name with room for x's and y's types, splits, the grid's dimension of these)."""

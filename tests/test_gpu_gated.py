@@ -67,6 +67,12 @@ def test_every_kernel(m, n, k, kind):
     check(m, n, k, "f16", kind, "gelu", out="f32", bias=n % 2 == 1, save=False, seed=2)
 
 
+@pytest.mark.parametrize("m,n,k", [c[:3] for c in gated_shapes.TWO])
+def test_whole_rounds_and_the_rest(m, n, k):
+    check(m, n, k, seed=3)
+    check(m, n, k, "f16", act="relu", out="f32", bias=False, pad=8, seed=4)
+
+
 @pytest.mark.parametrize("m", [1, 5, 40, 150])
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
 def test_activations(m, act):

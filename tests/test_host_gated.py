@@ -61,6 +61,26 @@ for m, n, k, weight, name, splits, dim in gated_shapes.cases():
 """)
 
 
+def test_whole_rounds_and_the_rest(host):  # noqa: F811
+    host(SETUP + """
+import ctypes, gated_shapes
+for m, n, k, (tn, tm), cols, (rn, rm) in gated_shapes.TWO:
+    for y in (2, 0):
+        hip.host_hip_fail(b"", 0)
+        assert gated(m=m, n=n, k=k, y_dtype=y, saved=at) == 0
+        c = launches("launch")
+        assert len(c) == 2, c
+        for line, (a, b), first, end in ((c[0], (tn, tm), 0, cols), (c[1], (rn, rm), cols, n)):
+            kernel = f"gated_large_kernelILi2ELi{y}ELi{a}ELi{b}E"
+            assert kernel in line, (m, n, k, c)
+            shape = (ctypes.c_uint * 6)()
+            assert hip.host_hip_shape(kernel.encode(), shape)
+            assert list(shape[:2]) == [-(-2 * (end - first) // a) * -(-m // b), 1], (m, n, k, list(shape))
+        hip.host_hip_fail(b"launch", 2)
+        assert gated(m=m, n=n, k=k, y_dtype=y) != 0
+""")
+
+
 def test_kernels_of_the_gradients(host):  # noqa: F811
     host(SETUP + """
 import gated_back_shapes as S
