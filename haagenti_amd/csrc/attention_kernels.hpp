@@ -36,7 +36,7 @@
 // there.  In the step kernel the other half of a column's query is zeros (that
 // kernel is bound by memory); in the tile kernel a wave's 32 columns belong to
 // one map and multiply its half of K only.  16 heads on 4 of 128: a token each
-// for 32 requests of up to 8000 30 us and 6 to join (143 MB at 4.8 TB/s), two
+// for 32 requests of up to 8000 30 us and 5.5 to join (143 MB at 4.8 TB/s), two
 // prompts of about 1500 rows over up to 2500 tokens 236 us, bound by the
 // softmax's vector work for both maps.
 //
@@ -496,54 +496,64 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void ATTENTION(step_kernel)(
 // W-th chunk.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void diff_join_kernel(const AttnArgs p) {
-    constexpr int W = 256 / (D / 4);
-    __shared__ __align__(16) float sum[W][D];
+    // rows of threads to a map; both maps at once: one after the other their
+    // loads' latencies add up (32 requests of 16 heads 6.3 us, so 5.5)
+    constexpr int W = 256 / (D / 4) / 2;
+    __shared__ __align__(16) float sum[2][W][D];
     __shared__ float parts[4];
     const uint32_t pairs = p.cols / 2, r = blockIdx.x, h = blockIdx.y / pairs, pair = blockIdx.y % pairs;
     const Request rq = request_of(p, r);
     const uint32_t cols = columns_of(p, rq);
     if (pair >= cols || cols > p.small || rq.seen <= (int32_t)p.chunk) return;
     const uint32_t n = ((uint32_t)rq.seen + p.chunk - 1) / p.chunk;
-    float value[2];
-    bool seen = false;
+    const uint64_t at = ((uint64_t)r * p.cache.kv_heads + h) * p.splits * p.cols + pair;
+    const float lambda = p.diff.d_lambda[h * p.group + pair % p.group];
+    // l in units of 2^own, the largest of O's units in the same
+    float m[2], rise[2], l[2];
 #pragma unroll
-    for (uint32_t map = 0; map < 2; map++) {
-        const uint64_t at = ((uint64_t)r * p.cache.kv_heads + h) * p.splits * p.cols + map * pairs + pair;
-        // l in units of 2^own, the largest of O's units in the same
-        float own = -__builtin_inff(), rise = -__builtin_inff(), l = 0.0f;
-        for (uint32_t s = threadIdx.x & 63u; s < n; s += 64) {
-            const float *ml = p.part_ml + 3 * (at + (uint64_t)s * p.cols);
-            const float now = fmaxf(own, ml[0]), down = own - base_of(now);
-            l = fmaf(ml[1], __builtin_amdgcn_exp2f(ml[0] - base_of(now)), l * __builtin_amdgcn_exp2f(down));
-            rise = fmaxf(rise + down, unit_of(ml[0], ml[2], now));
-            own = now;
+    for (int map = 0; map < 2; map++) m[map] = rise[map] = -__builtin_inff(), l[map] = 0.0f;
+    for (uint32_t s = threadIdx.x & 63u; s < n; s += 64)
+#pragma unroll
+        for (int map = 0; map < 2; map++) {
+            const float *ml = p.part_ml + 3 * (at + map * pairs + (uint64_t)s * p.cols);
+            const float now = fmaxf(m[map], ml[0]), down = m[map] - base_of(now);
+            l[map] = fmaf(ml[1], __builtin_amdgcn_exp2f(ml[0] - base_of(now)), l[map] * __builtin_amdgcn_exp2f(down));
+            rise[map] = fmaxf(rise[map] + down, unit_of(ml[0], ml[2], now));
+            m[map] = now;
         }
-        const float m = wave_max(own);
-        l *= __builtin_amdgcn_exp2f(own - base_of(m));
-        rise = wave_max(rise + (own - base_of(m)));
-        l = wave_sum(l);
-        const uint32_t part = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-        if (map) __syncthreads();
-        if (part < W) {
-            f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+    for (int map = 0; map < 2; map++) {
+        const float own = m[map];
+        m[map] = wave_max(own);
+        l[map] *= __builtin_amdgcn_exp2f(own - base_of(m[map]));
+        rise[map] = wave_max(rise[map] + (own - base_of(m[map])));
+        l[map] = wave_sum(l[map]);
+    }
+    const uint32_t part = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4, mine = part / W;
+    if (part < 2 * W) {
+        const float mm = mine ? m[1] : m[0], unit = base_of(mine ? rise[1] : rise[0]);
+        f32x4 o = {0, 0, 0, 0};
 #pragma unroll 8
-            for (uint32_t s = part; s < n; s += W) {
-                const uint64_t i = at + (uint64_t)s * p.cols;
-                o += __builtin_amdgcn_exp2f(unit_of(p.part_ml[3 * i], p.part_ml[3 * i + 2], m) - base_of(rise)) *
-                     *reinterpret_cast<const f32x4 *>(p.part_o + i * D + d);
-            }
-            *reinterpret_cast<f32x4 *>(&sum[part][d]) = o;
+        for (uint32_t s = part % W; s < n; s += W) {
+            const uint64_t i = at + mine * pairs + (uint64_t)s * p.cols;
+            o += __builtin_amdgcn_exp2f(unit_of(p.part_ml[3 * i], p.part_ml[3 * i + 2], mm) - unit) *
+                 *reinterpret_cast<const f32x4 *>(p.part_o + i * D + d);
         }
-        __syncthreads();
+        *reinterpret_cast<f32x4 *>(&sum[mine][part % W][d]) = o;
+    }
+    __syncthreads();
+    float value[2];
+#pragma unroll
+    for (int map = 0; map < 2; map++) {
         float o = 0.0f;
         if (threadIdx.x < D)
 #pragma unroll
-            for (int w = 0; w < W; w++) o += sum[w][threadIdx.x];
-        const float root = half_rise(rise > -__builtin_inff() ? rise : __builtin_inff());
-        value[map] = l != 0.0f ? o / l * root * root : 0.0f;
-        seen = l != 0.0f;
-        if (map) value[1] *= seen ? p.diff.d_lambda[h * p.group + pair % p.group] : 0.0f;
+            for (int w = 0; w < W; w++) o += sum[map][w][threadIdx.x];
+        const float root = half_rise(rise[map] > -__builtin_inff() ? rise[map] : __builtin_inff());
+        value[map] = l[map] != 0.0f ? o / l[map] * root * root : 0.0f;
     }
+    const bool seen = l[1] != 0.0f;
+    value[1] *= seen ? lambda : 0.0f;
     const float v = threadIdx.x < D ? value[0] - value[1] : 0.0f, squares = wave_sum(v * v);
     if ((threadIdx.x & 63u) == 0) parts[threadIdx.x >> 6] = squares;
     __syncthreads();
