@@ -5,7 +5,14 @@
 //    that the forward pass kept, rounded to x's type (half a step, what the
 //    matrix instructions take) into D = [dg | du]: m rows of 2 N columns, N =
 //    n rounded up to 64, zeros past both.  The biases' sums are taken here,
-//    before the rounding.  Bound by memory (14 bytes an element).
+//    before the rounding.  Bound by memory (14 bytes an element).  f16 has too
+//    short a range for this (dg above 65504 though dx isn't, or below 2^-24):
+//    there a first pass finds the largest |dg|, |du| of each row and of each
+//    column, and D is written twice, for dx with its rows scaled by powers of
+//    two to a largest of 2^14 to 2^15, for the weights with its columns; the
+//    products' results are scaled back in f32.  So a value is off by half a step
+//    of its own, and by at most 2^-39 of the largest of its row (column).  2048
+//    x 14336 x 4096 1037 us a call (917 without), 77 x 1003 x 1001 28 (20).
 // 2. dx = D [G; U]: a product over D's columns, the weights' rows.
 // 3. [dG; dU] = D^T x: a product over the rows of both.
 //
@@ -44,7 +51,13 @@ __device__ __forceinline__ f32x4 mma16(const u32x4 &a, const u32x4 &b, const f32
 struct SlopeArgs {
     const uint16_t *dy;
     const float *saved;   // [m][gate's n, up's n]
-    uint16_t *d;          // [rows][2 N]
+    uint16_t *d;          // [rows][2 N]; f16: for dx, or null
+    uint16_t *d_cols;     // f16: for the weights, or null
+    // f16: bits of the largest magnitudes
+    uint32_t *row_top;    // of D's rows, m rounded up to 64, and then
+    uint32_t *col_top;    // of its 2 N columns
+    uint32_t *row_part;   // [n / 256][m rounded up to 64], of 256 columns of a row, or null
+    uint32_t *col_part;   // [row block][2 N], or null
     float *part;          // [row block][2 n]: the biases' sums, or null
     float *gate_bias, *up_bias;
     uint64_t dy_stride;
@@ -84,18 +97,55 @@ __device__ __forceinline__ void act_and_slope(float z, int act, float &a, float 
     }
 }
 
+// The power of two that brings a largest magnitude (its bits) to 2^14 .. 2^15,
+// and what undoes it.  Infinities and NaN stay what they are, beside them what
+// is finite stays finite.
+__device__ __forceinline__ int power_of(uint32_t top) { return min(141 - (int)(top >> 23), 126); }
+__device__ __forceinline__ float scale_to(uint32_t top) { return __uint_as_float((uint32_t)(127 + power_of(top)) << 23); }
+__device__ __forceinline__ float scale_back(uint32_t top) { return __uint_as_float((uint32_t)(127 - power_of(top)) << 23); }
+
+__device__ __forceinline__ f32x4 scaled(const f32x4 &v, const f32x4 &by) {
+    return f32x4{v[0] * by[0], v[1] * by[1], v[2] * by[2], v[3] * by[3]};
+}
+template <int DT>
+__device__ __forceinline__ u32x2 packed(const f32x4 &v) {
+    return u32x2{f32_to_half<DT>(v[0]) | f32_to_half<DT>(v[1]) << 16, f32_to_half<DT>(v[2]) | f32_to_half<DT>(v[3]) << 16};
+}
+// Bits of the larger magnitude (NaN above all).
+__device__ __forceinline__ uint32_t larger(uint32_t top, float v) { return max(top, __float_as_uint(fabsf(v))); }
+
+// A wave's largest, in every lane.
+__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
+    auto with = [&](float other) { v = max(v, __float_as_uint(other)); };
+    with(dpp<0xb1>(__uint_as_float(v)));
+    with(dpp<0x4e>(__uint_as_float(v)));
+    with(dpp<0x141>(__uint_as_float(v)));
+    with(dpp<0x140>(__uint_as_float(v)));
+    const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((uint32_t)s[0], (uint32_t)s[1]);
+    const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max((uint32_t)t[0], (uint32_t)t[1]);
+}
+
 // 4 columns a lane, 256 a wave, every 4th row of the block a wave, R of them at
 // a time: all their loads are done, at places that are there (behind
 // conditions they wait for one another: 77 x 1003 14 us, so 4).  2048 x 14336:
-// 84 us, 411 MB at 4.9 TB/s.
-template <int DT, int R>
+// 84 us, 411 MB at 4.9 TB/s.  TOPS: the pass that finds the largest magnitudes.
+template <int DT, int R, bool TOPS>
 __global__ __launch_bounds__(256) void gated_slope_kernel(const SlopeArgs p) {
     __shared__ __align__(16) float sums[2][4][256];
     const uint32_t across = (p.wide + 255) / 256, block = blockIdx.x / across, c0 = blockIdx.x % across * 256;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = c0 + lane * 4, r0 = block * p.block_rows;
     const uint32_t end = min(r0 + p.block_rows, p.rows);
     f32x4 sg = {0, 0, 0, 0}, su = {0, 0, 0, 0};
-    if (c < p.wide) {
+    u32x4 top_g = {0, 0, 0, 0}, top_u = {0, 0, 0, 0};
+    f32x4 by_g = {1, 1, 1, 1}, by_u = {1, 1, 1, 1};  // f16: the columns' powers of two
+    if (TOPS || c < p.wide) {
+        if (!TOPS && DT == HH_F16 && p.d_cols) {
+            const u32x4 g = *reinterpret_cast<const u32x4 *>(p.col_top + c), u = *reinterpret_cast<const u32x4 *>(p.col_top + p.wide + c);
+#pragma unroll
+            for (int e = 0; e < 4; e++) by_g[e] = scale_to(g[e]), by_u[e] = scale_to(u[e]);
+        }
         for (uint32_t first = r0 + wave; first < end; first += 4 * R) {
             f32x4 d[R], g[R], u[R];
             if (c0 + 256 <= p.n) {
@@ -131,14 +181,48 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(const SlopeArgs p) {
                     act_and_slope(g[k][e], p.act, a, slope);
                     if (r < p.m && c + e < p.n) dg[e] = d[k][e] * u[k][e] * slope, du[e] = d[k][e] * a;
                 }
+                const uint64_t at = (uint64_t)r * 2 * p.wide + c;
+                if constexpr (TOPS) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        top_g[e] = larger(top_g[e], dg[e]), top_u[e] = larger(top_u[e], du[e]);
+                        top = larger(larger(top, dg[e]), du[e]);
+                    }
+                    top = wave_top(top);
+                    if (p.row_part && lane == 0) p.row_part[(uint64_t)(c0 / 256) * ((p.m + 63) / 64 * 64) + r] = top;
+                    continue;
+                }
                 sg += dg, su += du;
-                uint16_t *to = p.d + (uint64_t)r * 2 * p.wide + c;
-                *reinterpret_cast<u32x2 *>(to) = u32x2{f32_to_half<DT>(dg[0]) | f32_to_half<DT>(dg[1]) << 16,
-                                                       f32_to_half<DT>(dg[2]) | f32_to_half<DT>(dg[3]) << 16};
-                *reinterpret_cast<u32x2 *>(to + p.wide) = u32x2{f32_to_half<DT>(du[0]) | f32_to_half<DT>(du[1]) << 16,
-                                                                f32_to_half<DT>(du[2]) | f32_to_half<DT>(du[3]) << 16};
+                if constexpr (DT == HH_F16) {
+                    if (p.d) {
+                        const float by = r < p.m ? scale_to(p.row_top[r]) : 1.0f;
+                        *reinterpret_cast<u32x2 *>(p.d + at) = packed<DT>(dg * by);
+                        *reinterpret_cast<u32x2 *>(p.d + at + p.wide) = packed<DT>(du * by);
+                    }
+                    if (p.d_cols) {
+                        *reinterpret_cast<u32x2 *>(p.d_cols + at) = packed<DT>(scaled(dg, by_g));
+                        *reinterpret_cast<u32x2 *>(p.d_cols + at + p.wide) = packed<DT>(scaled(du, by_u));
+                    }
+                } else {
+                    *reinterpret_cast<u32x2 *>(p.d + at) = packed<DT>(dg);
+                    *reinterpret_cast<u32x2 *>(p.d + at + p.wide) = packed<DT>(du);
+                }
             }
         }
+    }
+    if constexpr (TOPS) {
+        if (!p.col_part) return;
+        uint32_t (*tops)[4][256] = reinterpret_cast<uint32_t (*)[4][256]>(sums);
+        *reinterpret_cast<u32x4 *>(&tops[0][wave][lane * 4]) = top_g;
+        *reinterpret_cast<u32x4 *>(&tops[1][wave][lane * 4]) = top_u;
+        __syncthreads();
+        if (c0 + threadIdx.x >= p.wide) return;
+#pragma unroll
+        for (uint32_t k = 0; k < 2; k++)
+            p.col_part[((uint64_t)block * 2 + k) * p.wide + c0 + threadIdx.x] =
+                max(max(tops[k][0][threadIdx.x], tops[k][1][threadIdx.x]), max(tops[k][2][threadIdx.x], tops[k][3][threadIdx.x]));
+        return;
     }
     if (!p.part) return;
     *reinterpret_cast<f32x4 *>(&sums[0][wave][lane * 4]) = sg;
@@ -168,6 +252,25 @@ __global__ __launch_bounds__(1024) void gated_bias_kernel(const SlopeArgs p, uin
     out[col] = s;
 }
 
+// The largest of the parts of 32 rows (columns) to a workgroup, its 32 rows of
+// threads over every 32nd part.
+__global__ __launch_bounds__(1024) void gated_tops_kernel(const SlopeArgs p, uint32_t rows, uint32_t across, uint32_t blocks) {
+    __shared__ uint32_t tops[32][33];
+    const uint32_t at = blockIdx.x * 32 + (threadIdx.x & 31u), q = threadIdx.x >> 5;
+    const bool row = blockIdx.x * 32 < rows;  // (rows are whole 64s)
+    const uint32_t *part = row ? p.row_part : p.col_part;
+    if (!part) return;
+    const uint32_t parts = row ? across : blocks, step = row ? rows : 2 * p.wide, col = row ? at : at - rows;
+    uint32_t top = 0;
+    if (!row || at < p.m)
+        for (uint32_t i = q; i < parts; i += 32) top = max(top, part[(uint64_t)i * step + col]);
+    tops[q][threadIdx.x & 31u] = top;
+    __syncthreads();
+    if (q) return;
+    for (int i = 1; i < 32; i++) top = max(top, tops[i][threadIdx.x & 31u]);
+    p.row_top[at] = top;
+}
+
 // ---------------------------------------------------------------- products
 //
 // C[r][c] = sum over t of R[r][t] L[t][c].  For dx: r the rows of x, c its
@@ -179,6 +282,7 @@ struct BackArgs {
     const uint16_t *l[2];    // the left matrix's parts: G and U, or x
     uint64_t l_stride[2];
     const uint16_t *d;
+    const uint32_t *top;     // f16: of each row of C, what D's was scaled by
     uint16_t *out[2];        // dx, or dG and dU
     uint64_t out_stride[2];
     float *partial;          // [split][rows][cols rounded up to 4], or null
@@ -233,13 +337,14 @@ __device__ __forceinline__ Place place_of(uint32_t rt, uint32_t ct) {
 
 // Outputs c .. c + 3 of row r.
 template <int DT, bool TURN>
-__device__ __forceinline__ void store_back(const BackArgs &p, uint32_t split, uint32_t r, uint32_t c, const f32x4 &v, bool wide) {
+__device__ __forceinline__ void store_back(const BackArgs &p, uint32_t split, uint32_t r, uint32_t c, f32x4 v, bool wide) {
     if (p.partial) {
         *reinterpret_cast<f32x4 *>(p.partial + ((uint64_t)split * p.rows + r) * ((p.cols + 3) / 4 * 4) + c) = v;
         return;
     }
     const uint32_t side = TURN && r >= p.wide, row = TURN && side ? r - p.wide : r;
     if (TURN && row >= p.n) return;
+    if constexpr (DT == HH_F16) v *= scale_back(p.top[r]);
     uint16_t *to = p.out[side] + row * p.out_stride[side] + c;
     if (wide && c + 4 <= p.cols) {
         *reinterpret_cast<u32x2_any *>(to) =
@@ -702,8 +807,12 @@ int32_t gated_backward(hh_context *ctx, const hh_gated_args &a, const hh_gated_g
     const uint32_t across = (wide + 255) / 256, block_rows = (uint64_t)(rows / 32) * across < 4 * (uint32_t)cus ? 4 : 32;
     const uint32_t blocks = rows / block_rows;
     if ((uint64_t)blocks * across >= 1u << 24 || px.tiles >= 1u << 23 || pw.tiles >= 1u << 23) return HH_ERR_UNSUPPORTED;
-    // D, the biases' sums of row blocks, the larger of the products' sums
-    const size_t d_bytes = (size_t)rows * 2 * wide * sizeof(uint16_t);
+    // D (f16: one for each product, the largest magnitudes and their parts),
+    // the biases' sums of row blocks, the larger of the products' sums
+    const bool f16 = DT == HH_F16 && (dx || dw);
+    const size_t one = (size_t)rows * 2 * wide * sizeof(uint16_t), tops = (size_t)rows + 2 * wide;
+    const size_t words = tops + (dx ? (size_t)across * rows : 0) + (dw ? (size_t)blocks * 2 * wide : 0);  // (whole 64s)
+    const size_t d_bytes = f16 ? one * (dx + dw) + words * sizeof(uint32_t) : one;
     const size_t b_bytes = bias ? ((size_t)blocks * 2 * a.n * sizeof(float) + 255) / 256 * 256 : 0;
     float *room = nullptr;
     const int32_t rc = op_room(ctx, s, d_bytes + b_bytes + (px.room > pw.room ? px.room : pw.room), &room);
@@ -711,27 +820,47 @@ int32_t gated_backward(hh_context *ctx, const hh_gated_args &a, const hh_gated_g
     uint8_t *at = reinterpret_cast<uint8_t *>(room);
     SlopeArgs sl = {};
     sl.dy = reinterpret_cast<const uint16_t *>(d.d_dy), sl.dy_stride = d.dy_stride;
-    sl.saved = a.d_saved, sl.d = reinterpret_cast<uint16_t *>(at);
+    sl.saved = a.d_saved, sl.d = DT == HH_F16 && !dx ? nullptr : reinterpret_cast<uint16_t *>(at);
     sl.part = bias ? reinterpret_cast<float *>(at + d_bytes) : nullptr;
     sl.gate_bias = d.d_dgate_bias, sl.up_bias = d.d_dup_bias;
     sl.m = a.m, sl.n = a.n, sl.wide = wide, sl.rows = dw ? rows : a.m, sl.act = a.activation;
     sl.block_rows = block_rows;
-    if (block_rows == 4)
-        hipLaunchKernelGGL((gated_slope_kernel<DT, 1>), dim3(across * blocks), dim3(256), 0, s, sl);
-    else
-        hipLaunchKernelGGL((gated_slope_kernel<DT, 4>), dim3(across * blocks), dim3(256), 0, s, sl);
-    int32_t e = from_hip(hipGetLastError());
+    const dim3 grid(across * blocks);
+    auto slope = [&](auto tops) {
+        constexpr bool TOPS = decltype(tops)::value;
+        if (block_rows == 4)
+            hipLaunchKernelGGL((gated_slope_kernel<DT, 1, TOPS>), grid, dim3(256), 0, s, sl);
+        else
+            hipLaunchKernelGGL((gated_slope_kernel<DT, 4, TOPS>), grid, dim3(256), 0, s, sl);
+        return from_hip(hipGetLastError());
+    };
+    int32_t e = HH_OK;
+    if (f16) {
+        uint8_t *d_cols = at + one * dx;
+        uint32_t *next = reinterpret_cast<uint32_t *>(d_cols + one * dw);
+        sl.row_top = next, sl.col_top = next + rows, next += tops;
+        if (dx) sl.row_part = next, next += (size_t)across * rows;
+        if (dw) sl.col_part = next;
+        sl.d_cols = dw ? reinterpret_cast<uint16_t *>(d_cols) : nullptr;
+        if constexpr (DT == HH_F16) e = slope(std::true_type());
+        if (e == HH_OK) {
+            hipLaunchKernelGGL(gated_tops_kernel, dim3((uint32_t)(tops / 32)), dim3(1024), 0, s, sl, rows, across, blocks);
+            e = from_hip(hipGetLastError());
+        }
+    }
+    if (e == HH_OK) e = slope(std::false_type());
     if (e == HH_OK && bias) {
         hipLaunchKernelGGL(gated_bias_kernel, dim3((a.n + 31) / 32, 2), dim3(1024), 0, s, sl, blocks);
         e = from_hip(hipGetLastError());
     }
     float *sums = reinterpret_cast<float *>(at + d_bytes + b_bytes);
     BackArgs p = {};
-    p.d = sl.d, p.cols = a.k, p.n = a.n, p.wide = wide;
+    p.cols = a.k, p.n = a.n, p.wide = wide;
     if (e == HH_OK && dx) {
         p.l[0] = reinterpret_cast<const uint16_t *>(a.d_gate), p.l[1] = reinterpret_cast<const uint16_t *>(a.d_up);
         p.l_stride[0] = a.gate_stride, p.l_stride[1] = a.up_stride;
         p.out[0] = reinterpret_cast<uint16_t *>(d.d_dx), p.out_stride[0] = d.dx_stride;
+        p.d = sl.d, p.top = sl.row_top;
         p.rows = a.m, p.depth = a.n;
         e = launch_back<DT, false>(p, px, x_aligned, sums, s);
     }
@@ -739,6 +868,7 @@ int32_t gated_backward(hh_context *ctx, const hh_gated_args &a, const hh_gated_g
         p.l[0] = reinterpret_cast<const uint16_t *>(a.d_x), p.l_stride[0] = a.x_stride;
         p.out[0] = reinterpret_cast<uint16_t *>(d.d_dgate), p.out[1] = reinterpret_cast<uint16_t *>(d.d_dup);
         p.out_stride[0] = d.dgate_stride, p.out_stride[1] = d.dup_stride;
+        p.d = f16 ? sl.d_cols : sl.d, p.top = sl.col_top;
         p.rows = 2 * wide, p.depth = a.m;
         e = launch_back<DT, true>(p, pw, w_aligned, sums, s);
     }

@@ -805,11 +805,15 @@ int32_t hh_gated_linear(hh_context *ctx, const hh_gated_args *args, void *stream
  * with dg = dy up act'(gate) and du = dy act(gate),
  *   dx = dg G + du U,  dG = dg^T x,  dU = du^T x,  sums of dg and du over the
  * rows for the biases (f32).  Any of the outputs may be NULL, dG and dU both
- * or neither.  dg and du are computed in f32 and rounded to x's type for the
- * products (the biases' sums are not), whose sums are f32; outputs are
- * rounded once, to x's type.  16-bit weights only (HH_ERR_UNSUPPORTED for
+ * or neither.  dg and du are computed in f32 and rounded for the products
+ * (the biases' sums are not), whose sums are f32; outputs are rounded once, to
+ * x's type.  bf16: to 8 bits.  f16: to 11 bits, or to 2^-39 of the largest
+ * magnitude among a row's dg and du (for dx) or among the rows of a column (for
+ * dG and dU), whatever that is: what leaves f16's range there doesn't matter,
+ * only what does in the outputs.  16-bit weights only (HH_ERR_UNSUPPORTED for
  * INT4 buffers).  d_y and the biases of args are not read.  relu's slope at 0
- * is 0. */
+ * is 0.  Outputs overlap neither each other nor anything that is read (not
+ * checked: a dx over x would change dG and dU). */
 typedef struct hh_gated_grads {
     const void *d_dy;
     void *d_dx, *d_dgate, *d_dup;
