@@ -16,7 +16,9 @@
 // memory bounds, adds the rest of P as a second f16 (22 bits; 48 requests 93.1
 // us, 92.2 without it, 131,001 tokens 52.3 and 51.8); for the tile kernel that
 // is half as much again of the matrix products (two prompts 573 us, 440
-// without) for errors below half a unit of its outputs.
+// without) for errors below half a unit of its outputs.  Not so where two maps
+// are subtracted, which may nearly cancel: with two maps it adds the rest too
+// (two prompts 277 us a call, 214 without).
 // P's exponent is z - m + share, share = log2(scale of V's block) - rise, rise
 // standing for M - m; the sum l takes the share out again per 16 tokens (a
 // share below 2^-40 counts as 2^-40: such a P is 0 in f16 anyway, and l keeps
@@ -37,8 +39,9 @@
 // kernel is bound by memory); in the tile kernel a wave's 32 columns belong to
 // one map and multiply its half of K only.  16 heads on 4 of 128: a token each
 // for 32 requests of up to 8000 30 us and 5.5 to join (143 MB at 4.8 TB/s), two
-// prompts of about 1500 rows over up to 2500 tokens 236 us, bound by the
-// softmax's vector work for both maps.
+// prompts of about 1500 rows over up to 2500 tokens 277 us a call, bound by the
+// softmax's vector work and the matrix products for both maps, one after the
+// other.
 //
 // bf16 queries are scaled by a power of two, to a largest magnitude of 2^14 to
 // 2^15 per row, before they become f16: exact down to 2^-31 of the largest, off
@@ -644,7 +647,7 @@ __global__ __launch_bounds__(64 * NW) void ATTENTION(tile_kernel)(const AttnArgs
     __shared__ __align__(16) float lks[2][4], lvs[2][4];  // K's scales, logarithms of V's
     // the last tiles of all requests and heads, which see most, first (by head
     // and request first: two prompts' 496 workgroups 520 us, so 486; two
-    // maps' 384 266 us, so 236)
+    // maps' 384 266 us, so 236, both without P's rest)
     const uint32_t lanes = p.a.requests * p.cache.kv_heads;
     const uint64_t id = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x;
     const uint32_t lane_of = (uint32_t)(id % lanes), r = lane_of / p.cache.kv_heads, h = lane_of % p.cache.kv_heads;
@@ -817,7 +820,7 @@ __global__ __launch_bounds__(64 * NW) void ATTENTION(tile_kernel)(const AttnArgs
             for (int u = 0; u < 4; u++) share[u] = share_of(log_vs[u], tops.rise);
         }
         const float ref = base_of(tops.m);
-        f16x8 pv[4];
+        f16x8 pv[4], rest[kDiff ? 4 : 1];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const float less = share[u] - ref;
@@ -827,6 +830,7 @@ __global__ __launch_bounds__(64 * NW) void ATTENTION(tile_kernel)(const AttnArgs
                 const float e = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + i], c[u], less));
                 sum += e;
                 pv[u][i] = (_Float16)e;
+                if constexpr (kDiff) rest[u][i] = (_Float16)(e - (float)pv[u][i]);
             }
             l = fmaf(sum, __builtin_amdgcn_exp2f(-share[u]), l);
         }
@@ -835,6 +839,7 @@ __global__ __launch_bounds__(64 * NW) void ATTENTION(tile_kernel)(const AttnArgs
 #pragma unroll
             for (int f = 0; f < 4; f++) {
                 const f16x8 a = *reinterpret_cast<const f16x8 *>(&lv[b][(t * 32 + (lane & 31)) * VP + f * 16 + hl * 8]);
+                if constexpr (kDiff) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, rest[f], o[t], 0, 0, 0);
                 o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pv[f], o[t], 0, 0, 0);
             }
     }

@@ -926,8 +926,8 @@ int32_t hh_kv_attention(hh_context *ctx, const hh_kv_cache *cache, const hh_kv_a
  * o / sqrt(mean(o^2) + eps) * norm_weight * gain over each head's dimensions,
  * else o * gain.  Arguments, limits and what rows see are hh_kv_attention's
  * (args); rows that see no token give zeros.  A row's probabilities are
- * rounded as there, each map's in units of its own largest: 22 bits for
- * requests of at most 8 rows times q_heads / kv_heads, else 11. */
+ * rounded to 22 bits, each map's in units of its own largest (of the largest
+ * product with a scale, as there): the maps may nearly cancel. */
 typedef struct hh_kv_diff_args {
     const float *d_lambda;      /* q_heads */
     const float *d_norm_weight; /* head_dim, or NULL */
