@@ -256,13 +256,15 @@ __device__ __forceinline__ void store4(uint16_t *to, bool wide, const float *v) 
 
 #if HH_DIFF
 // What the norm multiplies a head's outputs by, from the sum of their squares;
-// the weight of dimension d is apart.
+// the weight of dimension d is apart.  A row that sees nothing is zeros whatever
+// its weight is.
 template <int D>
 __device__ __forceinline__ float norm_factor(const AttnArgs &p, float squares) {
     return p.diff.d_norm_weight ? p.diff.gain / sqrtf(squares * (1.0f / D) + p.diff.eps) : p.diff.gain;
 }
-__device__ __forceinline__ float norm_weight(const AttnArgs &p, uint32_t d) {
-    return p.diff.d_norm_weight ? p.diff.d_norm_weight[d] : 1.0f;
+__device__ __forceinline__ float norm_weight(const AttnArgs &p, uint32_t d, bool seen) {
+    const float w = p.diff.d_norm_weight ? p.diff.d_norm_weight[d] : 1.0f;  // (loaded without a condition of the row)
+    return seen ? w : 1.0f;
 }
 #endif
 
@@ -472,7 +474,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void ATTENTION(step_kernel)(
         for (int t = 0; t < VT; t++) {
             float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = o[t][i] * factor * norm_weight(p, 16 * t + 4 * u + i);
+            for (int i = 0; i < 4; i++) v[i] = o[t][i] * factor * norm_weight(p, 16 * t + 4 * u + i, ll != 0.0f);
             store4<DT>(out + 16 * t + 4 * u, wide, v);
         }
 #else
@@ -564,7 +566,7 @@ __global__ __launch_bounds__(256) void diff_join_kernel(const AttnArgs p) {
     const float factor = seen ? norm_factor<D>(p, (parts[0] + parts[1]) + (parts[2] + parts[3])) : 0.0f;
     uint16_t *out = reinterpret_cast<uint16_t *>(p.a.d_out) + ((uint64_t)rq.q0 + pair / p.group) * p.a.out_token_stride +
                     (h * p.group + pair % p.group) * p.a.out_head_stride;
-    out[threadIdx.x] = (uint16_t)f32_to_half<DT>(v * factor * norm_weight(p, threadIdx.x));
+    out[threadIdx.x] = (uint16_t)f32_to_half<DT>(v * factor * norm_weight(p, threadIdx.x, seen));
 }
 #else
 // Joins the chunks of a request's column: one workgroup per request, head and
@@ -881,7 +883,7 @@ __global__ __launch_bounds__(64 * NW) void ATTENTION(tile_kernel)(const AttnArgs
         for (int i = 0; i < 16; i += 4) {
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = o[t][i + e] * factor * norm_weight(p, 32 * t + 2 * i + 4 * hl + e);
+            for (int e = 0; e < 4; e++) v[e] = o[t][i + e] * factor * norm_weight(p, 32 * t + 2 * i + 4 * hl + e, l != 0.0f);
             store4<DT>(out + 32 * t + 2 * i + 4 * hl, wide, v);
         }
 #else
