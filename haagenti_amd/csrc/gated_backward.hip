@@ -337,7 +337,7 @@ __device__ __forceinline__ Place place_of(uint32_t rt, uint32_t ct) {
 
 // Outputs c .. c + 3 of row r.
 template <int DT, bool TURN>
-__device__ __forceinline__ void store_back(const BackArgs &p, uint32_t split, uint32_t r, uint32_t c, f32x4 v, bool wide) {
+__device__ __forceinline__ void store_back(const BackArgs &p, uint32_t split, uint32_t r, uint32_t c, f32x4 v) {
     if (p.partial) {
         *reinterpret_cast<f32x4 *>(p.partial + ((uint64_t)split * p.rows + r) * ((p.cols + 3) / 4 * 4) + c) = v;
         return;
@@ -346,7 +346,7 @@ __device__ __forceinline__ void store_back(const BackArgs &p, uint32_t split, ui
     if (TURN && row >= p.n) return;
     if constexpr (DT == HH_F16) v *= scale_back(p.top[r]);
     uint16_t *to = p.out[side] + row * p.out_stride[side] + c;
-    if (wide && c + 4 <= p.cols) {
+    if (c + 4 <= p.cols) {
         *reinterpret_cast<u32x2_any *>(to) =
             u32x2{f32_to_half<DT>(v[0]) | f32_to_half<DT>(v[1]) << 16, f32_to_half<DT>(v[2]) | f32_to_half<DT>(v[3]) << 16};
         return;
@@ -605,7 +605,7 @@ __global__ __launch_bounds__(64 * WC * WR) void gated_back_kernel(const BackArgs
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 const f32x4 v = own[(4 * q + g) * Q + (r ^ (4 * q + g))];
-                if (row + 4 * q < p.rows && c < p.cols) store_back<DT, TURN>(p, blockIdx.y, row + 4 * q, c, v, true);
+                if (row + 4 * q < p.rows && c < p.cols) store_back<DT, TURN>(p, blockIdx.y, row + 4 * q, c, v);
             }
         }
 }
@@ -704,7 +704,7 @@ __global__ __launch_bounds__(256) void gated_back_any_kernel(const BackArgs p) {
 #pragma unroll
         for (int i = 0; i < F; i++) {
             const uint32_t row = r0 + wr + 16 * j + r, c = c0 + wc + 16 * i + 4 * g;
-            if (row < p.rows && c < p.cols) store_back<DT, TURN>(p, blockIdx.y, row, c, acc[i][j], true);
+            if (row < p.rows && c < p.cols) store_back<DT, TURN>(p, blockIdx.y, row, c, acc[i][j]);
         }
 }
 
@@ -721,7 +721,7 @@ __global__ __launch_bounds__(256) void gated_back_join_kernel(const BackArgs p, 
     for (uint32_t j = 0; j < splits; j++) s += *reinterpret_cast<const f32x4 *>(p.partial + j * step + (uint64_t)r * quads * 4 + c);
     BackArgs q = p;
     q.partial = nullptr;
-    store_back<DT, TURN>(q, 0, r, c, s, true);
+    store_back<DT, TURN>(q, 0, r, c, s);
 }
 
 // ---------------------------------------------------------------- host
