@@ -670,6 +670,7 @@ class KvCache:
         dimensions; with norm_weight (head_dim float32 values) the root mean
         square norm of each head's outputs times norm_weight, then times gain.
         lam: q_heads float32 values; scale defaults to (head_dim / 2) ** -0.5;
+        out lies, from its first to its last element, apart from what is read;
         the rest as for attention."""
         what, ctx = "diff_attention", self.ctx
         if q.dim() != 3:

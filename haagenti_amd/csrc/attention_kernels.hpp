@@ -18,7 +18,7 @@
 // is half as much again of the matrix products (two prompts 573 us, 440
 // without) for errors below half a unit of its outputs.  Not so where two maps
 // are subtracted, which may nearly cancel: with two maps it adds the rest too
-// (two prompts 277 us a call, 214 without).
+// (two prompts 277 to 283 us a call, 214 without).
 // P's exponent is z - m + share, share = log2(scale of V's block) - rise, rise
 // standing for M - m; the sum l takes the share out again per 16 tokens (a
 // share below 2^-40 counts as 2^-40: such a P is 0 in f16 anyway, and l keeps
@@ -39,7 +39,7 @@
 // kernel is bound by memory); in the tile kernel a wave's 32 columns belong to
 // one map and multiply its half of K only.  16 heads on 4 of 128: a token each
 // for 32 requests of up to 8000 30 us and 5.5 to join (143 MB at 4.8 TB/s), two
-// prompts of about 1500 rows over up to 2500 tokens 277 us a call, bound by the
+// prompts of about 1500 rows over up to 2500 tokens 277 to 283 us a call, bound by the
 // softmax's vector work and the matrix products for both maps, one after the
 // other.
 //
@@ -960,6 +960,11 @@ int32_t run_attention(hh_context *ctx, const hh_kv_cache *cache, const hh_kv_att
     p.group = group;
     p.bs_log = (uint32_t)__builtin_ctz(cache->block_size);
     p.block_step = cache->kv_heads * cache->block_size * cache->head_dim;
+    // Requests of more columns are the tile kernel's, which walks all their
+    // tokens in one workgroup to a cache head and tile.  So few rows over many
+    // tokens are slow from there on: a token of 16 heads on one over 131,000 at
+    // two maps 5256 us, 20 of 8 heads; 4 rows of 16 on 4 over 100,000 3999, 33 of
+    // 2 rows; with one map 4 rows of 32 on 4 3335, 32 of 16 on 4.
     p.small = kDiff ? 8 : 16;
     p.cols = (uint32_t)(most < 1 ? 1 : most < p.small ? most : p.small) * (kDiff ? 2 : 1);
     const uint64_t room = (uint64_t)a->table_width * cache->block_size;

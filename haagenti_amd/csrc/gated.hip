@@ -5,10 +5,12 @@
 //
 // Beside two products (up, then gate with the product as epilogue) x is read
 // once, up's output not written and read between, and one launch less.  bf16,
-// 14336 x 4096: a token 41 us (235 MB of weights at 5.7 TB/s); 16 tokens of
-// INT4 33 us (66 MB at 2 TB/s: loads of 64 bytes a row, and their scales); 2048
-// tokens with what is kept 405 and 99 us in two launches (950 TFLOP/s; the
-// library's bare product 415), bound by LDS beside the matrix pipes.
+// 14336 x 4096: a token 40 us (235 MB of weights at 5.9 TB/s); 16 tokens of
+// INT4 33 us (66 MB at 2 TB/s: loads of 64 bytes a row, and their scales), both
+// the kernel's by a profiler; a call of 2048 tokens 429 us, with what is kept 454
+// (1060 TFLOP/s; the library's bare product in the same run 334), bound by LDS
+// beside the matrix pipes.  INT4 of 2048 tokens, in tiles through registers 1082
+// us; of rows of 4097 values, whose groups cross rows, 1 to 16 tokens 166 to 170.
 #define HH_GATED 1
 #include "linear_kernels.hpp"
 
@@ -37,9 +39,11 @@ TilePlan plan_gated(const hh_linear_args &a, int cus, const Shape (&shapes)[N]) 
 }
 // Where a last round of tiles leaves CUs idle, whole rounds and then a launch
 // of smaller tiles for the other columns, if that is expected to be faster: the
-// first launch's columns (all of them: n) and the second's shape.  2048 x 14336
-// x 4096: 896 tiles of 256 x 256 on 256 CUs 561 us, 768 and 256 of 256 x 128
-// 542; 3000 x 5504 x 2048 174, so 148.
+// first launch's columns (all of them: n) and the second's shape.  The estimate
+// is the plain product's; what is kept, 8 bytes an output beside y's, isn't in
+// it.  Calls: 2048 x 14336 x 4096 in 896 tiles of 256 x 256 on 256 CUs 446 us
+// (470 with what is kept), in 768 and 256 of 256 x 128 428 (454); 3000 x 5504 x
+// 2048 169 (170), so 143 (144).
 uint32_t whole_rounds(const hh_linear_args &a, int cus, const TilePlan &plan, int *rest_shape) {
     if (plan.splits > 1) return a.n;
     const Shape &s = kLargeShapes[plan.shape];

@@ -23,9 +23,11 @@
 // read.  Nothing is transposed through memory (the weights alone would cost 85
 // us at 2 x 14336 x 4096).
 //
-// 2048 x 14336 x 4096 bf16: slope 84 us, dx 440 and 14 to join its two splits
-// (1090 TFLOP/s; the library's product 495), the weights'
-// 457 (1050; 559), bound by LDS reads beside the matrix pipes.
+// 2048 x 14336 x 4096 bf16, calls of one run: all 908 us; the slope alone 82,
+// with dx 490, so that dx and the join of its two splits take 408 (1180 TFLOP/s;
+// the library's product 395), with the weights' 481, so 399 (1200; 444).  By a
+// profiler, where all are slower: 85, 447 + 15 and 473.  Bound by LDS reads
+// beside the matrix pipes.
 #include <type_traits>
 
 #include "layer_ops.hpp"
@@ -359,7 +361,7 @@ __device__ __forceinline__ void store_back(const BackArgs &p, uint32_t split, ui
 // Aligned operands, copied straight to LDS in tiles 32 deep, four of them in
 // turn: three are on their way while one is multiplied (64 deep and two in
 // turn, a copy has one tile's products to arrive in: 483 and 479 us where
-// these take 440 and 457), 16-byte pieces at places that depend on their row.  One
+// these took 440 and 457, by a profiler), 16-byte pieces at places that depend on their row.  One
 // barrier a tile: before it a wave waits for its own part of the next tile's
 // copies, the oldest under way, and for its reads of the last one.
 __device__ __forceinline__ uint32_t shift_of(uint32_t row) { return (0u - (row >> 2)) & 3u; }
@@ -727,7 +729,12 @@ __global__ __launch_bounds__(256) void gated_back_join_kernel(const BackArgs p, 
 // ---------------------------------------------------------------- host
 
 // A tile shape (columns, rows), workgroups to a CU, microseconds per 64 t with
-// all of them and with one alone.
+// all of them and with one alone.  These are the forward kernels' figures; of
+// the kernels here, by a profiler, the weights' took 1.62, 0.88, 0.88, 0.97
+// (alone 0.65), 0.96 (0.49), through registers 1.53 (1.12), 1.27 (0.72), and
+// dx's 2.06, 1.40, 1.49, 1.41 (0.91), 1.60 (0.67), through registers 1.56
+// (1.24), 1.52 (0.76).  So they rank the shapes of a product, within a fifth for
+// most, and are no times of it; tables of their own were not tried.
 struct Shape {
     uint32_t c, r, per_cu;
     double us, alone;

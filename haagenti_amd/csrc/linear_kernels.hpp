@@ -295,7 +295,10 @@ __global__ __launch_bounds__(64 * KW) void PRODUCT(rows_kernel)(const Args p) {
     static_assert(!kGated || NT % 2 == 0, "both weights' rows");
     constexpr uint32_t STEP = 128 * KW;                       // columns between a wave's 128s
     constexpr int W = INT4 ? 1 : 4;                           // loads of 16 bytes per lane and 128 columns
-    constexpr int AHEAD = 2;       // 128s of W in registers, one in use
+    // 128s of W in registers, one in use.  (INT4: the compiler moves the scales
+    // between registers where a fetch is left out and waits for the newest loads
+    // there, so that nothing is on its way across every second 128.)
+    constexpr int AHEAD = 2;
     constexpr bool XA = MT <= 2;                              // x's values one 128 ahead, where registers allow
     __shared__ __align__(16) float part[kGated ? 2 : 1][KW][16 * MT][20];
     const hh_linear_args &a = p.a;

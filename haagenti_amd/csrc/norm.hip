@@ -11,9 +11,15 @@
 // and its variance is summed about its mean, in f32.  The backward pass
 // recomputes both from x, which it reads anyway: two sums over registers cost
 // less than statistics kept, passed and checked.  W = 1 needs no LDS and no
-// barrier; more waves take rows too long for one wave, and few rows.  8192 rows
-// of 4096 bf16: 24 us, 134 MB at 5.6 TB/s; gradients with add 58 us, 268 MB at
-// 4.7 TB/s, and 6 us to join the workgroups' sums; 8 rows 3.9 us.
+// barrier; more waves take rows too long for one wave, and few rows.  Kernels'
+// times, by a profiler: 8192 rows of 4096 bf16 24 us, 134 MB at 5.6 TB/s;
+// gradients with add 57 us, 268 MB at 4.7 TB/s, and 6 us to join the workgroups'
+// sums; 8 rows 3.6 us.
+//
+// The loops ask for the next row before they work on this one, but the compiler
+// waits for it at once (the request is under a condition, and what comes after
+// must hold either way): what hides a row's loads are the CU's other waves (at
+// 4096 values 16 forward and 8 backward).
 #include "layer_ops.hpp"
 
 namespace hh {
@@ -250,7 +256,7 @@ __global__ __launch_bounds__(64 * W * G) void norm_kernel(const NormArgs p) {
 template <int XT, int W, int G, int C>
 __global__ __launch_bounds__(64 * W * G) void norm_backward_kernel(const NormArgs p) {
     constexpr int V = Elem<XT>::V, T = 64 * W;
-    constexpr bool AHEAD = C * V <= 16;   // the next row on its way and the weights in registers, where these allow
+    constexpr bool AHEAD = C * V <= 16;   // the next row asked for early and the weights in registers, where these allow
     __shared__ float lds[2][W * G][3];
     __shared__ __align__(16) float join[G > 1 ? G : 1][G > 1 ? T * 4 : 4];
     const uint32_t t = threadIdx.x % T, group = threadIdx.x / T, step = gridDim.x * G;
@@ -402,10 +408,14 @@ __global__ __launch_bounds__(256) void norm_zero_kernel(const NormArgs p) {
 }
 
 // Waves to a row, rows to a workgroup at a time, pieces to a lane, workgroups
-// to a CU.  Few pieces to a lane, so that the next row is on its way while one
-// is worked on: layer norm of 8192 x 4096 bf16 takes 25 us with 4 waves of 2
-// pieces (30 with 2 of 4, 38 with one of 8), its gradients 70 (96, 127; 64
-// since).
+// to a CU.  Few pieces to a lane, so few registers and many waves: when this was
+// chosen a call of layer norm of 8192 x 4096 bf16 took 25 us with 4 waves of 2
+// pieces (30 with 2 of 4, 38 with one of 8), of its gradients 70 (96, 127; now
+// 52, with add 62 to 67).  Rows of more than 1024 pieces need 16 waves, whose
+// workgroups leave a lane 128 registers: too few for the gradients, which spill
+// 44 to 624 bytes a lane there (the forward pass 24 with 4 pieces).  Calls with
+// add: 8192 x 12288 bf16 710 us (1.1 TB/s; forward 97, 4.2 TB/s), 4096 x 16384
+// 408 (51); 2048 x 16384 f32 without add 275 (46).
 struct NormPlan {
     int w, g, c;
     uint32_t grid;
